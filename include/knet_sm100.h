@@ -343,6 +343,39 @@ KNET_BOTH_TYPES(KNET_DECL_SOFTMAX, softmax)
                                  int64_t K, int dims, int32_t *result, cudaStream_t s);
 KNET_BOTH_TYPES(KNET_DECL_NLL, nll)
 
+/* nll of a linear output layer, scores = W x (+ b), without the (V,N) score matrix: what
+ * `nll(W*x .+ b, labels)` composes from a matrix product, a broadcast and the loss
+ * (src/ops20/loss.jl:37-41, src/knetarrays/linalg.jl:11), for vocabularies whose scores,
+ * logsoftmax and score gradients should not all be kept.  W is (V,H) (transW 0) or (H,V)
+ * (transW 1: the embedding matrix of a tied model), x (H,N), b of V or NULL; labels 1-based
+ * Int32, 0 = skip the instance, anything outside 0..V makes the loss NaN.  All column-major.
+ * fwd: *total = sum over used instances of lse - s[label], *count = instances used,
+ *      per_instance of N their terms (0 when skipped); lse of 2N: log sum_v exp(s_vn) rounded,
+ *      then what the rounding left (both are what bwd reads).
+ * bwd: with g = dy (average 0) or dy / *count (average 1; *count 0 gives g = 0),
+ *      dx (H,N) = W' dS, dW (as W) = dS x', db (V) = sum over n of dS, where
+ *      dS = (softmax - onehot) g, 0 on skipped instances.  Any of dw, db, dx may be NULL; they
+ *      must not overlap an input.  The scores are computed again, a piece of the vocabulary at a
+ *      time.  Results are the same from run to run.
+ * Scores of -inf (a bias that masks a class) have probability 0; a class masked on every
+ * instance is fine, an instance with every class masked gives NaN, as the composed form does.
+ * workspace: at least knet_linear_nll_workspace_S(V, H, N, backward) bytes (0 for sizes that the
+ * entry points refuse), 256-byte aligned; calls that share one must be ordered on one stream.
+ * Nothing is allocated, nothing synchronises, calls can be captured.  V, H, N <= 2^22 - 64. */
+#define KNET_DECL_LINEAR_NLL(f, S, T)                                                          \
+  KNET_API size_t knet_linear_nll_workspace_##S(int64_t V, int64_t H, int64_t N, int backward); \
+  KNET_API int knet_linear_nll_fwd_##S(const T *w, int transW, const T *b, const T *x,         \
+                                       const int32_t *labels, int64_t V, int64_t H, int64_t N, \
+                                       T *total, int32_t *count, T *lse, T *per_instance,      \
+                                       void *workspace, size_t workspace_bytes,                \
+                                       cudaStream_t s);                                        \
+  KNET_API int knet_linear_nll_bwd_##S(const T *w, int transW, const T *b, const T *x,         \
+                                       const int32_t *labels, int64_t V, int64_t H, int64_t N, \
+                                       const T *lse, int average, T dy, const int32_t *count,  \
+                                       T *dw, T *db, T *dx, void *workspace,                   \
+                                       size_t workspace_bytes, cudaStream_t s);
+KNET_BOTH_TYPES(KNET_DECL_LINEAR_NLL, linear_nll)
+
 /* Whole-array reduction to a device scalar without a synchronisation or an allocation.
  * op: 0 sum 1 prod 2 maximum 3 minimum 4 sumabs 5 sumabs2 6 maxabs 7 minabs 8 countnz.
  * `workspace` is caller scratch of knet_reduce_workspace_bytes() bytes, 256-byte aligned;
@@ -478,6 +511,41 @@ KNET_API int64_t knet_multi_plan(knet_tensor_desc *host_table, int ntensors);
                                      double beta2, double eps, int t, double gscale,            \
                                      const double *factors, cudaStream_t s);
 KNET_BOTH_TYPES(KNET_DECL_MULTI, multi)
+
+/* The norm of all gradients of a parameter set taken as one vector, and clipping by it (the
+ * reference clips array by array, src/train20/update.jl:572-583).
+ * gnorm:        *norm = |gscale| * sqrt(sum over all tensors of g^2), in Float64.
+ * gclip_global: the same norm, and *factor = gclip / norm when norm > gclip, else 1 (also for a
+ *               NaN norm); gclip > 0.  Both take two launches and add in a fixed order;
+ *               `partials` is scratch of total_chunks doubles.
+ * gclip_apply:  g = lmul!(*factor, g) on every tensor; a factor of 1 touches nothing.
+ * _gc updates:  as the multi-tensor updates above with g replaced on load by lmul!(*factor, g);
+ *               adam_multi_gcg also reads its bias corrections from device memory (see
+ *               adam_multi_g), for a captured step. */
+#define KNET_DECL_GNORM(f, S, T)                                                                 \
+  KNET_API int knet_gnorm_##S(const knet_tensor_desc *table, int ntensors, int64_t total_chunks, \
+                              double gscale, double *partials, double *norm, cudaStream_t s);    \
+  KNET_API int knet_gclip_global_##S(const knet_tensor_desc *table, int ntensors,                \
+                                     int64_t total_chunks, double gclip, double gscale,          \
+                                     double *partials, double *norm, double *factor,             \
+                                     cudaStream_t s);                                            \
+  KNET_API int knet_gclip_apply_##S(const knet_tensor_desc *table, int ntensors,                 \
+                                    int64_t total_chunks, const double *factor, cudaStream_t s); \
+  KNET_API int knet_sgd_multi_gc_##S(const knet_tensor_desc *table, int ntensors,                \
+                                     int64_t total_chunks, double lr, double gscale,             \
+                                     const double *factor, cudaStream_t s);                      \
+  KNET_API int knet_momentum_multi_gc_##S(const knet_tensor_desc *table, int ntensors,           \
+                                          int64_t total_chunks, double lr, double gamma,         \
+                                          double gscale, const double *factor, cudaStream_t s);  \
+  KNET_API int knet_adam_multi_gc_##S(const knet_tensor_desc *table, int ntensors,               \
+                                      int64_t total_chunks, double lr, double beta1,             \
+                                      double beta2, double eps, int t, double gscale,            \
+                                      const double *factor, cudaStream_t s);                     \
+  KNET_API int knet_adam_multi_gcg_##S(const knet_tensor_desc *table, int ntensors,              \
+                                       int64_t total_chunks, double lr, double beta1,            \
+                                       double beta2, double eps, const T *bias_corr,             \
+                                       double gscale, const double *factor, cudaStream_t s);
+KNET_BOTH_TYPES(KNET_DECL_GNORM, gnorm)
 
 /* =====================================================================================
  * C. Data-parallel collectives (one process per GPU; NCCL over NVLink, loaded at run time).

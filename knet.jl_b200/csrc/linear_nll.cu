@@ -1,0 +1,368 @@
+// Softmax cross entropy of a linear output layer, scores = W x (+ b), without the score matrix:
+//   forward   lse_n = log sum_v exp(s_vn),  loss = sum over used n of lse_n - s_{label_n, n}
+//   backward  dS = (exp(s - lse) - onehot) * g,  dx = W' dS,  dW = dS x',  db = sum_n dS
+// The forward keeps per instance and tile of the vocabulary the maximum and the sum of
+// exponentials; the backward computes the scores again, a piece of the vocabulary at a time, turns
+// them into dS in the workspace and multiplies that piece by W and x.  Knet composes the same from
+// `W*x .+ b` and nll (src/ops20/loss.jl:37-41), which keeps scores, logsoftmax and their gradients.
+//
+// An instance's loss is lse - s[label]; the forward hands lse on as an unevaluated sum of two
+// numbers (its rounding alone would be a relative error of |lse| * 2^-24 in every p of that
+// instance), so that p = exp((s - hi) - lo).
+#include "linear_nll.cuh"
+
+namespace kn {
+
+// ---- matrix products on the FMA pipe ---------------------------------------------------------------
+// acc(i, j) = sum_c A(i, c) * B(j, c) for a 64x64 tile of (i, j), 4x4 per thread, c in steps of 16
+// through shared memory.  Operands have any strides with one of the two equal to 1.
+
+template <typename T> struct Strided {
+  const T* p;
+  int64_t si, sc;      // element (i, c) at p + i*si + c*sc
+};
+
+constexpr int kTile = 64, kStep = 16, kSimtThreads = 256;
+
+template <typename T>
+__device__ __forceinline__ void simt_load(T (&dst)[kStep][kTile + 4], const Strided<T>& a, int64_t i0, int64_t c0, int64_t I,
+                                          int64_t C) {
+#pragma unroll
+  for (int r = 0; r < 4; r++) {
+    int i, c;
+    if (a.sc == 1) {          // neighbouring threads walk the contiguous axis
+      c = threadIdx.x % kStep;
+      i = threadIdx.x / kStep + 16 * r;
+    } else {
+      i = threadIdx.x % kTile;
+      c = threadIdx.x / kTile + 4 * r;
+    }
+    T v = (T)0;
+    if (i0 + i < I && c0 + c < C) v = a.p[(i0 + i) * a.si + (c0 + c) * a.sc];
+    dst[c][i] = v;
+  }
+}
+
+template <typename T, typename Epi>
+__global__ void __launch_bounds__(kSimtThreads)
+simt_product_kernel(Strided<T> a, Strided<T> b, int64_t I, int64_t J, int64_t C, Epi epi) {
+  __shared__ __align__(16) T as[kStep][kTile + 4];
+  __shared__ __align__(16) T bs[kStep][kTile + 4];
+  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+  const int64_t i0 = (int64_t)blockIdx.y * kTile, j0 = (int64_t)blockIdx.x * kTile;
+  T acc[4][4];
+#pragma unroll
+  for (int u = 0; u < 4; u++)
+#pragma unroll
+    for (int w = 0; w < 4; w++) acc[u][w] = (T)0;
+  for (int64_t c0 = 0; c0 < C; c0 += kStep) {
+    simt_load<T>(as, a, i0, c0, I, C);
+    simt_load<T>(bs, b, j0, c0, J, C);
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < kStep; c++) {
+      T av[4], bv[4];
+#pragma unroll
+      for (int u = 0; u < 4; u++) av[u] = as[c][ty * 4 + u];
+#pragma unroll
+      for (int w = 0; w < 4; w++) bv[w] = bs[c][tx * 4 + w];
+#pragma unroll
+      for (int u = 0; u < 4; u++)
+#pragma unroll
+        for (int w = 0; w < 4; w++) acc[u][w] = Math<T>::fma(av[u], bv[w], acc[u][w]);
+    }
+    __syncthreads();
+  }
+  epi(acc, i0 + ty * 4, j0 + tx * 4, I, J);
+}
+
+// i = instance, j = class: the tile's maximum and sum of exponentials per instance, and the score at
+// the label.  The 16 threads of an instance row are neighbours in a half warp.
+template <typename T> struct StatsEpi {
+  const T* bias;
+  const int32_t* labels;
+  T *part_m, *part_s, *label_score;
+  int64_t N;
+  __device__ __forceinline__ void operator()(T (&acc)[4][4], int64_t i0, int64_t j0, int64_t I, int64_t J) const {
+    T bv[4];
+#pragma unroll
+    for (int w = 0; w < 4; w++) bv[w] = (bias && j0 + w < J) ? bias[j0 + w] : (T)0;
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const int64_t i = i0 + u;
+      const int32_t lab = i < I ? labels[i] : 0;
+      T m = -Math<T>::inf();
+#pragma unroll
+      for (int w = 0; w < 4; w++) {
+        acc[u][w] = j0 + w < J ? acc[u][w] + bv[w] : -Math<T>::inf();
+        m = fmax(m, acc[u][w]);
+        if (i < I && j0 + w < J && lab == j0 + w + 1) label_score[i] = acc[u][w];
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
+      T s = (T)0;
+#pragma unroll
+      for (int w = 0; w < 4; w++) s += exp_from(acc[u][w], m);
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      if (i < I && (threadIdx.x & 15) == 0) {
+        part_m[(int64_t)blockIdx.x * N + i] = m;
+        part_s[(int64_t)blockIdx.x * N + i] = s;
+      }
+    }
+  }
+};
+
+// i = instance, j = class of the piece: dS without the factor g
+template <typename T> struct GradScoresEpi {
+  const T* bias;               // of the piece's first class
+  const int32_t* labels;
+  const T* lse;                // N rounded values, then N remainders
+  T* ds;                       // [n][class of the piece], row pitch ld
+  int64_t N, ld, v0;
+  __device__ __forceinline__ void operator()(T (&acc)[4][4], int64_t i0, int64_t j0, int64_t I, int64_t J) const {
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const int64_t i = i0 + u;
+      if (i >= I) break;
+      const int32_t lab = labels[i];
+      const T hi = lse[i], lo = lse[N + i];
+#pragma unroll
+      for (int w = 0; w < 4; w++) {
+        if (j0 + w >= J) break;
+        const T s = acc[u][w] + (bias ? bias[j0 + w] : (T)0);
+        ds[i * ld + j0 + w] = grad_score(s, hi, lo, lab, v0 + j0 + w);
+      }
+    }
+  }
+};
+
+// out(i, j) (+)= g * acc
+template <typename T> struct StoreEpi {
+  T* out;
+  int64_t ld;
+  int add;
+  GradScale<T> g;
+  __device__ __forceinline__ void operator()(T (&acc)[4][4], int64_t i0, int64_t j0, int64_t I, int64_t J) const {
+    const T f = g.value();
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      if (i0 + u >= I) break;
+#pragma unroll
+      for (int w = 0; w < 4; w++) {
+        if (j0 + w >= J) break;
+        T* p = out + (i0 + u) * ld + j0 + w;
+        const T v = acc[u][w] * f;
+        *p = add ? *p + v : v;
+      }
+    }
+  }
+};
+
+// ---- joining the tiles of the vocabulary ---------------------------------------------------------------
+// A CTA takes 32 instances; its 8 warps share the tiles of the vocabulary.  lse and the loss are
+// formed in Float64 and rounded once.  A label outside 0..V gives a loss of NaN.
+template <typename T>
+__global__ void __launch_bounds__(256)
+lnll_join_kernel(const T* __restrict__ part_m, const T* __restrict__ part_s, const T* __restrict__ label_score,
+                 const int32_t* __restrict__ labels, int64_t N, int64_t V, int64_t tiles, T* __restrict__ lse,
+                 T* __restrict__ per_instance) {
+  __shared__ double sm[8][32], ss[8][32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t n = (int64_t)blockIdx.x * 32 + lane;
+  MaxSum a{-Math<double>::inf(), 0.0};
+  if (n < N)
+    for (int64_t t = w; t < tiles; t += 8) a = join(a, MaxSum{(double)part_m[t * N + n], (double)part_s[t * N + n]});
+  sm[w][lane] = a.m;
+  ss[w][lane] = a.s;
+  __syncthreads();
+  if (w == 0 && n < N) {
+    for (int k = 1; k < 8; k++) a = join(a, MaxSum{sm[k][lane], ss[k][lane]});
+    const double l = a.m + ::log(a.s);
+    const T hi = (T)l;
+    lse[n] = hi;
+    lse[N + n] = isfinite(hi) ? (T)(l - (double)hi) : (T)0;
+    const int32_t lab = labels[n];
+    T loss = (T)0;
+    if (lab < 0 || lab > V) loss = (T)NAN;
+    else if (lab > 0) loss = (T)(l - (double)label_score[n]);
+    per_instance[n] = loss;
+  }
+}
+
+// total and count over the instances in a fixed order, one CTA
+template <typename T>
+__global__ void __launch_bounds__(1024)
+lnll_total_kernel(const T* __restrict__ per_instance, const int32_t* __restrict__ labels, int64_t N, T* __restrict__ total,
+                  int32_t* __restrict__ count) {
+  __shared__ double sd[32];
+  __shared__ int sc[32];
+  double a = 0.0;
+  int c = 0;
+  for (int64_t n = threadIdx.x; n < N; n += 1024)
+    if (labels[n] != 0) {
+      a += (double)per_instance[n];
+      c++;
+    }
+  a = block_reduce(a, [](double x, double y) { return x + y; }, 0.0, sd);
+  c = block_reduce(c, [](int x, int y) { return x + y; }, 0, sc);
+  if (threadIdx.x == 0) {
+    *total = (T)a;
+    *count = c;
+  }
+}
+
+// db[j] = g * sum_n ds[n][j]: a CTA takes 32 classes, its 32 warps share the instances
+template <typename T>
+__global__ void __launch_bounds__(1024)
+lnll_bias_kernel(const T* __restrict__ ds, int64_t ld, int64_t N, int64_t J, T* __restrict__ db, GradScale<T> g) {
+  __shared__ T part[32][33];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t j = (int64_t)blockIdx.x * 32 + lane;
+  T a = (T)0;
+  if (j < J)
+    for (int64_t n = w; n < N; n += 32) a += ds[n * ld + j];
+  part[w][lane] = a;
+  __syncthreads();
+  if (w == 0 && j < J) {
+    for (int k = 1; k < 32; k++) a += part[k][lane];
+    db[j] = a * g.value();
+  }
+}
+
+template <typename T> __global__ void lnll_zero_kernel(T* p, int64_t n) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < n) p[i] = (T)0;
+}
+template <typename T> void lnll_zero(T* p, int64_t n, cudaStream_t st) {
+  if (p && n > 0) lnll_zero_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(p, n);
+}
+
+// ---- host ---------------------------------------------------------------------------------------------
+template <typename T> struct Head {
+  const T* w;
+  int trans;                   // 0: w is (V,H), 1: (H,V)
+  const T* bias;
+  const T* x;
+  const int32_t* labels;
+  int64_t V, H, N;
+  Strided<T> weights(int64_t v0) const {      // element (class v0 + i, feature c)
+    return trans ? Strided<T>{w + v0 * H, H, 1} : Strided<T>{w + v0, 1, V};
+  }
+};
+
+constexpr size_t kAlign = 256;
+inline size_t up(size_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
+
+// classes per piece of the backward: as many as keep dS within 64 MB, whole tiles
+template <typename T> int64_t simt_piece(int64_t V, int64_t N) {
+  int64_t v = (int64_t)((64u << 20) / sizeof(T)) / N / kTile * kTile;
+  if (v < kTile) v = kTile;
+  return v < V ? v : V;
+}
+
+template <typename T> size_t workspace(int64_t V, int64_t H, int64_t N, int backward) {
+  if (backward) return up((size_t)N * simt_piece<T>(V, N) * sizeof(T));
+  const int64_t tiles = (V + kTile - 1) / kTile;
+  return up((size_t)N * sizeof(T)) + 2 * up((size_t)tiles * N * sizeof(T));
+}
+template <typename T, typename Epi>
+void simt_product(Strided<T> a, Strided<T> b, int64_t I, int64_t J, int64_t C, Epi epi, cudaStream_t st) {
+  const dim3 grid((unsigned)((J + kTile - 1) / kTile), (unsigned)((I + kTile - 1) / kTile));
+  simt_product_kernel<T, Epi><<<grid, kSimtThreads, 0, st>>>(a, b, I, J, C, epi);
+}
+
+// sizes whose tile counts fit a launch grid (features are rows of a tile grid in dW)
+inline bool sizes_ok(int64_t V, int64_t H, int64_t N) {
+  const int64_t most = (int64_t)65535 * kTile;
+  return V <= 0x7fffffff && H <= most && N <= most && V <= most;
+}
+
+template <typename T> bool odd(const T* p) { return (uintptr_t)p % sizeof(T) != 0; }
+
+template <typename T> int check(const Head<T>& h, const void* ws, size_t have, size_t need) {
+  if (h.V <= 0 || h.H <= 0 || h.N < 0 || (h.trans != 0 && h.trans != 1)) return KN_EINVAL;
+  if (!sizes_ok(h.V, h.H, h.N)) return KN_ESIZE;
+  if (h.N == 0) return KN_OK;
+  if (!h.w || !h.x || !h.labels) return KN_EINVAL;
+  if (odd(h.w) || odd(h.x) || odd(h.bias) || odd(h.labels)) return KN_EALIGN;
+  if (!ws || have < need) return KN_EWORKSPACE;
+  if ((uintptr_t)ws % kAlign) return KN_EALIGN;
+  return KN_OK;
+}
+
+template <typename T>
+int linear_nll_fwd(const Head<T>& h, T* total, int32_t* count, T* lse, T* per_instance, void* ws, size_t have, cudaStream_t st) {
+  if (!total || !count || (h.N > 0 && (!lse || !per_instance))) return KN_EINVAL;
+  if (odd(total) || odd(lse) || odd(per_instance) || (uintptr_t)count % 4) return KN_EALIGN;
+  const size_t need = h.V > 0 && h.H > 0 && h.N > 0 && sizes_ok(h.V, h.H, h.N) ? workspace<T>(h.V, h.H, h.N, 0) : 0;
+  if (int rc = check(h, ws, have, need)) return rc;
+  if (h.N > 0) {
+    const int64_t tiles = (h.V + kTile - 1) / kTile;
+    char* p = (char*)ws;
+    T* label_score = (T*)p;
+    T* part_m = (T*)(p += up((size_t)h.N * sizeof(T)));
+    T* part_s = (T*)(p += up((size_t)tiles * h.N * sizeof(T)));
+    simt_product<T>(Strided<T>{h.x, h.H, 1}, h.weights(0), h.N, h.V, h.H,
+                    StatsEpi<T>{h.bias, h.labels, part_m, part_s, label_score, h.N}, st);
+    lnll_join_kernel<T><<<(unsigned)((h.N + 31) / 32), 256, 0, st>>>(part_m, part_s, label_score, h.labels, h.N, h.V, tiles, lse,
+                                                                   per_instance);
+  }
+  lnll_total_kernel<T><<<1, 1024, 0, st>>>(per_instance, h.labels, h.N, total, count);
+  return launch_status();
+}
+
+template <typename T>
+int linear_nll_bwd(const Head<T>& h, const T* lse, int average, T dy, const int32_t* count, T* dw, T* db, T* dx, void* ws,
+                   size_t have, cudaStream_t st) {
+  if (h.N > 0 && (!lse || (average && !count))) return KN_EINVAL;
+  if (odd(lse) || odd(dw) || odd(db) || odd(dx) || (uintptr_t)count % 4) return KN_EALIGN;
+  const size_t need = h.V > 0 && h.H > 0 && h.N > 0 && sizes_ok(h.V, h.H, h.N) ? workspace<T>(h.V, h.H, h.N, 1) : 0;
+  if (int rc = check(h, ws, have, need)) return rc;
+  if (h.N == 0) {
+    lnll_zero(dw, h.V * h.H, st);
+    lnll_zero(db, h.V, st);
+    return launch_status();
+  }
+  const GradScale<T> g{average ? count : nullptr, dy};
+  const int64_t piece = simt_piece<T>(h.V, h.N);
+  T* ds = (T*)ws;
+  for (int64_t v0 = 0; v0 < h.V; v0 += piece) {
+    const int64_t vp = h.V - v0 < piece ? h.V - v0 : piece;
+    const Strided<T> w = h.weights(v0);
+    simt_product<T>(Strided<T>{h.x, h.H, 1}, w, h.N, vp, h.H,
+                    GradScoresEpi<T>{h.bias ? h.bias + v0 : nullptr, h.labels, lse, ds, h.N, piece, v0}, st);
+    if (db) lnll_bias_kernel<T><<<(unsigned)((vp + 31) / 32), 1024, 0, st>>>(ds, piece, h.N, vp, db + v0, g);
+    if (dx)
+      simt_product<T>(Strided<T>{ds, piece, 1}, Strided<T>{w.p, w.sc, w.si}, h.N, h.H, vp, StoreEpi<T>{dx, h.H, v0 > 0, g}, st);
+    if (dw && h.trans)
+      simt_product<T>(Strided<T>{ds, 1, piece}, Strided<T>{h.x, 1, h.H}, vp, h.H, h.N, StoreEpi<T>{dw + v0 * h.H, h.H, 0, g}, st);
+    else if (dw)
+      simt_product<T>(Strided<T>{h.x, 1, h.H}, Strided<T>{ds, 1, piece}, h.H, vp, h.N, StoreEpi<T>{dw + v0, h.V, 0, g}, st);
+  }
+  return launch_status();
+}
+
+}  // namespace kn
+
+using namespace kn;
+
+#define KN_DEF_LNLL(f_, S, T)                                                                                       \
+  KN_EXPORT size_t knet_linear_nll_workspace_##S(int64_t V, int64_t H, int64_t N, int backward) {                   \
+    if (V <= 0 || H <= 0 || N <= 0 || !sizes_ok(V, H, N)) return 0;                                                 \
+    return workspace<T>(V, H, N, backward != 0);                                                                         \
+  }                                                                                                                 \
+  KN_EXPORT int knet_linear_nll_fwd_##S(const T* w, int transW, const T* b, const T* x, const int32_t* labels,      \
+                                        int64_t V, int64_t H, int64_t N, T* total, int32_t* count, T* lse,          \
+                                        T* per_instance, void* workspace, size_t workspace_bytes, cudaStream_t s) { \
+    return linear_nll_fwd<T>(Head<T>{w, transW, b, x, labels, V, H, N}, total, count, lse, per_instance, workspace, \
+                             workspace_bytes, s);                                                                   \
+  }                                                                                                                 \
+  KN_EXPORT int knet_linear_nll_bwd_##S(const T* w, int transW, const T* b, const T* x, const int32_t* labels,      \
+                                        int64_t V, int64_t H, int64_t N, const T* lse, int average, T dy,           \
+                                        const int32_t* count, T* dw, T* db, T* dx, void* workspace,                 \
+                                        size_t workspace_bytes, cudaStream_t s) {                                   \
+    return linear_nll_bwd<T>(Head<T>{w, transW, b, x, labels, V, H, N}, lse, average, dy, count, dw, db, dx,        \
+                             workspace, workspace_bytes, s);                                                        \
+  }
+KNET_BOTH_TYPES(KN_DEF_LNLL, lnll)

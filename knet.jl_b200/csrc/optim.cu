@@ -349,6 +349,99 @@ int run_clip_factors(const knet_tensor_desc* table, int ntensors, int64_t total_
   return launch_status();
 }
 
+// ---- one norm over all arrays -----------------------------------------------------------------------
+// Squares are added in Float64 (a square of Float32 is exact there and neither overflows nor
+// vanishes), per chunk and then over the chunks in a fixed order by one CTA.
+template <typename T>
+__global__ void __launch_bounds__(kOptThreads)
+gnorm_chunks_kernel(const knet_tensor_desc* __restrict__ table, int ntensors, double* __restrict__ partials) {
+  __shared__ int s_t;
+  __shared__ double red[32];
+  const knet_tensor_desc d = table[find_tensor(table, ntensors, blockIdx.x, &s_t)];
+  const int64_t start = ((int64_t)blockIdx.x - d.first_chunk) * KNET_MULTI_CHUNK;
+  const uint32_t cnt = start < d.n ? (uint32_t)min((int64_t)KNET_MULTI_CHUNK, d.n - start) : 0u;
+  const T* g = reinterpret_cast<const T*>(d.p[1]) + start;
+  double acc = 0.0;
+  segment_visit<T>(g, cnt, threadIdx.x, kOptThreads, [&](T v, uint32_t) { acc = ::fma((double)v, (double)v, acc); });
+  acc = block_reduce(acc, [](double a, double b) { return a + b; }, 0.0, red);
+  if (threadIdx.x == 0) partials[blockIdx.x] = acc;
+}
+
+__global__ void __launch_bounds__(1024)
+gnorm_finish_kernel(const double* __restrict__ partials, int64_t total_chunks, double gclip, double gscale,
+                    double* __restrict__ norm, double* __restrict__ factor) {
+  __shared__ double red[32];
+  double acc = 0.0;
+  for (int64_t c = threadIdx.x; c < total_chunks; c += 1024) acc += partials[c];
+  acc = block_reduce(acc, [](double a, double b) { return a + b; }, 0.0, red);
+  if (threadIdx.x == 0) {
+    const double nrm = ::sqrt(acc) * fabs(gscale);
+    if (norm) *norm = nrm;
+    if (factor) *factor = nrm > gclip ? gclip / nrm : 1.0;
+  }
+}
+
+// g = lmul!(factor, g) over every array; the whole grid returns at once when the factor is 1
+template <typename T> struct ScaleF {
+  enum { NP = 1, WMASK = 0x1 };
+  double factor;
+  __device__ __forceinline__ void operator()(T (&p)[NP]) const { p[0] = lmul<T>(factor, p[0]); }
+};
+template <typename T>
+__global__ void __launch_bounds__(kOptThreads)
+gclip_apply_kernel(const knet_tensor_desc* __restrict__ table, int ntensors, const double* __restrict__ factor) {
+  __shared__ int s_t;
+  const double f = *factor;
+  if (f == 1.0) return;
+  knet_tensor_desc d = table[find_tensor(table, ntensors, blockIdx.x, &s_t)];
+  d.p[0] = d.p[1];
+  opt_chunk<T, ScaleF<T>>(ScaleF<T>{f}, d, (int64_t)blockIdx.x - d.first_chunk);
+}
+
+// an update whose gradients are all multiplied by the same device-side factor
+template <typename T, typename F0>
+__global__ void __launch_bounds__(kOptThreads)
+opt_gclip_kernel(F0 f0, const knet_tensor_desc* __restrict__ table, int ntensors, const double* __restrict__ factor) {
+  const auto f = resolve(f0);
+  typedef typename std::remove_cv<typename std::remove_reference<decltype(f)>::type>::type F;
+  __shared__ int s_t;
+  const knet_tensor_desc d = table[find_tensor(table, ntensors, blockIdx.x, &s_t)];
+  opt_chunk<T, ClipF<F>>(ClipF<F>{f, *factor}, d, (int64_t)blockIdx.x - d.first_chunk);
+}
+
+template <typename T>
+int run_gnorm(const knet_tensor_desc* table, int ntensors, int64_t total_chunks, double gclip, double gscale, double* partials,
+              double* norm, double* factor, cudaStream_t st) {
+  if (ntensors < 0 || total_chunks < 0 || (!norm && !factor)) return KN_EINVAL;
+  if (total_chunks > 0 && (!table || ntensors == 0 || !partials)) return KN_EINVAL;
+  if ((uintptr_t)partials % 8 || (uintptr_t)norm % 8 || (uintptr_t)factor % 8) return KN_EALIGN;
+  if (total_chunks > 0x7fffffff) return KN_ESIZE;
+  if (total_chunks > 0) gnorm_chunks_kernel<T><<<(unsigned)total_chunks, kOptThreads, 0, st>>>(table, ntensors, partials);
+  gnorm_finish_kernel<<<1, 1024, 0, st>>>(partials, total_chunks, gclip, gscale, norm, factor);
+  return launch_status();
+}
+
+template <typename T>
+int run_gclip_apply(const knet_tensor_desc* table, int ntensors, int64_t total_chunks, const double* factor, cudaStream_t st) {
+  if (ntensors < 0 || total_chunks < 0) return KN_EINVAL;
+  if (ntensors == 0 || total_chunks == 0) return KN_OK;
+  if (!table || !factor) return KN_EINVAL;
+  if (total_chunks > 0x7fffffff) return KN_ESIZE;
+  gclip_apply_kernel<T><<<(unsigned)total_chunks, kOptThreads, 0, st>>>(table, ntensors, factor);
+  return launch_status();
+}
+
+template <typename T, typename F>
+int run_multi_gclip(const F& f, const knet_tensor_desc* table, int ntensors, int64_t total_chunks, const double* factor,
+                    cudaStream_t st) {
+  if (ntensors < 0 || total_chunks < 0) return KN_EINVAL;
+  if (ntensors == 0 || total_chunks == 0) return KN_OK;
+  if (!table || !factor) return KN_EINVAL;
+  if (total_chunks > 0x7fffffff) return KN_ESIZE;
+  opt_gclip_kernel<T, F><<<(unsigned)total_chunks, kOptThreads, 0, st>>>(f, table, ntensors, factor);
+  return launch_status();
+}
+
 template <typename T> GScale<T> make_gs(double gscale) { return GScale<T>{(T)gscale, gscale != 1.0}; }
 
 template <typename T> AdamF<T> make_adam(double lr, double beta1, double beta2, double eps, int t, double gscale) {
@@ -469,3 +562,50 @@ KN_EXPORT int64_t knet_multi_plan(knet_tensor_desc* host_table, int ntensors) {
     host_out[1] = f.b2t;                                                                             \
   }
 KNET_BOTH_TYPES(KN_DEF_OPT, opt)
+
+#define KN_DEF_GNORM(f_, S, T)                                                                       \
+  KN_EXPORT int knet_gnorm_##S(const knet_tensor_desc* table, int ntensors, int64_t total_chunks,    \
+                               double gscale, double* partials, double* norm, cudaStream_t s) {      \
+    if (!norm) return KN_EINVAL;                                                                     \
+    return run_gnorm<T>(table, ntensors, total_chunks, 0.0, gscale, partials, norm, nullptr, s);     \
+  }                                                                                                  \
+  KN_EXPORT int knet_gclip_global_##S(const knet_tensor_desc* table, int ntensors,                   \
+                                      int64_t total_chunks, double gclip, double gscale,             \
+                                      double* partials, double* norm, double* factor,                \
+                                      cudaStream_t s) {                                              \
+    if (!(gclip > 0) || !factor) return KN_EINVAL;                                                   \
+    return run_gnorm<T>(table, ntensors, total_chunks, gclip, gscale, partials, norm, factor, s);    \
+  }                                                                                                  \
+  KN_EXPORT int knet_gclip_apply_##S(const knet_tensor_desc* table, int ntensors,                    \
+                                     int64_t total_chunks, const double* factor, cudaStream_t s) {   \
+    return run_gclip_apply<T>(table, ntensors, total_chunks, factor, s);                             \
+  }                                                                                                  \
+  KN_EXPORT int knet_sgd_multi_gc_##S(const knet_tensor_desc* table, int ntensors,                   \
+                                      int64_t total_chunks, double lr, double gscale,                \
+                                      const double* factor, cudaStream_t s) {                        \
+    return run_multi_gclip<T>(SgdF<T>{(T)(-lr), make_gs<T>(gscale)}, table, ntensors, total_chunks,  \
+                              factor, s);                                                            \
+  }                                                                                                  \
+  KN_EXPORT int knet_momentum_multi_gc_##S(const knet_tensor_desc* table, int ntensors,              \
+                                           int64_t total_chunks, double lr, double gamma,            \
+                                           double gscale, const double* factor, cudaStream_t s) {    \
+    return run_multi_gclip<T>(MomentumF<T>{(T)(-lr), gamma, make_gs<T>(gscale)}, table, ntensors,    \
+                              total_chunks, factor, s);                                              \
+  }                                                                                                  \
+  KN_EXPORT int knet_adam_multi_gc_##S(const knet_tensor_desc* table, int ntensors,                  \
+                                       int64_t total_chunks, double lr, double beta1, double beta2,  \
+                                       double eps, int t, double gscale, const double* factor,       \
+                                       cudaStream_t s) {                                             \
+    if (t < 1) return KN_EINVAL;                                                                     \
+    return run_multi_gclip<T>(make_adam<T>(lr, beta1, beta2, eps, t, gscale), table, ntensors,       \
+                              total_chunks, factor, s);                                              \
+  }                                                                                                  \
+  KN_EXPORT int knet_adam_multi_gcg_##S(const knet_tensor_desc* table, int ntensors,                 \
+                                        int64_t total_chunks, double lr, double beta1, double beta2, \
+                                        double eps, const T* bias_corr, double gscale,               \
+                                        const double* factor, cudaStream_t s) {                      \
+    if (!bias_corr) return KN_EINVAL;                                                                \
+    return run_multi_gclip<T>(AdamDevF<T>{make_adam<T>(lr, beta1, beta2, eps, 1, gscale), bias_corr}, \
+                              table, ntensors, total_chunks, factor, s);                             \
+  }
+KNET_BOTH_TYPES(KN_DEF_GNORM, gnorm)

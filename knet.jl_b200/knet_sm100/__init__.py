@@ -26,7 +26,7 @@ from .lib import KnetError, libknet, knet, knet8, knet8r  # noqa: F401
 from .karray import KnetArray  # noqa: F401
 from . import autograd, indexing, ops, train  # noqa: F401
 from .ops import (relu, sigm, tanh, elu, selu, softmax, logsoftmax, logp, logsumexp, nll, accuracy,  # noqa: F401
-                  dropout, argmax)
+                  dropout, argmax, linear_nll)
 from .train import (SGD, Momentum, Nesterov, Adagrad, Rmsprop, Adadelta, Adam, Param, update_,  # noqa: F401
-                    update_multi_, MultiTensorPlan, param, param0)
+                    update_multi_, MultiTensorPlan, gnorm, gclip_global_, param, param0)
 from .mlp import MLP  # noqa: F401

@@ -454,12 +454,50 @@ def nll(scores, labels, dims=1, average=True):
     return _record(y, (scores,), lambda dy, _: (_nll_back(scores, res, dims, average, dy),))
 
 
-def minimize_step(f, args, algo, parameters=None):
+def linear_nll(w, x, labels, b=None, trans=False, average=True):
+    """nll(w*x .+ b, labels) (w' * x with `trans`) as one fused primitive that never holds the
+    scores; w, x and b may be tracked.  A backward sweep that is itself recorded (a gradient of a
+    gradient) spells the gradients with the primitives of this module instead, scores included."""
+    wv, xv, bv = _val(w), _val(x), _val(b)
+    res = ops.linear_nll_device(wv, xv, labels, bv, trans)
+    if not _tracked(w, x, b):
+        return res.value(average)
+    y = KnetArray((res.total / res.count.to(res.total.dtype)) if average else res.total.clone(), (1,))
+
+    def back(dy, _):
+        if recording():
+            return _linear_nll_composed(w, x, b, res, trans, average, dy)
+        need = tuple(isinstance(a, Value) for a in (w, x, b))
+        return ops.linear_nll_back(wv, xv, res, bv, trans, average, float(_val(dy).data.item()), need)
+
+    return _record(y, (w, x, b), back)
+
+
+def _linear_nll_composed(w, x, b, res, trans, average, dy):
+    """The gradients of linear_nll (dw, dx, db) out of tracked primitives."""
+    xv, bv = _val(x), _val(b)
+    H = xv.shape[0]
+    x2 = reshape(x, (H, len(xv) // H))
+    scores = At_mul_B(w, x2) if trans else matmul(w, x2)
+    if b is not None:
+        scores = add(scores, reshape(b, (len(bv), 1)))
+    ds = _nll_back(scores, res, 1, average, dy)
+    gw = (A_mul_Bt(x2, ds) if trans else A_mul_Bt(ds, x2)) if isinstance(w, Value) else None
+    gx = reshape(matmul(w, ds) if trans else At_mul_B(w, ds), xv.shape) if isinstance(x, Value) else None
+    gb = reshape(sum(ds, 2), bv.shape) if isinstance(b, Value) else None
+    return gw, gx, gb
+
+
+def minimize_step(f, args, algo, parameters=None, gclip_global=0):
     """One iteration of `minimize(f, data, algo)` (src/train20/train.jl:22-36): differentiate
-    f(args...), give every parameter a clone of `algo` on first sight, update!, return the loss."""
-    from .train import update_
+    f(args...), give every parameter a clone of `algo` on first sight, update!, return the loss.
+    `gclip_global` > 0 first clips the gradients to that norm taken over all of them."""
+    from .train import gclip_global_, update_
     tape = diff(f, *args)
-    for p in (parameters if parameters is not None else params(tape)):
+    ps = parameters if parameters is not None else params(tape)
+    if gclip_global:
+        gclip_global_([_val(p.grad) for p in ps if p.grad is not None], gclip_global)
+    for p in ps:
         if p.opt is None:
             p.opt = algo.clone()
         if p.grad is not None:

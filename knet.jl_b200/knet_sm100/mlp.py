@@ -17,20 +17,22 @@ import torch
 from . import dp, ops
 from .karray import KnetArray
 from .lib import knet, knet8, libknet, ptr, sfx
-from .train import Adam, Momentum, MultiTensorPlan, SGD, update_multi_
+from .train import Adam, Momentum, MultiTensorPlan, SGD, _global_norm, update_multi_
 
 
 class MLP:
     def __init__(self, sizes, batch, pdrop=0.0, dtype=torch.float32, seed=1, optimizer=None,
                  device="cuda", process_group=None, weights=None, dropout_seed=None, shard_update=False,
-                 fuse_bias_grad=True):
+                 fuse_bias_grad=True, gclip_global=0):
         """sizes = [in, hidden..., out]; `weights` optionally gives host (w, b) NumPy pairs
         (column-major Julia shapes) instead of the xavier draw; `process_group` turns on the
         gradient all-reduce (one rank per GPU, same weights everywhere, batch sharded).
         `shard_update` replaces it by reduce-scatter -> update of the rank's own 1/world of
         every layer -> all-gather of the weights, with optimizer state kept for that shard only.
         `fuse_bias_grad=False` computes the hidden layers' bias gradients with a separate
-        sum(dz, dims=2) instead of inside the dropback+reluback kernel."""
+        sum(dz, dims=2) instead of inside the dropback+reluback kernel.  `gclip_global` > 0 clips
+        the gradients by the norm of all of them inside the update; the norm of the last step stays
+        in `self.gnorm` (a device tensor)."""
         self.sizes, self.batch, self.pdrop, self.dtype = list(sizes), batch, pdrop, dtype
         self.device = torch.device(device)
         self.S = sfx(dtype)
@@ -118,6 +120,12 @@ class MLP:
             # the plan holds one slice per layer and rank, so per-array norms (gclip!, update.jl:572-583)
             # would be taken over parts of arrays
             raise ValueError("gradient clipping is not available with shard_update")
+        self.gclip_global, self.gnorm = gclip_global, None
+        if gclip_global:
+            if self.sharded:
+                raise ValueError("gradient clipping is not available with shard_update")
+            if not gclip_global > 0 or getattr(self.opt, "gclip", 0):
+                raise ValueError("gclip_global must be positive and the optimizer's gclip 0")
 
     def _kn(self, label, nbytes, call, *args, launches=1):
         """One library call; `nbytes` is its algorithmic traffic (for the optional probe)."""
@@ -226,7 +234,22 @@ class MLP:
     def update(self):
         nupd = int(self.offsets[-1]) // self.world if self.sharded else int(self.offsets[-1])
         per_param = (3 + 2 * len(self.state)) * self.esize          # read w, g, state; write w, state
-        if self._capturing and isinstance(self.opt, Adam):
+        if self.gclip_global:
+            # the norm reads the gradients once more; its two launches and the update's
+            nbytes, scale = nupd * (per_param + self.esize), dp.gradient_scale(self.world)
+            if self._capturing and isinstance(self.opt, Adam):
+                self.gnorm, factor = _global_norm(self.plan, self.gclip_global, scale)
+                self._kn("update! (multi-tensor, clipped)", nbytes, knet, f"knet_adam_multi_gcg_{self.S}", ptr(self.plan.table),
+                         self.plan.ntensors, self.plan.total_chunks, self.opt.lr, self.opt.beta1, self.opt.beta2,
+                         self.opt.eps, C.c_void_p(self._dev_step.data_ptr() + 8 * self.L), scale, ptr(factor), launches=3)
+            else:
+                if self.probe is not None:
+                    self.probe.begin("update! (multi-tensor, clipped)", nbytes)
+                self.gnorm = update_multi_(self.plan, self.opt, scale, gclip_global=self.gclip_global)
+                if self.probe is not None:
+                    self.probe.end()
+                self.launches += 3
+        elif self._capturing and isinstance(self.opt, Adam):
             self._kn("update! (multi-tensor)", nupd * per_param, knet, f"knet_adam_multi_g_{self.S}", ptr(self.plan.table),
                      self.plan.ntensors, self.plan.total_chunks, self.opt.lr, self.opt.beta1, self.opt.beta2, self.opt.eps,
                      C.c_void_p(self._dev_step.data_ptr() + 8 * self.L), dp.gradient_scale(self.world))

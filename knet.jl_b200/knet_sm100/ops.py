@@ -13,7 +13,7 @@ import numpy as np
 import torch
 
 from .karray import KnetArray, _prod
-from .lib import knet, knet8, knet8r, ptr, sfx
+from .lib import knet, knet8, knet8r, libknet, ptr, sfx
 
 _CT = {torch.float32: C.c_float, torch.float64: C.c_double}
 
@@ -368,6 +368,91 @@ def nll_back(scores, labels, dims=1, average=True, dy=1.0, count=None):
     knet(f"knet_nll_bwd_{sfx(scores.dtype)}", ptr(scores.data), ptr(lab), R, K, dims, int(average),
          _CT[scores.dtype](dy), ptr(count), ptr(dx.data))
     return dx
+
+
+class LinearNllResult(NllResult):
+    """Device-side result of linear_nll_device: NllResult plus log sum exp per instance, kept as its
+    rounded value (`lse`) and the remainder of that rounding, which the backward pass reads too."""
+
+    def __init__(self, total, count, per_instance, labels, lse_pair):
+        super().__init__(total, count, per_instance, labels)
+        self.lse_pair = lse_pair
+
+    @property
+    def lse(self):
+        return self.lse_pair[:self.lse_pair.numel() // 2]
+
+
+def _head_sizes(w, x, b, trans):
+    """(V, H, N) of scores = w*x (+ b), w being (V,H), or (H,V) with trans; checks what belongs together."""
+    if w.ndim != 2 or x.ndim < 1:
+        raise ValueError("DimensionMismatch: w must be a matrix and x a vector or matrix")
+    H, V = w.shape if trans else w.shape[::-1]
+    if x.shape[0] != H:
+        raise ValueError(f"DimensionMismatch: x has {x.shape[0]} features, w {H}")
+    if b is not None and len(b) != V:
+        raise ValueError(f"DimensionMismatch: b has {len(b)} entries for {V} classes")
+    for a in (x, b):
+        if a is not None and a.dtype != w.dtype:
+            raise TypeError("element types differ")
+        if a is not None and a.data.device != w.data.device:
+            raise ValueError("arrays live on different devices")
+    return V, H, (len(x) // H if H else 0)
+
+
+def _head_workspace(S, V, H, N, backward, device):
+    n = getattr(libknet, f"knet_linear_nll_workspace_{S}")(V, H, N, backward)
+    return torch.empty(max(n, 1), dtype=torch.uint8, device=device)
+
+
+def linear_nll_device(w, x, labels, b=None, trans=False):
+    """nll of scores = w*x (.+ b) without the score matrix, for a large number of classes: w is
+    (V,H), or (H,V) with `trans` (an embedding matrix used again at the output), x (H,N), labels
+    1-based with 0 = skip.  The result's total and count stay on the device, as nll_device's do."""
+    V, H, N = _head_sizes(w, x, b, trans)
+    dev, dt, S = w.data.device, w.dtype, sfx(w.dtype)
+    lab = _labels(labels, dev)
+    if lab.numel() != N:
+        raise ValueError("DimensionMismatch: one label per instance is needed")
+    with torch.cuda.device(dev):
+        total = torch.empty(1, dtype=dt, device=dev)
+        count = torch.empty(1, dtype=torch.int32, device=dev)
+        per = torch.empty(max(N, 1), dtype=dt, device=dev)
+        lse = torch.empty(2 * N, dtype=dt, device=dev)
+        ws = _head_workspace(S, V, H, N, 0, dev)
+        knet(f"knet_linear_nll_fwd_{S}", ptr(w.data), int(bool(trans)), ptr(None if b is None else b.data), ptr(x.data), ptr(lab),
+             V, H, N, ptr(total), ptr(count), ptr(lse), ptr(per), ptr(ws), ws.numel())
+    return LinearNllResult(total, count, per, lab, lse)
+
+
+def linear_nll(w, x, labels, b=None, trans=False, average=True):
+    """nll(w*x .+ b, labels) as a float, or (total, count) if not average; see linear_nll_device."""
+    return linear_nll_device(w, x, labels, b, trans).value(average)
+
+
+def linear_nll_back(w, x, res, b=None, trans=False, average=True, dy=1.0, need=(True, True, True), out=(None, None, None)):
+    """Gradients (dw, dx, db) of linear_nll from its forward result and the same w, x and b; db is
+    None without b.  `need` leaves some of them out (None); `out` gives arrays to write them to."""
+    V, H, N = _head_sizes(w, x, b, trans)
+    dev, S = w.data.device, sfx(w.dtype)
+    if res.labels.numel() != N or res.lse_pair.dtype != w.dtype:
+        raise ValueError("DimensionMismatch: the forward result belongs to other arrays")
+    grads = []
+    for a, want, o in zip((w, x, b), need, out):
+        if a is None or not want:
+            grads.append(None)
+            continue
+        if o is not None and (len(o) != len(a) or o.dtype != a.dtype or o.data.device != dev):
+            raise ValueError("DimensionMismatch: out does not match its array")
+        grads.append(a.similar() if o is None else o)
+    if all(g is None for g in grads):
+        return tuple(grads)
+    with torch.cuda.device(dev):
+        ws = _head_workspace(S, V, H, N, 1, dev)
+        knet(f"knet_linear_nll_bwd_{S}", ptr(w.data), int(bool(trans)), ptr(None if b is None else b.data), ptr(x.data),
+             ptr(res.labels), V, H, N, ptr(res.lse_pair), int(average), _CT[w.dtype](dy), ptr(res.count),
+             *[ptr(None if grads[k] is None else grads[k].data) for k in (0, 2, 1)], ptr(ws), ws.numel())
+    return tuple(grads)
 
 
 def argmax(x, dims=1):

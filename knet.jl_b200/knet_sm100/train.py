@@ -181,21 +181,96 @@ class MultiTensorPlan:
         raw = bytes(host)
         self.table = torch.frombuffer(bytearray(raw), dtype=torch.uint8).cuda()
         self._keep = arrays
+        held = [(host[i].p[1], host[i].n) for i in range(n) if host[i].p[1] and host[i].n]
+        self.repeated = len(set(held)) < len(held)
         self.clip_partials = self.clip_factors = None      # scratch of the fused gradient clipping
 
 
-def update_multi_(plan, p, gscale=1.0, advance=True):
+def _one_plan(grads):
+    """(plan over all gradients, plan over each buffer once).  A plan is taken as it is and must not
+    hold a gradient twice; a list may (two parameters whose gradient is one array)."""
+    if isinstance(grads, MultiTensorPlan):
+        if grads.repeated:
+            raise ValueError("the plan holds a gradient array twice")
+        return grads, grads
+    arrays = [g.data if isinstance(g, KnetArray) else g for g in grads]
+    if not arrays:
+        return None, None
+    for a in arrays:
+        sfx(a.dtype)
+        if not (a.is_cuda and a.is_contiguous()):
+            raise TypeError("gradients must be contiguous GPU arrays")
+        if a.dtype != arrays[0].dtype or a.device != arrays[0].device:
+            raise TypeError("gradients of one norm must share an element type and a device")
+    once = list({(a.data_ptr(), a.numel()): a for a in arrays}.values())
+    plan = MultiTensorPlan([(a, a) for a in arrays])
+    return plan, plan if len(once) == len(arrays) else MultiTensorPlan([(a, a) for a in once])
+
+
+def _global_norm(plan, gclip, gscale):
+    """(norm, factor) of a plan's gradients on the device; factor is None when gclip is None."""
+    dev = plan.table.device
+    partials = torch.empty(max(int(plan.total_chunks), 1), dtype=torch.float64, device=dev)
+    norm = torch.empty(1, dtype=torch.float64, device=dev)
+    S, head = sfx(plan.dtype), (ptr(plan.table), plan.ntensors, plan.total_chunks)
+    if gclip is None:
+        knet(f"knet_gnorm_{S}", *head, float(gscale), ptr(partials), ptr(norm))
+        return norm, None
+    factor = torch.empty(1, dtype=torch.float64, device=dev)
+    knet(f"knet_gclip_global_{S}", *head, float(gclip), float(gscale), ptr(partials), ptr(norm), ptr(factor))
+    return norm, factor
+
+
+def gnorm(grads, gscale=1.0):
+    """|gscale| * the norm of all gradients taken as one vector: a one-element Float64 tensor on the
+    device.  `grads` is a MultiTensorPlan or a list of arrays (a list costs an upload of its table)."""
+    plan, _ = _one_plan(grads)
+    if plan is None:
+        return torch.zeros(1, dtype=torch.float64, device="cuda")
+    with torch.cuda.device(plan.table.device):
+        return _global_norm(plan, None, gscale)[0]
+
+
+def gclip_global_(grads, gclip, gscale=1.0):
+    """Clip by the norm of all gradients: multiply every one in place by gclip / norm when
+    norm = gnorm(grads, gscale) exceeds gclip (gclip! does so array by array,
+    src/train20/update.jl:572-583).  Returns the norm before clipping, on the device; nothing
+    waits for it.  A norm that is NaN leaves the gradients as they are."""
+    if not gclip > 0:
+        raise ValueError("gclip must be positive")
+    plan, once = _one_plan(grads)
+    if plan is None:
+        return torch.zeros(1, dtype=torch.float64, device="cuda")
+    with torch.cuda.device(plan.table.device):
+        norm, factor = _global_norm(plan, gclip, gscale)
+        knet(f"knet_gclip_apply_{sfx(plan.dtype)}", ptr(once.table), once.ntensors, once.total_chunks, ptr(factor))
+    return norm
+
+
+def update_multi_(plan, p, gscale=1.0, advance=True, gclip_global=0):
     """One launch for every array of `plan` with optimizer `p` (state arrays are in the plan;
     Adam's step counter lives in `p`; `advance=False` keeps the counter where it is, for the
     second and later launches of one step whose parameter set was split over several plans).  With `p.gclip > 0` every array's gradient is clipped
     to that norm as `gclip!` does (src/train20/update.jl:572-583), without the host round
     trip of norm(g): two small launches leave the per-array factors on the device and the
-    update applies them to the gradient as it loads it."""
+    update applies them to the gradient as it loads it.  `gclip_global` > 0 clips by the norm of all
+    gradients of the plan instead (gclip_global_), also applied on load: the gradients in memory
+    stay as they are; that norm, a device tensor, is returned."""
     S = sfx(plan.dtype)
     clip = getattr(p, "gclip", 0) or 0
     tail = ()
     sfx_c = ""
-    if clip > 0:
+    norm = None
+    if gclip_global:
+        if clip > 0:
+            raise ValueError("clip by array (the optimizer's gclip) or by the global norm, not both")
+        if not gclip_global > 0:
+            raise ValueError("gclip_global must be positive")
+        if not isinstance(p, (Adam, Momentum, SGD)) or isinstance(p, Nesterov):
+            raise TypeError(f"no multi-tensor kernel for {type(p)}")
+        norm, factor = _global_norm(plan, gclip_global, gscale)
+        tail, sfx_c = (ptr(factor),), "_gc"
+    elif clip > 0:
         if plan.clip_partials is None:
             plan.clip_partials = torch.empty(max(int(plan.total_chunks), 1), dtype=plan.dtype, device=plan.table.device)
             plan.clip_factors = torch.ones(max(plan.ntensors, 1), dtype=torch.float64, device=plan.table.device)
@@ -214,6 +289,7 @@ def update_multi_(plan, p, gscale=1.0, advance=True):
         knet(f"knet_sgd_multi{sfx_c}_{S}", ptr(plan.table), plan.ntensors, plan.total_chunks, p.lr, gscale, *tail)
     else:
         raise TypeError(f"no multi-tensor kernel for {type(p)}")
+    return norm
 
 
 # ---- parameters and initialisation (src/train20/param.jl:22-24, distributions.jl:35-52) ------------

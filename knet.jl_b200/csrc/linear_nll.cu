@@ -10,13 +10,14 @@
 // numbers (its rounding alone would be a relative error of |lse| * 2^-24 in every p of that
 // instance), so that p = exp((s - hi) - lo).
 #include "linear_nll.cuh"
+#include "linear_nll_mma.cuh"
 
 namespace kn {
 
 // ---- matrix products on the FMA pipe ---------------------------------------------------------------
 // acc(i, j) = sum_c A(i, c) * B(j, c) for a 64x64 tile of (i, j), 4x4 per thread, c in steps of 16
-// through shared memory.  Operands have any strides with one of the two equal to 1.
-
+// through shared memory.  Operands have any strides with one of the two equal to 1.  Used for
+// Float64 and as the Float32 form where tensor-core tiles do not pay.
 template <typename T> struct Strided {
   const T* p;
   int64_t si, sc;      // element (i, c) at p + i*si + c*sc
@@ -261,11 +262,87 @@ template <typename T> int64_t simt_piece(int64_t V, int64_t N) {
   return v < V ? v : V;
 }
 
-template <typename T> size_t workspace(int64_t V, int64_t H, int64_t N, int backward) {
+// ---- plan of the tensor-core form (Float32) --------------------------------------------------------------
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// The tensor-core form pays from a few million products on; below, its launches cost more.
+template <typename T> bool use_mma(int64_t V, int64_t H, int64_t N) {
+  return sizeof(T) == 4 && N >= 32 && V >= 64 && H >= 16 && (double)V * H * N >= (double)(1 << 24);
+}
+
+// Pieces of the vocabulary and parts of dx's sum.  Workspace bounds: 256 MB of split weights in the
+// forward; 128 MB of dS and 64 MB of split weights in the backward.  Within them the backward takes
+// the piece with the fewest waves of tiles over its three products (a product's tiles are 128 x 256
+// and its time is proportional to the summed length), charging each piece for its launches.
+struct MmaPlan {
+  int64_t piece, wld, xld, dld;        // classes per piece; row pitches of split w, x and dS (elements)
+  int splits;                          // parts of dx's sum over a piece
+  size_t exps, absmax, xs, ws, label, part_m, part_s, ds, parts, db, total;
+};
+constexpr int kPlanSMs = 148;
+
+inline MmaPlan mma_plan(int64_t V, int64_t H, int64_t N, int trans, int backward) {
+  MmaPlan p{};
+  const int64_t all = ceil_div(V, kTN);
+  p.splits = 1;
+  if (!backward) {
+    int64_t m = (int64_t)(256u << 20) / 4 / H / kTN;
+    m = m < 1 ? 1 : m;
+    p.piece = kTN * ceil_div(all, ceil_div(all, m));
+  } else {
+    const int64_t nt = ceil_div(N, kTM), hj = ceil_div(H, kTN), hi = ceil_div(H, kTM);
+    double best = 0;
+    for (int64_t m = 1; m <= all; m++) {
+      if (m > 1 && (m * kTN * N * 4 > (128ll << 20) || m * kTN * H * 4 > (64ll << 20))) break;
+      int64_t sp = kPlanSMs / (nt * hj);
+      sp = sp < 1 ? 1 : sp > m ? m : sp > 16 ? 16 : sp;
+      const double t = (double)ceil_div(nt * m, kPlanSMs) * H + (double)ceil_div(nt * hj * sp, kPlanSMs) * ceil_div(m * kTN, sp) +
+                       (double)ceil_div(trans ? 2 * m * hj : hi * m, kPlanSMs) * N + 1500.0;
+      const double cost = t * ceil_div(all, m);
+      if (m == 1 || cost < best) {
+        best = cost;
+        p.piece = m * kTN;
+        p.splits = (int)sp;
+      }
+    }
+  }
+  const int64_t vp = p.piece < V ? p.piece : V;
+  p.wld = ceil_div(trans ? H : vp, 8) * 8;
+  p.xld = ceil_div(H, 8) * 8;
+  p.dld = ceil_div(vp, 8) * 8;
+  size_t at = 0;
+  auto put = [&](size_t& where, size_t bytes) {
+    where = at;
+    at += up(bytes);
+  };
+  put(p.exps, 16);
+  put(p.absmax, 2 * kMaxBlocks * 4);
+  put(p.xs, (size_t)N * p.xld * 4);
+  put(p.ws, (size_t)(trans ? vp : H) * p.wld * 4);
+  if (!backward) {
+    put(p.label, (size_t)N * 4);
+    put(p.part_m, (size_t)all * N * 4);
+    put(p.part_s, (size_t)all * N * 4);
+  } else {
+    put(p.ds, (size_t)N * p.dld * 4);
+    if (p.splits > 1) put(p.parts, (size_t)p.splits * N * H * 4);
+    put(p.db, (size_t)ceil_div(N, kTM) * vp * 4);
+  }
+  p.total = at;
+  return p;
+}
+
+template <typename T> size_t workspace(int64_t V, int64_t H, int64_t N, int trans, int backward) {
+  if (use_mma<T>(V, H, N)) return mma_plan(V, H, N, trans, backward).total;
   if (backward) return up((size_t)N * simt_piece<T>(V, N) * sizeof(T));
   const int64_t tiles = (V + kTile - 1) / kTile;
   return up((size_t)N * sizeof(T)) + 2 * up((size_t)tiles * N * sizeof(T));
 }
+template <typename T> size_t workspace_any(int64_t V, int64_t H, int64_t N, int backward) {
+  const size_t a = workspace<T>(V, H, N, 0, backward), b = workspace<T>(V, H, N, 1, backward);
+  return a > b ? a : b;
+}
+
 template <typename T, typename Epi>
 void simt_product(Strided<T> a, Strided<T> b, int64_t I, int64_t J, int64_t C, Epi epi, cudaStream_t st) {
   const dim3 grid((unsigned)((J + kTile - 1) / kTile), (unsigned)((I + kTile - 1) / kTile));
@@ -291,12 +368,131 @@ template <typename T> int check(const Head<T>& h, const void* ws, size_t have, s
   return KN_OK;
 }
 
+// One operand of a product: `rows` x `cols` in memory (cols contiguous), two planes.
+struct Planes {
+  const __half* p;
+  int64_t rows, cols, ld, plane;
+};
+// its map in the role of the tile's `tile` rows; mn: those rows are the contiguous axis
+inline int operand_map(CUtensorMap* map, const Planes& o, bool mn, int tile) {
+  return tensor_map_planes(map, o.p, o.rows, o.cols, o.ld, o.plane, mn ? 64 : kBK, mn ? kBK : tile,
+                           mn ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+template <typename Epi>
+int mma_product(const Planes& a, bool a_mn, const Planes& b, bool b_mn, int64_t I, int64_t J, int64_t C, int splits, const Epi& epi,
+                cudaStream_t st) {
+  static_assert(sizeof(CUtensorMap) == 128, "kernel parameter");
+  CUtensorMap am, bm;
+  if (int rc = operand_map(&am, a, a_mn, kTM)) return rc;
+  if (int rc = operand_map(&bm, b, b_mn, kTN)) return rc;
+  MmaTiles tl;
+  tl.i_tiles = (uint32_t)ceil_div(I, kTM);
+  tl.j_tiles = (uint32_t)ceil_div(J, kTN);
+  tl.blocks = (uint32_t)ceil_div(C, kBK);
+  tl.blocks_per_split = (uint32_t)ceil_div(tl.blocks, splits);
+  tl.splits = (uint32_t)splits;
+  tl.a_mn = a_mn;
+  tl.b_mn = b_mn;
+  if (cudaError_t e = cudaFuncSetAttribute(mma_kernel<Epi>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMmaSmem)) return (int)e;
+  const uint64_t tiles = (uint64_t)tl.i_tiles * tl.j_tiles * tl.splits;
+  if (tiles > 0x7fffffff) return KN_ESIZE;
+  const unsigned grid = (unsigned)(tiles < (uint64_t)sm_count() ? tiles : sm_count());
+  mma_kernel<Epi><<<grid, kMmaThreads, kMmaSmem, st>>>(am, bm, tl, epi);
+  return launch_status();
+}
+
+// absmax and split of w's classes [v0, v0 + vp) and, with the first piece, of x
+struct SplitState {
+  Planes w, x;
+};
+inline SplitState split_operands(const Head<float>& h, const MmaPlan& p, char* ws, int64_t v0, int64_t vp, bool with_x,
+                                 cudaStream_t st) {
+  SplitJob w, x;
+  w.src = h.trans ? h.w + v0 * h.H : h.w + v0;
+  w.rows = h.trans ? vp : h.H;
+  w.cols = h.trans ? h.H : vp;
+  w.pitch = h.trans ? h.H : h.V;
+  w.dst = (__half*)(ws + p.ws);
+  w.ld = p.wld;
+  w.plane = w.rows * p.wld;
+  x.src = h.x;
+  x.rows = h.N;
+  x.cols = x.pitch = h.H;
+  x.dst = (__half*)(ws + p.xs);
+  x.ld = p.xld;
+  x.plane = x.rows * p.xld;
+  const SplitState s{Planes{w.dst, w.rows, w.cols, w.ld, w.plane}, Planes{x.dst, x.rows, x.cols, x.ld, x.plane}};
+  if (!with_x) x.rows = 0;
+  uint32_t* absmax = (uint32_t*)(ws + p.absmax);
+  int* exps = (int*)(ws + p.exps);
+  const int64_t n = w.rows * w.cols + x.rows * x.cols;
+  const int64_t want = ceil_div(n, 4096);
+  const unsigned blocks = (unsigned)(want < kMaxBlocks ? want : kMaxBlocks);
+  lnll_absmax_kernel<<<blocks, 256, 0, st>>>(w, x, absmax);
+  const int64_t bw = ceil_div(w.rows * ceil_div(w.cols, 8), 1024), bx = ceil_div(x.rows * ceil_div(x.cols, 8), 1024);
+  const unsigned na = (unsigned)(bw < 8192 ? bw : 8192), nb = (unsigned)(bx < 8192 ? bx : 8192);
+  lnll_split_kernel<<<na + nb, 256, 0, st>>>(w, x, na, absmax, blocks, exps);
+  return s;
+}
+
+inline int linear_nll_fwd_mma(const Head<float>& h, float* total, int32_t* count, float* lse, float* per_instance, char* ws,
+                              cudaStream_t st) {
+  const MmaPlan p = mma_plan(h.V, h.H, h.N, h.trans, 0);
+  const int64_t all = ceil_div(h.V, kTN);
+  float *label = (float*)(ws + p.label), *pm = (float*)(ws + p.part_m), *ps = (float*)(ws + p.part_s);
+  for (int64_t v0 = 0; v0 < h.V; v0 += p.piece) {
+    const int64_t vp = h.V - v0 < p.piece ? h.V - v0 : p.piece;
+    const SplitState s = split_operands(h, p, ws, v0, vp, v0 == 0, st);
+    const MmaStats epi{(const int*)(ws + p.exps), h.bias ? h.bias + v0 : nullptr, h.labels, pm, ps, label, h.N, vp, v0, v0 / kTN};
+    if (int rc = mma_product(s.x, false, s.w, !h.trans, h.N, vp, h.H, 1, epi, st)) return rc;
+  }
+  lnll_join_kernel<float><<<(unsigned)ceil_div(h.N, 32), 256, 0, st>>>(pm, ps, label, h.labels, h.N, h.V, all, lse, per_instance);
+  lnll_total_kernel<float><<<1, 1024, 0, st>>>(per_instance, h.labels, h.N, total, count);
+  return launch_status();
+}
+
+inline int linear_nll_bwd_mma(const Head<float>& h, const float* lse, GradScale<float> g, float* dw, float* db, float* dx, char* ws,
+                              cudaStream_t st) {
+  const MmaPlan p = mma_plan(h.V, h.H, h.N, h.trans, 1);
+  const int* exps = (const int*)(ws + p.exps);
+  float* parts = (float*)(ws + p.parts);
+  float* dbp = db ? (float*)(ws + p.db) : nullptr;
+  for (int64_t v0 = 0; v0 < h.V; v0 += p.piece) {
+    const int64_t vp = h.V - v0 < p.piece ? h.V - v0 : p.piece;
+    const SplitState s = split_operands(h, p, ws, v0, vp, v0 == 0, st);
+    const Planes ds{(__half*)(ws + p.ds), h.N, vp, p.dld, h.N * p.dld};
+    const MmaGradScores e1{exps, h.bias ? h.bias + v0 : nullptr, h.labels, lse, (__half*)(ws + p.ds), h.N, vp, p.dld, ds.plane, v0, dbp};
+    if (int rc = mma_product(s.x, false, s.w, !h.trans, h.N, vp, h.H, 1, e1, st)) return rc;
+    if (db) lnll_bias_parts_kernel<<<(unsigned)ceil_div(vp, 256), 256, 0, st>>>(dbp, vp, ceil_div(h.N, kTM), db + v0, g);
+    if (dx) {
+      // every part has work: with fewer blocks of 32 than parts, fewer parts
+      const int64_t blocks = ceil_div(vp, kBK);
+      int splits = (int)(p.splits < blocks ? p.splits : blocks);
+      splits = (int)ceil_div(blocks, ceil_div(blocks, splits));
+      const bool one = splits == 1;
+      const MmaStore e2{exps, 0, one ? dx : parts, h.N, h.H, h.H, one ? 0 : h.N * h.H, one && v0 > 0, g};
+      if (int rc = mma_product(ds, false, s.w, (bool)h.trans, h.N, h.H, vp, splits, e2, st)) return rc;
+      if (!one) lnll_parts_kernel<<<(unsigned)ceil_div(h.N * h.H, 256), 256, 0, st>>>(parts, h.N * h.H, splits, dx, v0 > 0, g);
+    }
+    if (dw) {
+      const MmaStore e3{exps, 1, h.trans ? dw + v0 * h.H : dw + v0, h.trans ? vp : h.H, h.trans ? h.H : vp, h.trans ? h.H : h.V, 0, 0, g};
+      if (int rc = h.trans ? mma_product(ds, true, s.x, true, vp, h.H, h.N, 1, e3, st)
+                           : mma_product(s.x, true, ds, true, h.H, vp, h.N, 1, e3, st))
+        return rc;
+    }
+  }
+  return launch_status();
+}
+
 template <typename T>
 int linear_nll_fwd(const Head<T>& h, T* total, int32_t* count, T* lse, T* per_instance, void* ws, size_t have, cudaStream_t st) {
   if (!total || !count || (h.N > 0 && (!lse || !per_instance))) return KN_EINVAL;
   if (odd(total) || odd(lse) || odd(per_instance) || (uintptr_t)count % 4) return KN_EALIGN;
-  const size_t need = h.V > 0 && h.H > 0 && h.N > 0 && sizes_ok(h.V, h.H, h.N) ? workspace<T>(h.V, h.H, h.N, 0) : 0;
+  const size_t need = h.V > 0 && h.H > 0 && h.N > 0 && sizes_ok(h.V, h.H, h.N) ? workspace_any<T>(h.V, h.H, h.N, 0) : 0;
   if (int rc = check(h, ws, have, need)) return rc;
+  if constexpr (sizeof(T) == 4)
+    if (use_mma<T>(h.V, h.H, h.N)) return linear_nll_fwd_mma(h, total, count, lse, per_instance, (char*)ws, st);
   if (h.N > 0) {
     const int64_t tiles = (h.V + kTile - 1) / kTile;
     char* p = (char*)ws;
@@ -317,7 +513,7 @@ int linear_nll_bwd(const Head<T>& h, const T* lse, int average, T dy, const int3
                    size_t have, cudaStream_t st) {
   if (h.N > 0 && (!lse || (average && !count))) return KN_EINVAL;
   if (odd(lse) || odd(dw) || odd(db) || odd(dx) || (uintptr_t)count % 4) return KN_EALIGN;
-  const size_t need = h.V > 0 && h.H > 0 && h.N > 0 && sizes_ok(h.V, h.H, h.N) ? workspace<T>(h.V, h.H, h.N, 1) : 0;
+  const size_t need = h.V > 0 && h.H > 0 && h.N > 0 && sizes_ok(h.V, h.H, h.N) ? workspace_any<T>(h.V, h.H, h.N, 1) : 0;
   if (int rc = check(h, ws, have, need)) return rc;
   if (h.N == 0) {
     lnll_zero(dw, h.V * h.H, st);
@@ -325,6 +521,8 @@ int linear_nll_bwd(const Head<T>& h, const T* lse, int average, T dy, const int3
     return launch_status();
   }
   const GradScale<T> g{average ? count : nullptr, dy};
+  if constexpr (sizeof(T) == 4)
+    if (use_mma<T>(h.V, h.H, h.N)) return linear_nll_bwd_mma(h, lse, g, dw, db, dx, (char*)ws, st);
   const int64_t piece = simt_piece<T>(h.V, h.N);
   T* ds = (T*)ws;
   for (int64_t v0 = 0; v0 < h.V; v0 += piece) {
@@ -350,7 +548,7 @@ using namespace kn;
 #define KN_DEF_LNLL(f_, S, T)                                                                                       \
   KN_EXPORT size_t knet_linear_nll_workspace_##S(int64_t V, int64_t H, int64_t N, int backward) {                   \
     if (V <= 0 || H <= 0 || N <= 0 || !sizes_ok(V, H, N)) return 0;                                                 \
-    return workspace<T>(V, H, N, backward != 0);                                                                         \
+    return workspace_any<T>(V, H, N, backward != 0);                                                                         \
   }                                                                                                                 \
   KN_EXPORT int knet_linear_nll_fwd_##S(const T* w, int transW, const T* b, const T* x, const int32_t* labels,      \
                                         int64_t V, int64_t H, int64_t N, T* total, int32_t* count, T* lse,          \

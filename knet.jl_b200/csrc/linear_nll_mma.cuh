@@ -1,0 +1,529 @@
+// Float32 products of the linear-layer cross entropy on the tensor cores.
+//
+// A Float32 operand, scaled by a power of two that brings its largest magnitude into [2^14, 2^15), is
+// split into two fp16 terms, hi = fp16(x), lo = fp16(x - hi): together 22 bits, and never less than
+// 2^-25 of the scaled value's unit, so entries down to 2^-17 of the largest keep a relative error of
+// 2^-23.  A product takes three of the four partial products (lo*lo is below 2^-22 of it), which are
+// exact in Float32; the tensor core adds them.  Its additions truncate, so a long sum would lose
+// about 2^-25 per 16 terms, always towards zero: the accumulator in TMEM therefore takes only 128
+// summed indices, and the chunks are added in registers with rounding to nearest.
+//
+// A CTA owns a 128 x 256 tile of the result.  Warp 16 loads the operands with TMA into a ring of
+// stages of 32 summed indices (48 KB: both planes of 128 + 256 rows); warp 17 issues the products
+// into one of two halves of TMEM (256 columns each); warps 0-15 move finished chunks from the other
+// half into registers, 64 columns of one row per thread, and run the epilogue while the tensor core
+// works on the next tile.  The tile is as wide as TMEM allows with two halves: per summed index a CTA
+// loads 1.5 KB for 196 608 multiply-adds, 64 bytes per clock at the full rate.
+#pragma once
+#include <cuda_fp16.h>
+
+#include "linear_nll.cuh"
+#include "umma.cuh"
+
+namespace kn {
+
+constexpr int kTM = 128, kTN = 256, kBK = 32, kStages = 4;
+constexpr int kChunkBlocks = 4;                         // 128 summed indices per accumulator
+constexpr int kEpiWarps = 16, kMmaThreads = (kEpiWarps + 2) * 32;
+constexpr uint32_t kStageA = 2 * kTM * kBK * 2, kStageB = 2 * kTN * kBK * 2, kStageBytes = kStageA + kStageB;
+constexpr int kGradExp = 14;                            // dS lies in [-1, 1]
+
+struct MmaShared {
+  uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2], drain;
+  uint32_t tmem;
+  int gave_up;
+  float2 stat[2][4][kTM];                               // per tile parity, column quarter and row
+  float colsum[4][kTN];
+};
+constexpr size_t kMmaSmem = 1024 + (size_t)kStages * kStageBytes + sizeof(MmaShared);
+
+// how one launch walks its tiles: rows i fastest, then columns j, then parts of the summed axis
+struct MmaTiles {
+  uint32_t i_tiles, j_tiles, splits;
+  uint32_t blocks, blocks_per_split;                    // of 32 summed indices
+  int a_mn, b_mn;                                       // operand stored with its row index contiguous
+};
+
+// A wait that gives up (or finds that another role has) makes every role of the CTA leave.
+__device__ __forceinline__ bool mma_wait(uint64_t* bar, uint32_t parity, int* gave_up) {
+  for (uint32_t i = 0; i < kWaitSpins; i++) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (*(volatile int*)gave_up) return false;
+    if (i > 256) __nanosleep(128);
+  }
+  *(volatile int*)gave_up = 1;
+  note_wait_timeout();
+  return false;
+}
+
+// what the epilogue of one tile gets besides the accumulators
+struct TileAt {
+  int64_t i, j0;               // this thread's row and first of its 64 columns
+  uint32_t it, jt, split;      // tile
+  uint32_t turn;               // how many tiles this CTA has finished
+  int quarter, row;            // which 64 columns, which of the 128 rows
+  MmaShared* sh;
+};
+
+// barriers among the 512 epilogue threads; the second tells every one of them whether any says yes
+__device__ __forceinline__ void epi_sync() { asm volatile("barrier.cta.sync 1, 512;" ::: "memory"); }
+__device__ __forceinline__ bool epi_any(bool yes) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, 1, 512, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)yes)
+      : "memory");
+  return r != 0;
+}
+
+template <typename Epi>
+__global__ void __launch_bounds__(kMmaThreads, 1)
+mma_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap, MmaTiles tl, Epi epi) {
+  extern __shared__ uint8_t raw[];
+  uint8_t* stages = reinterpret_cast<uint8_t*>(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+  MmaShared* sh = reinterpret_cast<MmaShared*>(stages + (size_t)kStages * kStageBytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t tiles = tl.i_tiles * tl.j_tiles * tl.splits;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; s++) {
+      mbar_init(&sh->full[s], 1);
+      mbar_init(&sh->empty[s], 1);
+    }
+    for (int b = 0; b < 2; b++) {
+      mbar_init(&sh->acc_full[b], 1);
+      mbar_init(&sh->acc_empty[b], kEpiWarps);
+    }
+    mbar_init(&sh->drain, 1);
+    sh->gave_up = 0;
+    mbar_init_fence();
+  }
+  if (warp == kEpiWarps + 1) tmem_alloc(&sh->tmem, 512);
+  tcgen05_before_sync();
+  __syncthreads();
+  tcgen05_after_sync();
+  const uint32_t tmem = sh->tmem;
+
+  if (warp == kEpiWarps) {
+    // ---- loads
+    if (lane == 0) {
+      tma_prefetch_map(&amap);
+      tma_prefetch_map(&bmap);
+      uint32_t n = 0;                                   // stages filled so far
+      bool ok = true;
+      for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        const uint32_t it = t % tl.i_tiles, r = t / tl.i_tiles, jt = r % tl.j_tiles, sp = r / tl.j_tiles;
+        const uint32_t k0 = sp * tl.blocks_per_split, k1 = min(k0 + tl.blocks_per_split, tl.blocks);
+        const int32_t i0 = (int32_t)(it * kTM), j0 = (int32_t)(jt * kTN);
+        for (uint32_t k = k0; k < k1; k++, n++) {
+          const uint32_t s = n % kStages;
+          if (n >= kStages && !mma_wait(&sh->empty[s], (n / kStages - 1) & 1, &sh->gave_up)) {
+            ok = false;
+            break;
+          }
+          uint8_t* a = stages + (size_t)s * kStageBytes;
+          uint8_t* b = a + kStageA;
+          const int32_t c = (int32_t)(k * kBK);
+          mbar_arrive_expect_tx(&sh->full[s], kStageBytes);
+          if (tl.a_mn) {
+            for (int g = 0; g < kTM / 64; g++) tma_load_3d(a + g * 8192, &amap, i0 + g * 64, c, 0, &sh->full[s]);
+          } else {
+            tma_load_3d(a, &amap, c, i0, 0, &sh->full[s]);
+          }
+          if (tl.b_mn) {
+            for (int g = 0; g < kTN / 64; g++) tma_load_3d(b + g * 8192, &bmap, j0 + g * 64, c, 0, &sh->full[s]);
+          } else {
+            tma_load_3d(b, &bmap, c, j0, 0, &sh->full[s]);
+          }
+        }
+      }
+      // every load issued has landed before this CTA may leave
+      for (uint32_t m = n > kStages ? n - kStages : 0; m < n; m++)
+        for (uint32_t i = 0; i < kWaitSpins && !mbar_try_wait(&sh->full[m % kStages], (m / kStages) & 1); i++) __nanosleep(64);
+    }
+  } else if (warp == kEpiWarps + 1) {
+    // ---- products
+    if (lane == 0) {
+      const uint32_t idesc = umma_idesc(kTM, kTN, tl.a_mn, tl.b_mn);
+      const uint64_t ad = tl.a_mn ? umma_desc(8192, 1024, 2) : umma_desc(16, 8 * kBK * 2, 4);
+      const uint64_t bd = tl.b_mn ? umma_desc(8192, 1024, 2) : umma_desc(16, 8 * kBK * 2, 4);
+      // second plane, and 16 summed indices further, in bytes
+      const uint32_t alo = tl.a_mn ? 4096 : kTM * kBK * 2, blo = tl.b_mn ? 4096 : kTN * kBK * 2;
+      const uint32_t ak = tl.a_mn ? 2048 : 32, bk = tl.b_mn ? 2048 : 32;
+      uint32_t n = 0, ch = 0;                           // stages and chunks so far
+      bool ok = true;
+      for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        const uint32_t sp = t / (tl.i_tiles * tl.j_tiles);
+        const uint32_t k0 = sp * tl.blocks_per_split, k1 = min(k0 + tl.blocks_per_split, tl.blocks);
+        for (uint32_t k = k0; k < k1 && ok; ch++) {
+          const uint32_t buf = ch & 1, d = tmem + buf * kTN;
+          if (ch >= 2 && !mma_wait(&sh->acc_empty[buf], ((ch >> 1) - 1) & 1, &sh->gave_up)) {
+            ok = false;
+            break;
+          }
+          tcgen05_after_sync();
+          const uint32_t ke = min(k + kChunkBlocks, k1);
+          bool acc = false;
+          for (; k < ke; k++, n++) {
+            const uint32_t s = n % kStages;
+            if (!mma_wait(&sh->full[s], (n / kStages) & 1, &sh->gave_up)) {
+              ok = false;
+              break;
+            }
+            tcgen05_after_sync();
+            const uint32_t a = smem_u32(stages + (size_t)s * kStageBytes), b = a + kStageA;
+            // the small cross terms first, while the sum is small
+#pragma unroll
+            for (uint32_t q = 0; q < kBK / 16; q++) {
+              umma_f16(d, umma_at(ad, a + alo + q * ak), umma_at(bd, b + q * bk), idesc, acc);
+              umma_f16(d, umma_at(ad, a + q * ak), umma_at(bd, b + blo + q * bk), idesc, true);
+              acc = true;
+            }
+#pragma unroll
+            for (uint32_t q = 0; q < kBK / 16; q++) umma_f16(d, umma_at(ad, a + q * ak), umma_at(bd, b + q * bk), idesc, true);
+            umma_commit(&sh->empty[s]);
+          }
+          if (!ok) break;
+          umma_commit(&sh->acc_full[buf]);
+        }
+      }
+      // every product issued is done before TMEM is freed
+      umma_commit(&sh->drain);
+      for (uint32_t i = 0; i < kWaitSpins && !mbar_try_wait(&sh->drain, 0); i++) __nanosleep(64);
+    }
+  } else {
+    // ---- accumulators -> registers -> epilogue
+    const int q = warp & 3, quarter = warp >> 2;
+    const uint32_t lane_addr = (uint32_t)(q * 32) << 16;
+    uint32_t ch = 0, turn = 0;
+    bool ok = true;
+    for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x, turn++) {
+      const uint32_t it = t % tl.i_tiles, r = t / tl.i_tiles, jt = r % tl.j_tiles, sp = r / tl.j_tiles;
+      const uint32_t k0 = sp * tl.blocks_per_split, k1 = min(k0 + tl.blocks_per_split, tl.blocks);
+      float acc[64];
+#pragma unroll
+      for (int e = 0; e < 64; e++) acc[e] = 0.0f;
+      for (uint32_t k = k0; k < k1; k += kChunkBlocks, ch++) {
+        const uint32_t buf = ch & 1;
+        ok = __all_sync(0xffffffffu, mma_wait(&sh->acc_full[buf], (ch >> 1) & 1, &sh->gave_up));
+        if (!ok) break;
+        tcgen05_after_sync();
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          uint32_t v[32];
+          tmem_load32(tmem + lane_addr + buf * kTN + quarter * 64 + h * 32, v);
+          tmem_load_wait();
+#pragma unroll
+          for (int e = 0; e < 32; e++) acc[h * 32 + e] += __uint_as_float(v[e]);
+        }
+        tcgen05_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->acc_empty[buf]);
+      }
+      // the epilogue has barriers of its own: all of its warps run it, or none
+      if (epi_any(!ok)) break;
+      const TileAt at{(int64_t)it * kTM + q * 32 + lane, (int64_t)jt * kTN + quarter * 64, it, jt, sp, turn, quarter, q * 32 + lane, sh};
+      epi(acc, at);
+    }
+  }
+  __syncwarp();
+  tcgen05_before_sync();
+  __syncthreads();
+  tcgen05_after_sync();
+  if (warp == kEpiWarps + 1) tmem_free(tmem, 512);
+}
+
+// ---- scaling ------------------------------------------------------------------------------------------
+// exps[0] = exponent of w (of the piece), exps[1] = exponent of x: both were multiplied by 2^exp
+struct Unscale {
+  float a, b;
+  __device__ __forceinline__ float operator()(float v) const { return v * a * b; }
+};
+// 2^-e in two factors (e may exceed the exponent range of one Float32)
+__device__ __forceinline__ Unscale unscale(int e) {
+  const int h = e / 2;
+  return Unscale{scalbnf(1.0f, -h), scalbnf(1.0f, -(e - h))};
+}
+__device__ __forceinline__ int scale_exponent(uint32_t max_bits) {
+  if (max_bits == 0) return 0;
+  return 14 - ilogbf(__uint_as_float(max_bits));
+}
+
+struct SplitJob {
+  const float* src;            // rows x cols, row pitch `pitch`
+  int64_t rows, cols, pitch;
+  __half* dst;                 // two planes of rows x ld
+  int64_t ld, plane;
+};
+constexpr int kMaxBlocks = 592;                         // absmax blocks: 4 per SM
+
+// largest finite magnitude of each of two arrays, one value per block and array
+__global__ void __launch_bounds__(256)
+lnll_absmax_kernel(SplitJob a, SplitJob b, uint32_t* __restrict__ part) {
+  __shared__ uint32_t red[32];
+  for (int k = 0; k < 2; k++) {
+    const SplitJob& j = k ? b : a;
+    uint32_t m = 0;
+    const int64_t n = j.rows * j.cols;
+    const int64_t per = (n + gridDim.x - 1) / gridDim.x, lo = per * blockIdx.x, hi = min(lo + per, n);
+    auto take = [&](float v) {
+      const uint32_t u = __float_as_uint(v) & 0x7fffffffu;
+      m = max(m, u < 0x7f800000u ? u : 0u);
+    };
+    if (j.pitch == j.cols && lo < hi) {
+      const float* p = j.src + lo;
+      const int64_t len = hi - lo;
+      int64_t head = (((16 - ((uintptr_t)p & 15)) & 15) / 4);
+      if (head > len) head = len;
+      const int64_t nv = (len - head) / 4;
+      if (threadIdx.x < head) take(p[threadIdx.x]);
+      const float4* q = reinterpret_cast<const float4*>(p + head);
+      int64_t v = threadIdx.x;
+      for (; v + 3 * 256 < nv; v += 4 * 256) {
+        float4 t[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) t[u] = __ldg(q + v + u * 256);
+#pragma unroll
+        for (int u = 0; u < 4; u++) { take(t[u].x); take(t[u].y); take(t[u].z); take(t[u].w); }
+      }
+      for (; v < nv; v += 256) {
+        const float4 t = __ldg(q + v);
+        take(t.x); take(t.y); take(t.z); take(t.w);
+      }
+      const int64_t tail = head + nv * 4 + threadIdx.x;
+      if (tail < len) take(p[tail]);
+    } else {
+      for (int64_t i = lo + threadIdx.x; i < hi; i += 256) take(j.src[(i / j.cols) * j.pitch + i % j.cols]);
+    }
+    m = block_reduce(m, [](uint32_t x, uint32_t y) { return max(x, y); }, 0u, red);
+    if (threadIdx.x == 0) part[k * kMaxBlocks + blockIdx.x] = m;
+    __syncthreads();
+  }
+}
+
+// x * 2^e = hi + lo in fp16; an infinity goes to hi alone, so that hi + lo is not NaN
+__device__ __forceinline__ void split_half(float v, __half& hi, __half& lo) {
+  hi = __float2half_rn(v);
+  const float r = v - __half2float(hi);
+  lo = isinf(v) ? __float2half_rn(0.0f) : __float2half_rn(r);
+}
+
+// both operands into their two planes; rows are shared out over blocks, 8 columns per thread and turn
+__global__ void __launch_bounds__(256)
+lnll_split_kernel(SplitJob a, SplitJob b, uint32_t blocks_a, const uint32_t* __restrict__ part, uint32_t parts,
+                  int* __restrict__ exps) {
+  __shared__ uint32_t red[32];
+  const bool second = blockIdx.x >= blocks_a;
+  const SplitJob j = second ? b : a;
+  uint32_t m = 0;
+  for (uint32_t k = threadIdx.x; k < parts; k += 256) m = max(m, part[(second ? kMaxBlocks : 0) + k]);
+  m = block_reduce(m, [](uint32_t x, uint32_t y) { return max(x, y); }, 0u, red);
+  const int e = scale_exponent(m);
+  const uint32_t first = second ? blocks_a : 0, nb = (second ? gridDim.x - blocks_a : blocks_a);
+  if (blockIdx.x == first && threadIdx.x == 0) exps[second] = e;
+  const Unscale sc = unscale(-e);
+  const int64_t groups = (j.cols + 7) / 8;               // the pitch ld is a multiple of 8
+  const int64_t total = groups * j.rows;
+  for (int64_t g = (int64_t)(blockIdx.x - first) * 256 + threadIdx.x; g < total; g += (int64_t)nb * 256) {
+    const int64_t r = g / groups, c = (g - r * groups) * 8;
+    const float* p = j.src + r * j.pitch + c;
+    float v[8];
+    if (c + 8 <= j.cols && ((uintptr_t)p & 15) == 0) {
+      *reinterpret_cast<float4*>(v) = __ldg(reinterpret_cast<const float4*>(p));
+      *reinterpret_cast<float4*>(v + 4) = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; k++) v[k] = c + k < j.cols ? p[k] : 0.0f;
+    }
+    __align__(16) __half hi[8];
+    __align__(16) __half lo[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) split_half(sc(v[k]), hi[k], lo[k]);
+    *reinterpret_cast<uint4*>(j.dst + r * j.ld + c) = *reinterpret_cast<uint4*>(hi);
+    *reinterpret_cast<uint4*>(j.dst + j.plane + r * j.ld + c) = *reinterpret_cast<uint4*>(lo);
+  }
+}
+
+// ---- epilogues -------------------------------------------------------------------------------------------
+// i = instance, j = class: maximum and sum of exponentials of the tile's 256 classes per instance
+struct MmaStats {
+  const int* exps;
+  const float* bias;
+  const int32_t* labels;
+  float *part_m, *part_s, *label_score;
+  int64_t N, J;                // instances, classes of this launch
+  int64_t v0, tile0;           // first class and first tile of this launch
+  __device__ __forceinline__ void operator()(float (&acc)[64], const TileAt& at) const {
+    const Unscale us = unscale(exps[0] + exps[1]);
+    const bool live = at.i < N;
+    const int64_t lab = live ? (int64_t)labels[at.i] - 1 - v0 - at.j0 : -1;
+    float m = -CUDART_INF_F;
+    if (at.j0 + 64 <= J) {
+#pragma unroll
+      for (int e = 0; e < 64; e++) {
+        acc[e] = us(acc[e]) + (bias ? __ldg(bias + at.j0 + e) : 0.0f);
+        m = fmaxf(m, acc[e]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 64; e++) {
+        acc[e] = at.j0 + e < J ? us(acc[e]) + (bias ? __ldg(bias + at.j0 + e) : 0.0f) : -CUDART_INF_F;
+        m = fmaxf(m, acc[e]);
+      }
+    }
+    if (live && lab >= 0 && lab < 64) {
+      float s = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 64; e++)
+        if (lab == e) s = acc[e];
+      label_score[at.i] = s;
+    }
+    float s = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 64; e++) s += exp_from(acc[e], m);
+    float2(&st)[4][kTM] = at.sh->stat[at.turn & 1];
+    st[at.quarter][at.row] = make_float2(m, s);
+    epi_sync();
+    if (at.quarter == 0 && live) {
+      float mm = m;
+#pragma unroll
+      for (int k = 1; k < 4; k++) mm = fmaxf(mm, st[k][at.row].x);
+      float ss = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const float2 o = st[k][at.row];
+        if (o.y != 0.0f) ss += o.y * exp_from(o.x, mm);      // an empty quarter is (-inf, 0)
+      }
+      part_m[(tile0 + at.jt) * N + at.i] = mm;
+      part_s[(tile0 + at.jt) * N + at.i] = ss;
+    }
+  }
+};
+
+// 64 values per lane -> the sums over the 32 lanes of columns 2*lane and 2*lane+1
+__device__ __forceinline__ float2 lane_sums(float (&v)[64]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 16, half = 32; o > 0; o >>= 1, half >>= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int k = 0; k < 32; k++)
+      if (k < half) {
+        const float send = up ? v[k] : v[k + half], keep = up ? v[k + half] : v[k];
+        v[k] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+      }
+  }
+  return make_float2(v[0], v[1]);
+}
+
+// i = instance, j = class of the piece: dS without g in two fp16 planes, and its sums over the tile's
+// instances for the bias gradient
+struct MmaGradScores {
+  const int* exps;
+  const float* bias;           // of the piece's first class
+  const int32_t* labels;
+  const float* lse;            // N rounded values, N remainders
+  __half* ds;                  // [2][N][ld]
+  int64_t N, J, ld, plane, v0;
+  float* db_part;              // [instance tile][J] or null
+  __device__ __forceinline__ void operator()(float (&acc)[64], const TileAt& at) const {
+    const Unscale us = unscale(exps[0] + exps[1]);
+    const bool live = at.i < N;
+    const float hi = live ? __ldg(lse + at.i) : 0.0f, lo = live ? __ldg(lse + N + at.i) : 0.0f;
+    const int32_t lab = live ? __ldg(labels + at.i) : 0;    // rows past the last instance act as skipped
+    __half* row = ds + at.i * ld + at.j0;
+#pragma unroll
+    for (int g = 0; g < 8; g++) {
+      __align__(16) __half h[8];
+      __align__(16) __half l[8];
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        const int e = g * 8 + k;
+        const bool in = at.j0 + e < J;
+        const float s = us(acc[e]) + (bias && in ? __ldg(bias + at.j0 + e) : 0.0f);
+        const float d = in ? grad_score(s, hi, lo, lab, v0 + at.j0 + e) : 0.0f;
+        acc[e] = d;
+        split_half(d * (float)(1 << kGradExp), h[k], l[k]);
+      }
+      if (live && at.j0 + g * 8 < J) {                     // ld is a multiple of 8
+        *reinterpret_cast<uint4*>(row + g * 8) = *reinterpret_cast<uint4*>(h);
+        *reinterpret_cast<uint4*>(row + plane + g * 8) = *reinterpret_cast<uint4*>(l);
+      }
+    }
+    if (db_part) {
+      const float2 c = lane_sums(acc);
+      const int lane = threadIdx.x & 31, q = at.row >> 5;
+      *reinterpret_cast<float2*>(&at.sh->colsum[q][at.quarter * 64 + 2 * lane]) = c;
+      epi_sync();
+      const int col = threadIdx.x;
+      if (col < kTN) {
+        const int64_t j = (int64_t)at.jt * kTN + col;
+        if (j < J)
+          db_part[(int64_t)at.it * J + j] =
+              (at.sh->colsum[0][col] + at.sh->colsum[1][col]) + (at.sh->colsum[2][col] + at.sh->colsum[3][col]);
+      }
+    }
+  }
+};
+
+// out(i, j) = or += g * acc; with several parts of the summed axis the plain sums go to `out` + part
+struct MmaStore {
+  const int* exps;
+  int which;                   // the operand beside dS: 0 w, 1 x
+  float* out;
+  int64_t I, J, ld, part;      // part: elements between the parts' results (0: there is one)
+  int add;
+  GradScale<float> g;
+  __device__ __forceinline__ void operator()(float (&acc)[64], const TileAt& at) const {
+    if (at.i >= I) return;
+    const Unscale us = unscale(exps[which] + kGradExp);
+    const float f = part ? 1.0f : g.value();
+    float* p = out + at.split * part + at.i * ld + at.j0;
+    if (at.j0 + 64 <= J && ((uintptr_t)p & 15) == 0) {
+#pragma unroll
+      for (int e = 0; e < 64; e += 4) {
+        float4 v = make_float4(us(acc[e]) * f, us(acc[e + 1]) * f, us(acc[e + 2]) * f, us(acc[e + 3]) * f);
+        float4* q = reinterpret_cast<float4*>(p + e);
+        if (add) {
+          const float4 o = *q;
+          v = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
+        }
+        *q = v;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 64; e++)
+        if (at.j0 + e < J) {
+          const float v = us(acc[e]) * f;
+          p[e] = add ? p[e] + v : v;
+        }
+    }
+  }
+};
+
+// dx = or += g * (the parts' sums, added in order)
+__global__ void __launch_bounds__(256)
+lnll_parts_kernel(const float* __restrict__ parts, int64_t n, int splits, float* __restrict__ out, int add, GradScale<float> g) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float a = parts[i];
+  for (int s = 1; s < splits; s++) a += parts[(int64_t)s * n + i];
+  a *= g.value();
+  out[i] = add ? out[i] + a : a;
+}
+
+// db[j] = g * sum over the instance tiles of their sums
+__global__ void __launch_bounds__(256)
+lnll_bias_parts_kernel(const float* __restrict__ part, int64_t J, int64_t tiles, float* __restrict__ db, GradScale<float> g) {
+  const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (j >= J) return;
+  float a = 0.0f;
+  for (int64_t t = 0; t < tiles; t++) a += part[t * J + j];
+  db[j] = a * g.value();
+}
+
+}  // namespace kn

@@ -161,32 +161,48 @@ template <typename T> struct StoreEpi {
 };
 
 // ---- joining the tiles of the vocabulary ---------------------------------------------------------------
-// A CTA takes 32 instances; its 8 warps share the tiles of the vocabulary.  lse and the loss are
-// formed in Float64 and rounded once.  A label outside 0..V gives a loss of NaN.
+// A CTA takes 32 instances; its 8 warps share the tiles of the vocabulary: the maximum first, then the
+// sums relative to it, added in Float64.  lse and the loss are formed in Float64 and rounded once.  A label outside 0..V gives a loss of NaN.
 template <typename T>
 __global__ void __launch_bounds__(256)
 lnll_join_kernel(const T* __restrict__ part_m, const T* __restrict__ part_s, const T* __restrict__ label_score,
                  const int32_t* __restrict__ labels, int64_t N, int64_t V, int64_t tiles, T* __restrict__ lse,
                  T* __restrict__ per_instance) {
-  __shared__ double sm[8][32], ss[8][32];
+  __shared__ T sm[8][32];
+  __shared__ double ss[8][32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t n = (int64_t)blockIdx.x * 32 + lane;
-  MaxSum a{-Math<double>::inf(), 0.0};
-  if (n < N)
-    for (int64_t t = w; t < tiles; t += 8) a = join(a, MaxSum{(double)part_m[t * N + n], (double)part_s[t * N + n]});
-  sm[w][lane] = a.m;
-  ss[w][lane] = a.s;
+  T m = -Math<T>::inf();
+  if (n < N) {
+#pragma unroll 4
+    for (int64_t t = w; t < tiles; t += 8) m = fmax(m, part_m[t * N + n]);
+  }
+  sm[w][lane] = m;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 8; k++) m = fmax(m, sm[k][lane]);
+  double s = 0.0;
+  if (n < N) {
+#pragma unroll 4
+    for (int64_t t = w; t < tiles; t += 8) {
+      const T d = part_m[t * N + n] - m, v = part_s[t * N + n];
+      if (v != (T)0) s += (double)(v * exp(d));      // an empty tile is (-inf, 0)
+    }
+  }
+  ss[w][lane] = s;
   __syncthreads();
   if (w == 0 && n < N) {
-    for (int k = 1; k < 8; k++) a = join(a, MaxSum{sm[k][lane], ss[k][lane]});
-    const double l = a.m + ::log(a.s);
-    const T hi = (T)l;
+    s = ss[0][lane];
+    for (int k = 1; k < 8; k++) s += ss[k][lane];
+    const double ls = ::log(s);
+    const T hi = (T)((double)m + ls);
     lse[n] = hi;
-    lse[N + n] = isfinite(hi) ? (T)(l - (double)hi) : (T)0;
+    // in this order log s survives beside a maximum of the type's lowest value (every class masked by it)
+    lse[N + n] = isfinite(hi) ? (T)(((double)m - (double)hi) + ls) : (T)0;
     const int32_t lab = labels[n];
     T loss = (T)0;
     if (lab < 0 || lab > V) loss = (T)NAN;
-    else if (lab > 0) loss = (T)(l - (double)label_score[n]);
+    else if (lab > 0) loss = (T)(((double)m - (double)label_score[n]) + ls);
     per_instance[n] = loss;
   }
 }
@@ -271,7 +287,7 @@ template <typename T> bool use_mma(int64_t V, int64_t H, int64_t N) {
 }
 
 // Pieces of the vocabulary and parts of dx's sum.  Workspace bounds: 256 MB of split weights in the
-// forward; 128 MB of dS and 64 MB of split weights in the backward.  Within them the backward takes
+// forward; 128 MB of dS and 192 MB of split weights in the backward.  Within them the backward takes
 // the piece with the fewest waves of tiles over its three products (a product's tiles are 128 x 256
 // and its time is proportional to the summed length), charging each piece for its launches.
 struct MmaPlan {
@@ -293,7 +309,7 @@ inline MmaPlan mma_plan(int64_t V, int64_t H, int64_t N, int trans, int backward
     const int64_t nt = ceil_div(N, kTM), hj = ceil_div(H, kTN), hi = ceil_div(H, kTM);
     double best = 0;
     for (int64_t m = 1; m <= all; m++) {
-      if (m > 1 && (m * kTN * N * 4 > (128ll << 20) || m * kTN * H * 4 > (64ll << 20))) break;
+      if (m > 1 && (m * kTN * N * 4 > (128ll << 20) || m * kTN * H * 4 > (192ll << 20))) break;
       int64_t sp = kPlanSMs / (nt * hj);
       sp = sp < 1 ? 1 : sp > m ? m : sp > 16 ? 16 : sp;
       const double t = (double)ceil_div(nt * m, kPlanSMs) * H + (double)ceil_div(nt * hj * sp, kPlanSMs) * ceil_div(m * kTN, sp) +

@@ -11,16 +11,6 @@ template <typename T> __device__ __forceinline__ T exp_from(T v, T m) {
   return v == -Math<T>::inf() ? (T)0 : Math<T>::exp_fast(v - m);
 }
 
-struct MaxSum {
-  double m, s;
-};
-// the sum of exponentials relative to the larger maximum; an empty side (-inf, 0) leaves the other as it is
-__device__ __forceinline__ MaxSum join(const MaxSum& a, const MaxSum& b) {
-  const double m = fmax(a.m, b.m);
-  const double sa = a.s == 0.0 ? 0.0 : a.s * ::exp(a.m - m), sb = b.s == 0.0 ? 0.0 : b.s * ::exp(b.m - m);
-  return MaxSum{m, sa + sb};
-}
-
 // d loss / d score of class v (0-based) without the factor g: softmax minus one-hot, 0 on a skipped
 // instance whatever its scores are.
 template <typename T> __device__ __forceinline__ T grad_score(T s, T hi, T lo, int32_t label, int64_t v) {

@@ -33,6 +33,7 @@ struct MmaShared {
   uint32_t tmem;
   int gave_up;
   float2 stat[2][4][kTM];                               // per tile parity, column quarter and row
+  __align__(16) float bias[2][kTN];                     // per tile parity
   float colsum[4][kTN];
 };
 constexpr size_t kMmaSmem = 1024 + (size_t)kStages * kStageBytes + sizeof(MmaShared);
@@ -204,6 +205,7 @@ mma_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUt
     for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x, turn++) {
       const uint32_t it = t % tl.i_tiles, r = t / tl.i_tiles, jt = r % tl.j_tiles, sp = r / tl.j_tiles;
       const uint32_t k0 = sp * tl.blocks_per_split, k1 = min(k0 + tl.blocks_per_split, tl.blocks);
+      epi.stage((int64_t)jt * kTN, sh->bias[turn & 1]);  // read after the barrier below
       float acc[64];
 #pragma unroll
       for (int e = 0; e < 64; e++) acc[e] = 0.0f;
@@ -213,12 +215,12 @@ mma_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUt
         if (!ok) break;
         tcgen05_after_sync();
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          uint32_t v[32];
-          tmem_load32(tmem + lane_addr + buf * kTN + quarter * 64 + h * 32, v);
+        for (int h = 0; h < 4; h++) {
+          uint32_t v[16];
+          tmem_load16(tmem + lane_addr + buf * kTN + quarter * 64 + h * 16, v);
           tmem_load_wait();
 #pragma unroll
-          for (int e = 0; e < 32; e++) acc[h * 32 + e] += __uint_as_float(v[e]);
+          for (int e = 0; e < 16; e++) acc[h * 16 + e] += __uint_as_float(v[e]);
         }
         tcgen05_before_sync();
         __syncwarp();
@@ -261,47 +263,43 @@ struct SplitJob {
 };
 constexpr int kMaxBlocks = 592;                         // absmax blocks: 4 per SM
 
-// largest finite magnitude of each of two arrays, one value per block and array
+// Largest finite magnitude of each of two arrays, one value per block and array.  A block takes runs
+// of 8192 elements of a row in turn (a contiguous array is one row).
+constexpr int kRun = 8192;
 __global__ void __launch_bounds__(256)
 lnll_absmax_kernel(SplitJob a, SplitJob b, uint32_t* __restrict__ part) {
   __shared__ uint32_t red[32];
   for (int k = 0; k < 2; k++) {
     const SplitJob& j = k ? b : a;
+    const bool flat = j.pitch == j.cols;
+    const int64_t rows = flat ? (j.rows > 0 ? 1 : 0) : j.rows, cols = flat ? j.rows * j.cols : j.cols;
+    const int64_t runs = (cols + kRun - 1) / kRun;
     uint32_t m = 0;
-    const int64_t n = j.rows * j.cols;
-    const int64_t per = (n + gridDim.x - 1) / gridDim.x, lo = per * blockIdx.x, hi = min(lo + per, n);
     auto take = [&](float v) {
       const uint32_t u = __float_as_uint(v) & 0x7fffffffu;
       m = max(m, u < 0x7f800000u ? u : 0u);
     };
-    if (j.pitch == j.cols && lo < hi) {
-      const float* p = j.src + lo;
-      const int64_t len = hi - lo;
-      int64_t head = (((16 - ((uintptr_t)p & 15)) & 15) / 4);
+    for (int64_t t = blockIdx.x; t < rows * runs; t += gridDim.x) {
+      const int64_t r = t / runs, c = (t - r * runs) * kRun;
+      const float* p = j.src + r * j.pitch + c;
+      const int len = (int)min((int64_t)kRun, cols - c);
+      int head = (int)(((16 - ((uintptr_t)p & 15)) & 15) / 4);
       if (head > len) head = len;
-      const int64_t nv = (len - head) / 4;
+      const int nv = (len - head) / 4;
       if (threadIdx.x < head) take(p[threadIdx.x]);
       const float4* q = reinterpret_cast<const float4*>(p + head);
-      int64_t v = threadIdx.x;
-      for (; v + 3 * 256 < nv; v += 4 * 256) {
-        float4 t[4];
+      float4 v[8];
 #pragma unroll
-        for (int u = 0; u < 4; u++) t[u] = __ldg(q + v + u * 256);
+      for (int u = 0; u < 8; u++)
+        if (threadIdx.x + u * 256 < nv) v[u] = __ldg(q + threadIdx.x + u * 256);
 #pragma unroll
-        for (int u = 0; u < 4; u++) { take(t[u].x); take(t[u].y); take(t[u].z); take(t[u].w); }
-      }
-      for (; v < nv; v += 256) {
-        const float4 t = __ldg(q + v);
-        take(t.x); take(t.y); take(t.z); take(t.w);
-      }
-      const int64_t tail = head + nv * 4 + threadIdx.x;
+      for (int u = 0; u < 8; u++)
+        if (threadIdx.x + u * 256 < nv) { take(v[u].x); take(v[u].y); take(v[u].z); take(v[u].w); }
+      const int tail = head + nv * 4 + threadIdx.x;
       if (tail < len) take(p[tail]);
-    } else {
-      for (int64_t i = lo + threadIdx.x; i < hi; i += 256) take(j.src[(i / j.cols) * j.pitch + i % j.cols]);
     }
     m = block_reduce(m, [](uint32_t x, uint32_t y) { return max(x, y); }, 0u, red);
     if (threadIdx.x == 0) part[k * kMaxBlocks + blockIdx.x] = m;
-    __syncthreads();
   }
 }
 
@@ -349,6 +347,23 @@ lnll_split_kernel(SplitJob a, SplitJob b, uint32_t blocks_a, const uint32_t* __r
 }
 
 // ---- epilogues -------------------------------------------------------------------------------------------
+// A thread holds 64 columns of one row.  The epilogue has to stay below the time of two chunks (the
+// tensor core runs ahead by that much), about 6000 clocks: some 11 instructions per score plus 5 for
+// stores that cover whole 128-byte lines.
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float exp2_approx(float t) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(t));
+  return y;
+}
+
+// the bias of the tile's classes into shared memory, 0 without one and past the last class
+__device__ __forceinline__ void stage_bias(const float* bias, int64_t j0, int64_t J, float* to) {
+  const int col = threadIdx.x;
+  if (col < kTN) to[col] = bias && j0 + col < J ? __ldg(bias + j0 + col) : 0.0f;
+}
+
 // i = instance, j = class: maximum and sum of exponentials of the tile's 256 classes per instance
 struct MmaStats {
   const int* exps;
@@ -357,34 +372,40 @@ struct MmaStats {
   float *part_m, *part_s, *label_score;
   int64_t N, J;                // instances, classes of this launch
   int64_t v0, tile0;           // first class and first tile of this launch
+  __device__ __forceinline__ void stage(int64_t j0, float* to) const { stage_bias(bias, j0, J, to); }
   __device__ __forceinline__ void operator()(float (&acc)[64], const TileAt& at) const {
     const Unscale us = unscale(exps[0] + exps[1]);
     const bool live = at.i < N;
     const int64_t lab = live ? (int64_t)labels[at.i] - 1 - v0 - at.j0 : -1;
+    const float4* bs = reinterpret_cast<const float4*>(at.sh->bias[at.turn & 1] + at.quarter * 64);
     float m = -CUDART_INF_F;
-    if (at.j0 + 64 <= J) {
+    const int in = (int)min((int64_t)64, J - at.j0);        // columns that are classes
 #pragma unroll
-      for (int e = 0; e < 64; e++) {
-        acc[e] = us(acc[e]) + (bias ? __ldg(bias + at.j0 + e) : 0.0f);
-        m = fmaxf(m, acc[e]);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 64; e++) {
-        acc[e] = at.j0 + e < J ? us(acc[e]) + (bias ? __ldg(bias + at.j0 + e) : 0.0f) : -CUDART_INF_F;
-        m = fmaxf(m, acc[e]);
-      }
+    for (int g = 0; g < 16; g++) {
+      const float4 b = bs[g];
+      acc[4 * g] = fmaf(acc[4 * g] * us.a, us.b, b.x);
+      acc[4 * g + 1] = fmaf(acc[4 * g + 1] * us.a, us.b, b.y);
+      acc[4 * g + 2] = fmaf(acc[4 * g + 2] * us.a, us.b, b.z);
+      acc[4 * g + 3] = fmaf(acc[4 * g + 3] * us.a, us.b, b.w);
     }
-    if (live && lab >= 0 && lab < 64) {
+    if (in < 64) {
+#pragma unroll
+      for (int e = 0; e < 64; e++)
+        if (e >= in) acc[e] = -CUDART_INF_F;
+    }
+#pragma unroll
+    for (int e = 0; e < 64; e++) m = fmaxf(m, acc[e]);
+    if (lab >= 0 && lab < 64) {
       float s = 0.0f;
 #pragma unroll
       for (int e = 0; e < 64; e++)
         if (lab == e) s = acc[e];
       label_score[at.i] = s;
     }
+    const float ref = m == -CUDART_INF_F ? 0.0f : m;        // all masked: every term is 0
     float s = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 64; e++) s += exp_from(acc[e], m);
+    for (int e = 0; e < 64; e++) s += exp2_approx((acc[e] - ref) * kLog2e);
     float2(&st)[4][kTM] = at.sh->stat[at.turn & 1];
     st[at.quarter][at.row] = make_float2(m, s);
     epi_sync();
@@ -396,7 +417,7 @@ struct MmaStats {
 #pragma unroll
       for (int k = 0; k < 4; k++) {
         const float2 o = st[k][at.row];
-        if (o.y != 0.0f) ss += o.y * exp_from(o.x, mm);      // an empty quarter is (-inf, 0)
+        if (o.y != 0.0f) ss += o.y * exp2_approx((o.x - mm) * kLog2e);      // an empty quarter is (-inf, 0)
       }
       part_m[(tile0 + at.jt) * N + at.i] = mm;
       part_s[(tile0 + at.jt) * N + at.i] = ss;
@@ -404,20 +425,42 @@ struct MmaStats {
   }
 };
 
-// 64 values per lane -> the sums over the 32 lanes of columns 2*lane and 2*lane+1
-__device__ __forceinline__ float2 lane_sums(float (&v)[64]) {
+// 32 values per lane -> the sums over the 32 lanes of column `lane`
+__device__ __forceinline__ float lane_sum(float (&v)[32]) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int o = 16, half = 32; o > 0; o >>= 1, half >>= 1) {
+  for (int o = 16; o > 0; o >>= 1) {
     const bool up = lane & o;
 #pragma unroll
-    for (int k = 0; k < 32; k++)
-      if (k < half) {
-        const float send = up ? v[k] : v[k + half], keep = up ? v[k + half] : v[k];
+    for (int k = 0; k < 16; k++)
+      if (k < o) {
+        const float send = up ? v[k] : v[k + o], keep = up ? v[k + o] : v[k];
         v[k] = keep + __shfl_xor_sync(0xffffffffu, send, o);
       }
   }
-  return make_float2(v[0], v[1]);
+  return v[0];
+}
+
+// Eight lanes that hold one row of eight 16-byte groups each (32 words) exchange them so that lane r
+// (of the eight) holds group r of all eight rows: stores then cover 128 contiguous bytes per row
+// instead of 16 bytes in each of 32 lines.
+__device__ __forceinline__ void transpose8(uint32_t (&w)[32]) {
+  const int r = threadIdx.x & 7;
+#pragma unroll
+  for (int b = 1; b < 8; b <<= 1) {
+    const bool up = r & b;
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+      if (!(k & b)) {
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          const uint32_t send = up ? w[4 * k + c] : w[4 * (k | b) + c];
+          const uint32_t got = __shfl_xor_sync(0xffffffffu, send, b);
+          if (up) w[4 * k + c] = got;
+          else w[4 * (k | b) + c] = got;
+        }
+      }
+  }
 }
 
 // i = instance, j = class of the piece: dS without g in two fp16 planes, and its sums over the tile's
@@ -430,41 +473,70 @@ struct MmaGradScores {
   __half* ds;                  // [2][N][ld]
   int64_t N, J, ld, plane, v0;
   float* db_part;              // [instance tile][J] or null
+  __device__ __forceinline__ void stage(int64_t j0, float* to) const { stage_bias(bias, j0, J, to); }
   __device__ __forceinline__ void operator()(float (&acc)[64], const TileAt& at) const {
     const Unscale us = unscale(exps[0] + exps[1]);
     const bool live = at.i < N;
+    const int32_t label = live ? __ldg(labels + at.i) : 0;    // rows past the last instance act as skipped
     const float hi = live ? __ldg(lse + at.i) : 0.0f, lo = live ? __ldg(lse + N + at.i) : 0.0f;
-    const int32_t lab = live ? __ldg(labels + at.i) : 0;    // rows past the last instance act as skipped
-    __half* row = ds + at.i * ld + at.j0;
+    const int64_t hit64 = (int64_t)label - 1 - v0 - at.j0;
+    const int hit = hit64 >= 0 && hit64 < 64 ? (int)hit64 : -1;
+    const int in = (int)max((int64_t)0, min((int64_t)64, J - at.j0));
+    const float4* bs = reinterpret_cast<const float4*>(at.sh->bias[at.turn & 1] + at.quarter * 64);
+    const int lane = threadIdx.x & 31, r8 = lane & 7;
+    const int64_t row0 = at.i - lane + (lane & ~7);           // first of the eight rows of this lane's group
+    // after the exchange this lane holds, of each of the eight rows, 8 classes of one plane
+    const int64_t col = at.j0 + (r8 & 3) * 8;
+    __half* out = ds + (r8 >> 2) * plane + row0 * ld + col;
 #pragma unroll
-    for (int g = 0; g < 8; g++) {
-      __align__(16) __half h[8];
-      __align__(16) __half l[8];
+    for (int half = 0; half < 2; half++) {                    // 32 columns at a time: fewer live registers
+      float d[32];
 #pragma unroll
-      for (int k = 0; k < 8; k++) {
-        const int e = g * 8 + k;
-        const bool in = at.j0 + e < J;
-        const float s = us(acc[e]) + (bias && in ? __ldg(bias + at.j0 + e) : 0.0f);
-        const float d = in ? grad_score(s, hi, lo, lab, v0 + at.j0 + e) : 0.0f;
-        acc[e] = d;
-        split_half(d * (float)(1 << kGradExp), h[k], l[k]);
+      for (int g = 0; g < 8; g++) {
+        const float4 b4 = bs[half * 8 + g];
+        const float b[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const int e = 4 * g + k;
+          const float s = fmaf(acc[32 * half + e] * us.a, us.b, b[k]);
+          const float p = exp2_approx(((s - hi) - lo) * kLog2e);
+          d[e] = label == 0 ? 0.0f : p * (float)(1 << kGradExp);
+        }
       }
-      if (live && at.j0 + g * 8 < J) {                     // ld is a multiple of 8
-        *reinterpret_cast<uint4*>(row + g * 8) = *reinterpret_cast<uint4*>(h);
-        *reinterpret_cast<uint4*>(row + plane + g * 8) = *reinterpret_cast<uint4*>(l);
+      if (hit >> 5 == half) {
+#pragma unroll
+        for (int e = 0; e < 32; e++)
+          if ((hit & 31) == e) d[e] -= (float)(1 << kGradExp);
       }
+      if (in < 64) {
+#pragma unroll
+        for (int e = 0; e < 32; e++)
+          if (32 * half + e >= in) d[e] = 0.0f;
+      }
+      uint32_t w[32];                                          // 4 groups of the first plane, 4 of the second
+#pragma unroll
+      for (int k = 0; k < 16; k++) {
+        const __half2 h = __floats2half2_rn(d[2 * k], d[2 * k + 1]);
+        const float2 f = __half22float2(h);
+        const __half2 l = __floats2half2_rn(d[2 * k] - f.x, d[2 * k + 1] - f.y);
+        w[k] = *reinterpret_cast<const uint32_t*>(&h);
+        w[16 + k] = *reinterpret_cast<const uint32_t*>(&l);
+      }
+      if (db_part) at.sh->colsum[at.row >> 5][at.quarter * 64 + half * 32 + lane] = lane_sum(d);
+      transpose8(w);
+#pragma unroll
+      for (int q = 0; q < 8; q++)
+        if (col + half * 32 < J && row0 + q < N)               // ld is a multiple of 8
+          *reinterpret_cast<uint4*>(out + half * 32 + q * ld) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
     }
     if (db_part) {
-      const float2 c = lane_sums(acc);
-      const int lane = threadIdx.x & 31, q = at.row >> 5;
-      *reinterpret_cast<float2*>(&at.sh->colsum[q][at.quarter * 64 + 2 * lane]) = c;
       epi_sync();
-      const int col = threadIdx.x;
-      if (col < kTN) {
-        const int64_t j = (int64_t)at.jt * kTN + col;
+      const int c = threadIdx.x;
+      if (c < kTN) {
+        const int64_t j = (int64_t)at.jt * kTN + c;
         if (j < J)
-          db_part[(int64_t)at.it * J + j] =
-              (at.sh->colsum[0][col] + at.sh->colsum[1][col]) + (at.sh->colsum[2][col] + at.sh->colsum[3][col]);
+          db_part[(int64_t)at.it * J + j] = ((at.sh->colsum[0][c] + at.sh->colsum[1][c]) +
+                                             (at.sh->colsum[2][c] + at.sh->colsum[3][c])) * (1.0f / (1 << kGradExp));
       }
     }
   }
@@ -478,29 +550,42 @@ struct MmaStore {
   int64_t I, J, ld, part;      // part: elements between the parts' results (0: there is one)
   int add;
   GradScale<float> g;
+  __device__ __forceinline__ void stage(int64_t, float*) const {}
   __device__ __forceinline__ void operator()(float (&acc)[64], const TileAt& at) const {
-    if (at.i >= I) return;
     const Unscale us = unscale(exps[which] + kGradExp);
     const float f = part ? 1.0f : g.value();
-    float* p = out + at.split * part + at.i * ld + at.j0;
-    if (at.j0 + 64 <= J && ((uintptr_t)p & 15) == 0) {
+    const int lane = threadIdx.x & 31, r8 = lane & 7;
+    const int64_t row0 = at.i - lane + (lane & ~7);
+    float* base = out + at.split * part;
+    const bool wide = (ld & 3) == 0 && ((uintptr_t)base & 15) == 0;
 #pragma unroll
-      for (int e = 0; e < 64; e += 4) {
-        float4 v = make_float4(us(acc[e]) * f, us(acc[e + 1]) * f, us(acc[e + 2]) * f, us(acc[e + 3]) * f);
-        float4* q = reinterpret_cast<float4*>(p + e);
-        if (add) {
-          const float4 o = *q;
-          v = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
+    for (int h = 0; h < 2; h++) {
+      uint32_t w[32];
+#pragma unroll
+      for (int e = 0; e < 32; e++) w[e] = __float_as_uint(acc[32 * h + e] * us.a * us.b * f);
+      transpose8(w);
+      const int64_t j = at.j0 + 32 * h + 4 * r8;
+      float* p = base + row0 * ld + j;
+#pragma unroll
+      for (int q = 0; q < 8; q++) {
+        if (row0 + q >= I) break;
+        float v[4];
+#pragma unroll
+        for (int c = 0; c < 4; c++) v[c] = __uint_as_float(w[4 * q + c]);
+        float* d = p + q * ld;
+        if (wide && j + 4 <= J) {
+          float4 o = make_float4(v[0], v[1], v[2], v[3]);
+          if (add) {
+            const float4 t = *reinterpret_cast<const float4*>(d);
+            o = make_float4(t.x + o.x, t.y + o.y, t.z + o.z, t.w + o.w);
+          }
+          *reinterpret_cast<float4*>(d) = o;
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; c++)
+            if (j + c < J) d[c] = add ? d[c] + v[c] : v[c];
         }
-        *q = v;
       }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 64; e++)
-        if (at.j0 + e < J) {
-          const float v = us(acc[e]) * f;
-          p[e] = add ? p[e] + v : v;
-        }
     }
   }
 };

@@ -162,6 +162,25 @@ def test_masked_classes_and_bad_values(K, dtype, shape):
         c.labels[7] = 1
 
 
+@pytest.mark.parametrize("shape", [(300, 40, 50), (1000, 128, 300)], ids=str)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+def test_every_class_masked(K, dtype, shape):
+    """Masked by the type's lowest value, the softmax is uniform and the loss log V, as the score
+    matrix's logsoftmax gives; masked by -inf, NaN."""
+    c = Case(*shape, dtype, False, True, False)
+    c.b[:] = torch.finfo(dtype).min
+    kw, kx, kb = c.arrays(K)
+    res = K.ops.linear_nll_device(kw, kx, c.labels, b=kb)
+    tol = 1e-6 if dtype == torch.float32 else 1e-14
+    assert bool(((res.per_instance[:c.N] - math.log(c.V)).abs() <= tol * math.log(c.V)).all())
+    db = K.ops.linear_nll_back(kw, kx, res, b=kb)[2].data.double()
+    want = 1.0 / c.V - torch.bincount(c.labels.long() - 1, minlength=c.V).double() / c.N
+    assert bool(((db - want).abs() <= (16 * c.N + 32) * 2 * U[dtype] * (1.0 / c.V + want.abs())).all())
+    c.b[:] = -math.inf
+    res = K.ops.linear_nll_device(kw, kx, c.labels, b=K.KnetArray(c.b, (c.V,)))
+    assert bool(torch.isnan(res.per_instance[:c.N]).all())
+
+
 def test_labels_out_of_range_make_the_loss_nan(K):
     for bad in (-1, 301, 2 ** 31 - 1):
         c = Case(300, 40, 50, torch.float32, False, False, False)

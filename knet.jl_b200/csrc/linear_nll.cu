@@ -11,72 +11,11 @@
 // instance), so that p = exp((s - hi) - lo).
 #include "linear_nll.cuh"
 #include "linear_nll_mma.cuh"
+#include "linear_nll_small.cuh"
 
 namespace kn {
 
-// ---- matrix products on the FMA pipe ---------------------------------------------------------------
-// acc(i, j) = sum_c A(i, c) * B(j, c) for a 64x64 tile of (i, j), 4x4 per thread, c in steps of 16
-// through shared memory.  Operands have any strides with one of the two equal to 1.  Used for
-// Float64 and as the Float32 form where tensor-core tiles do not pay.
-template <typename T> struct Strided {
-  const T* p;
-  int64_t si, sc;      // element (i, c) at p + i*si + c*sc
-};
-
-constexpr int kTile = 64, kStep = 16, kSimtThreads = 256;
-
-template <typename T>
-__device__ __forceinline__ void simt_load(T (&dst)[kStep][kTile + 4], const Strided<T>& a, int64_t i0, int64_t c0, int64_t I,
-                                          int64_t C) {
-#pragma unroll
-  for (int r = 0; r < 4; r++) {
-    int i, c;
-    if (a.sc == 1) {          // neighbouring threads walk the contiguous axis
-      c = threadIdx.x % kStep;
-      i = threadIdx.x / kStep + 16 * r;
-    } else {
-      i = threadIdx.x % kTile;
-      c = threadIdx.x / kTile + 4 * r;
-    }
-    T v = (T)0;
-    if (i0 + i < I && c0 + c < C) v = a.p[(i0 + i) * a.si + (c0 + c) * a.sc];
-    dst[c][i] = v;
-  }
-}
-
-template <typename T, typename Epi>
-__global__ void __launch_bounds__(kSimtThreads)
-simt_product_kernel(Strided<T> a, Strided<T> b, int64_t I, int64_t J, int64_t C, Epi epi) {
-  __shared__ __align__(16) T as[kStep][kTile + 4];
-  __shared__ __align__(16) T bs[kStep][kTile + 4];
-  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-  const int64_t i0 = (int64_t)blockIdx.y * kTile, j0 = (int64_t)blockIdx.x * kTile;
-  T acc[4][4];
-#pragma unroll
-  for (int u = 0; u < 4; u++)
-#pragma unroll
-    for (int w = 0; w < 4; w++) acc[u][w] = (T)0;
-  for (int64_t c0 = 0; c0 < C; c0 += kStep) {
-    simt_load<T>(as, a, i0, c0, I, C);
-    simt_load<T>(bs, b, j0, c0, J, C);
-    __syncthreads();
-#pragma unroll
-    for (int c = 0; c < kStep; c++) {
-      T av[4], bv[4];
-#pragma unroll
-      for (int u = 0; u < 4; u++) av[u] = as[c][ty * 4 + u];
-#pragma unroll
-      for (int w = 0; w < 4; w++) bv[w] = bs[c][tx * 4 + w];
-#pragma unroll
-      for (int u = 0; u < 4; u++)
-#pragma unroll
-        for (int w = 0; w < 4; w++) acc[u][w] = Math<T>::fma(av[u], bv[w], acc[u][w]);
-    }
-    __syncthreads();
-  }
-  epi(acc, i0 + ty * 4, j0 + tx * 4, I, J);
-}
-
+// ---- pieces of the vocabulary on FMA tiles (what the other forms leave: many Float64 scores) ------------
 // i = instance, j = class: the tile's maximum and sum of exponentials per instance, and the score at
 // the label.  The 16 threads of an instance row are neighbours in a half warp.
 template <typename T> struct StatsEpi {
@@ -133,28 +72,6 @@ template <typename T> struct GradScoresEpi {
         if (j0 + w >= J) break;
         const T s = acc[u][w] + (bias ? bias[j0 + w] : (T)0);
         ds[i * ld + j0 + w] = grad_score(s, hi, lo, lab, v0 + j0 + w);
-      }
-    }
-  }
-};
-
-// out(i, j) (+)= g * acc
-template <typename T> struct StoreEpi {
-  T* out;
-  int64_t ld;
-  int add;
-  GradScale<T> g;
-  __device__ __forceinline__ void operator()(T (&acc)[4][4], int64_t i0, int64_t j0, int64_t I, int64_t J) const {
-    const T f = g.value();
-#pragma unroll
-    for (int u = 0; u < 4; u++) {
-      if (i0 + u >= I) break;
-#pragma unroll
-      for (int w = 0; w < 4; w++) {
-        if (j0 + w >= J) break;
-        T* p = out + (i0 + u) * ld + j0 + w;
-        const T v = acc[u][w] * f;
-        *p = add ? *p + v : v;
       }
     }
   }
@@ -278,12 +195,66 @@ template <typename T> int64_t simt_piece(int64_t V, int64_t N) {
   return v < V ? v : V;
 }
 
-// ---- plan of the tensor-core form (Float32) --------------------------------------------------------------
+constexpr int kPlanSMs = 148;
+
+// ---- plans; the tensor-core form (Float32) --------------------------------------------------------------
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// The tensor-core form pays from a few million products on; below, its launches cost more.
-template <typename T> bool use_mma(int64_t V, int64_t H, int64_t N) {
-  return sizeof(T) == 4 && N >= 32 && V >= 64 && H >= 16 && (double)V * H * N >= (double)(1 << 24);
+// Which form a call takes.
+//   kSmall   up to 2^24 scores and either few instances or little work: the scores go to the workspace
+//   kMma     Float32 beyond that
+//   kPieces  the rest (Float64 with many scores)
+// Few instances: kSmall reads W once per 16 instances, kMma about four times whatever their number (the
+// scale, the split, the product) and needs five launches.
+enum Form { kSmall, kMma, kPieces };
+constexpr int64_t kFewInstances = 48;
+template <typename T> Form form(int64_t V, int64_t H, int64_t N) {
+  const bool fits = N * V <= (1 << 24);
+  if (fits && N <= kFewInstances) return kSmall;
+  if (sizeof(T) == 4 && ((double)V * H * N >= (double)(1 << 26) || !fits)) return kMma;
+  return fits && (double)V * H * N < (double)(1ll << 32) ? kSmall : kPieces;
+}
+
+// Parts of the summed axes of the three products in kSmall: enough CTAs for two per SM, parts of at
+// least 64 (tiles) or 256 (few instances) terms, at most 64 parts.
+struct SmallPlan {
+  int64_t few, s_part, x_part, w_part;         // few: by vectors, not tiles; lengths of the parts
+  int s_parts, x_parts, w_parts;
+  size_t done, scores, parts, total;
+};
+template <typename T> SmallPlan small_plan(int64_t V, int64_t H, int64_t N, int trans, int backward) {
+  SmallPlan p{};
+  p.few = N <= 16 || (N <= kFewInstances && V * H >= (1 << 21));
+  const int64_t nb = sizeof(T) == 8 ? 8 : 16;
+  auto cut = [&](int64_t ctas, int64_t len, int64_t unit, int64_t bytes, int64_t& part, int& parts) {
+    int64_t k = (2 * kPlanSMs + ctas - 1) / ctas;
+    k = k > len / unit ? len / unit : k;
+    k = k > 64 ? 64 : k;
+    k = k > (64 << 20) / (bytes + 1) ? (64 << 20) / (bytes + 1) : k;
+    k = k < 1 ? 1 : k;
+    part = ceil_div(ceil_div(len, k), unit) * unit;
+    parts = (int)ceil_div(len, part);
+  };
+  const int64_t sz = sizeof(T), ntile = ceil_div(N, kTile), groups = ceil_div(N, nb);
+  if (p.few) {
+    cut(ceil_div(V, trans ? 32 : 128) * groups, H, 256, N * V * sz, p.s_part, p.s_parts);
+    cut(ceil_div(H, trans ? 128 : 32) * groups, V, 256, N * H * sz, p.x_part, p.x_parts);
+    p.w_parts = 1;
+  } else {
+    cut(ntile * ceil_div(V, kTile), H, 64, N * V * sz, p.s_part, p.s_parts);
+    cut(ntile * ceil_div(H, kTile), V, 64, N * H * sz, p.x_part, p.x_parts);
+    cut(ceil_div(V, kTile) * ceil_div(H, kTile), N, 64, V * H * sz, p.w_part, p.w_parts);
+  }
+  size_t at = up(4);
+  p.scores = at;
+  at += up((size_t)p.s_parts * N * V * sz);
+  p.parts = at;
+  if (backward) {
+    const size_t x = (size_t)p.x_parts * N * H * sz, w = p.w_parts > 1 ? (size_t)p.w_parts * V * H * sz : 0;
+    at += up(x > w ? x : w);
+  }
+  p.total = at;
+  return p;
 }
 
 // Pieces of the vocabulary and parts of dx's sum.  Workspace bounds: 256 MB of split weights in the
@@ -295,8 +266,6 @@ struct MmaPlan {
   int splits;                          // parts of dx's sum over a piece
   size_t exps, absmax, xs, ws, label, part_m, part_s, ds, parts, db, total;
 };
-constexpr int kPlanSMs = 148;
-
 inline MmaPlan mma_plan(int64_t V, int64_t H, int64_t N, int trans, int backward) {
   MmaPlan p{};
   const int64_t all = ceil_div(V, kTN);
@@ -349,7 +318,9 @@ inline MmaPlan mma_plan(int64_t V, int64_t H, int64_t N, int trans, int backward
 }
 
 template <typename T> size_t workspace(int64_t V, int64_t H, int64_t N, int trans, int backward) {
-  if (use_mma<T>(V, H, N)) return mma_plan(V, H, N, trans, backward).total;
+  const Form f = form<T>(V, H, N);
+  if (f == kMma) return mma_plan(V, H, N, trans, backward).total;
+  if (f == kSmall) return small_plan<T>(V, H, N, trans, backward).total;
   if (backward) return up((size_t)N * simt_piece<T>(V, N) * sizeof(T));
   const int64_t tiles = (V + kTile - 1) / kTile;
   return up((size_t)N * sizeof(T)) + 2 * up((size_t)tiles * N * sizeof(T));
@@ -360,9 +331,41 @@ template <typename T> size_t workspace_any(int64_t V, int64_t H, int64_t N, int 
 }
 
 template <typename T, typename Epi>
-void simt_product(Strided<T> a, Strided<T> b, int64_t I, int64_t J, int64_t C, Epi epi, cudaStream_t st) {
-  const dim3 grid((unsigned)((J + kTile - 1) / kTile), (unsigned)((I + kTile - 1) / kTile));
-  simt_product_kernel<T, Epi><<<grid, kSimtThreads, 0, st>>>(a, b, I, J, C, epi);
+void simt_product(Strided<T> a, Strided<T> b, int64_t I, int64_t J, int64_t C, int64_t c_part, uint32_t* done, Epi epi, cudaStream_t st) {
+  const dim3 grid((unsigned)ceil_div(J, kTile), (unsigned)ceil_div(I, kTile), (unsigned)ceil_div(C, c_part));
+  simt_product_kernel<T, Epi><<<grid, kSimtThreads, 0, st>>>(a, b, I, J, C, c_part, done, epi);
+}
+
+// packs of VEC elements are possible where base addresses and pitches are multiples of 16 bytes
+template <typename T> bool aligned16(const T* p, int64_t pitch) {
+  return ((uintptr_t)p & 15) == 0 && pitch * (int64_t)sizeof(T) % 16 == 0;
+}
+
+// parts of sum_c M(r, c) y(n, c) (by_row) or sum_r M(r, c) y(n, r)
+template <typename T, int NB>
+void few_product_nb(bool by_row, const Matrix<T>& m, const T* y, int64_t ldy, int64_t N, int64_t part, int parts, uint32_t* done, T* out,
+                    cudaStream_t st) {
+  constexpr int VEC = 16 / sizeof(T);
+  const unsigned groups = (unsigned)ceil_div(N, NB);
+  const bool wide = aligned16(m.p, m.pitch) && m.cols % VEC == 0;
+  if (by_row) {
+    const dim3 grid((unsigned)ceil_div(m.rows, 32), groups, (unsigned)parts);
+    if (wide && aligned16(y, ldy)) row_dot_kernel<T, NB, VEC><<<grid, 256, 0, st>>>(m, y, ldy, N, part, done, out);
+    else row_dot_kernel<T, NB, 1><<<grid, 256, 0, st>>>(m, y, ldy, N, part, done, out);
+  } else {
+    const dim3 grid((unsigned)ceil_div(m.cols, 128), groups, (unsigned)parts);
+    if (wide) col_sum_kernel<T, NB, VEC><<<grid, 256, 0, st>>>(m, y, ldy, N, part, done, out);
+    else col_sum_kernel<T, NB, 1><<<grid, 256, 0, st>>>(m, y, ldy, N, part, done, out);
+  }
+}
+template <typename T>
+void few_product(bool by_row, const Matrix<T>& m, const T* y, int64_t ldy, int64_t N, int64_t part, int parts, uint32_t* done, T* out,
+                 cudaStream_t st) {
+  if (N == 1) few_product_nb<T, 1>(by_row, m, y, ldy, N, part, parts, done, out, st);
+  else if (N == 2) few_product_nb<T, 2>(by_row, m, y, ldy, N, part, parts, done, out, st);
+  else if (N <= 4) few_product_nb<T, 4>(by_row, m, y, ldy, N, part, parts, done, out, st);
+  else if (N <= 8 || sizeof(T) == 8) few_product_nb<T, 8>(by_row, m, y, ldy, N, part, parts, done, out, st);
+  else if constexpr (sizeof(T) == 4) few_product_nb<T, 16>(by_row, m, y, ldy, N, part, parts, done, out, st);
 }
 
 // sizes whose tile counts fit a launch grid (features are rows of a tile grid in dW)
@@ -501,21 +504,96 @@ inline int linear_nll_bwd_mma(const Head<float>& h, const float* lse, GradScale<
   return launch_status();
 }
 
+// ---- few scores -----------------------------------------------------------------------------------------
+template <typename T> Matrix<T> weight_matrix(const Head<T>& h) {
+  return h.trans ? Matrix<T>{h.w, h.V, h.H, h.H} : Matrix<T>{h.w, h.H, h.V, h.V};
+}
+template <typename T> void small_scores(const Head<T>& h, const SmallPlan& p, uint32_t* done, T* scores, cudaStream_t st) {
+  if (p.few) few_product<T>(h.trans, weight_matrix(h), h.x, h.H, h.N, p.s_part, p.s_parts, done, scores, st);
+  else
+    simt_product<T>(Strided<T>{h.x, h.H, 1}, h.weights(0), h.N, h.V, h.H, p.s_part, done, PartsEpi<T>{scores}, st);
+}
+
+template <typename T>
+int linear_nll_fwd_small(const Head<T>& h, T* total, int32_t* count, T* lse, T* per_instance, char* ws, cudaStream_t st) {
+  const SmallPlan p = small_plan<T>(h.V, h.H, h.N, h.trans, 0);
+  uint32_t* done = (uint32_t*)ws;
+  T* scores = (T*)(ws + p.scores);
+  small_scores(h, p, done, scores, st);
+#define KN_ROWS(GROUP, THREADS)                                                                                      \
+  lnll_rows_kernel<T, GROUP><<<(unsigned)ceil_div(h.N, THREADS / GROUP), THREADS, 0, st>>>(scores, p.s_parts, h.bias, \
+                                                                          h.labels, h.N, h.V, lse, per_instance, total, count, done)
+  if (h.V <= 512) KN_ROWS(32, 256);
+  else if (h.V <= 8192) KN_ROWS(256, 256);
+  else KN_ROWS(1024, 1024);
+#undef KN_ROWS
+  return launch_status();
+}
+
+// out (contiguous I x J) = g * sum_c A(i, c) B(j, c) by tiles, through `parts` when the sum is cut
+template <typename T>
+void tile_product_out(Strided<T> a, Strided<T> b, int64_t I, int64_t J, int64_t C, int64_t c_part, int cuts, T* out, T* parts,
+                      GradScale<T> g, cudaStream_t st) {
+  if (cuts == 1) {
+    simt_product<T>(a, b, I, J, C, c_part, nullptr, StoreEpi<T>{out, J, 0, g}, st);
+    return;
+  }
+  simt_product<T>(a, b, I, J, C, c_part, nullptr, PartsEpi<T>{parts}, st);
+  lnll_sum_kernel<T><<<(unsigned)ceil_div(I * J, 256), 256, 0, st>>>(parts, I * J, cuts, out, 0, g);
+}
+
+template <typename T>
+int linear_nll_bwd_small(const Head<T>& h, const T* lse, GradScale<T> g, T* dw, T* db, T* dx, char* ws, cudaStream_t st) {
+  const SmallPlan p = small_plan<T>(h.V, h.H, h.N, h.trans, 1);
+  T *ds = (T*)(ws + p.scores), *parts = (T*)(ws + p.parts);
+  small_scores(h, p, nullptr, ds, st);
+  const int64_t blocks = ceil_div(h.V, 1024);
+  lnll_grad_kernel<T><<<(unsigned)(blocks * h.N), 256, 0, st>>>(ds, p.s_parts, h.bias, h.labels, lse, h.N, h.V, (uint32_t)blocks);
+  if (db) lnll_bias_kernel<T><<<(unsigned)ceil_div(h.V, 32), 1024, 0, st>>>(ds, h.V, h.N, h.V, db, g);
+  const Matrix<T> m = weight_matrix(h);
+  if (dx) {
+    if (p.few) {
+      few_product<T>(!h.trans, m, ds, h.V, h.N, p.x_part, p.x_parts, nullptr, parts, st);
+      lnll_sum_kernel<T><<<(unsigned)ceil_div(h.N * h.H, 256), 256, 0, st>>>(parts, h.N * h.H, p.x_parts, dx, 0, g);
+    } else {
+      const Strided<T> w = h.weights(0);
+      tile_product_out<T>(Strided<T>{ds, h.V, 1}, Strided<T>{w.p, w.sc, w.si}, h.N, h.H, h.V, p.x_part, p.x_parts, dx, parts, g, st);
+    }
+  }
+  if (dw) {
+    const int64_t R = m.rows, C = m.cols;
+    // rows and columns of W in terms of (dS, x)
+    const T *a = h.trans ? ds : h.x, *b = h.trans ? h.x : ds;
+    const int64_t lda = h.trans ? h.V : h.H, ldb = h.trans ? h.H : h.V;
+    if (p.few) {
+      constexpr int VEC = 16 / sizeof(T);
+      const dim3 grid((unsigned)ceil_div(R, 16), (unsigned)ceil_div(C, 128));
+      if (aligned16(b, ldb) && aligned16(dw, C)) outer_kernel<T, VEC><<<grid, 256, 0, st>>>(a, lda, b, ldb, h.N, R, C, dw, C, g);
+      else outer_kernel<T, 1><<<grid, 256, 0, st>>>(a, lda, b, ldb, h.N, R, C, dw, C, g);
+    } else {
+      tile_product_out<T>(Strided<T>{a, 1, lda}, Strided<T>{b, 1, ldb}, R, C, h.N, p.w_part, p.w_parts, dw, parts, g, st);
+    }
+  }
+  return launch_status();
+}
+
 template <typename T>
 int linear_nll_fwd(const Head<T>& h, T* total, int32_t* count, T* lse, T* per_instance, void* ws, size_t have, cudaStream_t st) {
   if (!total || !count || (h.N > 0 && (!lse || !per_instance))) return KN_EINVAL;
   if (odd(total) || odd(lse) || odd(per_instance) || (uintptr_t)count % 4) return KN_EALIGN;
   const size_t need = h.V > 0 && h.H > 0 && h.N > 0 && sizes_ok(h.V, h.H, h.N) ? workspace_any<T>(h.V, h.H, h.N, 0) : 0;
   if (int rc = check(h, ws, have, need)) return rc;
-  if constexpr (sizeof(T) == 4)
-    if (use_mma<T>(h.V, h.H, h.N)) return linear_nll_fwd_mma(h, total, count, lse, per_instance, (char*)ws, st);
   if (h.N > 0) {
+    const Form f = form<T>(h.V, h.H, h.N);
+    if constexpr (sizeof(T) == 4)
+      if (f == kMma) return linear_nll_fwd_mma(h, total, count, lse, per_instance, (char*)ws, st);
+    if (f == kSmall) return linear_nll_fwd_small<T>(h, total, count, lse, per_instance, (char*)ws, st);
     const int64_t tiles = (h.V + kTile - 1) / kTile;
     char* p = (char*)ws;
     T* label_score = (T*)p;
     T* part_m = (T*)(p += up((size_t)h.N * sizeof(T)));
     T* part_s = (T*)(p += up((size_t)tiles * h.N * sizeof(T)));
-    simt_product<T>(Strided<T>{h.x, h.H, 1}, h.weights(0), h.N, h.V, h.H,
+    simt_product<T>(Strided<T>{h.x, h.H, 1}, h.weights(0), h.N, h.V, h.H, h.H, nullptr,
                     StatsEpi<T>{h.bias, h.labels, part_m, part_s, label_score, h.N}, st);
     lnll_join_kernel<T><<<(unsigned)((h.N + 31) / 32), 256, 0, st>>>(part_m, part_s, label_score, h.labels, h.N, h.V, tiles, lse,
                                                                    per_instance);
@@ -537,22 +615,24 @@ int linear_nll_bwd(const Head<T>& h, const T* lse, int average, T dy, const int3
     return launch_status();
   }
   const GradScale<T> g{average ? count : nullptr, dy};
+  const Form f = form<T>(h.V, h.H, h.N);
   if constexpr (sizeof(T) == 4)
-    if (use_mma<T>(h.V, h.H, h.N)) return linear_nll_bwd_mma(h, lse, g, dw, db, dx, (char*)ws, st);
+    if (f == kMma) return linear_nll_bwd_mma(h, lse, g, dw, db, dx, (char*)ws, st);
+  if (f == kSmall) return linear_nll_bwd_small<T>(h, lse, g, dw, db, dx, (char*)ws, st);
   const int64_t piece = simt_piece<T>(h.V, h.N);
   T* ds = (T*)ws;
   for (int64_t v0 = 0; v0 < h.V; v0 += piece) {
     const int64_t vp = h.V - v0 < piece ? h.V - v0 : piece;
     const Strided<T> w = h.weights(v0);
-    simt_product<T>(Strided<T>{h.x, h.H, 1}, w, h.N, vp, h.H,
+    simt_product<T>(Strided<T>{h.x, h.H, 1}, w, h.N, vp, h.H, h.H, nullptr,
                     GradScoresEpi<T>{h.bias ? h.bias + v0 : nullptr, h.labels, lse, ds, h.N, piece, v0}, st);
     if (db) lnll_bias_kernel<T><<<(unsigned)((vp + 31) / 32), 1024, 0, st>>>(ds, piece, h.N, vp, db + v0, g);
     if (dx)
-      simt_product<T>(Strided<T>{ds, piece, 1}, Strided<T>{w.p, w.sc, w.si}, h.N, h.H, vp, StoreEpi<T>{dx, h.H, v0 > 0, g}, st);
+      simt_product<T>(Strided<T>{ds, piece, 1}, Strided<T>{w.p, w.sc, w.si}, h.N, h.H, vp, vp, nullptr, StoreEpi<T>{dx, h.H, v0 > 0, g}, st);
     if (dw && h.trans)
-      simt_product<T>(Strided<T>{ds, 1, piece}, Strided<T>{h.x, 1, h.H}, vp, h.H, h.N, StoreEpi<T>{dw + v0 * h.H, h.H, 0, g}, st);
+      simt_product<T>(Strided<T>{ds, 1, piece}, Strided<T>{h.x, 1, h.H}, vp, h.H, h.N, h.N, nullptr, StoreEpi<T>{dw + v0 * h.H, h.H, 0, g}, st);
     else if (dw)
-      simt_product<T>(Strided<T>{h.x, 1, h.H}, Strided<T>{ds, 1, piece}, h.H, vp, h.N, StoreEpi<T>{dw + v0, h.V, 0, g}, st);
+      simt_product<T>(Strided<T>{h.x, 1, h.H}, Strided<T>{ds, 1, piece}, h.H, vp, h.N, h.N, nullptr, StoreEpi<T>{dw + v0, h.V, 0, g}, st);
   }
   return launch_status();
 }

@@ -1,0 +1,493 @@
+// The linear-layer cross entropy where the instances times the classes are few: the scores fit a small
+// workspace, so a product leaves them there and a second kernel takes softmax statistics or gradients
+// from them.  Which product depends on what bounds it:
+//   few instances    W is read once at memory speed (row_dot or col_sum, by W's layout); tiles would
+//                    waste all but a few of their rows
+//   few outputs      64x64 tiles on the FMA pipe (Float64: on the FP64 tensor instruction) with the
+//                    summed axis split over CTAs, as there are too few tiles for the SMs
+// All of them leave sums as `parts`: [part of the summed axis][instance][column], added in order by
+// the kernel that reads them.
+#pragma once
+#include "linear_nll.cuh"
+
+namespace kn {
+
+template <typename T> struct Strided {
+  const T* p;
+  int64_t si, sc;      // element (i, c) at p + i*si + c*sc
+};
+
+// the counter of the statistics kernel that follows in the stream
+__device__ __forceinline__ void clear_done(uint32_t* done) {
+  if (done && threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) *done = 0;
+}
+
+// ---- tiles ---------------------------------------------------------------------------------------
+// acc(i, j) = sum_c A(i, c) * B(j, c) over a part of c, for a 64x64 tile of (i, j), c in steps of 16
+// through shared memory, the next step's operands loaded into registers meanwhile.  Operands have any
+// strides with one of the two equal to 1.
+constexpr int kTile = 64, kStep = 16, kSimtThreads = 256;
+
+template <typename T>
+__device__ __forceinline__ void tile_fetch(T (&reg)[4], const Strided<T>& a, int64_t i0, int64_t c0, int64_t I, int64_t C) {
+#pragma unroll
+  for (int r = 0; r < 4; r++) {
+    // neighbouring threads walk the contiguous axis
+    const int i = a.sc == 1 ? threadIdx.x / kStep + 16 * r : threadIdx.x % kTile;
+    const int c = a.sc == 1 ? threadIdx.x % kStep : threadIdx.x / kTile + 4 * r;
+    reg[r] = i0 + i < I && c0 + c < C ? a.p[(i0 + i) * a.si + (c0 + c) * a.sc] : (T)0;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void tile_put(T (&dst)[kStep][kTile + 4], const T (&reg)[4], bool c_contiguous) {
+#pragma unroll
+  for (int r = 0; r < 4; r++) {
+    if (c_contiguous) dst[threadIdx.x % kStep][threadIdx.x / kStep + 16 * r] = reg[r];
+    else dst[threadIdx.x / kTile + 4 * r][threadIdx.x % kTile] = reg[r];
+  }
+}
+
+// D += A * B for 8 x 8 doubles, 4 summed indices, by one warp: lane holds A(lane/4, lane%4),
+// B(lane%4, lane/4) and D(lane/4, 2*(lane%4) + {0, 1})
+__device__ __forceinline__ void dmma(double (&d)[2], double a, double b) {
+  asm("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};" : "+d"(d[0]), "+d"(d[1]) : "d"(a), "d"(b));
+}
+
+template <typename T> struct TileShared {
+  union {
+    struct {
+      T a[2][kStep][kTile + 4], b[2][kStep][kTile + 4];
+    } in;
+    T out[kTile][kTile + 1];
+  };
+};
+
+template <typename T, typename Epi>
+__global__ void __launch_bounds__(kSimtThreads)
+simt_product_kernel(Strided<T> a, Strided<T> b, int64_t I, int64_t J, int64_t C, int64_t c_part, uint32_t* done, Epi epi) {
+  clear_done(done);
+  __shared__ __align__(16) TileShared<T> sh;
+  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+  const int64_t i0 = (int64_t)blockIdx.y * kTile, j0 = (int64_t)blockIdx.x * kTile;
+  const int64_t c_lo = (int64_t)blockIdx.z * c_part, c_hi = min(C, c_lo + c_part);
+  T acc[4][4];
+#pragma unroll
+  for (int u = 0; u < 4; u++)
+#pragma unroll
+    for (int w = 0; w < 4; w++) acc[u][w] = (T)0;
+  // Float64: warp w owns rows 32*(w%2).. and columns 16*(w/2).. as 4 x 2 blocks of 8 x 8
+  const int lane = threadIdx.x & 31, wr = (threadIdx.x >> 5 & 1) * 32, wc = (threadIdx.x >> 6) * 16;
+  T ra[4], rb[4];
+  tile_fetch<T>(ra, a, i0, c_lo, I, c_hi);
+  tile_fetch<T>(rb, b, j0, c_lo, J, c_hi);
+  int buf = 0;
+  for (int64_t c0 = c_lo; c0 < c_hi; c0 += kStep, buf ^= 1) {
+    tile_put<T>(sh.in.a[buf], ra, a.sc == 1);
+    tile_put<T>(sh.in.b[buf], rb, b.sc == 1);
+    __syncthreads();
+    if (c0 + kStep < c_hi) {
+      tile_fetch<T>(ra, a, i0, c0 + kStep, I, c_hi);
+      tile_fetch<T>(rb, b, j0, c0 + kStep, J, c_hi);
+    }
+    if constexpr (sizeof(T) == 8) {
+#pragma unroll
+      for (int c = 0; c < kStep; c += 4) {
+        double av[4], bv[2];
+#pragma unroll
+        for (int u = 0; u < 4; u++) av[u] = sh.in.a[buf][c + (lane & 3)][wr + 8 * u + (lane >> 2)];
+#pragma unroll
+        for (int w = 0; w < 2; w++) bv[w] = sh.in.b[buf][c + (lane & 3)][wc + 8 * w + (lane >> 2)];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          dmma(reinterpret_cast<double(&)[2]>(acc[u][0]), av[u], bv[0]);
+          dmma(reinterpret_cast<double(&)[2]>(acc[u][2]), av[u], bv[1]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < kStep; c++) {
+        T av[4], bv[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) av[u] = sh.in.a[buf][c][ty * 4 + u];
+#pragma unroll
+        for (int w = 0; w < 4; w++) bv[w] = sh.in.b[buf][c][tx * 4 + w];
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+          for (int w = 0; w < 4; w++) acc[u][w] = Math<T>::fma(av[u], bv[w], acc[u][w]);
+      }
+    }
+  }
+  if constexpr (sizeof(T) == 8) {      // from the blocks to 4 x 4 per thread, as the epilogues expect it
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+#pragma unroll
+      for (int w = 0; w < 2; w++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) sh.out[wr + 8 * u + (lane >> 2)][wc + 8 * w + 2 * (lane & 3) + e] = acc[u][2 * w + e];
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+#pragma unroll
+      for (int w = 0; w < 4; w++) acc[u][w] = sh.out[ty * 4 + u][tx * 4 + w];
+  }
+  epi(acc, i0 + ty * 4, j0 + tx * 4, I, J);
+}
+
+// the sums of one part of c
+template <typename T> struct PartsEpi {
+  T* parts;
+  __device__ __forceinline__ void operator()(T (&acc)[4][4], int64_t i0, int64_t j0, int64_t I, int64_t J) const {
+    T* out = parts + (int64_t)blockIdx.z * I * J;
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+#pragma unroll
+      for (int w = 0; w < 4; w++)
+        if (i0 + u < I && j0 + w < J) out[(i0 + u) * J + j0 + w] = acc[u][w];
+  }
+};
+
+// out(i, j) (+)= g * acc
+template <typename T> struct StoreEpi {
+  T* out;
+  int64_t ld;
+  int add;
+  GradScale<T> g;
+  __device__ __forceinline__ void operator()(T (&acc)[4][4], int64_t i0, int64_t j0, int64_t I, int64_t J) const {
+    const T f = g.value();
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      if (i0 + u >= I) break;
+#pragma unroll
+      for (int w = 0; w < 4; w++) {
+        if (j0 + w >= J) break;
+        T* p = out + (i0 + u) * ld + j0 + w;
+        const T v = acc[u][w] * f;
+        *p = add ? *p + v : v;
+      }
+    }
+  }
+};
+
+// ---- few instances ------------------------------------------------------------------------------------
+// A matrix of `rows` rows of `cols` contiguous elements, pitch between rows, and NB vectors y.
+template <typename T> struct Matrix {
+  const T* p;
+  int64_t rows, cols, pitch;
+};
+
+template <typename T, int VEC> __device__ __forceinline__ Pack<T, VEC> ld_cached(const T* p) {
+  return *reinterpret_cast<const Pack<T, VEC>*>(p);
+}
+
+// parts[z part][n][row] = sum over a part of the columns of M(row, c) * y(n, c): a warp takes four
+// rows, its lanes the columns; the vectors come through L1.
+template <typename T, int NB, int VEC>
+__global__ void __launch_bounds__(256)
+row_dot_kernel(Matrix<T> m, const T* __restrict__ y, int64_t ldy, int64_t N, int64_t c_part, uint32_t* done, T* __restrict__ parts) {
+  clear_done(done);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t r0 = ((int64_t)blockIdx.x * 8 + warp) * 4;
+  const int64_t n0 = (int64_t)blockIdx.y * NB;
+  const int64_t c_lo = (int64_t)blockIdx.z * c_part, c_hi = min(m.cols, c_lo + c_part);
+  if (r0 >= m.rows) return;
+  T acc[4][NB];
+#pragma unroll
+  for (int r = 0; r < 4; r++)
+#pragma unroll
+    for (int n = 0; n < NB; n++) acc[r][n] = (T)0;
+  const T* row[4];
+#pragma unroll
+  for (int r = 0; r < 4; r++) row[r] = m.p + min(r0 + r, m.rows - 1) * m.pitch;
+  const T* yv[NB];
+#pragma unroll
+  for (int n = 0; n < NB; n++) yv[n] = y + min(n0 + n, N - 1) * ldy;
+  constexpr int UN = NB >= 8 ? 1 : 2;
+  for (int64_t c = c_lo + lane * VEC; c < c_hi; c += 32 * VEC * UN) {
+    Pack<T, VEC> w[UN][4];
+#pragma unroll
+    for (int u = 0; u < UN; u++)
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+        if (c + u * 32 * VEC < c_hi) w[u][r] = ld_stream<T, VEC>(row[r] + c + u * 32 * VEC);
+#pragma unroll
+    for (int u = 0; u < UN; u++)
+      if (c + u * 32 * VEC < c_hi) {
+#pragma unroll
+        for (int n = 0; n < NB; n++) {
+          const Pack<T, VEC> v = ld_cached<T, VEC>(yv[n] + c + u * 32 * VEC);
+#pragma unroll
+          for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int e = 0; e < VEC; e++) acc[r][n] = Math<T>::fma(w[u][r].v[e], v.v[e], acc[r][n]);
+        }
+      }
+  }
+#pragma unroll
+  for (int n = 0; n < NB; n++)
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      const T s = warp_reduce(acc[r][n], [](T a, T b) { return a + b; });
+      if (lane == 0 && r0 + r < m.rows && n0 + n < N) parts[((int64_t)blockIdx.z * N + n0 + n) * m.rows + r0 + r] = s;
+    }
+}
+
+// parts[z part][n][col] = sum over a part of the rows of M(r, col) * y(n, r): a CTA takes 128 columns,
+// its 8 warps share the rows; the vectors' entries come transposed through shared memory.
+constexpr int kColRows = 128;
+template <typename T, int NB, int VEC>
+__global__ void __launch_bounds__(256)
+col_sum_kernel(Matrix<T> m, const T* __restrict__ y, int64_t ldy, int64_t N, int64_t r_part, uint32_t* done, T* __restrict__ parts) {
+  clear_done(done);
+  constexpr int Q = 4 / VEC;                       // packs per thread: 4 columns
+  __shared__ __align__(16) T ys[kColRows][NB];
+  __shared__ __align__(16) T red[4][NB][128];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t j0 = (int64_t)blockIdx.x * 128, n0 = (int64_t)blockIdx.y * NB;
+  const int64_t r_lo = (int64_t)blockIdx.z * r_part, r_hi = min(m.rows, r_lo + r_part);
+  int64_t col[Q];
+  bool in[Q];
+#pragma unroll
+  for (int q = 0; q < Q; q++) {
+    col[q] = j0 + (lane + 32 * q) * VEC;
+    in[q] = col[q] < m.cols;                        // cols is a multiple of VEC where VEC > 1
+  }
+  T acc[NB][4];
+#pragma unroll
+  for (int n = 0; n < NB; n++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) acc[n][e] = (T)0;
+  for (int64_t rc = r_lo; rc < r_hi; rc += kColRows) {
+    __syncthreads();
+    for (int k = threadIdx.x; k < kColRows * NB; k += 256) {
+      const int n = k / kColRows, r = k % kColRows;
+      ys[r][n] = rc + r < r_hi && n0 + n < N ? y[(n0 + n) * ldy + rc + r] : (T)0;
+    }
+    __syncthreads();
+    constexpr int UN = 8;
+#pragma unroll 1
+    for (int u0 = warp; u0 < kColRows && rc + u0 < r_hi; u0 += 8 * UN) {
+      Pack<T, VEC> w[UN][Q];
+#pragma unroll
+      for (int u = 0; u < UN; u++)
+#pragma unroll
+        for (int q = 0; q < Q; q++) {
+          const int64_t r = rc + u0 + 8 * u;
+          if (in[q] && u0 + 8 * u < kColRows && r < r_hi) w[u][q] = ld_stream<T, VEC>(m.p + r * m.pitch + col[q]);
+          else
+#pragma unroll
+            for (int e = 0; e < VEC; e++) w[u][q].v[e] = (T)0;
+        }
+#pragma unroll
+      for (int u = 0; u < UN; u++) {
+        if (u0 + 8 * u >= kColRows || rc + u0 + 8 * u >= r_hi) break;
+#pragma unroll
+        for (int n = 0; n < NB; n++) {
+          const T v = ys[u0 + 8 * u][n];
+#pragma unroll
+          for (int q = 0; q < Q; q++)
+#pragma unroll
+            for (int e = 0; e < VEC; e++) acc[n][q * VEC + e] = Math<T>::fma(w[u][q].v[e], v, acc[n][q * VEC + e]);
+        }
+      }
+    }
+  }
+  // the warps' sums, the upper half of the warps handing over to the lower one in turn
+#pragma unroll
+  for (int h = 4; h > 0; h >>= 1) {
+    __syncthreads();
+    if (warp >= h && warp < 2 * h) {
+#pragma unroll
+      for (int n = 0; n < NB; n++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) red[warp - h][n][e * 32 + lane] = acc[n][e];
+    }
+    __syncthreads();
+    if (warp < h) {
+#pragma unroll
+      for (int n = 0; n < NB; n++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[n][e] += red[warp][n][e * 32 + lane];
+    }
+  }
+  if (warp == 0) {
+#pragma unroll
+    for (int n = 0; n < NB; n++)
+#pragma unroll
+      for (int q = 0; q < Q; q++)
+        if (in[q] && n0 + n < N)
+#pragma unroll
+          for (int e = 0; e < VEC; e++) parts[((int64_t)blockIdx.z * N + n0 + n) * m.cols + col[q] + e] = acc[n][q * VEC + e];
+  }
+}
+
+// out(r, c) = g * sum_n a(n, r) * b(n, c): few instances, bound by the stores.  A CTA takes 16 rows and
+// 128 columns, a warp two rows.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256)
+outer_kernel(const T* __restrict__ a, int64_t lda, const T* __restrict__ b, int64_t ldb, int64_t N, int64_t R, int64_t C,
+             T* __restrict__ out, int64_t ld, GradScale<T> g) {
+  constexpr int Q = 4 / VEC;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t r0 = (int64_t)blockIdx.x * 16 + warp * 2, j0 = (int64_t)blockIdx.y * 128;
+  if (r0 >= R) return;
+  const bool two = r0 + 1 < R;
+  T acc[2][4];
+#pragma unroll
+  for (int e = 0; e < 4; e++) acc[0][e] = acc[1][e] = (T)0;
+#pragma unroll 4
+  for (int64_t n = 0; n < N; n++) {
+    const T a0 = a[n * lda + r0], a1 = two ? a[n * lda + r0 + 1] : (T)0;
+#pragma unroll
+    for (int q = 0; q < Q; q++) {
+      const int64_t c = j0 + (lane + 32 * q) * VEC;
+      if (c < C) {
+        const Pack<T, VEC> v = ld_cached<T, VEC>(b + n * ldb + c);
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+          acc[0][q * VEC + e] = Math<T>::fma(a0, v.v[e], acc[0][q * VEC + e]);
+          acc[1][q * VEC + e] = Math<T>::fma(a1, v.v[e], acc[1][q * VEC + e]);
+        }
+      }
+    }
+  }
+  const T f = g.value();
+#pragma unroll
+  for (int q = 0; q < Q; q++) {
+    const int64_t c = j0 + (lane + 32 * q) * VEC;
+    if (c < C) {
+      Pack<T, VEC> v;
+#pragma unroll
+      for (int e = 0; e < VEC; e++) v.v[e] = acc[0][q * VEC + e] * f;
+      st_stream<T, VEC>(out + r0 * ld + c, v);
+      if (two) {
+#pragma unroll
+        for (int e = 0; e < VEC; e++) v.v[e] = acc[1][q * VEC + e] * f;
+        st_stream<T, VEC>(out + (r0 + 1) * ld + c, v);
+      }
+    }
+  }
+}
+
+// ---- from the scores ------------------------------------------------------------------------------------
+template <typename T> __device__ __forceinline__ T sum_parts(const T* p, int64_t stride, int parts) {
+  T s = p[0];
+  for (int k = 1; k < parts; k++) s += p[k * stride];
+  return s;
+}
+
+// lse and loss of each instance from the parts of its scores; GROUP threads (a warp or the CTA) per
+// instance.  The last CTA to finish adds the losses in a fixed order (`done` counts CTAs; the product
+// that ran before set it to 0).
+template <typename T, int GROUP>
+__global__ void __launch_bounds__(GROUP < 256 ? 256 : GROUP)
+lnll_rows_kernel(const T* __restrict__ scores, int parts, const T* __restrict__ bias, const int32_t* __restrict__ labels, int64_t N,
+                 int64_t V, T* __restrict__ lse, T* __restrict__ per_instance, T* __restrict__ total, int32_t* __restrict__ count,
+                 uint32_t* __restrict__ done) {
+  constexpr int THREADS = GROUP < 256 ? 256 : GROUP;
+  constexpr int KEEP = 8;                      // scores in flight per thread; the first ones stay in registers
+  __shared__ T red[32];
+  __shared__ double redd[32];
+  __shared__ int redi[32];
+  __shared__ uint32_t last;
+  const int sub = threadIdx.x % GROUP;
+  const int64_t n = (int64_t)blockIdx.x * (THREADS / GROUP) + threadIdx.x / GROUP;
+  const int64_t stride = N * V;
+  if (GROUP == THREADS || n < N) {
+    const T* x = scores + n * V;
+    auto score = [&](int64_t v) { return (T)(sum_parts(x + v, stride, parts) + (bias ? __ldg(bias + v) : (T)0)); };
+    T keep[KEEP];
+    T m = -Math<T>::inf();
+#pragma unroll
+    for (int k = 0; k < KEEP; k++) {
+      const int64_t v = sub + (int64_t)k * GROUP;
+      keep[k] = v < V ? score(v) : -Math<T>::inf();
+    }
+#pragma unroll
+    for (int k = 0; k < KEEP; k++) m = fmax(m, keep[k]);
+    for (int64_t v0 = sub + (int64_t)KEEP * GROUP; v0 < V; v0 += (int64_t)KEEP * GROUP) {
+      T t[KEEP];
+#pragma unroll
+      for (int k = 0; k < KEEP; k++) t[k] = v0 + (int64_t)k * GROUP < V ? score(v0 + (int64_t)k * GROUP) : -Math<T>::inf();
+#pragma unroll
+      for (int k = 0; k < KEEP; k++) m = fmax(m, t[k]);
+    }
+    auto larger = [](T a, T b) { return (T)fmax(a, b); };
+    if constexpr (GROUP == 32) m = warp_reduce(m, larger);
+    else m = block_reduce(m, larger, (T)-Math<T>::inf(), red);
+    double s = 0.0;
+#pragma unroll
+    for (int k = 0; k < KEEP; k++) s += (double)exp_from(keep[k], m);
+    for (int64_t v0 = sub + (int64_t)KEEP * GROUP; v0 < V; v0 += (int64_t)KEEP * GROUP) {
+      T t[KEEP];
+#pragma unroll
+      for (int k = 0; k < KEEP; k++) t[k] = v0 + (int64_t)k * GROUP < V ? score(v0 + (int64_t)k * GROUP) : -Math<T>::inf();
+      T e = (T)0;
+#pragma unroll
+      for (int k = 0; k < KEEP; k++) e += exp_from(t[k], m);
+      s += (double)e;
+    }
+    auto plus = [](double a, double b) { return a + b; };
+    if constexpr (GROUP == 32) s = warp_reduce(s, plus);
+    else s = block_reduce(s, plus, 0.0, redd);
+    if (sub == 0) {
+      const double ls = ::log(s);
+      const T hi = (T)((double)m + ls);
+      lse[n] = hi;
+      lse[N + n] = isfinite(hi) ? (T)(((double)m - (double)hi) + ls) : (T)0;
+      const int32_t lab = labels[n];
+      T loss = (T)0;
+      if (lab < 0 || lab > V) loss = (T)NAN;
+      else if (lab > 0) loss = (T)(((double)m - (double)score(lab - 1)) + ls);
+      per_instance[n] = loss;
+      __threadfence();
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(done, 1u);
+  __syncthreads();
+  if (last + 1 != gridDim.x) return;
+  __threadfence();
+  double a = 0.0;
+  int c = 0;
+  for (int64_t k = threadIdx.x; k < N; k += THREADS)
+    if (labels[k] != 0) {
+      a += (double)__ldcg(per_instance + k);
+      c++;
+    }
+  a = block_reduce(a, [](double x, double y) { return x + y; }, 0.0, redd);
+  c = block_reduce(c, [](int x, int y) { return x + y; }, 0, redi);
+  if (threadIdx.x == 0) {
+    *total = (T)a;
+    *count = c;
+  }
+}
+
+// dS (without g) over the first part of the scores; `blocks` CTAs per instance
+template <typename T>
+__global__ void __launch_bounds__(256)
+lnll_grad_kernel(T* __restrict__ scores, int parts, const T* __restrict__ bias, const int32_t* __restrict__ labels,
+                 const T* __restrict__ lse, int64_t N, int64_t V, uint32_t blocks) {
+  const int64_t n = blockIdx.x / blocks;
+  const T hi = lse[n], lo = lse[N + n];
+  const int32_t lab = labels[n];
+  T* x = scores + n * V;
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    const int64_t v = (int64_t)(blockIdx.x % blocks) * 1024 + k * 256 + threadIdx.x;
+    if (v < V) x[v] = grad_score((T)(sum_parts(x + v, N * V, parts) + (bias ? bias[v] : (T)0)), hi, lo, lab, v);
+  }
+}
+
+// out = g * (the parts, added in order)
+template <typename T>
+__global__ void __launch_bounds__(256)
+lnll_sum_kernel(const T* __restrict__ parts, int64_t n, int count, T* __restrict__ out, int add, GradScale<T> g) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const T a = sum_parts(parts + i, n, count) * g.value();
+  out[i] = add ? out[i] + a : a;
+}
+
+}  // namespace kn

@@ -9,6 +9,8 @@
 // An instance's loss is lse - s[label]; the forward hands lse on as an unevaluated sum of two
 // numbers (its rounding alone would be a relative error of |lse| * 2^-24 in every p of that
 // instance), so that p = exp((s - hi) - lo).
+#include <atomic>
+
 #include "linear_nll.cuh"
 #include "linear_nll_mma.cuh"
 #include "linear_nll_small.cuh"
@@ -111,16 +113,8 @@ lnll_join_kernel(const T* __restrict__ part_m, const T* __restrict__ part_s, con
   if (w == 0 && n < N) {
     s = ss[0][lane];
     for (int k = 1; k < 8; k++) s += ss[k][lane];
-    const double ls = ::log(s);
-    const T hi = (T)((double)m + ls);
-    lse[n] = hi;
-    // in this order log s survives beside a maximum of the type's lowest value (every class masked by it)
-    lse[N + n] = isfinite(hi) ? (T)(((double)m - (double)hi) + ls) : (T)0;
     const int32_t lab = labels[n];
-    T loss = (T)0;
-    if (lab < 0 || lab > V) loss = (T)NAN;
-    else if (lab > 0) loss = (T)(((double)m - (double)label_score[n]) + ls);
-    per_instance[n] = loss;
+    per_instance[n] = finish_instance(m, s, lab > 0 && lab <= V ? label_score[n] : (T)0, lab, V, lse + n, lse + N + n);
   }
 }
 
@@ -204,10 +198,10 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 //   kSmall   up to 2^24 scores and either few instances or little work: the scores go to the workspace
 //   kMma     Float32 beyond that
 //   kPieces  the rest (Float64 with many scores)
-// Few instances: kSmall reads W once per 16 instances, kMma about four times whatever their number (the
+// Few instances: kSmall reads W once per 8 instances, kMma about four times whatever their number (the
 // scale, the split, the product) and needs five launches.
 enum Form { kSmall, kMma, kPieces };
-constexpr int64_t kFewInstances = 48;
+constexpr int64_t kFewInstances = 8;
 template <typename T> Form form(int64_t V, int64_t H, int64_t N) {
   const bool fits = N * V <= (1 << 24);
   if (fits && N <= kFewInstances) return kSmall;
@@ -215,19 +209,20 @@ template <typename T> Form form(int64_t V, int64_t H, int64_t N) {
   return fits && (double)V * H * N < (double)(1ll << 32) ? kSmall : kPieces;
 }
 
-// Parts of the summed axes of the three products in kSmall: enough CTAs for two per SM, parts of at
-// least 64 (tiles) or 256 (few instances) terms, at most 64 parts.
+// Parts of the summed axes of the three products in kSmall: enough CTAs for two per SM (tiles) or eight
+// (few instances: two run at a time, so a last round of few CTAs costs little), parts of at least 64 or
+// 256 terms, at most 64 parts.
 struct SmallPlan {
   int64_t few, s_part, x_part, w_part;         // few: by vectors, not tiles; lengths of the parts
   int s_parts, x_parts, w_parts;
-  size_t done, scores, parts, total;
+  int64_t chunks;                              // of 2048 classes, where an instance has more than one
+  size_t scores, parts, stats, total;
 };
 template <typename T> SmallPlan small_plan(int64_t V, int64_t H, int64_t N, int trans, int backward) {
   SmallPlan p{};
-  p.few = N <= 16 || (N <= kFewInstances && V * H >= (1 << 21));
-  const int64_t nb = sizeof(T) == 8 ? 8 : 16;
+  p.few = N <= 4 * kFewInstances;
   auto cut = [&](int64_t ctas, int64_t len, int64_t unit, int64_t bytes, int64_t& part, int& parts) {
-    int64_t k = (2 * kPlanSMs + ctas - 1) / ctas;
+    int64_t k = ceil_div((unit == 64 ? 2 : 8) * kPlanSMs, ctas);
     k = k > len / unit ? len / unit : k;
     k = k > 64 ? 64 : k;
     k = k > (64 << 20) / (bytes + 1) ? (64 << 20) / (bytes + 1) : k;
@@ -235,20 +230,23 @@ template <typename T> SmallPlan small_plan(int64_t V, int64_t H, int64_t N, int 
     part = ceil_div(ceil_div(len, k), unit) * unit;
     parts = (int)ceil_div(len, part);
   };
-  const int64_t sz = sizeof(T), ntile = ceil_div(N, kTile), groups = ceil_div(N, nb);
+  const int64_t sz = sizeof(T), groups = ceil_div(N, 8);
   if (p.few) {
     cut(ceil_div(V, trans ? 32 : 128) * groups, H, 256, N * V * sz, p.s_part, p.s_parts);
     cut(ceil_div(H, trans ? 128 : 32) * groups, V, 256, N * H * sz, p.x_part, p.x_parts);
     p.w_parts = 1;
   } else {
-    cut(ntile * ceil_div(V, kTile), H, 64, N * V * sz, p.s_part, p.s_parts);
-    cut(ntile * ceil_div(H, kTile), V, 64, N * H * sz, p.x_part, p.x_parts);
+    cut(ceil_div(N, kTile) * ceil_div(V, kTile), H, 64, N * V * sz, p.s_part, p.s_parts);
+    cut(ceil_div(N, kTile) * ceil_div(H, kTile), V, 64, N * H * sz, p.x_part, p.x_parts);
     cut(ceil_div(V, kTile) * ceil_div(H, kTile), N, 64, V * H * sz, p.w_part, p.w_parts);
   }
   size_t at = up(4);
   p.scores = at;
   at += up((size_t)p.s_parts * N * V * sz);
   p.parts = at;
+  p.stats = at;
+  p.chunks = V > kChunk ? ceil_div(V, kChunk) : 0;
+  if (!backward && p.chunks) at += up((size_t)(2 * p.chunks + 1) * N * sz);
   if (backward) {
     const size_t x = (size_t)p.x_parts * N * H * sz, w = p.w_parts > 1 ? (size_t)p.w_parts * V * H * sz : 0;
     at += up(x > w ? x : w);
@@ -257,40 +255,56 @@ template <typename T> SmallPlan small_plan(int64_t V, int64_t H, int64_t N, int 
   return p;
 }
 
-// Pieces of the vocabulary and parts of dx's sum.  Workspace bounds: 256 MB of split weights in the
-// forward; 128 MB of dS and 192 MB of split weights in the backward.  Within them the backward takes
+// Pieces of the vocabulary and parts of the products' sums.  Workspace bounds: 256 MB of split weights in
+// the forward; 128 MB of dS and 192 MB of split weights in the backward.  Within them the backward takes
 // the piece with the fewest waves of tiles over its three products (a product's tiles are 128 x 256
-// and its time is proportional to the summed length), charging each piece for its launches.
+// and its time is proportional to the summed length), charging each piece for its launches.  Where a
+// product has tiles for less than half of the SMs, its sum is cut into parts of at least 128 (a chunk);
+// the scores only if they fit 64 MB with their parts, dW only if there is one piece.
 struct MmaPlan {
   int64_t piece, wld, xld, dld;        // classes per piece; row pitches of split w, x and dS (elements)
-  int splits;                          // parts of dx's sum over a piece
-  size_t exps, absmax, xs, ws, label, part_m, part_s, ds, parts, db, total;
+  int s_parts, x_parts, w_parts;
+  int64_t chunks;                      // of 2048 classes, where the scores are in the workspace (s_parts > 1)
+  size_t exps, absmax, xs, ws, label, part_m, part_s, scores, ds, parts, db, total;
 };
+
+inline int64_t cut_sum(int64_t tiles, int64_t len, int64_t bytes) {
+  if (tiles * 2 > kPlanSMs) return 1;
+  int64_t k = kPlanSMs / tiles;
+  k = k > ceil_div(len, 128) ? ceil_div(len, 128) : k;
+  k = k > (64 << 20) / (bytes + 1) ? (64 << 20) / (bytes + 1) : k;
+  return k < 1 ? 1 : k;
+}
+
 inline MmaPlan mma_plan(int64_t V, int64_t H, int64_t N, int trans, int backward) {
   MmaPlan p{};
-  const int64_t all = ceil_div(V, kTN);
-  p.splits = 1;
+  const int64_t all = ceil_div(V, kTN), nt = ceil_div(N, kTM), hj = ceil_div(H, kTN), hi = ceil_div(H, kTM);
+  p.s_parts = p.x_parts = p.w_parts = 1;
   if (!backward) {
     int64_t m = (int64_t)(256u << 20) / 4 / H / kTN;
     m = m < 1 ? 1 : m;
     p.piece = kTN * ceil_div(all, ceil_div(all, m));
   } else {
-    const int64_t nt = ceil_div(N, kTM), hj = ceil_div(H, kTN), hi = ceil_div(H, kTM);
     double best = 0;
     for (int64_t m = 1; m <= all; m++) {
       if (m > 1 && (m * kTN * N * 4 > (128ll << 20) || m * kTN * H * 4 > (192ll << 20))) break;
       int64_t sp = kPlanSMs / (nt * hj);
-      sp = sp < 1 ? 1 : sp > m ? m : sp > 16 ? 16 : sp;
+      sp = sp < 1 ? 1 : sp > 2 * m ? 2 * m : sp > 16 ? 16 : sp;
+      const int64_t wt = trans ? 2 * m * hj : hi * m;
+      const int64_t wp = m == all ? cut_sum(wt, N, V * H * 4) : 1;
       const double t = (double)ceil_div(nt * m, kPlanSMs) * H + (double)ceil_div(nt * hj * sp, kPlanSMs) * ceil_div(m * kTN, sp) +
-                       (double)ceil_div(trans ? 2 * m * hj : hi * m, kPlanSMs) * N + 1500.0;
+                       (double)ceil_div(wt * wp, kPlanSMs) * ceil_div(N, wp) + 1500.0;
       const double cost = t * ceil_div(all, m);
       if (m == 1 || cost < best) {
         best = cost;
         p.piece = m * kTN;
-        p.splits = (int)sp;
+        p.x_parts = (int)sp;
+        p.w_parts = (int)wp;
       }
     }
   }
+  if (p.piece >= V) p.s_parts = (int)cut_sum(nt * all, H, N * V * 4);
+  p.chunks = V > kChunk ? ceil_div(V, kChunk) : 0;
   const int64_t vp = p.piece < V ? p.piece : V;
   p.wld = ceil_div(trans ? H : vp, 8) * 8;
   p.xld = ceil_div(H, 8) * 8;
@@ -304,14 +318,16 @@ inline MmaPlan mma_plan(int64_t V, int64_t H, int64_t N, int trans, int backward
   put(p.absmax, 2 * kMaxBlocks * 4);
   put(p.xs, (size_t)N * p.xld * 4);
   put(p.ws, (size_t)(trans ? vp : H) * p.wld * 4);
+  if (p.s_parts > 1) put(p.scores, (size_t)p.s_parts * N * V * 4);
   if (!backward) {
     put(p.label, (size_t)N * 4);
-    put(p.part_m, (size_t)all * N * 4);
-    put(p.part_s, (size_t)all * N * 4);
+    put(p.part_m, (size_t)(p.s_parts > 1 ? p.chunks : all) * N * 4);
+    put(p.part_s, (size_t)(p.s_parts > 1 ? p.chunks : all) * N * 4);
   } else {
     put(p.ds, (size_t)N * p.dld * 4);
-    if (p.splits > 1) put(p.parts, (size_t)p.splits * N * H * 4);
-    put(p.db, (size_t)ceil_div(N, kTM) * vp * 4);
+    const size_t x = p.x_parts > 1 ? (size_t)p.x_parts * N * H * 4 : 0, w = p.w_parts > 1 ? (size_t)p.w_parts * V * H * 4 : 0;
+    put(p.parts, x > w ? x : w);
+    put(p.db, (size_t)ceil_div(N, kGradRows) * vp * 4);
   }
   p.total = at;
   return p;
@@ -364,8 +380,7 @@ void few_product(bool by_row, const Matrix<T>& m, const T* y, int64_t ldy, int64
   if (N == 1) few_product_nb<T, 1>(by_row, m, y, ldy, N, part, parts, done, out, st);
   else if (N == 2) few_product_nb<T, 2>(by_row, m, y, ldy, N, part, parts, done, out, st);
   else if (N <= 4) few_product_nb<T, 4>(by_row, m, y, ldy, N, part, parts, done, out, st);
-  else if (N <= 8 || sizeof(T) == 8) few_product_nb<T, 8>(by_row, m, y, ldy, N, part, parts, done, out, st);
-  else if constexpr (sizeof(T) == 4) few_product_nb<T, 16>(by_row, m, y, ldy, N, part, parts, done, out, st);
+  else few_product_nb<T, 8>(by_row, m, y, ldy, N, part, parts, done, out, st);
 }
 
 // sizes whose tile counts fit a launch grid (features are rows of a tile grid in dW)
@@ -398,6 +413,18 @@ inline int operand_map(CUtensorMap* map, const Planes& o, bool mn, int tile) {
                            mn ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
+// the kernel's shared memory is beyond the default limit: raised once per device
+template <typename Epi> int allow_smem() {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev)) return (int)e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return 0;
+  if (cudaError_t e = cudaFuncSetAttribute(mma_kernel<Epi>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMmaSmem)) return (int)e;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return 0;
+}
+
 template <typename Epi>
 int mma_product(const Planes& a, bool a_mn, const Planes& b, bool b_mn, int64_t I, int64_t J, int64_t C, int splits, const Epi& epi,
                 cudaStream_t st) {
@@ -413,7 +440,7 @@ int mma_product(const Planes& a, bool a_mn, const Planes& b, bool b_mn, int64_t 
   tl.splits = (uint32_t)splits;
   tl.a_mn = a_mn;
   tl.b_mn = b_mn;
-  if (cudaError_t e = cudaFuncSetAttribute(mma_kernel<Epi>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMmaSmem)) return (int)e;
+  if (int rc = allow_smem<Epi>()) return rc;
   const uint64_t tiles = (uint64_t)tl.i_tiles * tl.j_tiles * tl.splits;
   if (tiles > 0x7fffffff) return KN_ESIZE;
   const unsigned grid = (unsigned)(tiles < (uint64_t)sm_count() ? tiles : sm_count());
@@ -455,6 +482,35 @@ inline SplitState split_operands(const Head<float>& h, const MmaPlan& p, char* w
   return s;
 }
 
+// how many parts a sum of C terms really has (each has work, in blocks of 32)
+inline int mma_parts(int64_t C, int parts) {
+  const int64_t blocks = ceil_div(C, kBK);
+  const int64_t k = parts < blocks ? parts : blocks;
+  return (int)ceil_div(blocks, ceil_div(blocks, k));
+}
+// parts of the scores of all classes
+inline int mma_scores(const Head<float>& h, const MmaPlan& p, const SplitState& s, float* scores, uint32_t* done, char* ws,
+                      cudaStream_t st) {
+  const MmaStore epi{(const int*)(ws + p.exps), 2, scores, h.N, h.V, h.V, h.N * h.V, 0, done, GradScale<float>{nullptr, 1.0f}};
+  return mma_product(s.x, false, s.w, !h.trans, h.N, h.V, h.H, mma_parts(h.H, p.s_parts), epi, st);
+}
+
+// lse and loss from the parts of the scores
+template <typename T>
+void statistics(const Head<T>& h, const T* scores, int parts, int64_t chunks, T* stats, T* total, int32_t* count, T* lse,
+                T* per_instance, uint32_t* done, cudaStream_t st) {
+  if (chunks) {
+    T *pm = stats + h.N, *ps = pm + chunks * h.N;
+    lnll_chunks_kernel<T><<<(unsigned)(chunks * h.N), 256, 0, st>>>(scores, parts, h.bias, h.labels, h.N, h.V, (uint32_t)chunks, pm, ps,
+                                                                   stats, lse, per_instance, total, count, done);
+  } else if (h.V <= 512) {
+    lnll_rows_kernel<T, 32><<<(unsigned)ceil_div(h.N, 8), 256, 0, st>>>(scores, parts, h.bias, h.labels, h.N, h.V, lse, per_instance, total,
+                                                                       count, done);
+  } else {
+    lnll_rows_kernel<T, 256><<<(unsigned)h.N, 256, 0, st>>>(scores, parts, h.bias, h.labels, h.N, h.V, lse, per_instance, total, count, done);
+  }
+}
+
 inline int linear_nll_fwd_mma(const Head<float>& h, float* total, int32_t* count, float* lse, float* per_instance, char* ws,
                               cudaStream_t st) {
   const MmaPlan p = mma_plan(h.V, h.H, h.N, h.trans, 0);
@@ -463,6 +519,13 @@ inline int linear_nll_fwd_mma(const Head<float>& h, float* total, int32_t* count
   for (int64_t v0 = 0; v0 < h.V; v0 += p.piece) {
     const int64_t vp = h.V - v0 < p.piece ? h.V - v0 : p.piece;
     const SplitState s = split_operands(h, p, ws, v0, vp, v0 == 0, st);
+    if (p.s_parts > 1) {      // one piece
+      uint32_t* done = (uint32_t*)(ws + p.exps) + 2;
+      float* scores = (float*)(ws + p.scores);
+      if (int rc = mma_scores(h, p, s, scores, done, ws, st)) return rc;
+      statistics<float>(h, scores, mma_parts(h.H, p.s_parts), p.chunks, label, total, count, lse, per_instance, done, st);
+      return launch_status();
+    }
     const MmaStats epi{(const int*)(ws + p.exps), h.bias ? h.bias + v0 : nullptr, h.labels, pm, ps, label, h.N, vp, v0, v0 / kTN};
     if (int rc = mma_product(s.x, false, s.w, !h.trans, h.N, vp, h.H, 1, epi, st)) return rc;
   }
@@ -481,24 +544,32 @@ inline int linear_nll_bwd_mma(const Head<float>& h, const float* lse, GradScale<
     const int64_t vp = h.V - v0 < p.piece ? h.V - v0 : p.piece;
     const SplitState s = split_operands(h, p, ws, v0, vp, v0 == 0, st);
     const Planes ds{(__half*)(ws + p.ds), h.N, vp, p.dld, h.N * p.dld};
-    const MmaGradScores e1{exps, h.bias ? h.bias + v0 : nullptr, h.labels, lse, (__half*)(ws + p.ds), h.N, vp, p.dld, ds.plane, v0, dbp};
-    if (int rc = mma_product(s.x, false, s.w, !h.trans, h.N, vp, h.H, 1, e1, st)) return rc;
-    if (db) lnll_bias_parts_kernel<<<(unsigned)ceil_div(vp, 256), 256, 0, st>>>(dbp, vp, ceil_div(h.N, kTM), db + v0, g);
+    if (p.s_parts > 1) {
+      float* scores = (float*)(ws + p.scores);
+      if (int rc = mma_scores(h, p, s, scores, nullptr, ws, st)) return rc;
+      const dim3 grid((unsigned)ceil_div(p.dld, 256), (unsigned)ceil_div(h.N, kGradRows));
+      lnll_grad_planes_kernel<<<grid, 256, 0, st>>>(scores, mma_parts(h.H, p.s_parts), h.bias, h.labels, lse, h.N, h.V, (__half*)(ws + p.ds),
+                                                    p.dld, ds.plane, dbp);
+    } else {
+      const MmaGradScores e1{exps, h.bias ? h.bias + v0 : nullptr, h.labels, lse, (__half*)(ws + p.ds), h.N, vp, p.dld, ds.plane, v0, dbp};
+      if (int rc = mma_product(s.x, false, s.w, !h.trans, h.N, vp, h.H, 1, e1, st)) return rc;
+    }
+    if (db)
+      lnll_bias_parts_kernel<<<(unsigned)ceil_div(vp, 256), 256, 0, st>>>(dbp, vp, ceil_div(h.N, p.s_parts > 1 ? kGradRows : kTM), db + v0, g);
     if (dx) {
-      // every part has work: with fewer blocks of 32 than parts, fewer parts
-      const int64_t blocks = ceil_div(vp, kBK);
-      int splits = (int)(p.splits < blocks ? p.splits : blocks);
-      splits = (int)ceil_div(blocks, ceil_div(blocks, splits));
-      const bool one = splits == 1;
-      const MmaStore e2{exps, 0, one ? dx : parts, h.N, h.H, h.H, one ? 0 : h.N * h.H, one && v0 > 0, g};
-      if (int rc = mma_product(ds, false, s.w, (bool)h.trans, h.N, h.H, vp, splits, e2, st)) return rc;
-      if (!one) lnll_parts_kernel<<<(unsigned)ceil_div(h.N * h.H, 256), 256, 0, st>>>(parts, h.N * h.H, splits, dx, v0 > 0, g);
+      const int k = mma_parts(vp, p.x_parts);
+      const MmaStore e2{exps, 0, k == 1 ? dx : parts, h.N, h.H, h.H, k == 1 ? 0 : h.N * h.H, k == 1 && v0 > 0, nullptr, g};
+      if (int rc = mma_product(ds, false, s.w, (bool)h.trans, h.N, h.H, vp, k, e2, st)) return rc;
+      if (k > 1) lnll_sum_kernel<float><<<(unsigned)ceil_div(h.N * h.H, 256), 256, 0, st>>>(parts, h.N * h.H, k, dx, v0 > 0, g);
     }
     if (dw) {
-      const MmaStore e3{exps, 1, h.trans ? dw + v0 * h.H : dw + v0, h.trans ? vp : h.H, h.trans ? h.H : vp, h.trans ? h.H : h.V, 0, 0, g};
-      if (int rc = h.trans ? mma_product(ds, true, s.x, true, vp, h.H, h.N, 1, e3, st)
-                           : mma_product(s.x, true, ds, true, h.H, vp, h.N, 1, e3, st))
+      const int k = mma_parts(h.N, p.w_parts);           // more than one only where one piece holds all classes
+      const int64_t I = h.trans ? vp : h.H, J = h.trans ? h.H : vp;
+      float* out = h.trans ? dw + v0 * h.H : dw + v0;
+      const MmaStore e3{exps, 1, k == 1 ? out : parts, I, J, h.trans ? h.H : h.V, k == 1 ? 0 : h.V * h.H, 0, nullptr, g};
+      if (int rc = h.trans ? mma_product(ds, true, s.x, true, I, J, h.N, k, e3, st) : mma_product(s.x, true, ds, true, I, J, h.N, k, e3, st))
         return rc;
+      if (k > 1) lnll_sum_kernel<float><<<(unsigned)ceil_div(h.V * h.H, 256), 256, 0, st>>>(parts, h.V * h.H, k, dw, 0, g);
     }
   }
   return launch_status();
@@ -520,13 +591,7 @@ int linear_nll_fwd_small(const Head<T>& h, T* total, int32_t* count, T* lse, T* 
   uint32_t* done = (uint32_t*)ws;
   T* scores = (T*)(ws + p.scores);
   small_scores(h, p, done, scores, st);
-#define KN_ROWS(GROUP, THREADS)                                                                                      \
-  lnll_rows_kernel<T, GROUP><<<(unsigned)ceil_div(h.N, THREADS / GROUP), THREADS, 0, st>>>(scores, p.s_parts, h.bias, \
-                                                                          h.labels, h.N, h.V, lse, per_instance, total, count, done)
-  if (h.V <= 512) KN_ROWS(32, 256);
-  else if (h.V <= 8192) KN_ROWS(256, 256);
-  else KN_ROWS(1024, 1024);
-#undef KN_ROWS
+  statistics<T>(h, scores, p.s_parts, p.chunks, (T*)(ws + p.stats), total, count, lse, per_instance, done, st);
   return launch_status();
 }
 
@@ -567,7 +632,7 @@ int linear_nll_bwd_small(const Head<T>& h, const T* lse, GradScale<T> g, T* dw, 
     const int64_t lda = h.trans ? h.V : h.H, ldb = h.trans ? h.H : h.V;
     if (p.few) {
       constexpr int VEC = 16 / sizeof(T);
-      const dim3 grid((unsigned)ceil_div(R, 16), (unsigned)ceil_div(C, 128));
+      const dim3 grid((unsigned)ceil_div(R, 64), (unsigned)ceil_div(C, 128));
       if (aligned16(b, ldb) && aligned16(dw, C)) outer_kernel<T, VEC><<<grid, 256, 0, st>>>(a, lda, b, ldb, h.N, R, C, dw, C, g);
       else outer_kernel<T, 1><<<grid, 256, 0, st>>>(a, lda, b, ldb, h.N, R, C, dw, C, g);
     } else {

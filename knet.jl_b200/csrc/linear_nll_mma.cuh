@@ -545,14 +545,15 @@ struct MmaGradScores {
 // out(i, j) = or += g * acc; with several parts of the summed axis the plain sums go to `out` + part
 struct MmaStore {
   const int* exps;
-  int which;                   // the operand beside dS: 0 w, 1 x
+  int which;                   // the operand beside dS: 0 w, 1 x; 2: the product of w and x, without dS
   float* out;
   int64_t I, J, ld, part;      // part: elements between the parts' results (0: there is one)
   int add;
+  uint32_t* done;              // counter of the statistics kernel that follows, or null
   GradScale<float> g;
-  __device__ __forceinline__ void stage(int64_t, float*) const {}
+  __device__ __forceinline__ void stage(int64_t, float*) const { clear_done(done); }
   __device__ __forceinline__ void operator()(float (&acc)[64], const TileAt& at) const {
-    const Unscale us = unscale(exps[which] + kGradExp);
+    const Unscale us = unscale(which == 2 ? exps[0] + exps[1] : exps[which] + kGradExp);
     const float f = part ? 1.0f : g.value();
     const int lane = threadIdx.x & 31, r8 = lane & 7;
     const int64_t row0 = at.i - lane + (lane & ~7);
@@ -590,15 +591,29 @@ struct MmaStore {
   }
 };
 
-// dx = or += g * (the parts' sums, added in order)
+// dS in two fp16 planes from the parts of the scores, with its sums over groups of 8 instances
+constexpr int kGradRows = 8;
 __global__ void __launch_bounds__(256)
-lnll_parts_kernel(const float* __restrict__ parts, int64_t n, int splits, float* __restrict__ out, int add, GradScale<float> g) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  float a = parts[i];
-  for (int s = 1; s < splits; s++) a += parts[(int64_t)s * n + i];
-  a *= g.value();
-  out[i] = add ? out[i] + a : a;
+lnll_grad_planes_kernel(const float* __restrict__ scores, int parts, const float* __restrict__ bias, const int32_t* __restrict__ labels,
+                        const float* __restrict__ lse, int64_t N, int64_t V, __half* __restrict__ ds, int64_t ld, int64_t plane,
+                        float* __restrict__ db_part) {
+  const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x, n0 = (int64_t)blockIdx.y * kGradRows;
+  if (v >= ld) return;
+  const float b = bias && v < V ? bias[v] : 0.0f;
+  float sum = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kGradRows; k++) {
+    const int64_t n = n0 + k;
+    if (n >= N) break;
+    float d = 0.0f;
+    if (v < V) d = grad_score(sum_parts(scores + n * V + v, N * V, parts) + b, lse[n], lse[N + n], labels[n], v);
+    sum += d;
+    __half h, l;
+    split_half(d * (float)(1 << kGradExp), h, l);
+    ds[n * ld + v] = h;
+    ds[plane + n * ld + v] = l;
+  }
+  if (db_part && v < V) db_part[(int64_t)blockIdx.y * V + v] = sum;
 }
 
 // db[j] = g * sum over the instance tiles of their sums

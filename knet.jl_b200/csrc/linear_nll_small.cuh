@@ -17,11 +17,6 @@ template <typename T> struct Strided {
   int64_t si, sc;      // element (i, c) at p + i*si + c*sc
 };
 
-// the counter of the statistics kernel that follows in the stream
-__device__ __forceinline__ void clear_done(uint32_t* done) {
-  if (done && threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) *done = 0;
-}
-
 // ---- tiles ---------------------------------------------------------------------------------------
 // acc(i, j) = sum_c A(i, c) * B(j, c) over a part of c, for a 64x64 tile of (i, j), c in steps of 16
 // through shared memory, the next step's operands loaded into registers meanwhile.  Operands have any
@@ -203,7 +198,7 @@ row_dot_kernel(Matrix<T> m, const T* __restrict__ y, int64_t ldy, int64_t N, int
   const T* yv[NB];
 #pragma unroll
   for (int n = 0; n < NB; n++) yv[n] = y + min(n0 + n, N - 1) * ldy;
-  constexpr int UN = NB >= 8 ? 1 : 2;
+  constexpr int UN = NB >= 8 ? 1 : 2;              // packs per row in flight
   for (int64_t c = c_lo + lane * VEC; c < c_hi; c += 32 * VEC * UN) {
     Pack<T, VEC> w[UN][4];
 #pragma unroll
@@ -233,6 +228,44 @@ row_dot_kernel(Matrix<T> m, const T* __restrict__ y, int64_t ldy, int64_t N, int
     }
 }
 
+// the sums of the 8 warps of a CTA in warp 0: two warps at a time hand over to the others, so that two
+// slots of shared memory suffice
+template <typename T, int NB>
+__device__ __forceinline__ void join_warps(T (&acc)[NB][4], T (*red)[NB][128]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int h = 6; h > 0; h -= 2) {                 // warps h, h+1 -> 0, 1
+    __syncthreads();
+    if (warp == h || warp == h + 1) {
+#pragma unroll
+      for (int n = 0; n < NB; n++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) red[warp - h][n][e * 32 + lane] = acc[n][e];
+    }
+    __syncthreads();
+    if (warp < 2) {
+#pragma unroll
+      for (int n = 0; n < NB; n++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[n][e] += red[warp][n][e * 32 + lane];
+    }
+  }
+  __syncthreads();
+  if (warp == 1) {
+#pragma unroll
+    for (int n = 0; n < NB; n++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) red[0][n][e * 32 + lane] = acc[n][e];
+  }
+  __syncthreads();
+  if (warp == 0) {
+#pragma unroll
+    for (int n = 0; n < NB; n++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) acc[n][e] += red[0][n][e * 32 + lane];
+  }
+}
+
 // parts[z part][n][col] = sum over a part of the rows of M(r, col) * y(n, r): a CTA takes 128 columns,
 // its 8 warps share the rows; the vectors' entries come transposed through shared memory.
 constexpr int kColRows = 128;
@@ -241,8 +274,9 @@ __global__ void __launch_bounds__(256)
 col_sum_kernel(Matrix<T> m, const T* __restrict__ y, int64_t ldy, int64_t N, int64_t r_part, uint32_t* done, T* __restrict__ parts) {
   clear_done(done);
   constexpr int Q = 4 / VEC;                       // packs per thread: 4 columns
+  constexpr int YV = NB < 16 / (int)sizeof(T) ? NB : 16 / (int)sizeof(T);
   __shared__ __align__(16) T ys[kColRows][NB];
-  __shared__ __align__(16) T red[4][NB][128];
+  __shared__ __align__(16) T red[2][NB][128];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t j0 = (int64_t)blockIdx.x * 128, n0 = (int64_t)blockIdx.y * NB;
   const int64_t r_lo = (int64_t)blockIdx.z * r_part, r_hi = min(m.rows, r_lo + r_part);
@@ -265,52 +299,42 @@ col_sum_kernel(Matrix<T> m, const T* __restrict__ y, int64_t ldy, int64_t N, int
       ys[r][n] = rc + r < r_hi && n0 + n < N ? y[(n0 + n) * ldy + rc + r] : (T)0;
     }
     __syncthreads();
-    constexpr int UN = 8;
-#pragma unroll 1
-    for (int u0 = warp; u0 < kColRows && rc + u0 < r_hi; u0 += 8 * UN) {
-      Pack<T, VEC> w[UN][Q];
+    // rows warp, warp + 8, ... of the 128, UN at a time, the next batch in flight while one is used
+    constexpr int UN = NB >= 8 ? 4 : 8, BATCHES = kColRows / (8 * UN);
+    Pack<T, VEC> w[2][UN][Q];
+    auto fetch = [&](Pack<T, VEC> (&to)[UN][Q], int batch) {
 #pragma unroll
       for (int u = 0; u < UN; u++)
 #pragma unroll
         for (int q = 0; q < Q; q++) {
-          const int64_t r = rc + u0 + 8 * u;
-          if (in[q] && u0 + 8 * u < kColRows && r < r_hi) w[u][q] = ld_stream<T, VEC>(m.p + r * m.pitch + col[q]);
+          const int64_t r = rc + warp + 8 * (batch * UN + u);
+          if (in[q] && r < r_hi) to[u][q] = ld_stream<T, VEC>(m.p + r * m.pitch + col[q]);
           else
 #pragma unroll
-            for (int e = 0; e < VEC; e++) w[u][q].v[e] = (T)0;
+            for (int e = 0; e < VEC; e++) to[u][q].v[e] = (T)0;
         }
+    };
+    fetch(w[0], 0);
+#pragma unroll
+    for (int b = 0; b < BATCHES; b++) {
+      if (b + 1 < BATCHES) fetch(w[(b + 1) & 1], b + 1);
 #pragma unroll
       for (int u = 0; u < UN; u++) {
-        if (u0 + 8 * u >= kColRows || rc + u0 + 8 * u >= r_hi) break;
 #pragma unroll
-        for (int n = 0; n < NB; n++) {
-          const T v = ys[u0 + 8 * u][n];
+        for (int k = 0; k < NB; k += YV) {
+          const Pack<T, YV> v = *reinterpret_cast<const Pack<T, YV>*>(&ys[warp + 8 * (b * UN + u)][k]);
 #pragma unroll
-          for (int q = 0; q < Q; q++)
+          for (int n = 0; n < YV; n++)
 #pragma unroll
-            for (int e = 0; e < VEC; e++) acc[n][q * VEC + e] = Math<T>::fma(w[u][q].v[e], v, acc[n][q * VEC + e]);
+            for (int q = 0; q < Q; q++)
+#pragma unroll
+              for (int e = 0; e < VEC; e++)
+                acc[k + n][q * VEC + e] = Math<T>::fma(w[b & 1][u][q].v[e], v.v[n], acc[k + n][q * VEC + e]);
         }
       }
     }
   }
-  // the warps' sums, the upper half of the warps handing over to the lower one in turn
-#pragma unroll
-  for (int h = 4; h > 0; h >>= 1) {
-    __syncthreads();
-    if (warp >= h && warp < 2 * h) {
-#pragma unroll
-      for (int n = 0; n < NB; n++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) red[warp - h][n][e * 32 + lane] = acc[n][e];
-    }
-    __syncthreads();
-    if (warp < h) {
-#pragma unroll
-      for (int n = 0; n < NB; n++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) acc[n][e] += red[warp][n][e * 32 + lane];
-    }
-  }
+  join_warps<T, NB>(acc, red);
   if (warp == 0) {
 #pragma unroll
     for (int n = 0; n < NB; n++)
@@ -322,61 +346,66 @@ col_sum_kernel(Matrix<T> m, const T* __restrict__ y, int64_t ldy, int64_t N, int
   }
 }
 
-// out(r, c) = g * sum_n a(n, r) * b(n, c): few instances, bound by the stores.  A CTA takes 16 rows and
-// 128 columns, a warp two rows.
+// out(r, c) = g * sum_n a(n, r) * b(n, c): few instances, bound by the stores.  A CTA takes 64 rows and
+// 128 columns, a warp eight rows; a's entries come through shared memory, eight instances at a time.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
 outer_kernel(const T* __restrict__ a, int64_t lda, const T* __restrict__ b, int64_t ldb, int64_t N, int64_t R, int64_t C,
              T* __restrict__ out, int64_t ld, GradScale<T> g) {
-  constexpr int Q = 4 / VEC;
+  constexpr int Q = 4 / VEC, NB = 8;
+  __shared__ __align__(16) T as[NB][64];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t r0 = (int64_t)blockIdx.x * 16 + warp * 2, j0 = (int64_t)blockIdx.y * 128;
-  if (r0 >= R) return;
-  const bool two = r0 + 1 < R;
-  T acc[2][4];
+  const int64_t r0 = (int64_t)blockIdx.x * 64, j0 = (int64_t)blockIdx.y * 128;
+  T acc[8][4];
 #pragma unroll
-  for (int e = 0; e < 4; e++) acc[0][e] = acc[1][e] = (T)0;
-#pragma unroll 4
-  for (int64_t n = 0; n < N; n++) {
-    const T a0 = a[n * lda + r0], a1 = two ? a[n * lda + r0 + 1] : (T)0;
+  for (int r = 0; r < 8; r++)
 #pragma unroll
-    for (int q = 0; q < Q; q++) {
-      const int64_t c = j0 + (lane + 32 * q) * VEC;
-      if (c < C) {
-        const Pack<T, VEC> v = ld_cached<T, VEC>(b + n * ldb + c);
+    for (int e = 0; e < 4; e++) acc[r][e] = (T)0;
+  for (int64_t n0 = 0; n0 < N; n0 += NB) {
+    __syncthreads();
+    for (int k = threadIdx.x; k < NB * 64; k += 256) {
+      const int n = k >> 6, r = k & 63;
+      as[n][r] = n0 + n < N && r0 + r < R ? a[(n0 + n) * lda + r0 + r] : (T)0;
+    }
+    __syncthreads();
 #pragma unroll
-        for (int e = 0; e < VEC; e++) {
-          acc[0][q * VEC + e] = Math<T>::fma(a0, v.v[e], acc[0][q * VEC + e]);
-          acc[1][q * VEC + e] = Math<T>::fma(a1, v.v[e], acc[1][q * VEC + e]);
+    for (int n = 0; n < NB; n++) {
+      if (n0 + n >= N) break;
+      T av[8];
+#pragma unroll
+      for (int r = 0; r < 8; r++) av[r] = as[n][warp * 8 + r];
+#pragma unroll
+      for (int q = 0; q < Q; q++) {
+        const int64_t c = j0 + (lane + 32 * q) * VEC;
+        if (c < C) {
+          const Pack<T, VEC> v = ld_cached<T, VEC>(b + (n0 + n) * ldb + c);
+#pragma unroll
+          for (int r = 0; r < 8; r++)
+#pragma unroll
+            for (int e = 0; e < VEC; e++) acc[r][q * VEC + e] = Math<T>::fma(av[r], v.v[e], acc[r][q * VEC + e]);
         }
       }
     }
   }
   const T f = g.value();
 #pragma unroll
-  for (int q = 0; q < Q; q++) {
-    const int64_t c = j0 + (lane + 32 * q) * VEC;
-    if (c < C) {
-      Pack<T, VEC> v;
+  for (int r = 0; r < 8; r++) {
+    const int64_t row = r0 + warp * 8 + r;
+    if (row >= R) break;
 #pragma unroll
-      for (int e = 0; e < VEC; e++) v.v[e] = acc[0][q * VEC + e] * f;
-      st_stream<T, VEC>(out + r0 * ld + c, v);
-      if (two) {
+    for (int q = 0; q < Q; q++) {
+      const int64_t c = j0 + (lane + 32 * q) * VEC;
+      if (c < C) {
+        Pack<T, VEC> v;
 #pragma unroll
-        for (int e = 0; e < VEC; e++) v.v[e] = acc[1][q * VEC + e] * f;
-        st_stream<T, VEC>(out + (r0 + 1) * ld + c, v);
+        for (int e = 0; e < VEC; e++) v.v[e] = acc[r][q * VEC + e] * f;
+        st_stream<T, VEC>(out + row * ld + c, v);
       }
     }
   }
 }
 
 // ---- from the scores ------------------------------------------------------------------------------------
-template <typename T> __device__ __forceinline__ T sum_parts(const T* p, int64_t stride, int parts) {
-  T s = p[0];
-  for (int k = 1; k < parts; k++) s += p[k * stride];
-  return s;
-}
-
 // lse and loss of each instance from the parts of its scores; GROUP threads (a warp or the CTA) per
 // instance.  The last CTA to finish adds the losses in a fixed order (`done` counts CTAs; the product
 // that ran before set it to 0).
@@ -432,15 +461,8 @@ lnll_rows_kernel(const T* __restrict__ scores, int parts, const T* __restrict__ 
     if constexpr (GROUP == 32) s = warp_reduce(s, plus);
     else s = block_reduce(s, plus, 0.0, redd);
     if (sub == 0) {
-      const double ls = ::log(s);
-      const T hi = (T)((double)m + ls);
-      lse[n] = hi;
-      lse[N + n] = isfinite(hi) ? (T)(((double)m - (double)hi) + ls) : (T)0;
       const int32_t lab = labels[n];
-      T loss = (T)0;
-      if (lab < 0 || lab > V) loss = (T)NAN;
-      else if (lab > 0) loss = (T)(((double)m - (double)score(lab - 1)) + ls);
-      per_instance[n] = loss;
+      per_instance[n] = finish_instance(m, s, lab > 0 && lab <= V ? score(lab - 1) : (T)0, lab, V, lse + n, lse + N + n);
       __threadfence();
     }
   }
@@ -458,6 +480,79 @@ lnll_rows_kernel(const T* __restrict__ scores, int parts, const T* __restrict__ 
     }
   a = block_reduce(a, [](double x, double y) { return x + y; }, 0.0, redd);
   c = block_reduce(c, [](int x, int y) { return x + y; }, 0, redi);
+  if (threadIdx.x == 0) {
+    *total = (T)a;
+    *count = c;
+  }
+}
+
+// The same for many classes: a CTA takes 2048 classes of one instance and leaves their maximum and sum;
+// the last CTA to finish joins them, a warp per instance, and adds the losses.
+constexpr int kChunk = 2048;
+template <typename T>
+__global__ void __launch_bounds__(256)
+lnll_chunks_kernel(const T* __restrict__ scores, int parts, const T* __restrict__ bias, const int32_t* __restrict__ labels, int64_t N,
+                   int64_t V, uint32_t chunks, T* __restrict__ part_m, T* __restrict__ part_s, T* __restrict__ label_score,
+                   T* __restrict__ lse, T* __restrict__ per_instance, T* __restrict__ total, int32_t* __restrict__ count,
+                   uint32_t* __restrict__ done) {
+  __shared__ T red[32];
+  __shared__ double redd[32];
+  __shared__ int redi[32];
+  __shared__ uint32_t last;
+  const int64_t n = blockIdx.x / chunks, v0 = (int64_t)(blockIdx.x % chunks) * kChunk;
+  const T* x = scores + n * V;
+  T t[kChunk / 256];
+  T m = -Math<T>::inf();
+  const int64_t lab = (int64_t)labels[n] - 1 - v0;
+#pragma unroll
+  for (int k = 0; k < kChunk / 256; k++) {
+    const int c = k * 256 + threadIdx.x;
+    const int64_t v = v0 + c;
+    t[k] = v < V ? (T)(sum_parts(x + v, N * V, parts) + (bias ? __ldg(bias + v) : (T)0)) : -Math<T>::inf();
+    if (c == lab && v < V) label_score[n] = t[k];
+  }
+#pragma unroll
+  for (int k = 0; k < kChunk / 256; k++) m = fmax(m, t[k]);
+  m = block_reduce(m, [](T a, T b) { return (T)fmax(a, b); }, (T)-Math<T>::inf(), red);
+  T s = (T)0;
+#pragma unroll
+  for (int k = 0; k < kChunk / 256; k++) s += exp_from(t[k], m);
+  s = block_reduce(s, [](T a, T b) { return a + b; }, (T)0, red);
+  if (threadIdx.x == 0) {
+    part_m[n * chunks + blockIdx.x % chunks] = m;
+    part_s[n * chunks + blockIdx.x % chunks] = s;
+  }
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(done, 1u);
+  __syncthreads();
+  if (last + 1 != gridDim.x) return;
+  __threadfence();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  double a = 0.0;
+  int c = 0;
+  for (int64_t i = warp; i < N; i += 8) {
+    T mm = -Math<T>::inf();
+    for (uint32_t k = lane; k < chunks; k += 32) mm = fmax(mm, __ldcg(part_m + i * chunks + k));
+    mm = warp_reduce(mm, [](T p, T q) { return (T)fmax(p, q); });
+    double sd = 0.0;
+    for (uint32_t k = lane; k < chunks; k += 32) {
+      const T v = __ldcg(part_s + i * chunks + k), d = __ldcg(part_m + i * chunks + k) - mm;
+      if (v != (T)0) sd += (double)(v * exp(d));                 // an empty chunk is (-inf, 0)
+    }
+    sd = warp_reduce(sd, [](double p, double q) { return p + q; });
+    if (lane == 0) {
+      const int32_t l = labels[i];
+      const T loss = finish_instance(mm, sd, l > 0 && l <= V ? __ldcg(label_score + i) : (T)0, l, V, lse + i, lse + N + i);
+      per_instance[i] = loss;
+      if (l != 0) {
+        a += (double)loss;
+        c++;
+      }
+    }
+  }
+  a = block_reduce(a, [](double p, double q) { return p + q; }, 0.0, redd);
+  c = block_reduce(c, [](int p, int q) { return p + q; }, 0, redi);
   if (threadIdx.x == 0) {
     *total = (T)a;
     *count = c;

@@ -4,6 +4,7 @@ Mirrors src/libknet8/LibKnet8.jl:50-62: `knet8(fun, *args)` appends `_stream` to
 name and the current CUDA stream to the arguments; `knet8r` is the value-returning form.
 There is no fallback: if the shared library is missing the import of this module fails.
 """
+import contextlib
 import ctypes as C
 import os
 
@@ -38,12 +39,21 @@ def check(rc, name):
 
 
 def stream_ptr():
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    """The current stream's handle (the raw query costs a tenth of building a torch Stream object)."""
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
 def ptr(t):
     """Device pointer of a tensor (or None)."""
     return None if t is None else C.c_void_p(t.data_ptr())
+
+
+_here = contextlib.nullcontext()
+
+
+def on_device(dev):
+    """Context in which `dev` is the current device; free when it already is."""
+    return _here if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def knet8(fun, *args):

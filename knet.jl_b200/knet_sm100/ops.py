@@ -13,7 +13,7 @@ import numpy as np
 import torch
 
 from .karray import KnetArray, _prod
-from .lib import knet, knet8, knet8r, libknet, ptr, sfx
+from .lib import knet, knet8, knet8r, libknet, on_device, ptr, sfx
 
 _CT = {torch.float32: C.c_float, torch.float64: C.c_double}
 
@@ -317,6 +317,8 @@ def logsumexp_back(x, y, dy, dims=None):
 def _labels(labels, device):
     """Int32 device labels (1-based, 0 = skip); host arrays are uploaded once per call."""
     if isinstance(labels, torch.Tensor):
+        if labels.dtype == torch.int32 and labels.device == device and labels.dim() == 1 and labels.is_contiguous():
+            return labels
         return labels.to(device=device, dtype=torch.int32).contiguous().view(-1)
     return torch.from_numpy(np.ascontiguousarray(np.asarray(labels).reshape(-1, order="F"),
                                                  dtype=np.int32)).to(device)
@@ -385,24 +387,25 @@ class LinearNllResult(NllResult):
 
 def _head_sizes(w, x, b, trans):
     """(V, H, N) of scores = w*x (+ b), w being (V,H), or (H,V) with trans; checks what belongs together."""
-    if w.ndim != 2 or x.ndim < 1:
+    if len(w.shape) != 2 or not x.shape:
         raise ValueError("DimensionMismatch: w must be a matrix and x a vector or matrix")
     H, V = w.shape if trans else w.shape[::-1]
     if x.shape[0] != H:
         raise ValueError(f"DimensionMismatch: x has {x.shape[0]} features, w {H}")
-    if b is not None and len(b) != V:
+    if b is not None and b.data.numel() != V:
         raise ValueError(f"DimensionMismatch: b has {len(b)} entries for {V} classes")
     for a in (x, b):
-        if a is not None and a.dtype != w.dtype:
+        if a is None:
+            continue
+        if a.data.dtype != w.data.dtype:
             raise TypeError("element types differ")
-        if a is not None and a.data.device != w.data.device:
+        if a.data.device != w.data.device:
             raise ValueError("arrays live on different devices")
-    return V, H, (len(x) // H if H else 0)
+    return V, H, (x.data.numel() // H if H else 0)
 
 
-def _head_workspace(S, V, H, N, backward, device):
-    n = getattr(libknet, f"knet_linear_nll_workspace_{S}")(V, H, N, backward)
-    return torch.empty(max(n, 1), dtype=torch.uint8, device=device)
+def _address(a):
+    return None if a is None else a.data.data_ptr()
 
 
 def linear_nll_device(w, x, labels, b=None, trans=False):
@@ -410,18 +413,20 @@ def linear_nll_device(w, x, labels, b=None, trans=False):
     (V,H), or (H,V) with `trans` (an embedding matrix used again at the output), x (H,N), labels
     1-based with 0 = skip.  The result's total and count stay on the device, as nll_device's do."""
     V, H, N = _head_sizes(w, x, b, trans)
-    dev, dt, S = w.data.device, w.dtype, sfx(w.dtype)
+    dev, dt = w.data.device, w.data.dtype
+    S = sfx(dt)
     lab = _labels(labels, dev)
     if lab.numel() != N:
         raise ValueError("DimensionMismatch: one label per instance is needed")
-    with torch.cuda.device(dev):
+    with on_device(dev):
         total = torch.empty(1, dtype=dt, device=dev)
         count = torch.empty(1, dtype=torch.int32, device=dev)
         per = torch.empty(max(N, 1), dtype=dt, device=dev)
         lse = torch.empty(2 * N, dtype=dt, device=dev)
-        ws = _head_workspace(S, V, H, N, 0, dev)
-        knet(f"knet_linear_nll_fwd_{S}", ptr(w.data), int(bool(trans)), ptr(None if b is None else b.data), ptr(x.data), ptr(lab),
-             V, H, N, ptr(total), ptr(count), ptr(lse), ptr(per), ptr(ws), ws.numel())
+        size = getattr(libknet, f"knet_linear_nll_workspace_{S}")(V, H, N, 0)
+        ws = torch.empty(max(size, 1), dtype=torch.uint8, device=dev)
+        knet(f"knet_linear_nll_fwd_{S}", _address(w), 1 if trans else 0, _address(b), _address(x), lab.data_ptr(), V, H, N,
+             total.data_ptr(), count.data_ptr(), lse.data_ptr(), per.data_ptr(), ws.data_ptr(), size)
     return LinearNllResult(total, count, per, lab, lse)
 
 
@@ -434,25 +439,30 @@ def linear_nll_back(w, x, res, b=None, trans=False, average=True, dy=1.0, need=(
     """Gradients (dw, dx, db) of linear_nll from its forward result and the same w, x and b; db is
     None without b.  `need` leaves some of them out (None); `out` gives arrays to write them to."""
     V, H, N = _head_sizes(w, x, b, trans)
-    dev, S = w.data.device, sfx(w.dtype)
-    if res.labels.numel() != N or res.lse_pair.dtype != w.dtype:
+    dev, dt = w.data.device, w.data.dtype
+    if res.labels.numel() != N or res.lse_pair.dtype != dt or res.labels.device != dev:
         raise ValueError("DimensionMismatch: the forward result belongs to other arrays")
-    grads = []
-    for a, want, o in zip((w, x, b), need, out):
-        if a is None or not want:
-            grads.append(None)
-            continue
-        if o is not None and (len(o) != len(a) or o.dtype != a.dtype or o.data.device != dev):
-            raise ValueError("DimensionMismatch: out does not match its array")
-        grads.append(a.similar() if o is None else o)
-    if all(g is None for g in grads):
-        return tuple(grads)
-    with torch.cuda.device(dev):
-        ws = _head_workspace(S, V, H, N, 1, dev)
-        knet(f"knet_linear_nll_bwd_{S}", ptr(w.data), int(bool(trans)), ptr(None if b is None else b.data), ptr(x.data),
-             ptr(res.labels), V, H, N, ptr(res.lse_pair), int(average), _CT[w.dtype](dy), ptr(res.count),
-             *[ptr(None if grads[k] is None else grads[k].data) for k in (0, 2, 1)], ptr(ws), ws.numel())
-    return tuple(grads)
+    S = sfx(dt)
+    with on_device(dev):
+        grads = []
+        for a, want, o in zip((w, x, b), need, out):
+            if a is None or not want:
+                grads.append(None)
+            elif o is None:
+                grads.append(KnetArray(torch.empty_like(a.data), a.shape))
+            elif o.data.numel() != a.data.numel() or o.data.dtype != dt or o.data.device != dev:
+                raise ValueError("DimensionMismatch: out does not match its array")
+            else:
+                grads.append(o)
+        dw, dx, db = grads
+        if dw is None and dx is None and db is None:
+            return None, None, None
+        size = getattr(libknet, f"knet_linear_nll_workspace_{S}")(V, H, N, 1)
+        ws = torch.empty(max(size, 1), dtype=torch.uint8, device=dev)
+        knet(f"knet_linear_nll_bwd_{S}", _address(w), 1 if trans else 0, _address(b), _address(x), res.labels.data_ptr(), V, H, N,
+             res.lse_pair.data_ptr(), 1 if average else 0, dy, res.count.data_ptr(), _address(dw), _address(db), _address(dx),
+             ws.data_ptr(), size)
+    return dw, dx, db
 
 
 def argmax(x, dims=1):

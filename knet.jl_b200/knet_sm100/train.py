@@ -11,7 +11,7 @@ import ctypes as C
 import torch
 
 from .karray import KnetArray
-from .lib import knet, knet8, knet8r, libknet, ptr, sfx
+from .lib import knet, knet8, knet8r, libknet, on_device, ptr, sfx
 from . import ops
 
 
@@ -227,7 +227,7 @@ def gnorm(grads, gscale=1.0):
     plan, _ = _one_plan(grads)
     if plan is None:
         return torch.zeros(1, dtype=torch.float64, device="cuda")
-    with torch.cuda.device(plan.table.device):
+    with on_device(plan.table.device):
         return _global_norm(plan, None, gscale)[0]
 
 
@@ -241,7 +241,7 @@ def gclip_global_(grads, gclip, gscale=1.0):
     plan, once = _one_plan(grads)
     if plan is None:
         return torch.zeros(1, dtype=torch.float64, device="cuda")
-    with torch.cuda.device(plan.table.device):
+    with on_device(plan.table.device):
         norm, factor = _global_norm(plan, gclip, gscale)
         knet(f"knet_gclip_apply_{sfx(plan.dtype)}", ptr(once.table), once.ntensors, once.total_chunks, ptr(factor))
     return norm

@@ -54,4 +54,48 @@ template <typename T> __device__ __forceinline__ T sum_parts(const T* p, int64_t
   return s;
 }
 
+// total and count over the instances in a fixed order, by one CTA
+template <typename T, int THREADS>
+__device__ __forceinline__ void add_losses(const T* per_instance, const int32_t* __restrict__ labels, int64_t N, T* total, int32_t* count) {
+  __shared__ double sd[32];
+  __shared__ int sc[32];
+  double a = 0.0;
+  int c = 0;
+  for (int64_t n0 = threadIdx.x; n0 < N; n0 += 8 * THREADS) {      // eight loads in flight
+    T v[8];
+    int32_t l[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const int64_t n = n0 + (int64_t)k * THREADS;
+      l[k] = n < N ? __ldg(labels + n) : 0;
+      v[k] = n < N ? __ldcg(per_instance + n) : (T)0;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+      if (l[k] != 0) {
+        a += (double)v[k];
+        c++;
+      }
+  }
+  a = block_reduce(a, [](double x, double y) { return x + y; }, 0.0, sd);
+  c = block_reduce(c, [](int x, int y) { return x + y; }, 0, sc);
+  if (threadIdx.x == 0) {
+    *total = (T)a;
+    *count = c;
+  }
+}
+// the same by the last CTA of the grid to get here; `done` counts them
+template <typename T, int THREADS>
+__device__ __forceinline__ void last_adds_losses(const T* per_instance, const int32_t* __restrict__ labels, int64_t N, T* total,
+                                                 int32_t* count, uint32_t* done) {
+  __shared__ uint32_t last;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(done, 1u);
+  __syncthreads();
+  if (last + 1 != gridDim.x) return;
+  __threadfence();
+  add_losses<T, THREADS>(per_instance, labels, N, total, count);
+}
+
 }  // namespace kn

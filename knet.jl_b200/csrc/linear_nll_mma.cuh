@@ -4,9 +4,13 @@
 // split into two fp16 terms, hi = fp16(x), lo = fp16(x - hi): together 22 bits, and never less than
 // 2^-25 of the scaled value's unit, so entries down to 2^-17 of the largest keep a relative error of
 // 2^-23.  A product takes three of the four partial products (lo*lo is below 2^-22 of it), which are
-// exact in Float32; the tensor core adds them.  Its additions truncate, so a long sum would lose
-// about 2^-25 per 16 terms, always towards zero: the accumulator in TMEM therefore takes only 128
-// summed indices, and the chunks are added in registers with rounding to nearest.
+// exact in Float32; the tensor core adds them.  Its additions truncate: measured on sums of 1024 and 8192
+// products, an accumulator that takes n blocks of 32 summed indices comes out low by 0.75 n 2^-23 of its
+// value for terms of random signs (n = 4, 8, 16: 3.4e-7, 7.4e-7, 1.5e-6), about twice that for terms of
+// one sign.  The accumulator in TMEM therefore takes 256 summed indices, the chunks are added in registers
+// with rounding to nearest, and the epilogue multiplies by 1 + 0.75 n 2^-23, which leaves a relative error
+// of 5e-7 to 8e-7 in a product.  (Chunks of 128 halve the error; 256 give the epilogue 10 us instead of 5
+// before the tensor core has to wait for it: dS of 4608 classes x 4096 instances 123 -> 112 us.)
 //
 // A CTA owns a 128 x 256 tile of the result.  Warp 16 loads the operands with TMA into a ring of
 // stages of 32 summed indices (48 KB: both planes of 128 + 256 rows); warp 17 issues the products
@@ -23,8 +27,10 @@
 namespace kn {
 
 constexpr int kTM = 128, kTN = 256, kBK = 32, kStages = 4;
-constexpr int kChunkBlocks = 4;                         // 128 summed indices per accumulator
-constexpr int kEpiWarps = 16, kMmaThreads = (kEpiWarps + 2) * 32;
+constexpr int kChunkBlocks = 8;                         // 256 summed indices per accumulator
+// Registers: 640 threads start with 96 each; the four warps beside the epilogue give up all but 32 and
+// the epilogue's 512 threads take 112 (57 344 + 4 096 of 61 440).
+constexpr int kEpiWarps = 16, kMmaThreads = (kEpiWarps + 4) * 32;
 constexpr uint32_t kStageA = 2 * kTM * kBK * 2, kStageB = 2 * kTN * kBK * 2, kStageBytes = kStageA + kStageB;
 constexpr int kGradExp = 14;                            // dS lies in [-1, 1]
 
@@ -63,6 +69,7 @@ struct TileAt {
   uint32_t it, jt, split;      // tile
   uint32_t turn;               // how many tiles this CTA has finished
   int quarter, row;            // which 64 columns, which of the 128 rows
+  float gain;                  // makes up for the mean loss of the truncated additions
   MmaShared* sh;
 };
 
@@ -109,95 +116,99 @@ mma_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUt
   tcgen05_after_sync();
   const uint32_t tmem = sh->tmem;
 
-  if (warp == kEpiWarps) {
-    // ---- loads
-    if (lane == 0) {
-      tma_prefetch_map(&amap);
-      tma_prefetch_map(&bmap);
-      uint32_t n = 0;                                   // stages filled so far
-      bool ok = true;
-      for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-        const uint32_t it = t % tl.i_tiles, r = t / tl.i_tiles, jt = r % tl.j_tiles, sp = r / tl.j_tiles;
-        const uint32_t k0 = sp * tl.blocks_per_split, k1 = min(k0 + tl.blocks_per_split, tl.blocks);
-        const int32_t i0 = (int32_t)(it * kTM), j0 = (int32_t)(jt * kTN);
-        for (uint32_t k = k0; k < k1; k++, n++) {
-          const uint32_t s = n % kStages;
-          if (n >= kStages && !mma_wait(&sh->empty[s], (n / kStages - 1) & 1, &sh->gave_up)) {
-            ok = false;
-            break;
-          }
-          uint8_t* a = stages + (size_t)s * kStageBytes;
-          uint8_t* b = a + kStageA;
-          const int32_t c = (int32_t)(k * kBK);
-          mbar_arrive_expect_tx(&sh->full[s], kStageBytes);
-          if (tl.a_mn) {
-            for (int g = 0; g < kTM / 64; g++) tma_load_3d(a + g * 8192, &amap, i0 + g * 64, c, 0, &sh->full[s]);
-          } else {
-            tma_load_3d(a, &amap, c, i0, 0, &sh->full[s]);
-          }
-          if (tl.b_mn) {
-            for (int g = 0; g < kTN / 64; g++) tma_load_3d(b + g * 8192, &bmap, j0 + g * 64, c, 0, &sh->full[s]);
-          } else {
-            tma_load_3d(b, &bmap, c, j0, 0, &sh->full[s]);
+  if (warp >= kEpiWarps) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+    if (warp == kEpiWarps) {
+      // ---- loads
+      if (lane == 0) {
+        tma_prefetch_map(&amap);
+        tma_prefetch_map(&bmap);
+        uint32_t n = 0;                                   // stages filled so far
+        bool ok = true;
+        for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+          const uint32_t it = t % tl.i_tiles, r = t / tl.i_tiles, jt = r % tl.j_tiles, sp = r / tl.j_tiles;
+          const uint32_t k0 = sp * tl.blocks_per_split, k1 = min(k0 + tl.blocks_per_split, tl.blocks);
+          const int32_t i0 = (int32_t)(it * kTM), j0 = (int32_t)(jt * kTN);
+          for (uint32_t k = k0; k < k1; k++, n++) {
+            const uint32_t s = n % kStages;
+            if (n >= kStages && !mma_wait(&sh->empty[s], (n / kStages - 1) & 1, &sh->gave_up)) {
+              ok = false;
+              break;
+            }
+            uint8_t* a = stages + (size_t)s * kStageBytes;
+            uint8_t* b = a + kStageA;
+            const int32_t c = (int32_t)(k * kBK);
+            mbar_arrive_expect_tx(&sh->full[s], kStageBytes);
+            if (tl.a_mn) {
+              for (int g = 0; g < kTM / 64; g++) tma_load_3d(a + g * 8192, &amap, i0 + g * 64, c, 0, &sh->full[s]);
+            } else {
+              tma_load_3d(a, &amap, c, i0, 0, &sh->full[s]);
+            }
+            if (tl.b_mn) {
+              for (int g = 0; g < kTN / 64; g++) tma_load_3d(b + g * 8192, &bmap, j0 + g * 64, c, 0, &sh->full[s]);
+            } else {
+              tma_load_3d(b, &bmap, c, j0, 0, &sh->full[s]);
+            }
           }
         }
+        // every load issued has landed before this CTA may leave
+        for (uint32_t m = n > kStages ? n - kStages : 0; m < n; m++)
+          for (uint32_t i = 0; i < kWaitSpins && !mbar_try_wait(&sh->full[m % kStages], (m / kStages) & 1); i++) __nanosleep(64);
       }
-      // every load issued has landed before this CTA may leave
-      for (uint32_t m = n > kStages ? n - kStages : 0; m < n; m++)
-        for (uint32_t i = 0; i < kWaitSpins && !mbar_try_wait(&sh->full[m % kStages], (m / kStages) & 1); i++) __nanosleep(64);
-    }
-  } else if (warp == kEpiWarps + 1) {
-    // ---- products
-    if (lane == 0) {
-      const uint32_t idesc = umma_idesc(kTM, kTN, tl.a_mn, tl.b_mn);
-      const uint64_t ad = tl.a_mn ? umma_desc(8192, 1024, 2) : umma_desc(16, 8 * kBK * 2, 4);
-      const uint64_t bd = tl.b_mn ? umma_desc(8192, 1024, 2) : umma_desc(16, 8 * kBK * 2, 4);
-      // second plane, and 16 summed indices further, in bytes
-      const uint32_t alo = tl.a_mn ? 4096 : kTM * kBK * 2, blo = tl.b_mn ? 4096 : kTN * kBK * 2;
-      const uint32_t ak = tl.a_mn ? 2048 : 32, bk = tl.b_mn ? 2048 : 32;
-      uint32_t n = 0, ch = 0;                           // stages and chunks so far
-      bool ok = true;
-      for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-        const uint32_t sp = t / (tl.i_tiles * tl.j_tiles);
-        const uint32_t k0 = sp * tl.blocks_per_split, k1 = min(k0 + tl.blocks_per_split, tl.blocks);
-        for (uint32_t k = k0; k < k1 && ok; ch++) {
-          const uint32_t buf = ch & 1, d = tmem + buf * kTN;
-          if (ch >= 2 && !mma_wait(&sh->acc_empty[buf], ((ch >> 1) - 1) & 1, &sh->gave_up)) {
-            ok = false;
-            break;
-          }
-          tcgen05_after_sync();
-          const uint32_t ke = min(k + kChunkBlocks, k1);
-          bool acc = false;
-          for (; k < ke; k++, n++) {
-            const uint32_t s = n % kStages;
-            if (!mma_wait(&sh->full[s], (n / kStages) & 1, &sh->gave_up)) {
+    } else if (warp == kEpiWarps + 1) {
+      // ---- products
+      if (lane == 0) {
+        const uint32_t idesc = umma_idesc(kTM, kTN, tl.a_mn, tl.b_mn);
+        const uint64_t ad = tl.a_mn ? umma_desc(8192, 1024, 2) : umma_desc(16, 8 * kBK * 2, 4);
+        const uint64_t bd = tl.b_mn ? umma_desc(8192, 1024, 2) : umma_desc(16, 8 * kBK * 2, 4);
+        // second plane, and 16 summed indices further, in bytes
+        const uint32_t alo = tl.a_mn ? 4096 : kTM * kBK * 2, blo = tl.b_mn ? 4096 : kTN * kBK * 2;
+        const uint32_t ak = tl.a_mn ? 2048 : 32, bk = tl.b_mn ? 2048 : 32;
+        uint32_t n = 0, ch = 0;                           // stages and chunks so far
+        bool ok = true;
+        for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+          const uint32_t sp = t / (tl.i_tiles * tl.j_tiles);
+          const uint32_t k0 = sp * tl.blocks_per_split, k1 = min(k0 + tl.blocks_per_split, tl.blocks);
+          for (uint32_t k = k0; k < k1 && ok; ch++) {
+            const uint32_t buf = ch & 1, d = tmem + buf * kTN;
+            if (ch >= 2 && !mma_wait(&sh->acc_empty[buf], ((ch >> 1) - 1) & 1, &sh->gave_up)) {
               ok = false;
               break;
             }
             tcgen05_after_sync();
-            const uint32_t a = smem_u32(stages + (size_t)s * kStageBytes), b = a + kStageA;
-            // the small cross terms first, while the sum is small
+            const uint32_t ke = min(k + kChunkBlocks, k1);
+            bool acc = false;
+            for (; k < ke; k++, n++) {
+              const uint32_t s = n % kStages;
+              if (!mma_wait(&sh->full[s], (n / kStages) & 1, &sh->gave_up)) {
+                ok = false;
+                break;
+              }
+              tcgen05_after_sync();
+              const uint32_t a = smem_u32(stages + (size_t)s * kStageBytes), b = a + kStageA;
+              // the small cross terms first, while the sum is small
 #pragma unroll
-            for (uint32_t q = 0; q < kBK / 16; q++) {
-              umma_f16(d, umma_at(ad, a + alo + q * ak), umma_at(bd, b + q * bk), idesc, acc);
-              umma_f16(d, umma_at(ad, a + q * ak), umma_at(bd, b + blo + q * bk), idesc, true);
-              acc = true;
+              for (uint32_t q = 0; q < kBK / 16; q++) {
+                umma_f16(d, umma_at(ad, a + alo + q * ak), umma_at(bd, b + q * bk), idesc, acc);
+                umma_f16(d, umma_at(ad, a + q * ak), umma_at(bd, b + blo + q * bk), idesc, true);
+                acc = true;
+              }
+#pragma unroll
+              for (uint32_t q = 0; q < kBK / 16; q++) umma_f16(d, umma_at(ad, a + q * ak), umma_at(bd, b + q * bk), idesc, true);
+              umma_commit(&sh->empty[s]);
             }
-#pragma unroll
-            for (uint32_t q = 0; q < kBK / 16; q++) umma_f16(d, umma_at(ad, a + q * ak), umma_at(bd, b + q * bk), idesc, true);
-            umma_commit(&sh->empty[s]);
+            if (!ok) break;
+            umma_commit(&sh->acc_full[buf]);
           }
-          if (!ok) break;
-          umma_commit(&sh->acc_full[buf]);
         }
+        // every product issued is done before TMEM is freed
+        umma_commit(&sh->drain);
+        for (uint32_t i = 0; i < kWaitSpins && !mbar_try_wait(&sh->drain, 0); i++) __nanosleep(64);
       }
-      // every product issued is done before TMEM is freed
-      umma_commit(&sh->drain);
-      for (uint32_t i = 0; i < kWaitSpins && !mbar_try_wait(&sh->drain, 0); i++) __nanosleep(64);
     }
   } else {
     // ---- accumulators -> registers -> epilogue
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
     const int q = warp & 3, quarter = warp >> 2;
     const uint32_t lane_addr = (uint32_t)(q * 32) << 16;
     uint32_t ch = 0, turn = 0;
@@ -228,7 +239,8 @@ mma_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUt
       }
       // the epilogue has barriers of its own: all of its warps run it, or none
       if (epi_any(!ok)) break;
-      const TileAt at{(int64_t)it * kTM + q * 32 + lane, (int64_t)jt * kTN + quarter * 64, it, jt, sp, turn, quarter, q * 32 + lane, sh};
+      const TileAt at{(int64_t)it * kTM + q * 32 + lane, (int64_t)jt * kTN + quarter * 64, it, jt, sp, turn, quarter, q * 32 + lane,
+                      1.0f + 0.75f * 0x1p-23f * (float)min((uint32_t)kChunkBlocks, k1 - k0), sh};
       epi(acc, at);
     }
   }
@@ -246,9 +258,9 @@ struct Unscale {
   __device__ __forceinline__ float operator()(float v) const { return v * a * b; }
 };
 // 2^-e in two factors (e may exceed the exponent range of one Float32)
-__device__ __forceinline__ Unscale unscale(int e) {
+__device__ __forceinline__ Unscale unscale(int e, float gain = 1.0f) {
   const int h = e / 2;
-  return Unscale{scalbnf(1.0f, -h), scalbnf(1.0f, -(e - h))};
+  return Unscale{scalbnf(gain, -h), scalbnf(1.0f, -(e - h))};
 }
 __device__ __forceinline__ int scale_exponent(uint32_t max_bits) {
   if (max_bits == 0) return 0;
@@ -347,9 +359,8 @@ lnll_split_kernel(SplitJob a, SplitJob b, uint32_t blocks_a, const uint32_t* __r
 }
 
 // ---- epilogues -------------------------------------------------------------------------------------------
-// A thread holds 64 columns of one row.  The epilogue has to stay below the time of two chunks (the
-// tensor core runs ahead by that much), about 6000 clocks: some 11 instructions per score plus 5 for
-// stores that cover whole 128-byte lines.
+// A thread holds 64 columns of one row.  The epilogue has to stay below the time of two chunks, about
+// 12 000 clocks: the tensor core runs ahead by that much and then waits.
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float exp2_approx(float t) {
@@ -370,11 +381,15 @@ struct MmaStats {
   const float* bias;
   const int32_t* labels;
   float *part_m, *part_s, *label_score;
+  uint32_t* done;              // counter of the joining kernel that follows
   int64_t N, J;                // instances, classes of this launch
   int64_t v0, tile0;           // first class and first tile of this launch
-  __device__ __forceinline__ void stage(int64_t j0, float* to) const { stage_bias(bias, j0, J, to); }
+  __device__ __forceinline__ void stage(int64_t j0, float* to) const {
+    clear_done(done);
+    stage_bias(bias, j0, J, to);
+  }
   __device__ __forceinline__ void operator()(float (&acc)[64], const TileAt& at) const {
-    const Unscale us = unscale(exps[0] + exps[1]);
+    const Unscale us = unscale(exps[0] + exps[1], at.gain);
     const bool live = at.i < N;
     const int64_t lab = live ? (int64_t)labels[at.i] - 1 - v0 - at.j0 : -1;
     const float4* bs = reinterpret_cast<const float4*>(at.sh->bias[at.turn & 1] + at.quarter * 64);
@@ -475,7 +490,7 @@ struct MmaGradScores {
   float* db_part;              // [instance tile][J] or null
   __device__ __forceinline__ void stage(int64_t j0, float* to) const { stage_bias(bias, j0, J, to); }
   __device__ __forceinline__ void operator()(float (&acc)[64], const TileAt& at) const {
-    const Unscale us = unscale(exps[0] + exps[1]);
+    const Unscale us = unscale(exps[0] + exps[1], at.gain);
     const bool live = at.i < N;
     const int32_t label = live ? __ldg(labels + at.i) : 0;    // rows past the last instance act as skipped
     const float hi = live ? __ldg(lse + at.i) : 0.0f, lo = live ? __ldg(lse + N + at.i) : 0.0f;
@@ -553,7 +568,7 @@ struct MmaStore {
   GradScale<float> g;
   __device__ __forceinline__ void stage(int64_t, float*) const { clear_done(done); }
   __device__ __forceinline__ void operator()(float (&acc)[64], const TileAt& at) const {
-    const Unscale us = unscale(which == 2 ? exps[0] + exps[1] : exps[which] + kGradExp);
+    const Unscale us = unscale(which == 2 ? exps[0] + exps[1] : exps[which] + kGradExp, at.gain);
     const float f = part ? 1.0f : g.value();
     const int lane = threadIdx.x & 31, r8 = lane & 7;
     const int64_t row0 = at.i - lane + (lane & ~7);

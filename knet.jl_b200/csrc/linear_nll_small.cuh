@@ -418,8 +418,6 @@ lnll_rows_kernel(const T* __restrict__ scores, int parts, const T* __restrict__ 
   constexpr int KEEP = 8;                      // scores in flight per thread; the first ones stay in registers
   __shared__ T red[32];
   __shared__ double redd[32];
-  __shared__ int redi[32];
-  __shared__ uint32_t last;
   const int sub = threadIdx.x % GROUP;
   const int64_t n = (int64_t)blockIdx.x * (THREADS / GROUP) + threadIdx.x / GROUP;
   const int64_t stride = N * V;
@@ -466,28 +464,12 @@ lnll_rows_kernel(const T* __restrict__ scores, int parts, const T* __restrict__ 
       __threadfence();
     }
   }
-  __syncthreads();
-  if (threadIdx.x == 0) last = atomicAdd(done, 1u);
-  __syncthreads();
-  if (last + 1 != gridDim.x) return;
-  __threadfence();
-  double a = 0.0;
-  int c = 0;
-  for (int64_t k = threadIdx.x; k < N; k += THREADS)
-    if (labels[k] != 0) {
-      a += (double)__ldcg(per_instance + k);
-      c++;
-    }
-  a = block_reduce(a, [](double x, double y) { return x + y; }, 0.0, redd);
-  c = block_reduce(c, [](int x, int y) { return x + y; }, 0, redi);
-  if (threadIdx.x == 0) {
-    *total = (T)a;
-    *count = c;
-  }
+  last_adds_losses<T, THREADS>(per_instance, labels, N, total, count, done);
 }
 
-// The same for many classes: a CTA takes 2048 classes of one instance and leaves their maximum and sum;
-// the last CTA to finish joins them, a warp per instance, and adds the losses.
+// The same for many classes: a CTA takes 2048 classes of one instance and leaves their maximum and sum at
+// [chunk][instance], as the tiles of the larger forms do.  With `done` (few instances) the last CTA to
+// finish joins them, a warp per instance, and adds the losses; else lnll_join_kernel follows.
 constexpr int kChunk = 2048;
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -496,10 +478,8 @@ lnll_chunks_kernel(const T* __restrict__ scores, int parts, const T* __restrict_
                    T* __restrict__ lse, T* __restrict__ per_instance, T* __restrict__ total, int32_t* __restrict__ count,
                    uint32_t* __restrict__ done) {
   __shared__ T red[32];
-  __shared__ double redd[32];
-  __shared__ int redi[32];
   __shared__ uint32_t last;
-  const int64_t n = blockIdx.x / chunks, v0 = (int64_t)(blockIdx.x % chunks) * kChunk;
+  const int64_t n = blockIdx.x / chunks, chunk = blockIdx.x % chunks, v0 = chunk * kChunk;
   const T* x = scores + n * V;
   T t[kChunk / 256];
   T m = -Math<T>::inf();
@@ -519,9 +499,10 @@ lnll_chunks_kernel(const T* __restrict__ scores, int parts, const T* __restrict_
   for (int k = 0; k < kChunk / 256; k++) s += exp_from(t[k], m);
   s = block_reduce(s, [](T a, T b) { return a + b; }, (T)0, red);
   if (threadIdx.x == 0) {
-    part_m[n * chunks + blockIdx.x % chunks] = m;
-    part_s[n * chunks + blockIdx.x % chunks] = s;
+    part_m[chunk * N + n] = m;
+    part_s[chunk * N + n] = s;
   }
+  if (!done) return;
   __threadfence();
   __syncthreads();
   if (threadIdx.x == 0) last = atomicAdd(done, 1u);
@@ -529,34 +510,24 @@ lnll_chunks_kernel(const T* __restrict__ scores, int parts, const T* __restrict_
   if (last + 1 != gridDim.x) return;
   __threadfence();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  double a = 0.0;
-  int c = 0;
   for (int64_t i = warp; i < N; i += 8) {
     T mm = -Math<T>::inf();
-    for (uint32_t k = lane; k < chunks; k += 32) mm = fmax(mm, __ldcg(part_m + i * chunks + k));
+    for (uint32_t k = lane; k < chunks; k += 32) mm = fmax(mm, __ldcg(part_m + k * N + i));
     mm = warp_reduce(mm, [](T p, T q) { return (T)fmax(p, q); });
     double sd = 0.0;
     for (uint32_t k = lane; k < chunks; k += 32) {
-      const T v = __ldcg(part_s + i * chunks + k), d = __ldcg(part_m + i * chunks + k) - mm;
+      const T v = __ldcg(part_s + k * N + i), d = __ldcg(part_m + k * N + i) - mm;
       if (v != (T)0) sd += (double)(v * exp(d));                 // an empty chunk is (-inf, 0)
     }
     sd = warp_reduce(sd, [](double p, double q) { return p + q; });
     if (lane == 0) {
       const int32_t l = labels[i];
-      const T loss = finish_instance(mm, sd, l > 0 && l <= V ? __ldcg(label_score + i) : (T)0, l, V, lse + i, lse + N + i);
-      per_instance[i] = loss;
-      if (l != 0) {
-        a += (double)loss;
-        c++;
-      }
+      per_instance[i] = finish_instance(mm, sd, l > 0 && l <= V ? __ldcg(label_score + i) : (T)0, l, V, lse + i, lse + N + i);
     }
   }
-  a = block_reduce(a, [](double p, double q) { return p + q; }, 0.0, redd);
-  c = block_reduce(c, [](int p, int q) { return p + q; }, 0, redi);
-  if (threadIdx.x == 0) {
-    *total = (T)a;
-    *count = c;
-  }
+  __threadfence();
+  __syncthreads();
+  add_losses<T, 256>(per_instance, labels, N, total, count);
 }
 
 // dS (without g) over the first part of the scores; `blocks` CTAs per instance

@@ -194,8 +194,8 @@ template <typename T> Form form(int64_t V, int64_t H, int64_t N) {
   return fits && (double)V * H * N < (double)(1ll << 32) ? kSmall : kPieces;
 }
 
-// Parts of the summed axes of the three products in kSmall: enough CTAs for two per SM (tiles) or eight
-// (few instances: two run at a time, so a last round of few CTAs costs little), parts of at least 64 or
+// Parts of the summed axes of the three products in kSmall: no more CTAs than two per SM (tiles:
+// a second round would be nearly empty) or eight (few instances: the last round costs little), parts of at least 64 or
 // 256 terms, at most 64 parts.
 struct SmallPlan {
   int64_t few, s_part, x_part, w_part;         // few: by vectors, not tiles; lengths of the parts
@@ -207,7 +207,7 @@ template <typename T> SmallPlan small_plan(int64_t V, int64_t H, int64_t N, int 
   SmallPlan p{};
   p.few = N <= 4 * kFewInstances;
   auto cut = [&](int64_t ctas, int64_t len, int64_t unit, int64_t bytes, int64_t& part, int& parts) {
-    int64_t k = ceil_div((unit == 64 ? 2 : 8) * kPlanSMs, ctas);
+    int64_t k = unit == 64 ? 2 * kPlanSMs / ctas : ceil_div(8 * kPlanSMs, ctas);
     k = k > len / unit ? len / unit : k;
     k = k > 64 ? 64 : k;
     k = k > (64 << 20) / (bytes + 1) ? (64 << 20) / (bytes + 1) : k;

@@ -63,6 +63,33 @@ __device__ __forceinline__ bool mma_wait(uint64_t* bar, uint32_t parity, int* ga
   return false;
 }
 
+// Arithmetic on two neighbours in one instruction.  The epilogues share power and issue slots with the
+// tensor core: packed additions in the drain alone took the scores of 50257 classes x 4096 instances from
+// 857 to 830 us.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
 // what the epilogue of one tile gets besides the accumulators
 struct TileAt {
   int64_t i, j0;               // this thread's row and first of its 64 columns
@@ -217,9 +244,9 @@ mma_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUt
       const uint32_t it = t % tl.i_tiles, r = t / tl.i_tiles, jt = r % tl.j_tiles, sp = r / tl.j_tiles;
       const uint32_t k0 = sp * tl.blocks_per_split, k1 = min(k0 + tl.blocks_per_split, tl.blocks);
       epi.stage((int64_t)jt * kTN, sh->bias[turn & 1]);  // read after the barrier below
-      float acc[64];
+      float2 acc[32];                                   // 64 columns
 #pragma unroll
-      for (int e = 0; e < 64; e++) acc[e] = 0.0f;
+      for (int e = 0; e < 32; e++) acc[e] = both(0.0f);
       for (uint32_t k = k0; k < k1; k += kChunkBlocks, ch++) {
         const uint32_t buf = ch & 1;
         ok = __all_sync(0xffffffffu, mma_wait(&sh->acc_full[buf], (ch >> 1) & 1, &sh->gave_up));
@@ -231,7 +258,7 @@ mma_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUt
           tmem_load16(tmem + lane_addr + buf * kTN + quarter * 64 + h * 16, v);
           tmem_load_wait();
 #pragma unroll
-          for (int e = 0; e < 16; e++) acc[h * 16 + e] += __uint_as_float(v[e]);
+          for (int e = 0; e < 16; e += 2) acc[h * 8 + e / 2] = add2(acc[h * 8 + e / 2], make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
         }
         tcgen05_before_sync();
         __syncwarp();
@@ -388,39 +415,47 @@ struct MmaStats {
     clear_done(done);
     stage_bias(bias, j0, J, to);
   }
-  __device__ __forceinline__ void operator()(float (&acc)[64], const TileAt& at) const {
+  __device__ __forceinline__ void operator()(float2 (&acc)[32], const TileAt& at) const {
     const Unscale us = unscale(exps[0] + exps[1], at.gain);
     const bool live = at.i < N;
     const int64_t lab = live ? (int64_t)labels[at.i] - 1 - v0 - at.j0 : -1;
     const float4* bs = reinterpret_cast<const float4*>(at.sh->bias[at.turn & 1] + at.quarter * 64);
     float m = -CUDART_INF_F;
     const int in = (int)min((int64_t)64, J - at.j0);        // columns that are classes
+    const float2 ua = both(us.a), ub = both(us.b);
 #pragma unroll
     for (int g = 0; g < 16; g++) {
       const float4 b = bs[g];
-      acc[4 * g] = fmaf(acc[4 * g] * us.a, us.b, b.x);
-      acc[4 * g + 1] = fmaf(acc[4 * g + 1] * us.a, us.b, b.y);
-      acc[4 * g + 2] = fmaf(acc[4 * g + 2] * us.a, us.b, b.z);
-      acc[4 * g + 3] = fmaf(acc[4 * g + 3] * us.a, us.b, b.w);
+      acc[2 * g] = fma2(mul2(acc[2 * g], ua), ub, make_float2(b.x, b.y));
+      acc[2 * g + 1] = fma2(mul2(acc[2 * g + 1], ua), ub, make_float2(b.z, b.w));
     }
     if (in < 64) {
 #pragma unroll
-      for (int e = 0; e < 64; e++)
-        if (e >= in) acc[e] = -CUDART_INF_F;
+      for (int e = 0; e < 32; e++) {
+        if (2 * e >= in) acc[e].x = -CUDART_INF_F;
+        if (2 * e + 1 >= in) acc[e].y = -CUDART_INF_F;
+      }
     }
 #pragma unroll
-    for (int e = 0; e < 64; e++) m = fmaxf(m, acc[e]);
+    for (int e = 0; e < 32; e++) m = fmaxf(m, fmaxf(acc[e].x, acc[e].y));
     if (lab >= 0 && lab < 64) {
       float s = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 64; e++)
-        if (lab == e) s = acc[e];
+      for (int e = 0; e < 32; e++) {
+        if (lab == 2 * e) s = acc[e].x;
+        if (lab == 2 * e + 1) s = acc[e].y;
+      }
       label_score[at.i] = s;
     }
     const float ref = m == -CUDART_INF_F ? 0.0f : m;        // all masked: every term is 0
-    float s = 0.0f;
+    const float2 nref = both(-ref), l2e = both(kLog2e);
+    float2 s2 = both(0.0f);
 #pragma unroll
-    for (int e = 0; e < 64; e++) s += exp2_approx((acc[e] - ref) * kLog2e);
+    for (int e = 0; e < 32; e++) {
+      const float2 t = mul2(add2(acc[e], nref), l2e);
+      s2 = add2(s2, make_float2(exp2_approx(t.x), exp2_approx(t.y)));
+    }
+    const float s = s2.x + s2.y;
     float2(&st)[4][kTM] = at.sh->stat[at.turn & 1];
     st[at.quarter][at.row] = make_float2(m, s);
     epi_sync();
@@ -489,11 +524,12 @@ struct MmaGradScores {
   int64_t N, J, ld, plane, v0;
   float* db_part;              // [instance tile][J] or null
   __device__ __forceinline__ void stage(int64_t j0, float* to) const { stage_bias(bias, j0, J, to); }
-  __device__ __forceinline__ void operator()(float (&acc)[64], const TileAt& at) const {
+  __device__ __forceinline__ void operator()(float2 (&acc)[32], const TileAt& at) const {
     const Unscale us = unscale(exps[0] + exps[1], at.gain);
     const bool live = at.i < N;
     const int32_t label = live ? __ldg(labels + at.i) : 0;    // rows past the last instance act as skipped
     const float hi = live ? __ldg(lse + at.i) : 0.0f, lo = live ? __ldg(lse + N + at.i) : 0.0f;
+    const float2 ua = both(us.a), ub = both(us.b), nhi = both(-hi), nlo = both(-lo), l2e = both(kLog2e), scale = both((float)(1 << kGradExp));
     const int64_t hit64 = (int64_t)label - 1 - v0 - at.j0;
     const int hit = hit64 >= 0 && hit64 < 64 ? (int)hit64 : -1;
     const int in = (int)max((int64_t)0, min((int64_t)64, J - at.j0));
@@ -509,13 +545,14 @@ struct MmaGradScores {
 #pragma unroll
       for (int g = 0; g < 8; g++) {
         const float4 b4 = bs[half * 8 + g];
-        const float b[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-          const int e = 4 * g + k;
-          const float s = fmaf(acc[32 * half + e] * us.a, us.b, b[k]);
-          const float p = exp2_approx(((s - hi) - lo) * kLog2e);
-          d[e] = label == 0 ? 0.0f : p * (float)(1 << kGradExp);
+        for (int k = 0; k < 2; k++) {
+          const int e = 2 * g + k;
+          const float2 s = fma2(mul2(acc[16 * half + e], ua), ub, k ? make_float2(b4.z, b4.w) : make_float2(b4.x, b4.y));
+          const float2 t = mul2(add2(add2(s, nhi), nlo), l2e);
+          const float2 p = mul2(make_float2(exp2_approx(t.x), exp2_approx(t.y)), scale);
+          d[2 * e] = label == 0 ? 0.0f : p.x;
+          d[2 * e + 1] = label == 0 ? 0.0f : p.y;
         }
       }
       if (hit >> 5 == half) {
@@ -567,7 +604,7 @@ struct MmaStore {
   uint32_t* done;              // counter of the statistics kernel that follows, or null
   GradScale<float> g;
   __device__ __forceinline__ void stage(int64_t, float*) const { clear_done(done); }
-  __device__ __forceinline__ void operator()(float (&acc)[64], const TileAt& at) const {
+  __device__ __forceinline__ void operator()(float2 (&acc)[32], const TileAt& at) const {
     const Unscale us = unscale(which == 2 ? exps[0] + exps[1] : exps[which] + kGradExp, at.gain);
     const float f = part ? 1.0f : g.value();
     const int lane = threadIdx.x & 31, r8 = lane & 7;
@@ -578,7 +615,11 @@ struct MmaStore {
     for (int h = 0; h < 2; h++) {
       uint32_t w[32];
 #pragma unroll
-      for (int e = 0; e < 32; e++) w[e] = __float_as_uint(acc[32 * h + e] * us.a * us.b * f);
+      for (int e = 0; e < 16; e++) {
+        const float2 v = mul2(mul2(mul2(acc[16 * h + e], both(us.a)), both(us.b)), both(f));
+        w[2 * e] = __float_as_uint(v.x);
+        w[2 * e + 1] = __float_as_uint(v.y);
+      }
       transpose8(w);
       const int64_t j = at.j0 + 32 * h + 4 * r8;
       float* p = base + row0 * ld + j;

@@ -365,7 +365,8 @@ lnll_split_kernel(SplitJob a, SplitJob b, uint32_t blocks_a, const uint32_t* __r
   const Unscale sc = unscale(-e);
   const int64_t groups = (j.cols + 7) / 8;               // the pitch ld is a multiple of 8
   const int64_t total = groups * j.rows;
-  for (int64_t g = (int64_t)(blockIdx.x - first) * 256 + threadIdx.x; g < total; g += (int64_t)nb * 256) {
+  // from the end: what the maximum's pass read last is still in L2
+  for (int64_t g = total - 1 - ((int64_t)(blockIdx.x - first) * 256 + threadIdx.x); g >= 0; g -= (int64_t)nb * 256) {
     const int64_t r = g / groups, c = (g - r * groups) * 8;
     const float* p = j.src + r * j.pitch + c;
     float v[8];

@@ -194,8 +194,8 @@ template <typename T> Form form(int64_t V, int64_t H, int64_t N) {
   return fits && (double)V * H * N < (double)(1ll << 32) ? kSmall : kPieces;
 }
 
-// Parts of the summed axes of the three products in kSmall: no more CTAs than two per SM (tiles:
-// a second round would be nearly empty) or eight (few instances: the last round costs little), parts of at least 64 or
+// Parts of the summed axes of the three products in kSmall: no more CTAs than three per SM (tiles:
+// all run at once) or eight (few instances: the last round costs little), parts of at least 64 or
 // 256 terms, at most 64 parts.
 struct SmallPlan {
   int64_t few, s_part, x_part, w_part;         // few: by vectors, not tiles; lengths of the parts
@@ -207,7 +207,7 @@ template <typename T> SmallPlan small_plan(int64_t V, int64_t H, int64_t N, int 
   SmallPlan p{};
   p.few = N <= 4 * kFewInstances;
   auto cut = [&](int64_t ctas, int64_t len, int64_t unit, int64_t bytes, int64_t& part, int& parts) {
-    int64_t k = unit == 64 ? 2 * kPlanSMs / ctas : ceil_div(8 * kPlanSMs, ctas);
+    int64_t k = unit == 64 ? 3 * kPlanSMs / ctas : ceil_div(8 * kPlanSMs, ctas);
     k = k > len / unit ? len / unit : k;
     k = k > 64 ? 64 : k;
     k = k > (64 << 20) / (bytes + 1) ? (64 << 20) / (bytes + 1) : k;
@@ -494,7 +494,7 @@ void statistics(const Head<T>& h, const T* scores, int parts, int64_t chunks, T*
     if (!few)
       lnll_join_kernel<T><<<(unsigned)ceil_div(h.N, 32), 1024, 0, st>>>(pm, ps, stats, h.labels, h.N, h.V, chunks, lse, per_instance, total,
                                                                        count, done);
-  } else if (h.V <= 512) {
+  } else if (h.V <= 64 || (h.V <= 512 && h.N >= 2048)) {      // a warp per instance where there are many, or little to do
     lnll_rows_kernel<T, 32><<<(unsigned)ceil_div(h.N, 8), 256, 0, st>>>(scores, parts, h.bias, h.labels, h.N, h.V, lse, per_instance, total,
                                                                        count, done);
   } else {
@@ -602,9 +602,14 @@ template <typename T>
 int linear_nll_bwd_small(const Head<T>& h, const T* lse, GradScale<T> g, T* dw, T* db, T* dx, char* ws, cudaStream_t st) {
   const SmallPlan p = small_plan<T>(h.V, h.H, h.N, h.trans, 1);
   T *ds = (T*)(ws + p.scores), *parts = (T*)(ws + p.parts);
-  small_scores(h, p, nullptr, ds, st);
-  const int64_t blocks = ceil_div(h.V, 1024);
-  lnll_grad_kernel<T><<<(unsigned)(blocks * h.N), 256, 0, st>>>(ds, p.s_parts, h.bias, h.labels, lse, h.N, h.V, (uint32_t)blocks);
+  if (!p.few && p.s_parts == 1) {
+    simt_product<T>(Strided<T>{h.x, h.H, 1}, h.weights(0), h.N, h.V, h.H, h.H, nullptr,
+                    GradScoresEpi<T>{h.bias, h.labels, lse, ds, h.N, h.V, 0}, st);
+  } else {
+    small_scores(h, p, nullptr, ds, st);
+    const int64_t blocks = ceil_div(h.V, 1024);
+    lnll_grad_kernel<T><<<(unsigned)(blocks * h.N), 256, 0, st>>>(ds, p.s_parts, h.bias, h.labels, lse, h.N, h.V, (uint32_t)blocks);
+  }
   if (db) lnll_bias_kernel<T><<<(unsigned)ceil_div(h.V, 32), 1024, 0, st>>>(ds, h.V, h.N, h.V, db, g);
   const Matrix<T> m = weight_matrix(h);
   if (dx) {

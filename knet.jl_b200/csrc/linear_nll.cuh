@@ -54,6 +54,24 @@ template <typename T> __device__ __forceinline__ T sum_parts(const T* p, int64_t
   return s;
 }
 
+// K scores v, v + STEP, ... of one instance: their parts in order, one part of all of them at a time so
+// that the loads overlap, and the bias; -inf past the last class
+template <typename T, int K, int STEP>
+__device__ __forceinline__ void load_scores(T (&t)[K], const T* x, int64_t v, int64_t V, int64_t stride, int parts, const T* bias) {
+#pragma unroll
+  for (int k = 0; k < K; k++) t[k] = v + k * STEP < V ? x[v + k * STEP] : -Math<T>::inf();
+  for (int p = 1; p < parts; p++) {
+#pragma unroll
+    for (int k = 0; k < K; k++)
+      if (v + k * STEP < V) t[k] += x[p * stride + v + k * STEP];
+  }
+  if (bias) {
+#pragma unroll
+    for (int k = 0; k < K; k++)
+      if (v + k * STEP < V) t[k] += __ldg(bias + v + k * STEP);
+  }
+}
+
 // total and count over the instances in a fixed order, by one CTA
 template <typename T, int THREADS>
 __device__ __forceinline__ void add_losses(const T* per_instance, const int32_t* __restrict__ labels, int64_t N, T* total, int32_t* count) {

@@ -657,13 +657,19 @@ lnll_grad_planes_kernel(const float* __restrict__ scores, int parts, const float
   const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x, n0 = (int64_t)blockIdx.y * kGradRows;
   if (v >= ld) return;
   const float b = bias && v < V ? bias[v] : 0.0f;
-  float sum = 0.0f;
+  float t[kGradRows], sum = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kGradRows; k++) t[k] = v < V && n0 + k < N ? scores[(n0 + k) * V + v] : 0.0f;
+  for (int p = 1; p < parts; p++) {
+#pragma unroll
+    for (int k = 0; k < kGradRows; k++)
+      if (v < V && n0 + k < N) t[k] += scores[p * N * V + (n0 + k) * V + v];
+  }
 #pragma unroll
   for (int k = 0; k < kGradRows; k++) {
     const int64_t n = n0 + k;
     if (n >= N) break;
-    float d = 0.0f;
-    if (v < V) d = grad_score(sum_parts(scores + n * V + v, N * V, parts) + b, lse[n], lse[N + n], labels[n], v);
+    const float d = v < V ? grad_score(t[k] + b, lse[n], lse[N + n], labels[n], v) : 0.0f;
     sum += d;
     __half h, l;
     split_half(d * (float)(1 << kGradExp), h, l);

@@ -18,29 +18,46 @@ template <typename T> struct Strided {
 };
 
 // ---- tiles ---------------------------------------------------------------------------------------
-// acc(i, j) = sum_c A(i, c) * B(j, c) over a part of c, for a 64x64 tile of (i, j), c in steps of 16
-// through shared memory, the next step's operands loaded into registers meanwhile.  Operands have any
-// strides with one of the two equal to 1.
-constexpr int kTile = 64, kStep = 16, kSimtThreads = 256;
+// acc(i, j) = sum_c A(i, c) * B(j, c) over a part of c, for a 64x64 tile of (i, j), c in steps through
+// shared memory: four steps of 16 (Float64: 8) are in flight as asynchronous copies of single elements,
+// which may go anywhere, so operands have any strides with one of the two equal to 1.
+constexpr int kTile = 64, kSimtThreads = 256, kSimtStages = 4;
+template <typename T> constexpr int kStep = sizeof(T) == 8 ? 8 : 16;
 
-template <typename T>
-__device__ __forceinline__ void tile_fetch(T (&reg)[4], const Strided<T>& a, int64_t i0, int64_t c0, int64_t I, int64_t C) {
-#pragma unroll
-  for (int r = 0; r < 4; r++) {
-    // neighbouring threads walk the contiguous axis
-    const int i = a.sc == 1 ? threadIdx.x / kStep + 16 * r : threadIdx.x % kTile;
-    const int c = a.sc == 1 ? threadIdx.x % kStep : threadIdx.x / kTile + 4 * r;
-    reg[r] = i0 + i < I && c0 + c < C ? a.p[(i0 + i) * a.si + (c0 + c) * a.sc] : (T)0;
-  }
+// one element into shared memory, 0 where `in` is false (the address is then not read)
+template <typename T> __device__ __forceinline__ void copy_element(T* dst, const T* src, bool in) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src),
+               "n"((int)sizeof(T)), "r"(in ? (int)sizeof(T) : 0)
+               : "memory");
 }
-template <typename T>
-__device__ __forceinline__ void tile_put(T (&dst)[kStep][kTile + 4], const T (&reg)[4], bool c_contiguous) {
+
+// this thread's elements of one operand's steps: neighbouring threads walk the contiguous axis
+template <typename T> struct TileCopy {
+  static constexpr int S = kStep<T>, PER = S * kTile / kSimtThreads;
+  const T* p[PER];
+  uint32_t at[PER];            // places in a stage
+  int c[PER];                  // summed index in a step; past any bound for a row outside
+  int64_t advance;
+  __device__ __forceinline__ TileCopy(const Strided<T>& a, int64_t i0, int64_t c0, int64_t I) : advance(S * a.sc) {
 #pragma unroll
-  for (int r = 0; r < 4; r++) {
-    if (c_contiguous) dst[threadIdx.x % kStep][threadIdx.x / kStep + 16 * r] = reg[r];
-    else dst[threadIdx.x / kTile + 4 * r][threadIdx.x % kTile] = reg[r];
+    for (int r = 0; r < PER; r++) {
+      const int i = a.sc == 1 ? threadIdx.x / S + kSimtThreads / S * r : threadIdx.x % kTile;
+      const int k = a.sc == 1 ? threadIdx.x % S : threadIdx.x / kTile + kSimtThreads / kTile * r;
+      const bool in = i0 + i < I;
+      p[r] = in ? a.p + (i0 + i) * a.si + (c0 + k) * a.sc : a.p;
+      at[r] = (uint32_t)(k * (kTile + 4) + i);
+      c[r] = in ? k : 1 << 30;
+    }
   }
-}
+  // step k into `stage`; `left` summed indices remain from its first on
+  __device__ __forceinline__ void start(T* stage, int k, int64_t left) {
+#pragma unroll
+    for (int r = 0; r < PER; r++) {
+      const bool in = c[r] < left;
+      copy_element(stage + at[r], in ? p[r] + k * advance : p[r], in);
+    }
+  }
+};
 
 // D += A * B for 8 x 8 doubles, 4 summed indices, by one warp: lane holds A(lane/4, lane%4),
 // B(lane%4, lane/4) and D(lane/4, 2*(lane%4) + {0, 1})
@@ -51,14 +68,14 @@ __device__ __forceinline__ void dmma(double (&d)[2], double a, double b) {
 template <typename T> struct TileShared {
   union {
     struct {
-      T a[2][kStep][kTile + 4], b[2][kStep][kTile + 4];
+      T a[kSimtStages][kStep<T>][kTile + 4], b[kSimtStages][kStep<T>][kTile + 4];
     } in;
     T out[kTile][kTile + 1];
   };
 };
 
 template <typename T, typename Epi>
-__global__ void __launch_bounds__(kSimtThreads)
+__global__ void __launch_bounds__(kSimtThreads, 3)
 simt_product_kernel(Strided<T> a, Strided<T> b, int64_t I, int64_t J, int64_t C, int64_t c_part, uint32_t* done, Epi epi) {
   clear_done(done);
   __shared__ __align__(16) TileShared<T> sh;
@@ -72,21 +89,27 @@ simt_product_kernel(Strided<T> a, Strided<T> b, int64_t I, int64_t J, int64_t C,
     for (int w = 0; w < 4; w++) acc[u][w] = (T)0;
   // Float64: warp w owns rows 32*(w%2).. and columns 16*(w/2).. as 4 x 2 blocks of 8 x 8
   const int lane = threadIdx.x & 31, wr = (threadIdx.x >> 5 & 1) * 32, wc = (threadIdx.x >> 6) * 16;
-  T ra[4], rb[4];
-  tile_fetch<T>(ra, a, i0, c_lo, I, c_hi);
-  tile_fetch<T>(rb, b, j0, c_lo, J, c_hi);
-  int buf = 0;
-  for (int64_t c0 = c_lo; c0 < c_hi; c0 += kStep, buf ^= 1) {
-    tile_put<T>(sh.in.a[buf], ra, a.sc == 1);
-    tile_put<T>(sh.in.b[buf], rb, b.sc == 1);
-    __syncthreads();
-    if (c0 + kStep < c_hi) {
-      tile_fetch<T>(ra, a, i0, c0 + kStep, I, c_hi);
-      tile_fetch<T>(rb, b, j0, c0 + kStep, J, c_hi);
+  constexpr int S = kStep<T>;
+  const int steps = (int)((c_hi - c_lo + S - 1) / S);
+  TileCopy<T> ca(a, i0, c_lo, I), cb(b, j0, c_lo, J);
+  auto start = [&](int k) {
+    if (k < steps) {
+      const int64_t left = c_hi - c_lo - (int64_t)k * S;
+      ca.start(&sh.in.a[k % kSimtStages][0][0], k, left);
+      cb.start(&sh.in.b[k % kSimtStages][0][0], k, left);
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");      // empty past the last step, so that the count stays right
+  };
+#pragma unroll
+  for (int k = 0; k < kSimtStages - 1; k++) start(k);
+  for (int k = 0; k < steps; k++) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kSimtStages - 2) : "memory");
+    __syncthreads();                                          // step k has landed; step k - 1 has been used by all
+    start(k + kSimtStages - 1);
+    const int buf = k % kSimtStages;
     if constexpr (sizeof(T) == 8) {
 #pragma unroll
-      for (int c = 0; c < kStep; c += 4) {
+      for (int c = 0; c < S; c += 4) {
         double av[4], bv[2];
 #pragma unroll
         for (int u = 0; u < 4; u++) av[u] = sh.in.a[buf][c + (lane & 3)][wr + 8 * u + (lane >> 2)];
@@ -100,7 +123,7 @@ simt_product_kernel(Strided<T> a, Strided<T> b, int64_t I, int64_t J, int64_t C,
       }
     } else {
 #pragma unroll
-      for (int c = 0; c < kStep; c++) {
+      for (int c = 0; c < S; c++) {
         T av[4], bv[4];
 #pragma unroll
         for (int u = 0; u < 4; u++) av[u] = sh.in.a[buf][c][ty * 4 + u];
@@ -114,6 +137,7 @@ simt_product_kernel(Strided<T> a, Strided<T> b, int64_t I, int64_t J, int64_t C,
     }
   }
   if constexpr (sizeof(T) == 8) {      // from the blocks to 4 x 4 per thread, as the epilogues expect it
+    asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < 4; u++)
@@ -423,20 +447,14 @@ lnll_rows_kernel(const T* __restrict__ scores, int parts, const T* __restrict__ 
   const int64_t stride = N * V;
   if (GROUP == THREADS || n < N) {
     const T* x = scores + n * V;
-    auto score = [&](int64_t v) { return (T)(sum_parts(x + v, stride, parts) + (bias ? __ldg(bias + v) : (T)0)); };
     T keep[KEEP];
     T m = -Math<T>::inf();
-#pragma unroll
-    for (int k = 0; k < KEEP; k++) {
-      const int64_t v = sub + (int64_t)k * GROUP;
-      keep[k] = v < V ? score(v) : -Math<T>::inf();
-    }
+    load_scores<T, KEEP, GROUP>(keep, x, sub, V, stride, parts, bias);
 #pragma unroll
     for (int k = 0; k < KEEP; k++) m = fmax(m, keep[k]);
     for (int64_t v0 = sub + (int64_t)KEEP * GROUP; v0 < V; v0 += (int64_t)KEEP * GROUP) {
       T t[KEEP];
-#pragma unroll
-      for (int k = 0; k < KEEP; k++) t[k] = v0 + (int64_t)k * GROUP < V ? score(v0 + (int64_t)k * GROUP) : -Math<T>::inf();
+      load_scores<T, KEEP, GROUP>(t, x, v0, V, stride, parts, bias);
 #pragma unroll
       for (int k = 0; k < KEEP; k++) m = fmax(m, t[k]);
     }
@@ -448,8 +466,7 @@ lnll_rows_kernel(const T* __restrict__ scores, int parts, const T* __restrict__ 
     for (int k = 0; k < KEEP; k++) s += (double)exp_from(keep[k], m);
     for (int64_t v0 = sub + (int64_t)KEEP * GROUP; v0 < V; v0 += (int64_t)KEEP * GROUP) {
       T t[KEEP];
-#pragma unroll
-      for (int k = 0; k < KEEP; k++) t[k] = v0 + (int64_t)k * GROUP < V ? score(v0 + (int64_t)k * GROUP) : -Math<T>::inf();
+      load_scores<T, KEEP, GROUP>(t, x, v0, V, stride, parts, bias);
       T e = (T)0;
 #pragma unroll
       for (int k = 0; k < KEEP; k++) e += exp_from(t[k], m);
@@ -460,7 +477,8 @@ lnll_rows_kernel(const T* __restrict__ scores, int parts, const T* __restrict__ 
     else s = block_reduce(s, plus, 0.0, redd);
     if (sub == 0) {
       const int32_t lab = labels[n];
-      per_instance[n] = finish_instance(m, s, lab > 0 && lab <= V ? score(lab - 1) : (T)0, lab, V, lse + n, lse + N + n);
+      per_instance[n] = finish_instance(m, s, lab > 0 && lab <= V ? (T)(sum_parts(x + lab - 1, stride, parts) + (bias ? bias[lab - 1] : (T)0)) : (T)0,
+                                        lab, V, lse + n, lse + N + n);
       __threadfence();
     }
   }
@@ -484,13 +502,10 @@ lnll_chunks_kernel(const T* __restrict__ scores, int parts, const T* __restrict_
   T t[kChunk / 256];
   T m = -Math<T>::inf();
   const int64_t lab = (int64_t)labels[n] - 1 - v0;
+  load_scores<T, kChunk / 256, 256>(t, x, v0 + threadIdx.x, V, N * V, parts, bias);
 #pragma unroll
-  for (int k = 0; k < kChunk / 256; k++) {
-    const int c = k * 256 + threadIdx.x;
-    const int64_t v = v0 + c;
-    t[k] = v < V ? (T)(sum_parts(x + v, N * V, parts) + (bias ? __ldg(bias + v) : (T)0)) : -Math<T>::inf();
-    if (c == lab && v < V) label_score[n] = t[k];
-  }
+  for (int k = 0; k < kChunk / 256; k++)
+    if (k * 256 + threadIdx.x == lab && v0 + lab < V) label_score[n] = t[k];
 #pragma unroll
   for (int k = 0; k < kChunk / 256; k++) m = fmax(m, t[k]);
   m = block_reduce(m, [](T a, T b) { return (T)fmax(a, b); }, (T)-Math<T>::inf(), red);
@@ -539,11 +554,12 @@ lnll_grad_kernel(T* __restrict__ scores, int parts, const T* __restrict__ bias, 
   const T hi = lse[n], lo = lse[N + n];
   const int32_t lab = labels[n];
   T* x = scores + n * V;
+  const int64_t v0 = (int64_t)(blockIdx.x % blocks) * 1024 + threadIdx.x;
+  T t[4];
+  load_scores<T, 4, 256>(t, x, v0, V, N * V, parts, bias);
 #pragma unroll
-  for (int k = 0; k < 4; k++) {
-    const int64_t v = (int64_t)(blockIdx.x % blocks) * 1024 + k * 256 + threadIdx.x;
-    if (v < V) x[v] = grad_score((T)(sum_parts(x + v, N * V, parts) + (bias ? bias[v] : (T)0)), hi, lo, lab, v);
-  }
+  for (int k = 0; k < 4; k++)
+    if (v0 + k * 256 < V) x[v0 + k * 256] = grad_score(t[k], hi, lo, lab, v0 + k * 256);
 }
 
 // out = g * (the parts, added in order)

@@ -393,9 +393,10 @@ gclip_apply_kernel(const knet_tensor_desc* __restrict__ table, int ntensors, con
   __shared__ int s_t;
   const double f = *factor;
   if (f == 1.0) return;
-  knet_tensor_desc d = table[find_tensor(table, ntensors, blockIdx.x, &s_t)];
+  const int chunk = (int)(gridDim.x - 1 - blockIdx.x);      // from the end, which the norm's pass read last
+  knet_tensor_desc d = table[find_tensor(table, ntensors, chunk, &s_t)];
   d.p[0] = d.p[1];
-  opt_chunk<T, ScaleF<T>>(ScaleF<T>{f}, d, (int64_t)blockIdx.x - d.first_chunk);
+  opt_chunk<T, ScaleF<T>>(ScaleF<T>{f}, d, (int64_t)chunk - d.first_chunk);
 }
 
 // an update whose gradients are all multiplied by the same device-side factor
@@ -405,8 +406,9 @@ opt_gclip_kernel(F0 f0, const knet_tensor_desc* __restrict__ table, int ntensors
   const auto f = resolve(f0);
   typedef typename std::remove_cv<typename std::remove_reference<decltype(f)>::type>::type F;
   __shared__ int s_t;
-  const knet_tensor_desc d = table[find_tensor(table, ntensors, blockIdx.x, &s_t)];
-  opt_chunk<T, ClipF<F>>(ClipF<F>{f, *factor}, d, (int64_t)blockIdx.x - d.first_chunk);
+  const int chunk = (int)(gridDim.x - 1 - blockIdx.x);      // from the end, which the norm's pass read last
+  const knet_tensor_desc d = table[find_tensor(table, ntensors, chunk, &s_t)];
+  opt_chunk<T, ClipF<F>>(ClipF<F>{f, *factor}, d, (int64_t)chunk - d.first_chunk);
 }
 
 template <typename T>

@@ -196,7 +196,7 @@ template <typename T> Form form(int64_t V, int64_t H, int64_t N) {
 
 // Parts of the summed axes of the three products in kSmall: no more CTAs than three per SM (tiles:
 // all run at once) or eight (few instances: the last round costs little), parts of at least 64 or
-// 256 terms, at most 64 parts.
+// 128 terms, at most 64 parts.
 struct SmallPlan {
   int64_t few, s_part, x_part, w_part;         // few: by vectors, not tiles; lengths of the parts
   int s_parts, x_parts, w_parts;
@@ -217,8 +217,8 @@ template <typename T> SmallPlan small_plan(int64_t V, int64_t H, int64_t N, int 
   };
   const int64_t sz = sizeof(T), groups = ceil_div(N, 8);
   if (p.few) {
-    cut(ceil_div(V, trans ? 32 : 128) * groups, H, 256, N * V * sz, p.s_part, p.s_parts);
-    cut(ceil_div(H, trans ? 128 : 32) * groups, V, 256, N * H * sz, p.x_part, p.x_parts);
+    cut(ceil_div(V, trans ? 32 : 128) * groups, H, 128, N * V * sz, p.s_part, p.s_parts);
+    cut(ceil_div(H, trans ? 128 : 32) * groups, V, 128, N * H * sz, p.x_part, p.x_parts);
     p.w_parts = 1;
   } else {
     cut(ceil_div(N, kTile) * ceil_div(V, kTile), H, 64, N * V * sz, p.s_part, p.s_parts);
@@ -546,7 +546,7 @@ inline int linear_nll_bwd_mma(const Head<float>& h, const float* lse, GradScale<
       if (int rc = mma_product(s.x, false, s.w, !h.trans, h.N, vp, h.H, 1, e1, st)) return rc;
     }
     if (db)
-      lnll_bias_parts_kernel<<<(unsigned)ceil_div(vp, 256), 256, 0, st>>>(dbp, vp, ceil_div(h.N, p.s_parts > 1 ? kGradRows : kTM), db + v0, g);
+      lnll_bias_kernel<float><<<(unsigned)ceil_div(vp, 32), 1024, 0, st>>>(dbp, vp, ceil_div(h.N, p.s_parts > 1 ? kGradRows : kTM), vp, db + v0, g);
     if (dx) {
       const int k = mma_parts(vp, p.x_parts);
       const MmaStore e2{exps, 0, k == 1 ? dx : parts, h.N, h.H, h.H, k == 1 ? 0 : h.N * h.H, k == 1 && v0 > 0, nullptr, g};

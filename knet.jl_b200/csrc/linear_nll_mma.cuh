@@ -514,6 +514,23 @@ __device__ __forceinline__ void transpose8(uint32_t (&w)[32]) {
   }
 }
 
+// The 32 rows of 32 words of a warp turned: lane c then holds word c of every row.
+__device__ __forceinline__ void transpose32(uint32_t (&w)[32]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int b = 16; b > 0; b >>= 1) {
+    const bool up = lane & b;
+#pragma unroll
+    for (int k = 0; k < 32; k++)
+      if (!(k & b)) {
+        const uint32_t send = up ? w[k] : w[k | b];
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, send, b);
+        if (up) w[k] = got;
+        else w[k | b] = got;
+      }
+  }
+}
+
 // i = instance, j = class of the piece: dS without g in two fp16 planes, and its sums over the tile's
 // instances for the bias gradient
 struct MmaGradScores {
@@ -537,50 +554,63 @@ struct MmaGradScores {
     const float4* bs = reinterpret_cast<const float4*>(at.sh->bias[at.turn & 1] + at.quarter * 64);
     const int lane = threadIdx.x & 31, r8 = lane & 7;
     const int64_t row0 = at.i - lane + (lane & ~7);           // first of the eight rows of this lane's group
-    // after the exchange this lane holds, of each of the eight rows, 8 classes of one plane
-    const int64_t col = at.j0 + (r8 & 3) * 8;
-    __half* out = ds + (r8 >> 2) * plane + row0 * ld + col;
+    const int64_t col = at.j0 + r8 * 8;                       // after the exchange: 8 classes of each of the eight rows
+    __half* out = ds + row0 * ld + col;
 #pragma unroll
-    for (int half = 0; half < 2; half++) {                    // 32 columns at a time: fewer live registers
-      float d[32];
+    for (int g = 0; g < 16; g++) {
+      const float4 b4 = bs[g];
 #pragma unroll
-      for (int g = 0; g < 8; g++) {
-        const float4 b4 = bs[half * 8 + g];
+      for (int k = 0; k < 2; k++) {
+        float2& d = acc[2 * g + k];
+        const float2 s = fma2(mul2(d, ua), ub, k ? make_float2(b4.z, b4.w) : make_float2(b4.x, b4.y));
+        const float2 t = mul2(add2(add2(s, nhi), nlo), l2e);
+        const float2 p = mul2(make_float2(exp2_approx(t.x), exp2_approx(t.y)), scale);
+        d = label == 0 ? both(0.0f) : p;
+      }
+    }
+    if (hit >= 0) {
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
-          const int e = 2 * g + k;
-          const float2 s = fma2(mul2(acc[16 * half + e], ua), ub, k ? make_float2(b4.z, b4.w) : make_float2(b4.x, b4.y));
-          const float2 t = mul2(add2(add2(s, nhi), nlo), l2e);
-          const float2 p = mul2(make_float2(exp2_approx(t.x), exp2_approx(t.y)), scale);
-          d[2 * e] = label == 0 ? 0.0f : p.x;
-          d[2 * e + 1] = label == 0 ? 0.0f : p.y;
+      for (int e = 0; e < 32; e++) {
+        if (hit == 2 * e) acc[e].x -= (float)(1 << kGradExp);
+        if (hit == 2 * e + 1) acc[e].y -= (float)(1 << kGradExp);
+      }
+    }
+    if (in < 64) {
+#pragma unroll
+      for (int e = 0; e < 32; e++) {
+        if (2 * e >= in) acc[e].x = 0.0f;
+        if (2 * e + 1 >= in) acc[e].y = 0.0f;
+      }
+    }
+    if (db_part) {
+#pragma unroll
+      for (int half = 0; half < 2; half++) {
+        float v[32];
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          v[2 * e] = acc[16 * half + e].x;
+          v[2 * e + 1] = acc[16 * half + e].y;
         }
+        at.sh->colsum[at.row >> 5][at.quarter * 64 + half * 32 + lane] = lane_sum(v);
       }
-      if (hit >> 5 == half) {
+    }
 #pragma unroll
-        for (int e = 0; e < 32; e++)
-          if ((hit & 31) == e) d[e] -= (float)(1 << kGradExp);
-      }
-      if (in < 64) {
+    for (int pl = 0; pl < 2; pl++) {
+      uint32_t w[32];
 #pragma unroll
-        for (int e = 0; e < 32; e++)
-          if (32 * half + e >= in) d[e] = 0.0f;
-      }
-      uint32_t w[32];                                          // 4 groups of the first plane, 4 of the second
-#pragma unroll
-      for (int k = 0; k < 16; k++) {
-        const __half2 h = __floats2half2_rn(d[2 * k], d[2 * k + 1]);
-        const float2 f = __half22float2(h);
-        const __half2 l = __floats2half2_rn(d[2 * k] - f.x, d[2 * k + 1] - f.y);
+      for (int k = 0; k < 32; k++) {
+        __half2 h = __floats2half2_rn(acc[k].x, acc[k].y);
+        if (pl) {
+          const float2 f = __half22float2(h);
+          h = __floats2half2_rn(acc[k].x - f.x, acc[k].y - f.y);
+        }
         w[k] = *reinterpret_cast<const uint32_t*>(&h);
-        w[16 + k] = *reinterpret_cast<const uint32_t*>(&l);
       }
-      if (db_part) at.sh->colsum[at.row >> 5][at.quarter * 64 + half * 32 + lane] = lane_sum(d);
       transpose8(w);
 #pragma unroll
       for (int q = 0; q < 8; q++)
-        if (col + half * 32 < J && row0 + q < N)               // ld is a multiple of 8
-          *reinterpret_cast<uint4*>(out + half * 32 + q * ld) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+        if (col < J && row0 + q < N)                           // ld is a multiple of 8
+          *reinterpret_cast<uint4*>(out + pl * plane + q * ld) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
     }
     if (db_part) {
       epi_sync();
@@ -611,7 +641,7 @@ struct MmaStore {
     const int lane = threadIdx.x & 31, r8 = lane & 7;
     const int64_t row0 = at.i - lane + (lane & ~7);
     float* base = out + at.split * part;
-    const bool wide = (ld & 3) == 0 && ((uintptr_t)base & 15) == 0;
+    const bool wide = (ld & 3) == 0 && (J & 3) == 0 && ((uintptr_t)base & 15) == 0;
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       uint32_t w[32];
@@ -621,28 +651,32 @@ struct MmaStore {
         w[2 * e] = __float_as_uint(v.x);
         w[2 * e + 1] = __float_as_uint(v.y);
       }
-      transpose8(w);
-      const int64_t j = at.j0 + 32 * h + 4 * r8;
-      float* p = base + row0 * ld + j;
+      if (wide) {
+        transpose8(w);
+        const int64_t j = at.j0 + 32 * h + 4 * r8;             // J is a multiple of 4 here
+        float* p = base + row0 * ld + j;
 #pragma unroll
-      for (int q = 0; q < 8; q++) {
-        if (row0 + q >= I) break;
-        float v[4];
-#pragma unroll
-        for (int c = 0; c < 4; c++) v[c] = __uint_as_float(w[4 * q + c]);
-        float* d = p + q * ld;
-        if (wide && j + 4 <= J) {
-          float4 o = make_float4(v[0], v[1], v[2], v[3]);
-          if (add) {
-            const float4 t = *reinterpret_cast<const float4*>(d);
-            o = make_float4(t.x + o.x, t.y + o.y, t.z + o.z, t.w + o.w);
+        for (int q = 0; q < 8; q++)
+          if (row0 + q < I && j < J) {
+            float4 o = make_float4(__uint_as_float(w[4 * q]), __uint_as_float(w[4 * q + 1]), __uint_as_float(w[4 * q + 2]),
+                                   __uint_as_float(w[4 * q + 3]));
+            float4* d = reinterpret_cast<float4*>(p + q * ld);
+            if (add) {
+              const float4 t = *d;
+              o = make_float4(t.x + o.x, t.y + o.y, t.z + o.z, t.w + o.w);
+            }
+            *d = o;
           }
-          *reinterpret_cast<float4*>(d) = o;
-        } else {
+      } else {                                                  // rows start anywhere: a row's 32 columns at a time
+        transpose32(w);
+        const int64_t i0 = at.i - lane, j = at.j0 + 32 * h + lane;
+        float* p = base + i0 * ld + j;
 #pragma unroll
-          for (int c = 0; c < 4; c++)
-            if (j + c < J) d[c] = add ? d[c] + v[c] : v[c];
-        }
+        for (int q = 0; q < 32; q++)
+          if (i0 + q < I && j < J) {
+            float* d = p + q * ld;
+            *d = add ? *d + __uint_as_float(w[q]) : __uint_as_float(w[q]);
+          }
       }
     }
   }
@@ -677,16 +711,6 @@ lnll_grad_planes_kernel(const float* __restrict__ scores, int parts, const float
     ds[plane + n * ld + v] = l;
   }
   if (db_part && v < V) db_part[(int64_t)blockIdx.y * V + v] = sum;
-}
-
-// db[j] = g * sum over the instance tiles of their sums
-__global__ void __launch_bounds__(256)
-lnll_bias_parts_kernel(const float* __restrict__ part, int64_t J, int64_t tiles, float* __restrict__ db, GradScale<float> g) {
-  const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (j >= J) return;
-  float a = 0.0f;
-  for (int64_t t = 0; t < tiles; t++) a += part[t * J + j];
-  db[j] = a * g.value();
 }
 
 }  // namespace kn

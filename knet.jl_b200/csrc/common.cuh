@@ -38,6 +38,30 @@ inline int launch_status() {
   return e == cudaSuccess ? KN_OK : (int)e;
 }
 
+// ---- chains of launches ---------------------------------------------------------------------------
+// A kernel of a chain starts with chain_begin(): the next one may be launched now (its blocks take the
+// room that this grid leaves) and nothing is read or written before the one in front has finished and
+// its results are visible.  launch_chained() allows that early start; behind any other work it is an
+// ordinary launch.  The gap between two dependent kernels shrinks from about 2 us to below 1.
+__device__ __forceinline__ void chain_begin() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_chained(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
 // ---- 16-byte packs ----------------------------------------------------------------------
 template <typename T, int N> struct alignas(sizeof(T) * N) Pack { T v[N]; };
 

@@ -87,6 +87,7 @@ __global__ void __launch_bounds__(1024)
 lnll_join_kernel(const T* __restrict__ part_m, const T* __restrict__ part_s, const T* __restrict__ label_score,
                  const int32_t* __restrict__ labels, int64_t N, int64_t V, int64_t tiles, T* __restrict__ lse,
                  T* __restrict__ per_instance, T* __restrict__ total, int32_t* __restrict__ count, uint32_t* __restrict__ done) {
+  chain_begin();
   __shared__ T sm[32][32];
   __shared__ double ss[32][32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -121,6 +122,7 @@ lnll_join_kernel(const T* __restrict__ part_m, const T* __restrict__ part_s, con
 
 // an empty batch
 template <typename T> __global__ void lnll_none_kernel(T* total, int32_t* count) {
+  chain_begin();
   *total = (T)0;
   *count = 0;
 }
@@ -129,6 +131,7 @@ template <typename T> __global__ void lnll_none_kernel(T* total, int32_t* count)
 template <typename T>
 __global__ void __launch_bounds__(1024)
 lnll_bias_kernel(const T* __restrict__ ds, int64_t ld, int64_t N, int64_t J, T* __restrict__ db, GradScale<T> g) {
+  chain_begin();
   __shared__ T part[32][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t j = (int64_t)blockIdx.x * 32 + lane;
@@ -144,11 +147,12 @@ lnll_bias_kernel(const T* __restrict__ ds, int64_t ld, int64_t N, int64_t J, T* 
 }
 
 template <typename T> __global__ void lnll_zero_kernel(T* p, int64_t n) {
+  chain_begin();
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i < n) p[i] = (T)0;
 }
 template <typename T> void lnll_zero(T* p, int64_t n, cudaStream_t st) {
-  if (p && n > 0) lnll_zero_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(p, n);
+  if (p && n > 0) launch_chained(lnll_zero_kernel<T>, (unsigned)((n + 255) / 256), 256, 0, st, p, n);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------
@@ -336,7 +340,7 @@ template <typename T> size_t workspace_any(int64_t V, int64_t H, int64_t N, int 
 template <typename T, typename Epi>
 void simt_product(Strided<T> a, Strided<T> b, int64_t I, int64_t J, int64_t C, int64_t c_part, uint32_t* done, Epi epi, cudaStream_t st) {
   const dim3 grid((unsigned)ceil_div(J, kTile), (unsigned)ceil_div(I, kTile), (unsigned)ceil_div(C, c_part));
-  simt_product_kernel<T, Epi><<<grid, kSimtThreads, 0, st>>>(a, b, I, J, C, c_part, done, epi);
+  launch_chained(simt_product_kernel<T, Epi>, grid, kSimtThreads, 0, st, a, b, I, J, C, c_part, done, epi);
 }
 
 // packs of VEC elements are possible where base addresses and pitches are multiples of 16 bytes
@@ -353,12 +357,12 @@ void few_product_nb(bool by_row, const Matrix<T>& m, const T* y, int64_t ldy, in
   const bool wide = aligned16(m.p, m.pitch) && m.cols % VEC == 0;
   if (by_row) {
     const dim3 grid((unsigned)ceil_div(m.rows, 32), groups, (unsigned)parts);
-    if (wide && aligned16(y, ldy)) row_dot_kernel<T, NB, VEC><<<grid, 256, 0, st>>>(m, y, ldy, N, part, done, out);
-    else row_dot_kernel<T, NB, 1><<<grid, 256, 0, st>>>(m, y, ldy, N, part, done, out);
+    if (wide && aligned16(y, ldy)) launch_chained(row_dot_kernel<T, NB, VEC>, grid, 256, 0, st, m, y, ldy, N, part, done, out);
+    else launch_chained(row_dot_kernel<T, NB, 1>, grid, 256, 0, st, m, y, ldy, N, part, done, out);
   } else {
     const dim3 grid((unsigned)ceil_div(m.cols, 128), groups, (unsigned)parts);
-    if (wide) col_sum_kernel<T, NB, VEC><<<grid, 256, 0, st>>>(m, y, ldy, N, part, done, out);
-    else col_sum_kernel<T, NB, 1><<<grid, 256, 0, st>>>(m, y, ldy, N, part, done, out);
+    if (wide) launch_chained(col_sum_kernel<T, NB, VEC>, grid, 256, 0, st, m, y, ldy, N, part, done, out);
+    else launch_chained(col_sum_kernel<T, NB, 1>, grid, 256, 0, st, m, y, ldy, N, part, done, out);
   }
 }
 template <typename T>
@@ -431,7 +435,7 @@ int mma_product(const Planes& a, bool a_mn, const Planes& b, bool b_mn, int64_t 
   const uint64_t tiles = (uint64_t)tl.i_tiles * tl.j_tiles * tl.splits;
   if (tiles > 0x7fffffff) return KN_ESIZE;
   const unsigned grid = (unsigned)(tiles < (uint64_t)sm_count() ? tiles : sm_count());
-  mma_kernel<Epi><<<grid, kMmaThreads, kMmaSmem, st>>>(am, bm, tl, epi);
+  launch_chained(mma_kernel<Epi>, grid, kMmaThreads, kMmaSmem, st, am, bm, tl, epi);
   return launch_status();
 }
 
@@ -462,10 +466,10 @@ inline SplitState split_operands(const Head<float>& h, const MmaPlan& p, char* w
   const int64_t n = w.rows * w.cols + x.rows * x.cols;
   const int64_t want = ceil_div(n, 4096);
   const unsigned blocks = (unsigned)(want < kMaxBlocks ? want : kMaxBlocks);
-  lnll_absmax_kernel<<<blocks, 256, 0, st>>>(w, x, absmax);
+  launch_chained(lnll_absmax_kernel, blocks, 256, 0, st, w, x, absmax);
   const int64_t bw = ceil_div(w.rows * ceil_div(w.cols, 8), 1024), bx = ceil_div(x.rows * ceil_div(x.cols, 8), 1024);
   const unsigned na = (unsigned)(bw < 8192 ? bw : 8192), nb = (unsigned)(bx < 8192 ? bx : 8192);
-  lnll_split_kernel<<<na + nb, 256, 0, st>>>(w, x, na, absmax, blocks, exps);
+  launch_chained(lnll_split_kernel, na + nb, 256, 0, st, w, x, na, absmax, blocks, exps);
   return s;
 }
 
@@ -489,16 +493,16 @@ void statistics(const Head<T>& h, const T* scores, int parts, int64_t chunks, T*
   if (chunks) {
     T *pm = stats + h.N, *ps = pm + chunks * h.N;
     const bool few = h.N <= 16;
-    lnll_chunks_kernel<T><<<(unsigned)(chunks * h.N), 256, 0, st>>>(scores, parts, h.bias, h.labels, h.N, h.V, (uint32_t)chunks, pm, ps,
+    launch_chained(lnll_chunks_kernel<T>, (unsigned)(chunks * h.N), 256, 0, st, scores, parts, h.bias, h.labels, h.N, h.V, (uint32_t)chunks, pm, ps,
                                                                    stats, lse, per_instance, total, count, few ? done : nullptr);
     if (!few)
-      lnll_join_kernel<T><<<(unsigned)ceil_div(h.N, 32), 1024, 0, st>>>(pm, ps, stats, h.labels, h.N, h.V, chunks, lse, per_instance, total,
+      launch_chained(lnll_join_kernel<T>, (unsigned)ceil_div(h.N, 32), 1024, 0, st, pm, ps, stats, h.labels, h.N, h.V, chunks, lse, per_instance, total,
                                                                        count, done);
   } else if (h.V <= 64 || (h.V <= 512 && h.N >= 2048)) {      // a warp per instance where there are many, or little to do
-    lnll_rows_kernel<T, 32><<<(unsigned)ceil_div(h.N, 8), 256, 0, st>>>(scores, parts, h.bias, h.labels, h.N, h.V, lse, per_instance, total,
+    launch_chained(lnll_rows_kernel<T, 32>, (unsigned)ceil_div(h.N, 8), 256, 0, st, scores, parts, h.bias, h.labels, h.N, h.V, lse, per_instance, total,
                                                                        count, done);
   } else {
-    lnll_rows_kernel<T, 256><<<(unsigned)h.N, 256, 0, st>>>(scores, parts, h.bias, h.labels, h.N, h.V, lse, per_instance, total, count, done);
+    launch_chained(lnll_rows_kernel<T, 256>, (unsigned)h.N, 256, 0, st, scores, parts, h.bias, h.labels, h.N, h.V, lse, per_instance, total, count, done);
   }
 }
 
@@ -520,7 +524,7 @@ inline int linear_nll_fwd_mma(const Head<float>& h, float* total, int32_t* count
     const MmaStats epi{(const int*)(ws + p.exps), h.bias ? h.bias + v0 : nullptr, h.labels, pm, ps, label, done, h.N, vp, v0, v0 / kTN};
     if (int rc = mma_product(s.x, false, s.w, !h.trans, h.N, vp, h.H, 1, epi, st)) return rc;
   }
-  lnll_join_kernel<float><<<(unsigned)ceil_div(h.N, 32), 1024, 0, st>>>(pm, ps, label, h.labels, h.N, h.V, all, lse, per_instance, total,
+  launch_chained(lnll_join_kernel<float>, (unsigned)ceil_div(h.N, 32), 1024, 0, st, pm, ps, label, h.labels, h.N, h.V, all, lse, per_instance, total,
                                                                        count, done);
   return launch_status();
 }
@@ -539,19 +543,19 @@ inline int linear_nll_bwd_mma(const Head<float>& h, const float* lse, GradScale<
       float* scores = (float*)(ws + p.scores);
       if (int rc = mma_scores(h, p, s, scores, nullptr, ws, st)) return rc;
       const dim3 grid((unsigned)ceil_div(p.dld, 256), (unsigned)ceil_div(h.N, kGradRows));
-      lnll_grad_planes_kernel<<<grid, 256, 0, st>>>(scores, mma_parts(h.H, p.s_parts), h.bias, h.labels, lse, h.N, h.V, (__half*)(ws + p.ds),
+      launch_chained(lnll_grad_planes_kernel, grid, 256, 0, st, scores, mma_parts(h.H, p.s_parts), h.bias, h.labels, lse, h.N, h.V, (__half*)(ws + p.ds),
                                                     p.dld, ds.plane, dbp);
     } else {
       const MmaGradScores e1{exps, h.bias ? h.bias + v0 : nullptr, h.labels, lse, (__half*)(ws + p.ds), h.N, vp, p.dld, ds.plane, v0, dbp};
       if (int rc = mma_product(s.x, false, s.w, !h.trans, h.N, vp, h.H, 1, e1, st)) return rc;
     }
     if (db)
-      lnll_bias_kernel<float><<<(unsigned)ceil_div(vp, 32), 1024, 0, st>>>(dbp, vp, ceil_div(h.N, p.s_parts > 1 ? kGradRows : kTM), vp, db + v0, g);
+      launch_chained(lnll_bias_kernel<float>, (unsigned)ceil_div(vp, 32), 1024, 0, st, dbp, vp, ceil_div(h.N, p.s_parts > 1 ? kGradRows : kTM), vp, db + v0, g);
     if (dx) {
       const int k = mma_parts(vp, p.x_parts);
       const MmaStore e2{exps, 0, k == 1 ? dx : parts, h.N, h.H, h.H, k == 1 ? 0 : h.N * h.H, k == 1 && v0 > 0, nullptr, g};
       if (int rc = mma_product(ds, false, s.w, (bool)h.trans, h.N, h.H, vp, k, e2, st)) return rc;
-      if (k > 1) lnll_sum_kernel<float><<<(unsigned)ceil_div(h.N * h.H, 256), 256, 0, st>>>(parts, h.N * h.H, k, dx, v0 > 0, g);
+      if (k > 1) launch_chained(lnll_sum_kernel<float>, (unsigned)ceil_div(h.N * h.H, 256), 256, 0, st, parts, h.N * h.H, k, dx, v0 > 0, g);
     }
     if (dw) {
       const int k = mma_parts(h.N, p.w_parts);           // more than one only where one piece holds all classes
@@ -560,7 +564,7 @@ inline int linear_nll_bwd_mma(const Head<float>& h, const float* lse, GradScale<
       const MmaStore e3{exps, 1, k == 1 ? out : parts, I, J, h.trans ? h.H : h.V, k == 1 ? 0 : h.V * h.H, 0, nullptr, g};
       if (int rc = h.trans ? mma_product(ds, true, s.x, true, I, J, h.N, k, e3, st) : mma_product(s.x, true, ds, true, I, J, h.N, k, e3, st))
         return rc;
-      if (k > 1) lnll_sum_kernel<float><<<(unsigned)ceil_div(h.V * h.H, 256), 256, 0, st>>>(parts, h.V * h.H, k, dw, 0, g);
+      if (k > 1) launch_chained(lnll_sum_kernel<float>, (unsigned)ceil_div(h.V * h.H, 256), 256, 0, st, parts, h.V * h.H, k, dw, 0, g);
     }
   }
   return launch_status();
@@ -595,7 +599,7 @@ void tile_product_out(Strided<T> a, Strided<T> b, int64_t I, int64_t J, int64_t 
     return;
   }
   simt_product<T>(a, b, I, J, C, c_part, nullptr, PartsEpi<T>{parts}, st);
-  lnll_sum_kernel<T><<<(unsigned)ceil_div(I * J, 256), 256, 0, st>>>(parts, I * J, cuts, out, 0, g);
+  launch_chained(lnll_sum_kernel<T>, (unsigned)ceil_div(I * J, 256), 256, 0, st, parts, I * J, cuts, out, 0, g);
 }
 
 template <typename T>
@@ -608,14 +612,14 @@ int linear_nll_bwd_small(const Head<T>& h, const T* lse, GradScale<T> g, T* dw, 
   } else {
     small_scores(h, p, nullptr, ds, st);
     const int64_t blocks = ceil_div(h.V, 1024);
-    lnll_grad_kernel<T><<<(unsigned)(blocks * h.N), 256, 0, st>>>(ds, p.s_parts, h.bias, h.labels, lse, h.N, h.V, (uint32_t)blocks);
+    launch_chained(lnll_grad_kernel<T>, (unsigned)(blocks * h.N), 256, 0, st, ds, p.s_parts, h.bias, h.labels, lse, h.N, h.V, (uint32_t)blocks);
   }
-  if (db) lnll_bias_kernel<T><<<(unsigned)ceil_div(h.V, 32), 1024, 0, st>>>(ds, h.V, h.N, h.V, db, g);
+  if (db) launch_chained(lnll_bias_kernel<T>, (unsigned)ceil_div(h.V, 32), 1024, 0, st, ds, h.V, h.N, h.V, db, g);
   const Matrix<T> m = weight_matrix(h);
   if (dx) {
     if (p.few) {
       few_product<T>(!h.trans, m, ds, h.V, h.N, p.x_part, p.x_parts, nullptr, parts, st);
-      lnll_sum_kernel<T><<<(unsigned)ceil_div(h.N * h.H, 256), 256, 0, st>>>(parts, h.N * h.H, p.x_parts, dx, 0, g);
+      launch_chained(lnll_sum_kernel<T>, (unsigned)ceil_div(h.N * h.H, 256), 256, 0, st, parts, h.N * h.H, p.x_parts, dx, 0, g);
     } else {
       const Strided<T> w = h.weights(0);
       tile_product_out<T>(Strided<T>{ds, h.V, 1}, Strided<T>{w.p, w.sc, w.si}, h.N, h.H, h.V, p.x_part, p.x_parts, dx, parts, g, st);
@@ -629,8 +633,8 @@ int linear_nll_bwd_small(const Head<T>& h, const T* lse, GradScale<T> g, T* dw, 
     if (p.few) {
       constexpr int VEC = 16 / sizeof(T);
       const dim3 grid((unsigned)ceil_div(R, 64), (unsigned)ceil_div(C, 128));
-      if (aligned16(b, ldb) && aligned16(dw, C)) outer_kernel<T, VEC><<<grid, 256, 0, st>>>(a, lda, b, ldb, h.N, R, C, dw, C, g);
-      else outer_kernel<T, 1><<<grid, 256, 0, st>>>(a, lda, b, ldb, h.N, R, C, dw, C, g);
+      if (aligned16(b, ldb) && aligned16(dw, C)) launch_chained(outer_kernel<T, VEC>, grid, 256, 0, st, a, lda, b, ldb, h.N, R, C, dw, C, g);
+      else launch_chained(outer_kernel<T, 1>, grid, 256, 0, st, a, lda, b, ldb, h.N, R, C, dw, C, g);
     } else {
       tile_product_out<T>(Strided<T>{a, 1, lda}, Strided<T>{b, 1, ldb}, R, C, h.N, p.w_part, p.w_parts, dw, parts, g, st);
     }
@@ -645,7 +649,7 @@ int linear_nll_fwd(const Head<T>& h, T* total, int32_t* count, T* lse, T* per_in
   const size_t need = h.V > 0 && h.H > 0 && h.N > 0 && sizes_ok(h.V, h.H, h.N) ? workspace_any<T>(h.V, h.H, h.N, 0) : 0;
   if (int rc = check(h, ws, have, need)) return rc;
   if (h.N == 0) {
-    lnll_none_kernel<T><<<1, 1, 0, st>>>(total, count);
+    launch_chained(lnll_none_kernel<T>, 1, 1, 0, st, total, count);
     return launch_status();
   }
   const Form f = form<T>(h.V, h.H, h.N);
@@ -660,7 +664,7 @@ int linear_nll_fwd(const Head<T>& h, T* total, int32_t* count, T* lse, T* per_in
   T* part_s = (T*)(p += up((size_t)tiles * h.N * sizeof(T)));
   simt_product<T>(Strided<T>{h.x, h.H, 1}, h.weights(0), h.N, h.V, h.H, h.H, done,
                   StatsEpi<T>{h.bias, h.labels, part_m, part_s, label_score, h.N}, st);
-  lnll_join_kernel<T><<<(unsigned)ceil_div(h.N, 32), 1024, 0, st>>>(part_m, part_s, label_score, h.labels, h.N, h.V, tiles, lse, per_instance,
+  launch_chained(lnll_join_kernel<T>, (unsigned)ceil_div(h.N, 32), 1024, 0, st, part_m, part_s, label_score, h.labels, h.N, h.V, tiles, lse, per_instance,
                                                                    total, count, done);
   return launch_status();
 }
@@ -689,7 +693,7 @@ int linear_nll_bwd(const Head<T>& h, const T* lse, int average, T dy, const int3
     const Strided<T> w = h.weights(v0);
     simt_product<T>(Strided<T>{h.x, h.H, 1}, w, h.N, vp, h.H, h.H, nullptr,
                     GradScoresEpi<T>{h.bias ? h.bias + v0 : nullptr, h.labels, lse, ds, h.N, piece, v0}, st);
-    if (db) lnll_bias_kernel<T><<<(unsigned)((vp + 31) / 32), 1024, 0, st>>>(ds, piece, h.N, vp, db + v0, g);
+    if (db) launch_chained(lnll_bias_kernel<T>, (unsigned)((vp + 31) / 32), 1024, 0, st, ds, piece, h.N, vp, db + v0, g);
     if (dx)
       simt_product<T>(Strided<T>{ds, piece, 1}, Strided<T>{w.p, w.sc, w.si}, h.N, h.H, vp, vp, nullptr, StoreEpi<T>{dx, h.H, v0 > 0, g}, st);
     if (dw && h.trans)

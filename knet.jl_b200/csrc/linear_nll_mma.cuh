@@ -142,6 +142,7 @@ mma_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUt
   __syncthreads();
   tcgen05_after_sync();
   const uint32_t tmem = sh->tmem;
+  chain_begin();
 
   if (warp >= kEpiWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
@@ -307,6 +308,7 @@ constexpr int kMaxBlocks = 592;                         // absmax blocks: 4 per 
 constexpr int kRun = 8192;
 __global__ void __launch_bounds__(256)
 lnll_absmax_kernel(SplitJob a, SplitJob b, uint32_t* __restrict__ part) {
+  chain_begin();
   __shared__ uint32_t red[32];
   for (int k = 0; k < 2; k++) {
     const SplitJob& j = k ? b : a;
@@ -353,6 +355,7 @@ __device__ __forceinline__ void split_half(float v, __half& hi, __half& lo) {
 __global__ void __launch_bounds__(256)
 lnll_split_kernel(SplitJob a, SplitJob b, uint32_t blocks_a, const uint32_t* __restrict__ part, uint32_t parts,
                   int* __restrict__ exps) {
+  chain_begin();
   __shared__ uint32_t red[32];
   const bool second = blockIdx.x >= blocks_a;
   const SplitJob j = second ? b : a;
@@ -688,6 +691,7 @@ __global__ void __launch_bounds__(256)
 lnll_grad_planes_kernel(const float* __restrict__ scores, int parts, const float* __restrict__ bias, const int32_t* __restrict__ labels,
                         const float* __restrict__ lse, int64_t N, int64_t V, __half* __restrict__ ds, int64_t ld, int64_t plane,
                         float* __restrict__ db_part) {
+  chain_begin();
   const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x, n0 = (int64_t)blockIdx.y * kGradRows;
   if (v >= ld) return;
   const float b = bias && v < V ? bias[v] : 0.0f;

@@ -77,6 +77,7 @@ template <typename T> struct TileShared {
 template <typename T, typename Epi>
 __global__ void __launch_bounds__(kSimtThreads, 3)
 simt_product_kernel(Strided<T> a, Strided<T> b, int64_t I, int64_t J, int64_t C, int64_t c_part, uint32_t* done, Epi epi) {
+  chain_begin();
   clear_done(done);
   __shared__ __align__(16) TileShared<T> sh;
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
@@ -205,6 +206,7 @@ template <typename T, int VEC> __device__ __forceinline__ Pack<T, VEC> ld_cached
 template <typename T, int NB, int VEC>
 __global__ void __launch_bounds__(256)
 row_dot_kernel(Matrix<T> m, const T* __restrict__ y, int64_t ldy, int64_t N, int64_t c_part, uint32_t* done, T* __restrict__ parts) {
+  chain_begin();
   clear_done(done);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t r0 = ((int64_t)blockIdx.x * 8 + warp) * 4;
@@ -296,6 +298,7 @@ constexpr int kColRows = 128;
 template <typename T, int NB, int VEC>
 __global__ void __launch_bounds__(256)
 col_sum_kernel(Matrix<T> m, const T* __restrict__ y, int64_t ldy, int64_t N, int64_t r_part, uint32_t* done, T* __restrict__ parts) {
+  chain_begin();
   clear_done(done);
   constexpr int Q = 4 / VEC;                       // packs per thread: 4 columns
   constexpr int YV = NB < 16 / (int)sizeof(T) ? NB : 16 / (int)sizeof(T);
@@ -376,6 +379,7 @@ template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
 outer_kernel(const T* __restrict__ a, int64_t lda, const T* __restrict__ b, int64_t ldb, int64_t N, int64_t R, int64_t C,
              T* __restrict__ out, int64_t ld, GradScale<T> g) {
+  chain_begin();
   constexpr int Q = 4 / VEC, NB = 8;
   __shared__ __align__(16) T as[NB][64];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -438,6 +442,7 @@ __global__ void __launch_bounds__(GROUP < 256 ? 256 : GROUP)
 lnll_rows_kernel(const T* __restrict__ scores, int parts, const T* __restrict__ bias, const int32_t* __restrict__ labels, int64_t N,
                  int64_t V, T* __restrict__ lse, T* __restrict__ per_instance, T* __restrict__ total, int32_t* __restrict__ count,
                  uint32_t* __restrict__ done) {
+  chain_begin();
   constexpr int THREADS = GROUP < 256 ? 256 : GROUP;
   constexpr int KEEP = 8;                      // scores in flight per thread; the first ones stay in registers
   __shared__ T red[32];
@@ -495,6 +500,7 @@ lnll_chunks_kernel(const T* __restrict__ scores, int parts, const T* __restrict_
                    int64_t V, uint32_t chunks, T* __restrict__ part_m, T* __restrict__ part_s, T* __restrict__ label_score,
                    T* __restrict__ lse, T* __restrict__ per_instance, T* __restrict__ total, int32_t* __restrict__ count,
                    uint32_t* __restrict__ done) {
+  chain_begin();
   __shared__ T red[32];
   __shared__ uint32_t last;
   const int64_t n = blockIdx.x / chunks, chunk = blockIdx.x % chunks, v0 = chunk * kChunk;
@@ -550,6 +556,7 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 lnll_grad_kernel(T* __restrict__ scores, int parts, const T* __restrict__ bias, const int32_t* __restrict__ labels,
                  const T* __restrict__ lse, int64_t N, int64_t V, uint32_t blocks) {
+  chain_begin();
   const int64_t n = blockIdx.x / blocks;
   const T hi = lse[n], lo = lse[N + n];
   const int32_t lab = labels[n];
@@ -566,6 +573,7 @@ lnll_grad_kernel(T* __restrict__ scores, int parts, const T* __restrict__ bias, 
 template <typename T>
 __global__ void __launch_bounds__(256)
 lnll_sum_kernel(const T* __restrict__ parts, int64_t n, int count, T* __restrict__ out, int add, GradScale<T> g) {
+  chain_begin();
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= n) return;
   const T a = sum_parts(parts + i, n, count) * g.value();

@@ -355,6 +355,7 @@ int run_clip_factors(const knet_tensor_desc* table, int ntensors, int64_t total_
 template <typename T>
 __global__ void __launch_bounds__(kOptThreads)
 gnorm_chunks_kernel(const knet_tensor_desc* __restrict__ table, int ntensors, double* __restrict__ partials) {
+  chain_begin();
   __shared__ int s_t;
   __shared__ double red[32];
   const knet_tensor_desc d = table[find_tensor(table, ntensors, blockIdx.x, &s_t)];
@@ -370,6 +371,7 @@ gnorm_chunks_kernel(const knet_tensor_desc* __restrict__ table, int ntensors, do
 __global__ void __launch_bounds__(1024)
 gnorm_finish_kernel(const double* __restrict__ partials, int64_t total_chunks, double gclip, double gscale,
                     double* __restrict__ norm, double* __restrict__ factor) {
+  chain_begin();
   __shared__ double red[32];
   double acc = 0.0;
   for (int64_t c = threadIdx.x; c < total_chunks; c += 1024) acc += partials[c];
@@ -390,6 +392,7 @@ template <typename T> struct ScaleF {
 template <typename T>
 __global__ void __launch_bounds__(kOptThreads)
 gclip_apply_kernel(const knet_tensor_desc* __restrict__ table, int ntensors, const double* __restrict__ factor) {
+  chain_begin();
   __shared__ int s_t;
   const double f = *factor;
   if (f == 1.0) return;
@@ -403,6 +406,7 @@ gclip_apply_kernel(const knet_tensor_desc* __restrict__ table, int ntensors, con
 template <typename T, typename F0>
 __global__ void __launch_bounds__(kOptThreads)
 opt_gclip_kernel(F0 f0, const knet_tensor_desc* __restrict__ table, int ntensors, const double* __restrict__ factor) {
+  chain_begin();
   const auto f = resolve(f0);
   typedef typename std::remove_cv<typename std::remove_reference<decltype(f)>::type>::type F;
   __shared__ int s_t;
@@ -418,8 +422,8 @@ int run_gnorm(const knet_tensor_desc* table, int ntensors, int64_t total_chunks,
   if (total_chunks > 0 && (!table || ntensors == 0 || !partials)) return KN_EINVAL;
   if ((uintptr_t)partials % 8 || (uintptr_t)norm % 8 || (uintptr_t)factor % 8) return KN_EALIGN;
   if (total_chunks > 0x7fffffff) return KN_ESIZE;
-  if (total_chunks > 0) gnorm_chunks_kernel<T><<<(unsigned)total_chunks, kOptThreads, 0, st>>>(table, ntensors, partials);
-  gnorm_finish_kernel<<<1, 1024, 0, st>>>(partials, total_chunks, gclip, gscale, norm, factor);
+  if (total_chunks > 0) launch_chained(gnorm_chunks_kernel<T>, (unsigned)total_chunks, kOptThreads, 0, st, table, ntensors, partials);
+  launch_chained(gnorm_finish_kernel, 1, 1024, 0, st, partials, total_chunks, gclip, gscale, norm, factor);
   return launch_status();
 }
 
@@ -429,7 +433,7 @@ int run_gclip_apply(const knet_tensor_desc* table, int ntensors, int64_t total_c
   if (ntensors == 0 || total_chunks == 0) return KN_OK;
   if (!table || !factor) return KN_EINVAL;
   if (total_chunks > 0x7fffffff) return KN_ESIZE;
-  gclip_apply_kernel<T><<<(unsigned)total_chunks, kOptThreads, 0, st>>>(table, ntensors, factor);
+  launch_chained(gclip_apply_kernel<T>, (unsigned)total_chunks, kOptThreads, 0, st, table, ntensors, factor);
   return launch_status();
 }
 
@@ -440,7 +444,7 @@ int run_multi_gclip(const F& f, const knet_tensor_desc* table, int ntensors, int
   if (ntensors == 0 || total_chunks == 0) return KN_OK;
   if (!table || !factor) return KN_EINVAL;
   if (total_chunks > 0x7fffffff) return KN_ESIZE;
-  opt_gclip_kernel<T, F><<<(unsigned)total_chunks, kOptThreads, 0, st>>>(f, table, ntensors, factor);
+  launch_chained(opt_gclip_kernel<T, F>, (unsigned)total_chunks, kOptThreads, 0, st, f, table, ntensors, factor);
   return launch_status();
 }
 

@@ -17,7 +17,7 @@
 
 namespace kn {
 
-// ---- pieces of the vocabulary on FMA tiles (what the other forms leave: many Float64 scores) ------------
+// ---- epilogues of the FMA and FP64 tiles -----------------------------------------------------------------
 // i = instance, j = class: the tile's maximum and sum of exponentials per instance, and the score at
 // the label.  The 16 threads of an instance row are neighbours in a half warp.
 template <typename T> struct StatsEpi {
@@ -380,6 +380,8 @@ inline bool sizes_ok(int64_t V, int64_t H, int64_t N) {
   return V <= 0x7fffffff && H <= most && N <= most && V <= most;
 }
 
+int linear_nll_wait_flag_read_clear() { return wait_flag_read_clear(); }
+
 template <typename T> bool odd(const T* p) { return (uintptr_t)p % sizeof(T) != 0; }
 
 template <typename T> int check(const Head<T>& h, const void* ws, size_t have, size_t need) {
@@ -644,50 +646,23 @@ int linear_nll_bwd_small(const Head<T>& h, const T* lse, GradScale<T> g, T* dw, 
   return launch_status();
 }
 
+// ---- many Float64 scores: pieces of the vocabulary on FP64 tiles -------------------------------------------
 template <typename T>
-int linear_nll_fwd(const Head<T>& h, T* total, int32_t* count, T* lse, T* per_instance, void* ws, size_t have, cudaStream_t st) {
-  if (!total || !count || (h.N > 0 && (!lse || !per_instance))) return KN_EINVAL;
-  if (odd(total) || odd(lse) || odd(per_instance) || (uintptr_t)count % 4) return KN_EALIGN;
-  const size_t need = h.V > 0 && h.H > 0 && h.N > 0 && sizes_ok(h.V, h.H, h.N) ? workspace_any<T>(h.V, h.H, h.N, 0) : 0;
-  if (int rc = check(h, ws, have, need)) return rc;
-  if (h.N == 0) {
-    launch_chained(lnll_none_kernel<T>, 1, 1, 0, st, total, count);
-    return launch_status();
-  }
-  const Form f = form<T>(h.V, h.H, h.N);
-  if constexpr (sizeof(T) == 4)
-    if (f == kMma) return linear_nll_fwd_mma(h, total, count, lse, per_instance, (char*)ws, st);
-  if (f == kSmall) return linear_nll_fwd_small<T>(h, total, count, lse, per_instance, (char*)ws, st);
+int linear_nll_fwd_pieces(const Head<T>& h, T* total, int32_t* count, T* lse, T* per_instance, char* p, cudaStream_t st) {
   const int64_t tiles = ceil_div(h.V, kTile);
-  char* p = (char*)ws;
   uint32_t* done = (uint32_t*)p;
   T* label_score = (T*)(p += up(4));
   T* part_m = (T*)(p += up((size_t)h.N * sizeof(T)));
   T* part_s = (T*)(p += up((size_t)tiles * h.N * sizeof(T)));
   simt_product<T>(Strided<T>{h.x, h.H, 1}, h.weights(0), h.N, h.V, h.H, h.H, done,
                   StatsEpi<T>{h.bias, h.labels, part_m, part_s, label_score, h.N}, st);
-  launch_chained(lnll_join_kernel<T>, (unsigned)ceil_div(h.N, 32), 1024, 0, st, part_m, part_s, label_score, h.labels, h.N, h.V, tiles, lse, per_instance,
-                                                                   total, count, done);
+  launch_chained(lnll_join_kernel<T>, (unsigned)ceil_div(h.N, 32), 1024, 0, st, part_m, part_s, label_score, h.labels, h.N, h.V, tiles, lse,
+                 per_instance, total, count, done);
   return launch_status();
 }
 
 template <typename T>
-int linear_nll_bwd(const Head<T>& h, const T* lse, int average, T dy, const int32_t* count, T* dw, T* db, T* dx, void* ws,
-                   size_t have, cudaStream_t st) {
-  if (h.N > 0 && (!lse || (average && !count))) return KN_EINVAL;
-  if (odd(lse) || odd(dw) || odd(db) || odd(dx) || (uintptr_t)count % 4) return KN_EALIGN;
-  const size_t need = h.V > 0 && h.H > 0 && h.N > 0 && sizes_ok(h.V, h.H, h.N) ? workspace_any<T>(h.V, h.H, h.N, 1) : 0;
-  if (int rc = check(h, ws, have, need)) return rc;
-  if (h.N == 0) {
-    lnll_zero(dw, h.V * h.H, st);
-    lnll_zero(db, h.V, st);
-    return launch_status();
-  }
-  const GradScale<T> g{average ? count : nullptr, dy};
-  const Form f = form<T>(h.V, h.H, h.N);
-  if constexpr (sizeof(T) == 4)
-    if (f == kMma) return linear_nll_bwd_mma(h, lse, g, dw, db, dx, (char*)ws, st);
-  if (f == kSmall) return linear_nll_bwd_small<T>(h, lse, g, dw, db, dx, (char*)ws, st);
+int linear_nll_bwd_pieces(const Head<T>& h, const T* lse, GradScale<T> g, T* dw, T* db, T* dx, char* ws, cudaStream_t st) {
   const int64_t piece = simt_piece<T>(h.V, h.N);
   T* ds = (T*)ws;
   for (int64_t v0 = 0; v0 < h.V; v0 += piece) {
@@ -695,7 +670,7 @@ int linear_nll_bwd(const Head<T>& h, const T* lse, int average, T dy, const int3
     const Strided<T> w = h.weights(v0);
     simt_product<T>(Strided<T>{h.x, h.H, 1}, w, h.N, vp, h.H, h.H, nullptr,
                     GradScoresEpi<T>{h.bias ? h.bias + v0 : nullptr, h.labels, lse, ds, h.N, piece, v0}, st);
-    if (db) launch_chained(lnll_bias_kernel<T>, (unsigned)((vp + 31) / 32), 1024, 0, st, ds, piece, h.N, vp, db + v0, g);
+    if (db) launch_chained(lnll_bias_kernel<T>, (unsigned)ceil_div(vp, 32), 1024, 0, st, ds, piece, h.N, vp, db + v0, g);
     if (dx)
       simt_product<T>(Strided<T>{ds, piece, 1}, Strided<T>{w.p, w.sc, w.si}, h.N, h.H, vp, vp, nullptr, StoreEpi<T>{dx, h.H, v0 > 0, g}, st);
     if (dw && h.trans)
@@ -704,6 +679,47 @@ int linear_nll_bwd(const Head<T>& h, const T* lse, int average, T dy, const int3
       simt_product<T>(Strided<T>{h.x, 1, h.H}, Strided<T>{ds, 1, piece}, h.H, vp, h.N, h.N, nullptr, StoreEpi<T>{dw + v0, h.V, 0, g}, st);
   }
   return launch_status();
+}
+
+template <typename T>
+int linear_nll_fwd(const Head<T>& h, T* total, int32_t* count, T* lse, T* per_instance, void* ws, size_t have, cudaStream_t st) {
+  if (!total || !count || (h.N > 0 && (!lse || !per_instance))) return KN_EINVAL;
+  if (odd(total) || odd(lse) || odd(per_instance) || (uintptr_t)count % 4) return KN_EALIGN;
+  const size_t need = h.V > 0 && h.H > 0 && h.N > 0 && sizes_ok(h.V, h.H, h.N) ? workspace<T>(h.V, h.H, h.N, h.trans, 0) : 0;
+  if (int rc = check(h, ws, have, need)) return rc;
+  if (h.N == 0) {
+    launch_chained(lnll_none_kernel<T>, 1, 1, 0, st, total, count);
+    return launch_status();
+  }
+  const Form f = form<T>(h.V, h.H, h.N);
+  if constexpr (sizeof(T) == 4) {
+    if (f == kMma) return linear_nll_fwd_mma(h, total, count, lse, per_instance, (char*)ws, st);
+  } else if (f == kPieces) {
+    return linear_nll_fwd_pieces<T>(h, total, count, lse, per_instance, (char*)ws, st);
+  }
+  return linear_nll_fwd_small<T>(h, total, count, lse, per_instance, (char*)ws, st);
+}
+
+template <typename T>
+int linear_nll_bwd(const Head<T>& h, const T* lse, int average, T dy, const int32_t* count, T* dw, T* db, T* dx, void* ws,
+                   size_t have, cudaStream_t st) {
+  if (h.N > 0 && (!lse || (average && !count))) return KN_EINVAL;
+  if (odd(lse) || odd(dw) || odd(db) || odd(dx) || (uintptr_t)count % 4) return KN_EALIGN;
+  const size_t need = h.V > 0 && h.H > 0 && h.N > 0 && sizes_ok(h.V, h.H, h.N) ? workspace<T>(h.V, h.H, h.N, h.trans, 1) : 0;
+  if (int rc = check(h, ws, have, need)) return rc;
+  if (h.N == 0) {
+    lnll_zero(dw, h.V * h.H, st);
+    lnll_zero(db, h.V, st);
+    return launch_status();
+  }
+  const GradScale<T> g{average ? count : nullptr, dy};
+  const Form f = form<T>(h.V, h.H, h.N);
+  if constexpr (sizeof(T) == 4) {
+    if (f == kMma) return linear_nll_bwd_mma(h, lse, g, dw, db, dx, (char*)ws, st);
+  } else if (f == kPieces) {
+    return linear_nll_bwd_pieces<T>(h, lse, g, dw, db, dx, (char*)ws, st);
+  }
+  return linear_nll_bwd_small<T>(h, lse, g, dw, db, dx, (char*)ws, st);
 }
 
 }  // namespace kn

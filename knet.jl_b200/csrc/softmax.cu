@@ -1265,12 +1265,13 @@ using namespace kn;
 
 namespace kn {
 int index_wait_flag_read_clear();   // index.cu: the flag of the staged row kernels and of the wait probe
+int linear_nll_wait_flag_read_clear();   // linear_nll.cu: the tensor-core products
 }
 
 KN_EXPORT int knet_device_status(void) {
-  const int a = wait_flag_read_clear(), b = index_wait_flag_read_clear();
-  if (a < 0 || b < 0) return -1;
-  return (a | b) ? 1 : 0;
+  const int a = wait_flag_read_clear(), b = index_wait_flag_read_clear(), c = linear_nll_wait_flag_read_clear();
+  if (a < 0 || b < 0 || c < 0) return -1;
+  return (a | b | c) ? 1 : 0;
 }
 
 #define KN_DEF_SOFTMAX(f, S, T)                                                                     \

@@ -350,8 +350,9 @@ KNET_BOTH_TYPES(KNET_DECL_NLL, nll)
  * (transW 1: the embedding matrix of a tied model), x (H,N), b of V or NULL; labels 1-based
  * Int32, 0 = skip the instance, anything outside 0..V makes the loss NaN.  All column-major.
  * fwd: *total = sum over used instances of lse - s[label], *count = instances used,
- *      per_instance of N their terms (0 when skipped); lse of 2N: log sum_v exp(s_vn) rounded,
- *      then what the rounding left (both are what bwd reads).
+ *      per_instance of N their terms (0 when skipped); lse of 2N + 2: log sum_v exp(s_vn)
+ *      rounded, then what the rounding left, then the scales of W and x.  bwd reads all of it and
+ *      takes the same W, x, b and sizes.
  * bwd: with g = dy (average 0) or dy / *count (average 1; *count 0 gives g = 0),
  *      dx (H,N) = W' dS, dW (as W) = dS x', db (V) = sum over n of dS, where
  *      dS = (softmax - onehot) g, 0 on skipped instances.  Any of dw, db, dx may be NULL; they

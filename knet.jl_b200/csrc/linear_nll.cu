@@ -441,12 +441,29 @@ int mma_product(const Planes& a, bool a_mn, const Planes& b, bool b_mn, int64_t 
   return launch_status();
 }
 
-// absmax and split of w's classes [v0, v0 + vp) and, with the first piece, of x
+// the largest magnitudes of w and x, one value per block of each
+inline unsigned scale_operands(const Head<float>& h, const MmaPlan& p, char* ws, cudaStream_t st) {
+  SplitJob w{}, x{};
+  w.src = h.w;
+  w.rows = h.H;
+  w.cols = w.pitch = h.V;      // whole and contiguous in either layout
+  x.src = h.x;
+  x.rows = h.N;
+  x.cols = x.pitch = h.H;
+  const int64_t want = ceil_div(h.V * h.H + h.N * h.H, 4096);
+  const unsigned blocks = (unsigned)(want < kMaxBlocks ? want : kMaxBlocks);
+  // an ordinary launch: placed under the tail of another kernel, its equal shares would land unevenly on the
+  // SMs (32000x4096 n512, where it ran once per piece: 2.20 against 2.10 ms)
+  lnll_absmax_kernel<<<blocks, 256, 0, st>>>(w, x, (uint32_t*)(ws + p.absmax));
+  return blocks;
+}
+
+// w's classes [v0, v0 + vp) and, with the first piece, x in two planes; see lnll_split_kernel for the scales
 struct SplitState {
   Planes w, x;
 };
-inline SplitState split_operands(const Head<float>& h, const MmaPlan& p, char* ws, int64_t v0, int64_t vp, bool with_x,
-                                 cudaStream_t st) {
+inline SplitState split_operands(const Head<float>& h, const MmaPlan& p, char* ws, int64_t v0, int64_t vp, unsigned parts,
+                                 const float* given, float* saved, cudaStream_t st) {
   SplitJob w, x;
   w.src = h.trans ? h.w + v0 * h.H : h.w + v0;
   w.rows = h.trans ? vp : h.H;
@@ -462,18 +479,10 @@ inline SplitState split_operands(const Head<float>& h, const MmaPlan& p, char* w
   x.ld = p.xld;
   x.plane = x.rows * p.xld;
   const SplitState s{Planes{w.dst, w.rows, w.cols, w.ld, w.plane}, Planes{x.dst, x.rows, x.cols, x.ld, x.plane}};
-  if (!with_x) x.rows = 0;
-  uint32_t* absmax = (uint32_t*)(ws + p.absmax);
-  int* exps = (int*)(ws + p.exps);
-  const int64_t n = w.rows * w.cols + x.rows * x.cols;
-  const int64_t want = ceil_div(n, 4096);
-  const unsigned blocks = (unsigned)(want < kMaxBlocks ? want : kMaxBlocks);
-  // an ordinary launch: placed under the tail of another kernel, its equal shares would land unevenly on the
-  // SMs (32000x4096 n512: 2.20 against 2.10 ms)
-  lnll_absmax_kernel<<<blocks, 256, 0, st>>>(w, x, absmax);
-  const int64_t bw = ceil_div(w.rows * ceil_div(w.cols, 8), 1024), bx = ceil_div(x.rows * ceil_div(x.cols, 8), 1024);
+  const int64_t bw = ceil_div(w.rows * ceil_div(w.cols, 8), 1024), bx = v0 ? 0 : ceil_div(x.rows * ceil_div(x.cols, 8), 1024);
   const unsigned na = (unsigned)(bw < 8192 ? bw : 8192), nb = (unsigned)(bx < 8192 ? bx : 8192);
-  launch_chained(lnll_split_kernel, na + nb, 256, 0, st, w, x, na, absmax, blocks, exps);
+  launch_chained(lnll_split_kernel, na + nb, 256, 0, st, w, x, na, (const uint32_t*)(ws + p.absmax), parts, given, saved,
+                 (int*)(ws + p.exps));
   return s;
 }
 
@@ -514,11 +523,12 @@ inline int linear_nll_fwd_mma(const Head<float>& h, float* total, int32_t* count
                               cudaStream_t st) {
   const MmaPlan p = mma_plan(h.V, h.H, h.N, h.trans, 0);
   const int64_t all = ceil_div(h.V, kTN);
+  const unsigned parts = scale_operands(h, p, ws, st);
   uint32_t* done = (uint32_t*)(ws + p.exps) + 2;
   float *label = (float*)(ws + p.label), *pm = (float*)(ws + p.part_m), *ps = (float*)(ws + p.part_s);
   for (int64_t v0 = 0; v0 < h.V; v0 += p.piece) {
     const int64_t vp = h.V - v0 < p.piece ? h.V - v0 : p.piece;
-    const SplitState s = split_operands(h, p, ws, v0, vp, v0 == 0, st);
+    const SplitState s = split_operands(h, p, ws, v0, vp, parts, nullptr, lse + 2 * h.N, st);
     if (p.s_parts > 1) {      // one piece
       float* scores = (float*)(ws + p.scores);
       if (int rc = mma_scores(h, p, s, scores, done, ws, st)) return rc;
@@ -541,7 +551,7 @@ inline int linear_nll_bwd_mma(const Head<float>& h, const float* lse, GradScale<
   float* dbp = db ? (float*)(ws + p.db) : nullptr;
   for (int64_t v0 = 0; v0 < h.V; v0 += p.piece) {
     const int64_t vp = h.V - v0 < p.piece ? h.V - v0 : p.piece;
-    const SplitState s = split_operands(h, p, ws, v0, vp, v0 == 0, st);
+    const SplitState s = split_operands(h, p, ws, v0, vp, 0, lse + 2 * h.N, nullptr, st);
     const Planes ds{(__half*)(ws + p.ds), h.N, vp, p.dld, h.N * p.dld};
     if (p.s_parts > 1) {
       float* scores = (float*)(ws + p.scores);

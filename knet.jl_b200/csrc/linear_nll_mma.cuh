@@ -280,19 +280,19 @@ mma_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUt
 }
 
 // ---- scaling ------------------------------------------------------------------------------------------
-// exps[0] = exponent of w (of the piece), exps[1] = exponent of x: both were multiplied by 2^exp
+// exps[0] = exponent of w, exps[1] = exponent of x: both were multiplied by 2^exp.  2^126 is the largest
+// factor: data below 2^-112 stays below 2^14, with terms as fine as before.
+__device__ __forceinline__ float power2(int e) { return __int_as_float((127 + e) << 23); }
+__device__ __forceinline__ int scale_exponent(uint32_t max_bits) {
+  return max_bits ? min(126, 14 - ilogbf(__uint_as_float(max_bits))) : 0;
+}
+// 2^-e in two factors (the exponents of two operands add up to -226 .. 252)
 struct Unscale {
   float a, b;
-  __device__ __forceinline__ float operator()(float v) const { return v * a * b; }
 };
-// 2^-e in two factors (e may exceed the exponent range of one Float32)
 __device__ __forceinline__ Unscale unscale(int e, float gain = 1.0f) {
   const int h = e / 2;
-  return Unscale{scalbnf(gain, -h), scalbnf(1.0f, -(e - h))};
-}
-__device__ __forceinline__ int scale_exponent(uint32_t max_bits) {
-  if (max_bits == 0) return 0;
-  return 14 - ilogbf(__uint_as_float(max_bits));
+  return Unscale{gain * power2(-h), power2(-(e - h))};
 }
 
 struct SplitJob {
@@ -344,48 +344,74 @@ lnll_absmax_kernel(SplitJob a, SplitJob b, uint32_t* __restrict__ part) {
   }
 }
 
-// x * 2^e = hi + lo in fp16; an infinity goes to hi alone, so that hi + lo is not NaN
-__device__ __forceinline__ void split_half(float v, __half& hi, __half& lo) {
-  hi = __float2half_rn(v);
-  const float r = v - __half2float(hi);
-  lo = isinf(v) ? __float2half_rn(0.0f) : __float2half_rn(r);
+// v = hi + lo in fp16 for two values; what is not finite goes to hi alone, so that an infinity is not NaN
+__device__ __forceinline__ void split_pair(float v0, float v1, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(v0, v1);
+  const float2 f = __half22float2(h);
+  float r0 = v0 - f.x, r1 = v1 - f.y;
+  r0 = r0 == r0 ? r0 : 0.0f;
+  r1 = r1 == r1 ? r1 : 0.0f;
+  const __half2 l = __floats2half2_rn(r0, r1);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
-// both operands into their two planes; rows are shared out over blocks, 8 columns per thread and turn
+// Eight consecutive floats of a row that starts at any alignment: aligned 16-byte loads that lie inside the
+// row, shifted by the row's offset in a line; single loads at its ends.
+__device__ __forceinline__ void load8(const float* row, int64_t c, int64_t cols, float (&v)[8]) {
+  const int off = (int)(((uintptr_t)row >> 2) & 3);
+  if (c - off >= 0 && c - off + (off ? 12 : 8) <= cols) {
+    const float4* q = reinterpret_cast<const float4*>(row + c - off);
+    const float4 a = __ldg(q), b = __ldg(q + 1);
+    const float4 d = off ? __ldg(q + 2) : b;
+    const float t[12] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, d.x, d.y, d.z, d.w};
+#pragma unroll
+    for (int k = 0; k < 8; k++) v[k] = off == 0 ? t[k] : off == 1 ? t[k + 1] : off == 2 ? t[k + 2] : t[k + 3];
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; k++) v[k] = c + k < cols ? __ldg(row + c + k) : 0.0f;
+  }
+}
+
+// Both operands into their two planes; rows are shared out over blocks, 8 columns per thread and turn.
+// The exponents come from the maxima in `part` (and are left in `saved` for the backward) or, in the
+// backward, from what the forward left (`given`).
 __global__ void __launch_bounds__(256)
 lnll_split_kernel(SplitJob a, SplitJob b, uint32_t blocks_a, const uint32_t* __restrict__ part, uint32_t parts,
-                  int* __restrict__ exps) {
+                  const float* __restrict__ given, float* __restrict__ saved, int* __restrict__ exps) {
   chain_begin();
   __shared__ uint32_t red[32];
   const bool second = blockIdx.x >= blocks_a;
   const SplitJob j = second ? b : a;
-  uint32_t m = 0;
-  for (uint32_t k = threadIdx.x; k < parts; k += 256) m = max(m, part[(second ? kMaxBlocks : 0) + k]);
-  m = block_reduce(m, [](uint32_t x, uint32_t y) { return max(x, y); }, 0u, red);
-  const int e = scale_exponent(m);
+  int e;
+  if (given) {
+    e = max(-113, min(126, (int)given[second]));
+  } else {
+    uint32_t m = 0;
+    for (uint32_t k = threadIdx.x; k < parts; k += 256) m = max(m, part[(second ? kMaxBlocks : 0) + k]);
+    m = block_reduce(m, [](uint32_t x, uint32_t y) { return max(x, y); }, 0u, red);
+    e = scale_exponent(m);
+  }
   const uint32_t first = second ? blocks_a : 0, nb = (second ? gridDim.x - blocks_a : blocks_a);
-  if (blockIdx.x == first && threadIdx.x == 0) exps[second] = e;
-  const Unscale sc = unscale(-e);
+  if (blockIdx.x == first && threadIdx.x == 0) {
+    exps[second] = e;
+    if (saved) saved[second] = (float)e;
+  }
+  const float f = power2(e);
   const int64_t groups = (j.cols + 7) / 8;               // the pitch ld is a multiple of 8
   const int64_t total = groups * j.rows;
   // from the end: what the maximum's pass read last is still in L2
   for (int64_t g = total - 1 - ((int64_t)(blockIdx.x - first) * 256 + threadIdx.x); g >= 0; g -= (int64_t)nb * 256) {
     const int64_t r = g / groups, c = (g - r * groups) * 8;
-    const float* p = j.src + r * j.pitch + c;
     float v[8];
-    if (c + 8 <= j.cols && ((uintptr_t)p & 15) == 0) {
-      *reinterpret_cast<float4*>(v) = __ldg(reinterpret_cast<const float4*>(p));
-      *reinterpret_cast<float4*>(v + 4) = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; k++) v[k] = c + k < j.cols ? p[k] : 0.0f;
-    }
-    __align__(16) __half hi[8];
-    __align__(16) __half lo[8];
-#pragma unroll
-    for (int k = 0; k < 8; k++) split_half(sc(v[k]), hi[k], lo[k]);
-    *reinterpret_cast<uint4*>(j.dst + r * j.ld + c) = *reinterpret_cast<uint4*>(hi);
-    *reinterpret_cast<uint4*>(j.dst + j.plane + r * j.ld + c) = *reinterpret_cast<uint4*>(lo);
+    load8(j.src + r * j.pitch, c, j.cols, v);
+    uint4 hi, lo;
+    split_pair(v[0] * f, v[1] * f, hi.x, lo.x);
+    split_pair(v[2] * f, v[3] * f, hi.y, lo.y);
+    split_pair(v[4] * f, v[5] * f, hi.z, lo.z);
+    split_pair(v[6] * f, v[7] * f, hi.w, lo.w);
+    *reinterpret_cast<uint4*>(j.dst + r * j.ld + c) = hi;
+    *reinterpret_cast<uint4*>(j.dst + j.plane + r * j.ld + c) = lo;
   }
 }
 
@@ -709,10 +735,10 @@ lnll_grad_planes_kernel(const float* __restrict__ scores, int parts, const float
     if (n >= N) break;
     const float d = v < V ? grad_score(t[k] + b, lse[n], lse[N + n], labels[n], v) : 0.0f;
     sum += d;
-    __half h, l;
-    split_half(d * (float)(1 << kGradExp), h, l);
-    ds[n * ld + v] = h;
-    ds[plane + n * ld + v] = l;
+    uint32_t h, l;
+    split_pair(d * (float)(1 << kGradExp), 0.0f, h, l);
+    ds[n * ld + v] = __ushort_as_half((unsigned short)h);
+    ds[plane + n * ld + v] = __ushort_as_half((unsigned short)l);
   }
   if (db_part && v < V) db_part[(int64_t)blockIdx.y * V + v] = sum;
 }

@@ -243,6 +243,50 @@ end
 
 Base.close(c::DpComm) = (check(ccall((:knet_dp_destroy, libknet8), Cint, (Ptr{Cvoid},), c.handle), :knet_dp_destroy); nothing)
 
+# ---- nll of a linear layer without its score matrix, clipping by the norm of all gradients --------------
+for (T, S) in ((Float32, "32"), (Float64, "64"))
+    wsf, fwd, bwd = Symbol("knet_linear_nll_workspace_", S), Symbol("knet_linear_nll_fwd_", S), Symbol("knet_linear_nll_bwd_", S)
+    gcl, app = Symbol("knet_gclip_global_", S), Symbol("knet_gclip_apply_", S)
+    @eval begin
+        # nll(W*x .+ b, labels), W (V,H) or, with trans, (H,V); b may be nothing.  Returns total, count
+        # and the lse pair that the backward call needs; nothing waits for the device.
+        function linear_nll(w::DevArray{$T}, x::DevArray{$T}, labels::CuArray{Int32}; b=nothing, trans=false)
+            H = size(x, 1); N = div(length(x), H); V = div(length(w), H)
+            ws = CuArray{UInt8}(undef, ccall(($(QuoteNode(wsf)), libknet8), Csize_t, (Int64, Int64, Int64, Cint), V, H, N, 0))
+            total = CuArray{$T}(undef, 1); count = CuArray{Int32}(undef, 1)
+            lse = CuArray{$T}(undef, 2N + 2); per = CuArray{$T}(undef, N)
+            check(ccall(($(QuoteNode(fwd)), libknet8), Cint,
+                        (CuPtr{$T}, Cint, CuPtr{$T}, CuPtr{$T}, CuPtr{Int32}, Int64, Int64, Int64, CuPtr{$T}, CuPtr{Int32},
+                         CuPtr{$T}, CuPtr{$T}, CuPtr{UInt8}, Csize_t, CUDA.CUstream),
+                        w, trans, b === nothing ? CU_NULL : b, x, labels, V, H, N, total, count, lse, per, ws, length(ws),
+                        CUDA.stream()), $(QuoteNode(fwd)))
+            (total, count, lse)
+        end
+        function linear_nll_back(w::DevArray{$T}, x::DevArray{$T}, labels::CuArray{Int32}, lse, count, dy; b=nothing, trans=false,
+                                 average=true)
+            H = size(x, 1); N = div(length(x), H); V = div(length(w), H)
+            ws = CuArray{UInt8}(undef, ccall(($(QuoteNode(wsf)), libknet8), Csize_t, (Int64, Int64, Int64, Cint), V, H, N, 1))
+            dw = similar(w); dx = similar(x); db = b === nothing ? nothing : similar(b)
+            check(ccall(($(QuoteNode(bwd)), libknet8), Cint,
+                        (CuPtr{$T}, Cint, CuPtr{$T}, CuPtr{$T}, CuPtr{Int32}, Int64, Int64, Int64, CuPtr{$T}, Cint, $T,
+                         CuPtr{Int32}, CuPtr{$T}, CuPtr{$T}, CuPtr{$T}, CuPtr{UInt8}, Csize_t, CUDA.CUstream),
+                        w, trans, b === nothing ? CU_NULL : b, x, labels, V, H, N, lse, average, dy, count, dw,
+                        db === nothing ? CU_NULL : db, dx, ws, length(ws), CUDA.stream()), $(QuoteNode(bwd)))
+            (dw, dx, db)
+        end
+        # table, ntensors and chunks as for the multi-tensor updates; returns the norm on the device
+        function gclip_global!(table, ntensors, chunks, ::Type{$T}, gclip; gscale=1.0)
+            partials = CuArray{Float64}(undef, max(chunks, 1)); norm = CuArray{Float64}(undef, 1); factor = CuArray{Float64}(undef, 1)
+            check(ccall(($(QuoteNode(gcl)), libknet8), Cint,
+                        (CuPtr{Cvoid}, Cint, Int64, Cdouble, Cdouble, CuPtr{Float64}, CuPtr{Float64}, CuPtr{Float64}, CUDA.CUstream),
+                        table, ntensors, chunks, gclip, gscale, partials, norm, factor, CUDA.stream()), $(QuoteNode(gcl)))
+            check(ccall(($(QuoteNode(app)), libknet8), Cint, (CuPtr{Cvoid}, Cint, Int64, CuPtr{Float64}, CUDA.CUstream),
+                        table, ntensors, chunks, factor, CUDA.stream()), $(QuoteNode(app)))
+            norm
+        end
+    end
+end
+
 # ---- matrix products (section D of knet_sm100.h) ----------------------------------------------------
 # gemm!(transA, transB, alpha, A, B, beta, C) for KnetArray (src/knetarrays/linalg.jl:27-55) through
 # knet_gemm_S_S: the same cuBLAS product, with GEMM_MODE[] = 1 asking cuBLAS (12.9 or later, e.g.

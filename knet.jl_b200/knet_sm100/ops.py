@@ -373,16 +373,16 @@ def nll_back(scores, labels, dims=1, average=True, dy=1.0, count=None):
 
 
 class LinearNllResult(NllResult):
-    """Device-side result of linear_nll_device: NllResult plus log sum exp per instance, kept as its
-    rounded value (`lse`) and the remainder of that rounding, which the backward pass reads too."""
+    """Device-side result of linear_nll_device: NllResult plus `saved`, what the backward pass reads: log
+    sum exp per instance as its rounded value (`lse`) and the remainder of that rounding, and two scales."""
 
-    def __init__(self, total, count, per_instance, labels, lse_pair):
+    def __init__(self, total, count, per_instance, labels, saved):
         super().__init__(total, count, per_instance, labels)
-        self.lse_pair = lse_pair
+        self.saved = saved
 
     @property
     def lse(self):
-        return self.lse_pair[:self.lse_pair.numel() // 2]
+        return self.saved[:self.saved.numel() // 2 - 1]
 
 
 def _head_sizes(w, x, b, trans):
@@ -422,7 +422,7 @@ def linear_nll_device(w, x, labels, b=None, trans=False):
         total = torch.empty(1, dtype=dt, device=dev)
         count = torch.empty(1, dtype=torch.int32, device=dev)
         per = torch.empty(max(N, 1), dtype=dt, device=dev)
-        lse = torch.empty(2 * N, dtype=dt, device=dev)
+        lse = torch.empty(2 * N + 2, dtype=dt, device=dev)
         size = getattr(libknet, f"knet_linear_nll_workspace_{S}")(V, H, N, 0)
         ws = torch.empty(max(size, 1), dtype=torch.uint8, device=dev)
         knet(f"knet_linear_nll_fwd_{S}", _address(w), 1 if trans else 0, _address(b), _address(x), lab.data_ptr(), V, H, N,
@@ -440,7 +440,7 @@ def linear_nll_back(w, x, res, b=None, trans=False, average=True, dy=1.0, need=(
     None without b.  `need` leaves some of them out (None); `out` gives arrays to write them to."""
     V, H, N = _head_sizes(w, x, b, trans)
     dev, dt = w.data.device, w.data.dtype
-    if res.labels.numel() != N or res.lse_pair.dtype != dt or res.labels.device != dev:
+    if res.labels.numel() != N or res.saved.dtype != dt or res.labels.device != dev:
         raise ValueError("DimensionMismatch: the forward result belongs to other arrays")
     S = sfx(dt)
     with on_device(dev):
@@ -460,7 +460,7 @@ def linear_nll_back(w, x, res, b=None, trans=False, average=True, dy=1.0, need=(
         size = getattr(libknet, f"knet_linear_nll_workspace_{S}")(V, H, N, 1)
         ws = torch.empty(max(size, 1), dtype=torch.uint8, device=dev)
         knet(f"knet_linear_nll_bwd_{S}", _address(w), 1 if trans else 0, _address(b), _address(x), res.labels.data_ptr(), V, H, N,
-             res.lse_pair.data_ptr(), 1 if average else 0, dy, res.count.data_ptr(), _address(dw), _address(db), _address(dx),
+             res.saved.data_ptr(), 1 if average else 0, dy, res.count.data_ptr(), _address(dw), _address(db), _address(dx),
              ws.data_ptr(), size)
     return dw, dx, db
 

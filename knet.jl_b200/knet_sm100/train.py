@@ -179,7 +179,8 @@ class MultiTensorPlan:
         self.ntensors = n
         self.total_chunks = libknet.knet_multi_plan(C.cast(host, C.c_void_p), n)
         raw = bytes(host)
-        self.table = torch.frombuffer(bytearray(raw), dtype=torch.uint8).cuda()
+        first = arrays[0][0].data if isinstance(arrays[0][0], KnetArray) else arrays[0][0]
+        self.table = torch.frombuffer(bytearray(raw), dtype=torch.uint8).to(first.device)      # beside its arrays
         self._keep = arrays
         held = [(host[i].p[1], host[i].n) for i in range(n) if host[i].p[1] and host[i].n]
         self.repeated = len(set(held)) < len(held)
@@ -223,7 +224,8 @@ def _global_norm(plan, gclip, gscale):
 
 def gnorm(grads, gscale=1.0):
     """|gscale| * the norm of all gradients taken as one vector: a one-element Float64 tensor on the
-    device.  `grads` is a MultiTensorPlan or a list of arrays (a list costs an upload of its table)."""
+    device.  `grads` is a MultiTensorPlan or a list of arrays (a list costs an upload of its table and
+    cannot be used while a graph is captured)."""
     plan, _ = _one_plan(grads)
     if plan is None:
         return torch.zeros(1, dtype=torch.float64, device="cuda")
@@ -256,40 +258,41 @@ def update_multi_(plan, p, gscale=1.0, advance=True, gclip_global=0):
     update applies them to the gradient as it loads it.  `gclip_global` > 0 clips by the norm of all
     gradients of the plan instead (gclip_global_), also applied on load: the gradients in memory
     stay as they are; that norm, a device tensor, is returned."""
-    S = sfx(plan.dtype)
-    clip = getattr(p, "gclip", 0) or 0
-    tail = ()
-    sfx_c = ""
-    norm = None
-    if gclip_global:
-        if clip > 0:
-            raise ValueError("clip by array (the optimizer's gclip) or by the global norm, not both")
-        if not gclip_global > 0:
-            raise ValueError("gclip_global must be positive")
-        if not isinstance(p, (Adam, Momentum, SGD)) or isinstance(p, Nesterov):
+    with on_device(plan.table.device):
+        S = sfx(plan.dtype)
+        clip = getattr(p, "gclip", 0) or 0
+        tail = ()
+        sfx_c = ""
+        norm = None
+        if gclip_global:
+            if clip > 0:
+                raise ValueError("clip by array (the optimizer's gclip) or by the global norm, not both")
+            if not gclip_global > 0:
+                raise ValueError("gclip_global must be positive")
+            if not isinstance(p, (Adam, Momentum, SGD)) or isinstance(p, Nesterov):
+                raise TypeError(f"no multi-tensor kernel for {type(p)}")
+            norm, factor = _global_norm(plan, gclip_global, gscale)
+            tail, sfx_c = (ptr(factor),), "_gc"
+        elif clip > 0:
+            if plan.clip_partials is None:
+                plan.clip_partials = torch.empty(max(int(plan.total_chunks), 1), dtype=plan.dtype, device=plan.table.device)
+                plan.clip_factors = torch.ones(max(plan.ntensors, 1), dtype=torch.float64, device=plan.table.device)
+            knet(f"knet_gclip_factors_{S}", ptr(plan.table), plan.ntensors, plan.total_chunks, float(clip), float(gscale),
+                 ptr(plan.clip_partials), ptr(plan.clip_factors))
+            tail, sfx_c = (ptr(plan.clip_factors),), "_c"
+        if isinstance(p, Adam):
+            if advance:
+                p.t += 1
+            knet(f"knet_adam_multi{sfx_c}_{S}", ptr(plan.table), plan.ntensors, plan.total_chunks, p.lr, p.beta1,
+                 p.beta2, p.eps, p.t, gscale, *tail)
+        elif isinstance(p, Momentum) and not isinstance(p, Nesterov):
+            knet(f"knet_momentum_multi{sfx_c}_{S}", ptr(plan.table), plan.ntensors, plan.total_chunks, p.lr, p.gamma,
+                 gscale, *tail)
+        elif isinstance(p, SGD):
+            knet(f"knet_sgd_multi{sfx_c}_{S}", ptr(plan.table), plan.ntensors, plan.total_chunks, p.lr, gscale, *tail)
+        else:
             raise TypeError(f"no multi-tensor kernel for {type(p)}")
-        norm, factor = _global_norm(plan, gclip_global, gscale)
-        tail, sfx_c = (ptr(factor),), "_gc"
-    elif clip > 0:
-        if plan.clip_partials is None:
-            plan.clip_partials = torch.empty(max(int(plan.total_chunks), 1), dtype=plan.dtype, device=plan.table.device)
-            plan.clip_factors = torch.ones(max(plan.ntensors, 1), dtype=torch.float64, device=plan.table.device)
-        knet(f"knet_gclip_factors_{S}", ptr(plan.table), plan.ntensors, plan.total_chunks, float(clip), float(gscale),
-             ptr(plan.clip_partials), ptr(plan.clip_factors))
-        tail, sfx_c = (ptr(plan.clip_factors),), "_c"
-    if isinstance(p, Adam):
-        if advance:
-            p.t += 1
-        knet(f"knet_adam_multi{sfx_c}_{S}", ptr(plan.table), plan.ntensors, plan.total_chunks, p.lr, p.beta1,
-             p.beta2, p.eps, p.t, gscale, *tail)
-    elif isinstance(p, Momentum) and not isinstance(p, Nesterov):
-        knet(f"knet_momentum_multi{sfx_c}_{S}", ptr(plan.table), plan.ntensors, plan.total_chunks, p.lr, p.gamma,
-             gscale, *tail)
-    elif isinstance(p, SGD):
-        knet(f"knet_sgd_multi{sfx_c}_{S}", ptr(plan.table), plan.ntensors, plan.total_chunks, p.lr, gscale, *tail)
-    else:
-        raise TypeError(f"no multi-tensor kernel for {type(p)}")
-    return norm
+        return norm
 
 
 # ---- parameters and initialisation (src/train20/param.jl:22-24, distributions.jl:35-52) ------------

@@ -407,38 +407,47 @@ inline int operand_map(CUtensorMap* map, const Planes& o, bool mn, int tile) {
 }
 
 // the kernel's shared memory is beyond the default limit: raised once per device
-template <typename Epi> int allow_smem() {
+template <int CG, typename Epi> int allow_smem() {
   static std::atomic<uint64_t> done{0};
   int dev = 0;
   if (cudaError_t e = cudaGetDevice(&dev)) return (int)e;
   const uint64_t bit = dev < 64 ? 1ull << dev : 0;
   if (done.load(std::memory_order_relaxed) & bit) return 0;
-  if (cudaError_t e = cudaFuncSetAttribute(mma_kernel<Epi>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMmaSmem)) return (int)e;
+  if (cudaError_t e = cudaFuncSetAttribute(mma_kernel<CG, Epi>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMmaSmem)) return (int)e;
   done.fetch_or(bit, std::memory_order_relaxed);
   return 0;
 }
 
-template <typename Epi>
-int mma_product(const Planes& a, bool a_mn, const Planes& b, bool b_mn, int64_t I, int64_t J, int64_t C, int splits, const Epi& epi,
-                cudaStream_t st) {
+template <int CG, typename Epi>
+int mma_product_cg(const Planes& a, bool a_mn, const Planes& b, bool b_mn, int64_t I, int64_t J, int64_t C, int splits, const Epi& epi,
+                   cudaStream_t st) {
   static_assert(sizeof(CUtensorMap) == 128, "kernel parameter");
   CUtensorMap am, bm;
   if (int rc = operand_map(&am, a, a_mn, kTM)) return rc;
-  if (int rc = operand_map(&bm, b, b_mn, kTN)) return rc;
+  if (int rc = operand_map(&bm, b, b_mn, kTN / CG)) return rc;
   MmaTiles tl;
-  tl.i_tiles = (uint32_t)ceil_div(I, kTM);
+  tl.i_tiles = (uint32_t)ceil_div(I, kTM * CG);
   tl.j_tiles = (uint32_t)ceil_div(J, kTN);
   tl.blocks = (uint32_t)ceil_div(C, kBK);
   tl.blocks_per_split = (uint32_t)ceil_div(tl.blocks, splits);
   tl.splits = (uint32_t)splits;
   tl.a_mn = a_mn;
   tl.b_mn = b_mn;
-  if (int rc = allow_smem<Epi>()) return rc;
+  if (int rc = allow_smem<CG, Epi>()) return rc;
   const uint64_t tiles = (uint64_t)tl.i_tiles * tl.j_tiles * tl.splits;
   if (tiles > 0x7fffffff) return KN_ESIZE;
-  const unsigned grid = (unsigned)(tiles < (uint64_t)sm_count() ? tiles : sm_count());
-  launch_chained(mma_kernel<Epi>, grid, kMmaThreads, kMmaSmem, st, am, bm, tl, epi);
-  return launch_status();
+  const uint64_t workers = (uint64_t)sm_count() / CG;
+  const unsigned grid = (unsigned)(tiles < workers ? tiles : workers) * CG;
+  return (int)launch_chained_cluster(CG, mma_kernel<CG, Epi>, grid, kMmaThreads, kMmaSmem, st, am, bm, tl, epi);
+}
+
+// Pairs of CTAs need tiles of 256 rows: not where those would leave more than a seventh of the rows empty.
+template <typename Epi>
+int mma_product(const Planes& a, bool a_mn, const Planes& b, bool b_mn, int64_t I, int64_t J, int64_t C, int splits, const Epi& epi,
+                cudaStream_t st) {
+  const int64_t one = ceil_div(I, kTM), two = 2 * ceil_div(I, 2 * kTM);
+  if (6 * two <= 7 * one) return mma_product_cg<2>(a, a_mn, b, b_mn, I, J, C, splits, epi, st);
+  return mma_product_cg<1>(a, a_mn, b, b_mn, I, J, C, splits, epi, st);
 }
 
 // the largest magnitudes of w and x, one value per block of each

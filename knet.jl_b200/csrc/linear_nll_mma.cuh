@@ -12,12 +12,16 @@
 // of 5e-7 to 8e-7 in a product.  (Chunks of 128 halve the error; 256 give the epilogue 10 us instead of 5
 // before the tensor core has to wait for it: dS of 4608 classes x 4096 instances 123 -> 112 us.)
 //
-// A CTA owns a 128 x 256 tile of the result.  Warp 16 loads the operands with TMA into a ring of
-// stages of 32 summed indices (48 KB: both planes of 128 + 256 rows); warp 17 issues the products
-// into one of two halves of TMEM (256 columns each); warps 0-15 move finished chunks from the other
-// half into registers, 64 columns of one row per thread, and run the epilogue while the tensor core
-// works on the next tile.  The tile is as wide as TMEM allows with two halves: per summed index a CTA
-// loads 1.5 KB for 196 608 multiply-adds, 64 bytes per clock at the full rate.
+// A CTA owns a 128 x 256 tile of the result, or a pair of CTAs (a cluster) one of 256 x 256.  Warp 16 loads
+// the operands with TMA into a ring of stages of 32 summed indices (both planes of 128 rows of A and of 256
+// rows of B, or the CTA's 128 of them); warp 17, of a pair the first CTA's, issues the products into one of
+// two halves of TMEM (256 columns each); warps 0-15 move finished chunks from the other half into registers,
+// 64 columns of one row per thread, and run the epilogue while the tensor core works on the next tile.
+//
+// Alone, a CTA writes 48 KB and reads 72 KB of shared memory per 32 summed indices, 160 bytes per clock at the
+// tensor core's full rate where shared memory has 128; in a pair, where each loads half of B, 32 + 48 KB or 107
+// bytes.  Scores of 50257 classes x 4096 instances: 818 us alone, 748 us in pairs (1692 TFLOP/s of fp16
+// products; the device's own library reaches 1658 on bf16).
 #pragma once
 #include <cuda_fp16.h>
 
@@ -26,23 +30,29 @@
 
 namespace kn {
 
-constexpr int kTM = 128, kTN = 256, kBK = 32, kStages = 4;
+constexpr int kTM = 128, kTN = 256, kBK = 32;
 constexpr int kChunkBlocks = 8;                         // 256 summed indices per accumulator
 // Registers: 640 threads start with 96 each; the four warps beside the epilogue give up all but 32 and
 // the epilogue's 512 threads take 112 (57 344 + 4 096 of 61 440).
 constexpr int kEpiWarps = 16, kMmaThreads = (kEpiWarps + 4) * 32;
-constexpr uint32_t kStageA = 2 * kTM * kBK * 2, kStageB = 2 * kTN * kBK * 2, kStageBytes = kStageA + kStageB;
+constexpr uint32_t kStageA = 2 * kTM * kBK * 2;
+// a CTA's share of B in a stage, and the stages: 48 KB x 4 alone, 32 KB x 6 in a pair
+template <int CG> constexpr uint32_t kStageB = 2 * (kTN / CG) * kBK * 2;
+template <int CG> constexpr uint32_t kStageBytes = kStageA + kStageB<CG>;
+template <int CG> constexpr uint32_t kStages = CG == 1 ? 4 : 6;
+constexpr int kMaxStages = 6;
 constexpr int kGradExp = 14;                            // dS lies in [-1, 1]
 
 struct MmaShared {
-  uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2], drain;
+  uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2], drain;
   uint32_t tmem;
   int gave_up;
   float2 stat[2][4][kTM];                               // per tile parity, column quarter and row
   __align__(16) float bias[2][kTN];                     // per tile parity
   float colsum[4][kTN];
 };
-constexpr size_t kMmaSmem = 1024 + (size_t)kStages * kStageBytes + sizeof(MmaShared);
+constexpr size_t kMmaSmem = 1024 + (size_t)kStages<1> * kStageBytes<1> + sizeof(MmaShared);
+static_assert(kStages<1> * kStageBytes<1> == kStages<2> * kStageBytes<2>, "one size");
 
 // how one launch walks its tiles: rows i fastest, then columns j, then parts of the summed axis
 struct MmaTiles {
@@ -51,10 +61,11 @@ struct MmaTiles {
   int a_mn, b_mn;                                       // operand stored with its row index contiguous
 };
 
-// A wait that gives up (or finds that another role has) makes every role of the CTA leave.
-__device__ __forceinline__ bool mma_wait(uint64_t* bar, uint32_t parity, int* gave_up) {
+// A wait that gives up (or finds that another role has) makes every role of the CTA leave; the other CTA of
+// a pair then runs into its own limits.
+template <int CG> __device__ __forceinline__ bool mma_wait(uint64_t* bar, uint32_t parity, int* gave_up) {
   for (uint32_t i = 0; i < kWaitSpins; i++) {
-    if (mbar_try_wait(bar, parity)) return true;
+    if (CG == 1 ? mbar_try_wait(bar, parity) : mbar_try_wait_cluster(bar, parity)) return true;
     if (*(volatile int*)gave_up) return false;
     if (i > 256) __nanosleep(128);
   }
@@ -115,31 +126,36 @@ __device__ __forceinline__ bool epi_any(bool yes) {
   return r != 0;
 }
 
-template <typename Epi>
+template <int CG, typename Epi>
 __global__ void __launch_bounds__(kMmaThreads, 1)
 mma_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap, MmaTiles tl, Epi epi) {
+  constexpr uint32_t STAGES = kStages<CG>, STAGE = kStageBytes<CG>, BN = kTN / CG;
   extern __shared__ uint8_t raw[];
   uint8_t* stages = reinterpret_cast<uint8_t*>(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
-  MmaShared* sh = reinterpret_cast<MmaShared*>(stages + (size_t)kStages * kStageBytes);
+  MmaShared* sh = reinterpret_cast<MmaShared*>(stages + (size_t)STAGES * STAGE);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 1 ? 0 : cluster_rank();
+  const uint32_t worker = blockIdx.x / CG, workers = gridDim.x / CG;     // a CTA or a pair
   const uint32_t tiles = tl.i_tiles * tl.j_tiles * tl.splits;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; s++) {
+    for (uint32_t s = 0; s < STAGES; s++) {
       mbar_init(&sh->full[s], 1);
       mbar_init(&sh->empty[s], 1);
     }
     for (int b = 0; b < 2; b++) {
       mbar_init(&sh->acc_full[b], 1);
-      mbar_init(&sh->acc_empty[b], kEpiWarps);
+      mbar_init(&sh->acc_empty[b], kEpiWarps * CG);
     }
     mbar_init(&sh->drain, 1);
     sh->gave_up = 0;
     mbar_init_fence();
   }
-  if (warp == kEpiWarps + 1) tmem_alloc(&sh->tmem, 512);
+  __syncwarp();
+  if (warp == kEpiWarps + 1) tmem_alloc<CG>(&sh->tmem, 512);
   tcgen05_before_sync();
-  __syncthreads();
+  if constexpr (CG == 1) __syncthreads();
+  else cluster_barrier();
   tcgen05_after_sync();
   const uint32_t tmem = sh->tmem;
   chain_begin();
@@ -147,59 +163,70 @@ mma_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUt
   if (warp >= kEpiWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
     if (warp == kEpiWarps) {
-      // ---- loads
+      // ---- loads: this CTA's rows of A and its share of B; in a pair all bytes count on the first CTA's barrier
       if (lane == 0) {
         tma_prefetch_map(&amap);
         tma_prefetch_map(&bmap);
         uint32_t n = 0;                                   // stages filled so far
         bool ok = true;
-        for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        for (uint32_t t = worker; t < tiles && ok; t += workers) {
           const uint32_t it = t % tl.i_tiles, r = t / tl.i_tiles, jt = r % tl.j_tiles, sp = r / tl.j_tiles;
           const uint32_t k0 = sp * tl.blocks_per_split, k1 = min(k0 + tl.blocks_per_split, tl.blocks);
-          const int32_t i0 = (int32_t)(it * kTM), j0 = (int32_t)(jt * kTN);
+          const int32_t i0 = (int32_t)((it * CG + rank) * kTM), j0 = (int32_t)(jt * kTN + rank * BN);
           for (uint32_t k = k0; k < k1; k++, n++) {
-            const uint32_t s = n % kStages;
-            if (n >= kStages && !mma_wait(&sh->empty[s], (n / kStages - 1) & 1, &sh->gave_up)) {
+            const uint32_t s = n % STAGES;
+            if (n >= STAGES && !mma_wait<CG>(&sh->empty[s], (n / STAGES - 1) & 1, &sh->gave_up)) {
               ok = false;
               break;
             }
-            uint8_t* a = stages + (size_t)s * kStageBytes;
+            uint8_t* a = stages + (size_t)s * STAGE;
             uint8_t* b = a + kStageA;
             const int32_t c = (int32_t)(k * kBK);
-            mbar_arrive_expect_tx(&sh->full[s], kStageBytes);
+            if (rank == 0) mbar_arrive_expect_tx(&sh->full[s], STAGE * CG);
+            const uint32_t bar = CG == 1 ? 0 : mapa_u32(&sh->full[s], 0);
+            auto load = [&](uint8_t* to, const CUtensorMap* map, int32_t x, int32_t y) {
+              if constexpr (CG == 1) tma_load_3d(to, map, x, y, 0, &sh->full[s]);
+              else tma_load_3d_pair(to, map, x, y, 0, bar);
+            };
             if (tl.a_mn) {
-              for (int g = 0; g < kTM / 64; g++) tma_load_3d(a + g * 8192, &amap, i0 + g * 64, c, 0, &sh->full[s]);
+              for (int g = 0; g < kTM / 64; g++) load(a + g * 8192, &amap, i0 + g * 64, c);
             } else {
-              tma_load_3d(a, &amap, c, i0, 0, &sh->full[s]);
+              load(a, &amap, c, i0);
             }
             if (tl.b_mn) {
-              for (int g = 0; g < kTN / 64; g++) tma_load_3d(b + g * 8192, &bmap, j0 + g * 64, c, 0, &sh->full[s]);
+              for (uint32_t g = 0; g < BN / 64; g++) load(b + g * 8192, &bmap, j0 + (int32_t)g * 64, c);
             } else {
-              tma_load_3d(b, &bmap, c, j0, 0, &sh->full[s]);
+              load(b, &bmap, c, j0);
             }
           }
         }
-        // every load issued has landed before this CTA may leave
-        for (uint32_t m = n > kStages ? n - kStages : 0; m < n; m++)
-          for (uint32_t i = 0; i < kWaitSpins && !mbar_try_wait(&sh->full[m % kStages], (m / kStages) & 1); i++) __nanosleep(64);
+        // every load issued has landed before this CTA may leave: the first CTA sees it on its barriers (the
+        // products that it waits for below have read the second CTA's); after a wait that gave up the second
+        // CTA leaves its own loads a millisecond
+        if (rank == 0) {
+          for (uint32_t m = n > STAGES ? n - STAGES : 0; m < n; m++)
+            for (uint32_t i = 0; i < kWaitSpins && !mbar_try_wait(&sh->full[m % STAGES], (m / STAGES) & 1); i++) __nanosleep(64);
+        } else if (!ok) {
+          for (int i = 0; i < 1000; i++) __nanosleep(1000);
+        }
       }
     } else if (warp == kEpiWarps + 1) {
-      // ---- products
-      if (lane == 0) {
-        const uint32_t idesc = umma_idesc(kTM, kTN, tl.a_mn, tl.b_mn);
+      // ---- products, by the first CTA
+      if (lane == 0 && rank == 0) {
+        const uint32_t idesc = umma_idesc(kTM * CG, kTN, tl.a_mn, tl.b_mn);
         const uint64_t ad = tl.a_mn ? umma_desc(8192, 1024, 2) : umma_desc(16, 8 * kBK * 2, 4);
         const uint64_t bd = tl.b_mn ? umma_desc(8192, 1024, 2) : umma_desc(16, 8 * kBK * 2, 4);
         // second plane, and 16 summed indices further, in bytes
-        const uint32_t alo = tl.a_mn ? 4096 : kTM * kBK * 2, blo = tl.b_mn ? 4096 : kTN * kBK * 2;
+        const uint32_t alo = tl.a_mn ? 4096 : kTM * kBK * 2, blo = tl.b_mn ? 4096 : BN * kBK * 2;
         const uint32_t ak = tl.a_mn ? 2048 : 32, bk = tl.b_mn ? 2048 : 32;
         uint32_t n = 0, ch = 0;                           // stages and chunks so far
         bool ok = true;
-        for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        for (uint32_t t = worker; t < tiles && ok; t += workers) {
           const uint32_t sp = t / (tl.i_tiles * tl.j_tiles);
           const uint32_t k0 = sp * tl.blocks_per_split, k1 = min(k0 + tl.blocks_per_split, tl.blocks);
           for (uint32_t k = k0; k < k1 && ok; ch++) {
             const uint32_t buf = ch & 1, d = tmem + buf * kTN;
-            if (ch >= 2 && !mma_wait(&sh->acc_empty[buf], ((ch >> 1) - 1) & 1, &sh->gave_up)) {
+            if (ch >= 2 && !mma_wait<CG>(&sh->acc_empty[buf], ((ch >> 1) - 1) & 1, &sh->gave_up)) {
               ok = false;
               break;
             }
@@ -207,30 +234,30 @@ mma_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUt
             const uint32_t ke = min(k + kChunkBlocks, k1);
             bool acc = false;
             for (; k < ke; k++, n++) {
-              const uint32_t s = n % kStages;
-              if (!mma_wait(&sh->full[s], (n / kStages) & 1, &sh->gave_up)) {
+              const uint32_t s = n % STAGES;
+              if (!mma_wait<CG>(&sh->full[s], (n / STAGES) & 1, &sh->gave_up)) {
                 ok = false;
                 break;
               }
               tcgen05_after_sync();
-              const uint32_t a = smem_u32(stages + (size_t)s * kStageBytes), b = a + kStageA;
+              const uint32_t a = smem_u32(stages + (size_t)s * STAGE), b = a + kStageA;
               // the small cross terms first, while the sum is small
 #pragma unroll
               for (uint32_t q = 0; q < kBK / 16; q++) {
-                umma_f16(d, umma_at(ad, a + alo + q * ak), umma_at(bd, b + q * bk), idesc, acc);
-                umma_f16(d, umma_at(ad, a + q * ak), umma_at(bd, b + blo + q * bk), idesc, true);
+                umma_f16<CG>(d, umma_at(ad, a + alo + q * ak), umma_at(bd, b + q * bk), idesc, acc);
+                umma_f16<CG>(d, umma_at(ad, a + q * ak), umma_at(bd, b + blo + q * bk), idesc, true);
                 acc = true;
               }
 #pragma unroll
-              for (uint32_t q = 0; q < kBK / 16; q++) umma_f16(d, umma_at(ad, a + q * ak), umma_at(bd, b + q * bk), idesc, true);
-              umma_commit(&sh->empty[s]);
+              for (uint32_t q = 0; q < kBK / 16; q++) umma_f16<CG>(d, umma_at(ad, a + q * ak), umma_at(bd, b + q * bk), idesc, true);
+              umma_commit<CG>(&sh->empty[s]);
             }
             if (!ok) break;
-            umma_commit(&sh->acc_full[buf]);
+            umma_commit<CG>(&sh->acc_full[buf]);
           }
         }
         // every product issued is done before TMEM is freed
-        umma_commit(&sh->drain);
+        umma_commit<CG>(&sh->drain);
         for (uint32_t i = 0; i < kWaitSpins && !mbar_try_wait(&sh->drain, 0); i++) __nanosleep(64);
       }
     }
@@ -241,7 +268,7 @@ mma_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUt
     const uint32_t lane_addr = (uint32_t)(q * 32) << 16;
     uint32_t ch = 0, turn = 0;
     bool ok = true;
-    for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x, turn++) {
+    for (uint32_t t = worker; t < tiles && ok; t += workers, turn++) {
       const uint32_t it = t % tl.i_tiles, r = t / tl.i_tiles, jt = r % tl.j_tiles, sp = r / tl.j_tiles;
       const uint32_t k0 = sp * tl.blocks_per_split, k1 = min(k0 + tl.blocks_per_split, tl.blocks);
       epi.stage((int64_t)jt * kTN, sh->bias[turn & 1]);  // read after the barrier below
@@ -250,7 +277,7 @@ mma_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUt
       for (int e = 0; e < 32; e++) acc[e] = both(0.0f);
       for (uint32_t k = k0; k < k1; k += kChunkBlocks, ch++) {
         const uint32_t buf = ch & 1;
-        ok = __all_sync(0xffffffffu, mma_wait(&sh->acc_full[buf], (ch >> 1) & 1, &sh->gave_up));
+        ok = __all_sync(0xffffffffu, mma_wait<CG>(&sh->acc_full[buf], (ch >> 1) & 1, &sh->gave_up));
         if (!ok) break;
         tcgen05_after_sync();
 #pragma unroll
@@ -263,20 +290,26 @@ mma_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUt
         }
         tcgen05_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->acc_empty[buf]);
+        if (lane == 0) {
+          if constexpr (CG == 1) mbar_arrive(&sh->acc_empty[buf]);
+          else mbar_arrive_remote(mapa_u32(&sh->acc_empty[buf], 0));
+        }
       }
       // the epilogue has barriers of its own: all of its warps run it, or none
       if (epi_any(!ok)) break;
-      const TileAt at{(int64_t)it * kTM + q * 32 + lane, (int64_t)jt * kTN + quarter * 64, it, jt, sp, turn, quarter, q * 32 + lane,
+      const uint32_t rows = it * CG + rank;              // 128-row tile
+      const TileAt at{(int64_t)rows * kTM + q * 32 + lane, (int64_t)jt * kTN + quarter * 64, rows, jt, sp, turn, quarter, q * 32 + lane,
                       1.0f + 0.75f * 0x1p-23f * (float)min((uint32_t)kChunkBlocks, k1 - k0), sh};
       epi(acc, at);
     }
   }
   __syncwarp();
   tcgen05_before_sync();
-  __syncthreads();
+  if constexpr (CG == 1) __syncthreads();
+  else cluster_barrier();
   tcgen05_after_sync();
-  if (warp == kEpiWarps + 1) tmem_free(tmem, 512);
+  if (warp == kEpiWarps + 1) tmem_free<CG>(tmem, 512);
+  if constexpr (CG == 2) cluster_barrier();              // neither CTA leaves while the other still frees or signals
 }
 
 // ---- scaling ------------------------------------------------------------------------------------------
@@ -646,7 +679,7 @@ struct MmaGradScores {
       const int c = threadIdx.x;
       if (c < kTN) {
         const int64_t j = (int64_t)at.jt * kTN + c;
-        if (j < J)
+        if (j < J && (int64_t)at.it * kTM < N)                // a pair's second tile may lie past the last instance
           db_part[(int64_t)at.it * J + j] = ((at.sh->colsum[0][c] + at.sh->colsum[1][c]) +
                                              (at.sh->colsum[2][c] + at.sh->colsum[3][c])) * (1.0f / (1 << kGradExp));
       }

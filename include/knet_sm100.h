@@ -360,8 +360,11 @@ KNET_BOTH_TYPES(KNET_DECL_NLL, nll)
  *      time.  Results are the same from run to run.
  * Scores of -inf (a bias that masks a class) have probability 0; a class masked on every
  * instance is fine, an instance with every class masked gives NaN, as the composed form does.
- * An infinity or a NaN in W or x may make every score that it enters NaN.  Float32 products of
- * any size are as exact as Float32 arithmetic (errors against 64 bits of 1e-6 and less).
+ * An infinity or a NaN in W or x may make every score that it enters NaN.  What x holds in a
+ * skipped instance reaches neither the loss nor a gradient (its lse is then of no use).
+ * Large Float32 products (V*H*N from 2^26, or more than 2^24 scores) hold W, x (used instances)
+ * and dS to 2^-40 of the largest magnitude of each array: as exact as Float32 arithmetic for
+ * entries down to 2^-17 of it, less so below.
  * Up to 2^24 scores may pass through the workspace where that is faster.
  * workspace: at least knet_linear_nll_workspace_S(V, H, N, backward) bytes (0 for sizes that the
  * entry points refuse), 256-byte aligned; calls that share one must be ordered on one stream.

@@ -340,7 +340,16 @@ template <typename T> size_t workspace_any(int64_t V, int64_t H, int64_t N, int 
 template <typename T, typename Epi>
 void simt_product(Strided<T> a, Strided<T> b, int64_t I, int64_t J, int64_t C, int64_t c_part, uint32_t* done, Epi epi, cudaStream_t st) {
   const dim3 grid((unsigned)ceil_div(J, kTile), (unsigned)ceil_div(I, kTile), (unsigned)ceil_div(C, c_part));
-  launch_chained(simt_product_kernel<T, Epi>, grid, kSimtThreads, 0, st, a, b, I, J, C, c_part, done, epi);
+  launch_chained(simt_product_kernel<T, false, Epi>, grid, kSimtThreads, 0, st, a, b, (const int32_t*)nullptr, (const int32_t*)nullptr, I, J, C,
+                 c_part, done, epi);
+}
+// dW's: the sum runs over the instances, of which the labels tell the skipped ones in the operand that is x
+template <typename T, typename Epi>
+void simt_product_dw(Strided<T> a, Strided<T> b, bool a_is_x, const int32_t* labels, int64_t I, int64_t J, int64_t N, int64_t c_part,
+                     const Epi& epi, cudaStream_t st) {
+  const dim3 grid((unsigned)ceil_div(J, kTile), (unsigned)ceil_div(I, kTile), (unsigned)ceil_div(N, c_part));
+  launch_chained(simt_product_kernel<T, true, Epi>, grid, kSimtThreads, 0, st, a, b, a_is_x ? labels : nullptr, a_is_x ? nullptr : labels, I, J, N,
+                 c_part, (uint32_t*)nullptr, epi);
 }
 
 // packs of VEC elements are possible where base addresses and pitches are multiples of 16 bytes
@@ -452,18 +461,11 @@ int mma_product(const Planes& a, bool a_mn, const Planes& b, bool b_mn, int64_t 
 
 // the largest magnitudes of w and x, one value per block of each
 inline unsigned scale_operands(const Head<float>& h, const MmaPlan& p, char* ws, cudaStream_t st) {
-  SplitJob w{}, x{};
-  w.src = h.w;
-  w.rows = h.H;
-  w.cols = w.pitch = h.V;      // whole and contiguous in either layout
-  x.src = h.x;
-  x.rows = h.N;
-  x.cols = x.pitch = h.H;
   const int64_t want = ceil_div(h.V * h.H + h.N * h.H, 4096);
   const unsigned blocks = (unsigned)(want < kMaxBlocks ? want : kMaxBlocks);
   // an ordinary launch: placed under the tail of another kernel, its equal shares would land unevenly on the
   // SMs (32000x4096 n512, where it ran once per piece: 2.20 against 2.10 ms)
-  lnll_absmax_kernel<<<blocks, 256, 0, st>>>(w, x, (uint32_t*)(ws + p.absmax));
+  lnll_absmax_kernel<<<blocks, 256, 0, st>>>(h.w, h.V * h.H, h.x, h.labels, h.N, h.H, (uint32_t*)(ws + p.absmax));
   return blocks;
 }
 
@@ -481,12 +483,14 @@ inline SplitState split_operands(const Head<float>& h, const MmaPlan& p, char* w
   w.dst = (__half*)(ws + p.ws);
   w.ld = p.wld;
   w.plane = w.rows * p.wld;
+  w.labels = nullptr;
   x.src = h.x;
   x.rows = h.N;
   x.cols = x.pitch = h.H;
   x.dst = (__half*)(ws + p.xs);
   x.ld = p.xld;
   x.plane = x.rows * p.xld;
+  x.labels = h.labels;
   const SplitState s{Planes{w.dst, w.rows, w.cols, w.ld, w.plane}, Planes{x.dst, x.rows, x.cols, x.ld, x.plane}};
   const int64_t bw = ceil_div(w.rows * ceil_div(w.cols, 8), 1024), bx = v0 ? 0 : ceil_div(x.rows * ceil_div(x.cols, 8), 1024);
   const unsigned na = (unsigned)(bw < 8192 ? bw : 8192), nb = (unsigned)(bx < 8192 ? bx : 8192);
@@ -613,18 +617,6 @@ int linear_nll_fwd_small(const Head<T>& h, T* total, int32_t* count, T* lse, T* 
   return launch_status();
 }
 
-// out (contiguous I x J) = g * sum_c A(i, c) B(j, c) by tiles, through `parts` when the sum is cut
-template <typename T>
-void tile_product_out(Strided<T> a, Strided<T> b, int64_t I, int64_t J, int64_t C, int64_t c_part, int cuts, T* out, T* parts,
-                      GradScale<T> g, cudaStream_t st) {
-  if (cuts == 1) {
-    simt_product<T>(a, b, I, J, C, c_part, nullptr, StoreEpi<T>{out, J, 0, g}, st);
-    return;
-  }
-  simt_product<T>(a, b, I, J, C, c_part, nullptr, PartsEpi<T>{parts}, st);
-  launch_chained(lnll_sum_kernel<T>, (unsigned)ceil_div(I * J, 256), 256, 0, st, parts, I * J, cuts, out, 0, g);
-}
-
 template <typename T>
 int linear_nll_bwd_small(const Head<T>& h, const T* lse, GradScale<T> g, T* dw, T* db, T* dx, char* ws, cudaStream_t st) {
   const SmallPlan p = small_plan<T>(h.V, h.H, h.N, h.trans, 1);
@@ -645,7 +637,13 @@ int linear_nll_bwd_small(const Head<T>& h, const T* lse, GradScale<T> g, T* dw, 
       launch_chained(lnll_sum_kernel<T>, (unsigned)ceil_div(h.N * h.H, 256), 256, 0, st, parts, h.N * h.H, p.x_parts, dx, 0, g);
     } else {
       const Strided<T> w = h.weights(0);
-      tile_product_out<T>(Strided<T>{ds, h.V, 1}, Strided<T>{w.p, w.sc, w.si}, h.N, h.H, h.V, p.x_part, p.x_parts, dx, parts, g, st);
+      const Strided<T> sd{ds, h.V, 1}, sw{w.p, w.sc, w.si};
+      if (p.x_parts == 1) {
+        simt_product<T>(sd, sw, h.N, h.H, h.V, h.V, nullptr, StoreEpi<T>{dx, h.H, 0, g}, st);
+      } else {
+        simt_product<T>(sd, sw, h.N, h.H, h.V, p.x_part, nullptr, PartsEpi<T>{parts}, st);
+        launch_chained(lnll_sum_kernel<T>, (unsigned)ceil_div(h.N * h.H, 256), 256, 0, st, parts, h.N * h.H, p.x_parts, dx, 0, g);
+      }
     }
   }
   if (dw) {
@@ -656,10 +654,16 @@ int linear_nll_bwd_small(const Head<T>& h, const T* lse, GradScale<T> g, T* dw, 
     if (p.few) {
       constexpr int VEC = 16 / sizeof(T);
       const dim3 grid((unsigned)ceil_div(R, 64), (unsigned)ceil_div(C, 128));
-      if (aligned16(b, ldb) && aligned16(dw, C)) launch_chained(outer_kernel<T, VEC>, grid, 256, 0, st, a, lda, b, ldb, h.N, R, C, dw, C, g);
-      else launch_chained(outer_kernel<T, 1>, grid, 256, 0, st, a, lda, b, ldb, h.N, R, C, dw, C, g);
+      if (aligned16(b, ldb) && aligned16(dw, C)) launch_chained(outer_kernel<T, VEC>, grid, 256, 0, st, a, lda, b, ldb, h.labels, h.N, R, C, dw, C, g);
+      else launch_chained(outer_kernel<T, 1>, grid, 256, 0, st, a, lda, b, ldb, h.labels, h.N, R, C, dw, C, g);
     } else {
-      tile_product_out<T>(Strided<T>{a, 1, lda}, Strided<T>{b, 1, ldb}, R, C, h.N, p.w_part, p.w_parts, dw, parts, g, st);
+      const Strided<T> sa{a, 1, lda}, sb{b, 1, ldb};
+      if (p.w_parts == 1) {
+        simt_product_dw<T>(sa, sb, !h.trans, h.labels, R, C, h.N, h.N, StoreEpi<T>{dw, C, 0, g}, st);
+      } else {
+        simt_product_dw<T>(sa, sb, !h.trans, h.labels, R, C, h.N, p.w_part, PartsEpi<T>{parts}, st);
+        launch_chained(lnll_sum_kernel<T>, (unsigned)ceil_div(R * C, 256), 256, 0, st, parts, R * C, p.w_parts, dw, 0, g);
+      }
     }
   }
   return launch_status();
@@ -693,9 +697,9 @@ int linear_nll_bwd_pieces(const Head<T>& h, const T* lse, GradScale<T> g, T* dw,
     if (dx)
       simt_product<T>(Strided<T>{ds, piece, 1}, Strided<T>{w.p, w.sc, w.si}, h.N, h.H, vp, vp, nullptr, StoreEpi<T>{dx, h.H, v0 > 0, g}, st);
     if (dw && h.trans)
-      simt_product<T>(Strided<T>{ds, 1, piece}, Strided<T>{h.x, 1, h.H}, vp, h.H, h.N, h.N, nullptr, StoreEpi<T>{dw + v0 * h.H, h.H, 0, g}, st);
+      simt_product_dw<T>(Strided<T>{ds, 1, piece}, Strided<T>{h.x, 1, h.H}, false, h.labels, vp, h.H, h.N, h.N, StoreEpi<T>{dw + v0 * h.H, h.H, 0, g}, st);
     else if (dw)
-      simt_product<T>(Strided<T>{h.x, 1, h.H}, Strided<T>{ds, 1, piece}, h.H, vp, h.N, h.N, nullptr, StoreEpi<T>{dw + v0, h.V, 0, g}, st);
+      simt_product_dw<T>(Strided<T>{h.x, 1, h.H}, Strided<T>{ds, 1, piece}, true, h.labels, h.H, vp, h.N, h.N, StoreEpi<T>{dw + v0, h.V, 0, g}, st);
   }
   return launch_status();
 }

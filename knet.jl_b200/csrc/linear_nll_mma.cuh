@@ -333,48 +333,58 @@ struct SplitJob {
   int64_t rows, cols, pitch;
   __half* dst;                 // two planes of rows x ld
   int64_t ld, plane;
+  const int32_t* labels;       // of the rows, or null: see lnll_split_kernel
 };
 constexpr int kMaxBlocks = 592;                         // absmax blocks: 4 per SM
 
-// Largest finite magnitude of each of two arrays, one value per block and array.  A block takes runs
-// of 8192 elements of a row in turn (a contiguous array is one row).
-constexpr int kRun = 8192;
+// Largest finite magnitude of each of two arrays, one value per block and array.  W, contiguous, goes to
+// the blocks in turns of 8192 elements; x goes to the warps, 1024 elements of one instance at a time, and
+// a skipped instance (label 0) does not count: a padded batch may hold anything there.
+constexpr int kRun = 8192, kWarpRun = 1024;
+// len <= 32 * LANES values from p on, by LANES threads of which this is number t
+template <int LANES> __device__ __forceinline__ uint32_t run_absmax(const float* p, int len, int t) {
+  uint32_t m = 0;
+  auto take = [&](float v) {
+    const uint32_t u = __float_as_uint(v) & 0x7fffffffu;
+    m = max(m, u < 0x7f800000u ? u : 0u);
+  };
+  int head = (int)(((16 - ((uintptr_t)p & 15)) & 15) / 4);
+  if (head > len) head = len;
+  const int nv = (len - head) / 4;
+  if (t < head) take(p[t]);
+  const float4* q = reinterpret_cast<const float4*>(p + head);
+  float4 v[8];
+#pragma unroll
+  for (int u = 0; u < 8; u++)
+    if (t + u * LANES < nv) v[u] = __ldg(q + t + u * LANES);
+#pragma unroll
+  for (int u = 0; u < 8; u++)
+    if (t + u * LANES < nv) { take(v[u].x); take(v[u].y); take(v[u].z); take(v[u].w); }
+  const int tail = head + nv * 4 + t;
+  if (tail < len) take(p[tail]);
+  return m;
+}
 __global__ void __launch_bounds__(256)
-lnll_absmax_kernel(SplitJob a, SplitJob b, uint32_t* __restrict__ part) {
+lnll_absmax_kernel(const float* __restrict__ w, int64_t n, const float* __restrict__ x, const int32_t* __restrict__ labels, int64_t N,
+                   int64_t H, uint32_t* __restrict__ part) {
   chain_begin();
   __shared__ uint32_t red[32];
-  for (int k = 0; k < 2; k++) {
-    const SplitJob& j = k ? b : a;
-    const bool flat = j.pitch == j.cols;
-    const int64_t rows = flat ? (j.rows > 0 ? 1 : 0) : j.rows, cols = flat ? j.rows * j.cols : j.cols;
-    const int64_t runs = (cols + kRun - 1) / kRun;
-    uint32_t m = 0;
-    auto take = [&](float v) {
-      const uint32_t u = __float_as_uint(v) & 0x7fffffffu;
-      m = max(m, u < 0x7f800000u ? u : 0u);
-    };
-    for (int64_t t = blockIdx.x; t < rows * runs; t += gridDim.x) {
-      const int64_t r = t / runs, c = (t - r * runs) * kRun;
-      const float* p = j.src + r * j.pitch + c;
-      const int len = (int)min((int64_t)kRun, cols - c);
-      int head = (int)(((16 - ((uintptr_t)p & 15)) & 15) / 4);
-      if (head > len) head = len;
-      const int nv = (len - head) / 4;
-      if (threadIdx.x < head) take(p[threadIdx.x]);
-      const float4* q = reinterpret_cast<const float4*>(p + head);
-      float4 v[8];
-#pragma unroll
-      for (int u = 0; u < 8; u++)
-        if (threadIdx.x + u * 256 < nv) v[u] = __ldg(q + threadIdx.x + u * 256);
-#pragma unroll
-      for (int u = 0; u < 8; u++)
-        if (threadIdx.x + u * 256 < nv) { take(v[u].x); take(v[u].y); take(v[u].z); take(v[u].w); }
-      const int tail = head + nv * 4 + threadIdx.x;
-      if (tail < len) take(p[tail]);
-    }
-    m = block_reduce(m, [](uint32_t x, uint32_t y) { return max(x, y); }, 0u, red);
-    if (threadIdx.x == 0) part[k * kMaxBlocks + blockIdx.x] = m;
+  auto larger = [](uint32_t a, uint32_t b) { return max(a, b); };
+  uint32_t m = 0;
+  for (int64_t c = (int64_t)blockIdx.x * kRun; c < n; c += (int64_t)gridDim.x * kRun)
+    m = max(m, run_absmax<256>(w + c, (int)min((int64_t)kRun, n - c), threadIdx.x));
+  m = block_reduce(m, larger, 0u, red);
+  if (threadIdx.x == 0) part[blockIdx.x] = m;
+  m = 0;
+  const int64_t runs = (H + kWarpRun - 1) / kWarpRun;
+  for (int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); t < N * runs; t += (int64_t)gridDim.x * 8) {
+    const int64_t i = t / runs, c = (t - i * runs) * kWarpRun;
+    const bool used = __ldg(labels + i) != 0;          // does not hold up the loads
+    const uint32_t v = run_absmax<32>(x + i * H + c, (int)min((int64_t)kWarpRun, H - c), threadIdx.x & 31);
+    m = used ? max(m, v) : m;
   }
+  m = block_reduce(m, larger, 0u, red);
+  if (threadIdx.x == 0) part[kMaxBlocks + blockIdx.x] = m;
 }
 
 // v = hi + lo in fp16 for two values; what is not finite goes to hi alone, so that an infinity is not NaN
@@ -408,7 +418,8 @@ __device__ __forceinline__ void load8(const float* row, int64_t c, int64_t cols,
 
 // Both operands into their two planes; rows are shared out over blocks, 8 columns per thread and turn.
 // The exponents come from the maxima in `part` (and are left in `saved` for the backward) or, in the
-// backward, from what the forward left (`given`).
+// backward, from what the forward left (`given`).  In a skipped instance (label 0), which the scale does not
+// regard, whatever has no fp16 value becomes 0: its dS is 0, which times infinity would be NaN in dW.
 __global__ void __launch_bounds__(256)
 lnll_split_kernel(SplitJob a, SplitJob b, uint32_t blocks_a, const uint32_t* __restrict__ part, uint32_t parts,
                   const float* __restrict__ given, float* __restrict__ saved, int* __restrict__ exps) {
@@ -437,12 +448,18 @@ lnll_split_kernel(SplitJob a, SplitJob b, uint32_t blocks_a, const uint32_t* __r
   for (int64_t g = total - 1 - ((int64_t)(blockIdx.x - first) * 256 + threadIdx.x); g >= 0; g -= (int64_t)nb * 256) {
     const int64_t r = g / groups, c = (g - r * groups) * 8;
     float v[8];
+    const bool skipped = j.labels && __ldg(j.labels + r) == 0;
     load8(j.src + r * j.pitch, c, j.cols, v);
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      v[k] *= f;
+      if (skipped && !(fabsf(v[k]) <= 65504.0f)) v[k] = 0.0f;
+    }
     uint4 hi, lo;
-    split_pair(v[0] * f, v[1] * f, hi.x, lo.x);
-    split_pair(v[2] * f, v[3] * f, hi.y, lo.y);
-    split_pair(v[4] * f, v[5] * f, hi.z, lo.z);
-    split_pair(v[6] * f, v[7] * f, hi.w, lo.w);
+    split_pair(v[0], v[1], hi.x, lo.x);
+    split_pair(v[2], v[3], hi.y, lo.y);
+    split_pair(v[4], v[5], hi.z, lo.z);
+    split_pair(v[6], v[7], hi.w, lo.w);
     *reinterpret_cast<uint4*>(j.dst + r * j.ld + c) = hi;
     *reinterpret_cast<uint4*>(j.dst + j.plane + r * j.ld + c) = lo;
   }

@@ -31,14 +31,19 @@ template <typename T> __device__ __forceinline__ void copy_element(T* dst, const
                : "memory");
 }
 
-// this thread's elements of one operand's steps: neighbouring threads walk the contiguous axis
-template <typename T> struct TileCopy {
+// this thread's elements of one operand's steps: neighbouring threads walk the contiguous axis.  MASK: where
+// the summed axis is the instances, x of a skipped one (label 0) is taken as 0, since its dS of 0 times what a
+// padded batch holds there may be NaN.
+template <typename T, bool MASK> struct TileCopy {
   static constexpr int S = kStep<T>, PER = S * kTile / kSimtThreads;
   const T* p[PER];
   uint32_t at[PER];            // places in a stage
   int c[PER];                  // summed index in a step; past any bound for a row outside
   int64_t advance;
-  __device__ __forceinline__ TileCopy(const Strided<T>& a, int64_t i0, int64_t c0, int64_t I) : advance(S * a.sc) {
+  const int32_t* labels;       // of the summed indices from this part's first on, or null
+  int32_t used[PER];           // the next step's
+  __device__ __forceinline__ TileCopy(const Strided<T>& a, int64_t i0, int64_t c0, int64_t I, const int32_t* labels_, int64_t left)
+      : advance(S * a.sc), labels(labels_ ? labels_ + c0 : nullptr) {
 #pragma unroll
     for (int r = 0; r < PER; r++) {
       const int i = a.sc == 1 ? threadIdx.x / S + kSimtThreads / S * r : threadIdx.x % kTile;
@@ -48,14 +53,20 @@ template <typename T> struct TileCopy {
       at[r] = (uint32_t)(k * (kTile + 4) + i);
       c[r] = in ? k : 1 << 30;
     }
+    if constexpr (MASK) look(0, left);
+  }
+  __device__ __forceinline__ void look(int k, int64_t left) {
+#pragma unroll
+    for (int r = 0; r < PER; r++) used[r] = !labels || (c[r] < left && __ldg(labels + (int64_t)k * S + c[r]) != 0);
   }
   // step k into `stage`; `left` summed indices remain from its first on
   __device__ __forceinline__ void start(T* stage, int k, int64_t left) {
 #pragma unroll
     for (int r = 0; r < PER; r++) {
-      const bool in = c[r] < left;
+      const bool in = c[r] < left && (!MASK || used[r]);
       copy_element(stage + at[r], in ? p[r] + k * advance : p[r], in);
     }
+    if constexpr (MASK) look(k + 1, left - S);
   }
 };
 
@@ -74,9 +85,10 @@ template <typename T> struct TileShared {
   };
 };
 
-template <typename T, typename Epi>
+template <typename T, bool MASK, typename Epi>
 __global__ void __launch_bounds__(kSimtThreads, 3)
-simt_product_kernel(Strided<T> a, Strided<T> b, int64_t I, int64_t J, int64_t C, int64_t c_part, uint32_t* done, Epi epi) {
+simt_product_kernel(Strided<T> a, Strided<T> b, const int32_t* mask_a, const int32_t* mask_b, int64_t I, int64_t J, int64_t C, int64_t c_part,
+                    uint32_t* done, Epi epi) {
   chain_begin();
   clear_done(done);
   __shared__ __align__(16) TileShared<T> sh;
@@ -92,7 +104,7 @@ simt_product_kernel(Strided<T> a, Strided<T> b, int64_t I, int64_t J, int64_t C,
   const int lane = threadIdx.x & 31, wr = (threadIdx.x >> 5 & 1) * 32, wc = (threadIdx.x >> 6) * 16;
   constexpr int S = kStep<T>;
   const int steps = (int)((c_hi - c_lo + S - 1) / S);
-  TileCopy<T> ca(a, i0, c_lo, I), cb(b, j0, c_lo, J);
+  TileCopy<T, MASK> ca(a, i0, c_lo, I, mask_a, c_hi - c_lo), cb(b, j0, c_lo, J, mask_b, c_hi - c_lo);
   auto start = [&](int k) {
     if (k < steps) {
       const int64_t left = c_hi - c_lo - (int64_t)k * S;
@@ -375,10 +387,11 @@ col_sum_kernel(Matrix<T> m, const T* __restrict__ y, int64_t ldy, int64_t N, int
 
 // out(r, c) = g * sum_n a(n, r) * b(n, c): few instances, bound by the stores.  A CTA takes 64 rows and
 // 128 columns, a warp eight rows; a's entries come through shared memory, eight instances at a time.
+// Skipped instances (label 0) are passed over: 0 times what a padded batch holds there may be NaN.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
-outer_kernel(const T* __restrict__ a, int64_t lda, const T* __restrict__ b, int64_t ldb, int64_t N, int64_t R, int64_t C,
-             T* __restrict__ out, int64_t ld, GradScale<T> g) {
+outer_kernel(const T* __restrict__ a, int64_t lda, const T* __restrict__ b, int64_t ldb, const int32_t* __restrict__ labels, int64_t N,
+             int64_t R, int64_t C, T* __restrict__ out, int64_t ld, GradScale<T> g) {
   chain_begin();
   constexpr int Q = 4 / VEC, NB = 8;
   __shared__ __align__(16) T as[NB][64];
@@ -399,6 +412,7 @@ outer_kernel(const T* __restrict__ a, int64_t lda, const T* __restrict__ b, int6
 #pragma unroll
     for (int n = 0; n < NB; n++) {
       if (n0 + n >= N) break;
+      if (__ldg(labels + n0 + n) == 0) continue;
       T av[8];
 #pragma unroll
       for (int r = 0; r < 8; r++) av[r] = as[n][warp * 8 + r];

@@ -345,3 +345,29 @@ def test_refusals(K):
         K.ops.linear_nll_back(kw, z.zeros((8, 12)), res)
     with pytest.raises(ValueError):
         K.ops.linear_nll_back(kw, kx, res, out=(z.zeros((30, 9)), None, None))
+
+
+# every form: few instances; FMA and FP64 tiles, the sum of dW whole and cut; tensor-core tiles, sums cut and whole;
+# Float64 pieces
+@pytest.mark.parametrize("shape", [(300, 64, 8), (300, 40, 50), (1000, 784, 400), (40, 70, 5000), (1000, 256, 300), (5000, 100, 3000),
+                                   (9000, 96, 2100)], ids=str)
+@pytest.mark.parametrize("trans", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+def test_skipped_instances_may_hold_anything(K, dtype, trans, shape):
+    """What a padded batch has in a skipped instance changes no bit of the loss, the gradients or the used
+    instances' lse."""
+    c = Case(*shape, dtype, trans, True, True)
+    skip = c.labels == 0
+
+    def run():
+        kw, kx, kb = c.arrays(K)
+        res = K.ops.linear_nll_device(kw, kx, c.labels, b=kb, trans=trans)
+        dw, dx, db = K.ops.linear_nll_back(kw, kx, res, b=kb, trans=trans)
+        assert not dx.data.view(c.N, c.H)[skip].any()
+        return [res.total, res.per_instance[:c.N], res.lse[~skip], dw.data, dx.data, db.data]
+
+    c.x[skip] = 0
+    want = run()
+    for bad in (math.nan, math.inf, -math.inf, 1e30, torch.finfo(dtype).min):
+        c.x[skip] = bad
+        assert all(torch.equal(a, b) for a, b in zip(run(), want)), bad

@@ -363,8 +363,9 @@ KNET_BOTH_TYPES(KNET_DECL_NLL, nll)
  * An infinity or a NaN in W or x may make every score that it enters NaN.  What x holds in a
  * skipped instance reaches neither the loss nor a gradient (its lse is then of no use).
  * Large Float32 products (V*H*N from 2^26, or more than 2^24 scores) hold W, x (used instances)
- * and dS to 2^-40 of the largest magnitude of each array: as exact as Float32 arithmetic for
- * entries down to 2^-17 of it, less so below.
+ * to 2^-39 of the largest magnitude of each and dS without g to 2^-39: as exact as Float32
+ * arithmetic for entries down to 2^-16 of the largest (of 1), less so below; a dW of a class whose
+ * probabilities are all about 2^-28 has 2^-11 of relative error per term.
  * Up to 2^24 scores may pass through the workspace where that is faster.
  * workspace: at least knet_linear_nll_workspace_S(V, H, N, backward) bytes (0 for sizes that the
  * entry points refuse), 256-byte aligned; calls that share one must be ordered on one stream.

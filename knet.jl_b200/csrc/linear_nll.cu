@@ -127,22 +127,25 @@ template <typename T> __global__ void lnll_none_kernel(T* total, int32_t* count)
   *count = 0;
 }
 
-// db[j] = g * sum_n ds[n][j]: a CTA takes 32 classes, its 32 warps share the instances
+// db[j] = g * sum_n ds[n][j]: a CTA takes 32 classes, its 32 warps share the instances.  Cut over gridDim.y
+// parts of `rows` instances, the plain sums of each go to parts[part][j].
 template <typename T>
 __global__ void __launch_bounds__(1024)
-lnll_bias_kernel(const T* __restrict__ ds, int64_t ld, int64_t N, int64_t J, T* __restrict__ db, GradScale<T> g) {
+lnll_bias_kernel(const T* __restrict__ ds, int64_t ld, int64_t N, int64_t J, int64_t rows, T* __restrict__ out, GradScale<T> g) {
   chain_begin();
   __shared__ T part[32][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t j = (int64_t)blockIdx.x * 32 + lane;
+  const int64_t n0 = (int64_t)blockIdx.y * rows, n1 = min(N, n0 + rows);
   T a = (T)0;
   if (j < J)
-    for (int64_t n = w; n < N; n += 32) a += ds[n * ld + j];
+#pragma unroll 8
+    for (int64_t n = n0 + w; n < n1; n += 32) a += ds[n * ld + j];
   part[w][lane] = a;
   __syncthreads();
   if (w == 0 && j < J) {
     for (int k = 1; k < 32; k++) a += part[k][lane];
-    db[j] = a * g.value();
+    out[blockIdx.y * J + j] = gridDim.y > 1 ? a : a * g.value();
   }
 }
 
@@ -183,6 +186,16 @@ constexpr int kPlanSMs = 148;
 // ---- plans; the tensor-core form (Float32) --------------------------------------------------------------
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// The bias gradient's rows of dS are cut where there are many and few classes: one CTA of 32 warps would
+// walk them alone.  At most 64 parts of 2048 rows or more, together two CTAs per SM.
+inline int64_t bias_parts(int64_t rows, int64_t J) {
+  int64_t k = 2 * kPlanSMs / ceil_div(J, 32);
+  k = k > rows / 2048 ? rows / 2048 : k;
+  return k > 64 ? 64 : k < 1 ? 1 : k;
+}
+// numbers in the parts of any J classes: more than one part of ceil(J / 32) CTAs are at most two CTAs per SM
+constexpr size_t kBiasRoom = 2 * kPlanSMs * 32;
+
 // Which form a call takes.
 //   kSmall   up to 2^24 scores and either few instances or little work: the scores go to the workspace
 //   kMma     Float32 beyond that
@@ -205,7 +218,7 @@ struct SmallPlan {
   int64_t few, s_part, x_part, w_part;         // few: by vectors, not tiles; lengths of the parts
   int s_parts, x_parts, w_parts;
   int64_t chunks;                              // of 2048 classes, where an instance has more than one
-  size_t scores, parts, stats, total;
+  size_t scores, parts, stats, bias, total;
 };
 template <typename T> SmallPlan small_plan(int64_t V, int64_t H, int64_t N, int trans, int backward) {
   SmallPlan p{};
@@ -239,6 +252,8 @@ template <typename T> SmallPlan small_plan(int64_t V, int64_t H, int64_t N, int 
   if (backward) {
     const size_t x = (size_t)p.x_parts * N * H * sz, w = p.w_parts > 1 ? (size_t)p.w_parts * V * H * sz : 0;
     at += up(x > w ? x : w);
+    p.bias = at;
+    at += up(kBiasRoom * sz);
   }
   p.total = at;
   return p;
@@ -246,15 +261,17 @@ template <typename T> SmallPlan small_plan(int64_t V, int64_t H, int64_t N, int 
 
 // Pieces of the vocabulary and parts of the products' sums.  Workspace bounds: 256 MB of split weights in
 // the forward; 128 MB of dS and 192 MB of split weights in the backward.  Within them the backward takes
-// the piece with the fewest waves of tiles over its three products (a product's tiles are 128 x 256
-// and its time is proportional to the summed length), charging each piece for its launches.  Where a
+// the piece with the fewest waves of tiles over its three products (a product's tiles are 128 x 256, a
+// pair's two of them, and its time is proportional to the summed length), charging each piece for its
+// launches.  Only the smallest piece of each number of pieces is tried: for four million classes that takes the host
+// 10 us, every size of a piece 0.7 ms.  Where a
 // product has tiles for less than half of the SMs, its sum is cut into parts of at least 128 (a chunk);
 // the scores only if they fit 64 MB with their parts, dW only if there is one piece.
 struct MmaPlan {
   int64_t piece, wld, xld, dld;        // classes per piece; row pitches of split w, x and dS (elements)
   int s_parts, x_parts, w_parts;
   int64_t chunks;                      // of 2048 classes, where the scores are in the workspace (s_parts > 1)
-  size_t exps, absmax, xs, ws, label, part_m, part_s, scores, ds, parts, db, total;
+  size_t exps, absmax, xs, ws, label, part_m, part_s, scores, ds, parts, db, bias, total;
 };
 
 inline int64_t cut_sum(int64_t tiles, int64_t len, int64_t bytes) {
@@ -270,26 +287,33 @@ inline MmaPlan mma_plan(int64_t V, int64_t H, int64_t N, int trans, int backward
   const int64_t all = ceil_div(V, kTN), nt = ceil_div(N, kTM), hj = ceil_div(H, kTN), hi = ceil_div(H, kTM);
   p.s_parts = p.x_parts = p.w_parts = 1;
   if (!backward) {
-    int64_t m = (int64_t)(256u << 20) / 4 / H / kTN;
+    int64_t m = (int64_t)(256u << 20) / 4 / (ceil_div(H, 64) * 64) / kTN;
     m = m < 1 ? 1 : m;
     p.piece = kTN * ceil_div(all, ceil_div(all, m));
   } else {
+    // the largest piece within the bounds, then the smallest piece of each number of pieces
+    const int64_t row = ceil_div(H, 64) * 64 * 4 * kTN, most_ds = (128ll << 20) / (kTN * N * 4), most_w = (192ll << 20) / row;
+    int64_t m = most_ds < most_w ? most_ds : most_w;
+    m = m < 1 ? 1 : m > all ? all : m;
     double best = 0;
-    for (int64_t m = 1; m <= all; m++) {
-      if (m > 1 && (m * kTN * N * 4 > (128ll << 20) || m * kTN * H * 4 > (192ll << 20))) break;
+    for (bool first = true; m > 0; first = false) {
+      const int64_t pieces = ceil_div(all, m);
+      if (!first && pieces * 1500.0 >= best) break;
+      m = ceil_div(all, pieces);
       int64_t sp = kPlanSMs / (nt * hj);
       sp = sp < 1 ? 1 : sp > 2 * m ? 2 * m : sp > 16 ? 16 : sp;
       const int64_t wt = trans ? 2 * m * hj : hi * m;
       const int64_t wp = m == all ? cut_sum(wt, N, V * H * 4) : 1;
       const double t = (double)ceil_div(nt * m, kPlanSMs) * H + (double)ceil_div(nt * hj * sp, kPlanSMs) * ceil_div(m * kTN, sp) +
                        (double)ceil_div(wt * wp, kPlanSMs) * ceil_div(N, wp) + 1500.0;
-      const double cost = t * ceil_div(all, m);
-      if (m == 1 || cost < best) {
+      const double cost = t * pieces;
+      if (first || cost <= best) {
         best = cost;
         p.piece = m * kTN;
         p.x_parts = (int)sp;
         p.w_parts = (int)wp;
       }
+      m--;
     }
   }
   if (p.piece >= V) p.s_parts = (int)cut_sum(nt * all, H, N * V * 4);
@@ -319,6 +343,7 @@ inline MmaPlan mma_plan(int64_t V, int64_t H, int64_t N, int trans, int backward
     const size_t x = p.x_parts > 1 ? (size_t)p.x_parts * N * H * 4 : 0, w = p.w_parts > 1 ? (size_t)p.w_parts * V * H * 4 : 0;
     put(p.parts, x > w ? x : w);
     put(p.db, (size_t)ceil_div(N, kGradRows) * vp * 4);
+    put(p.bias, kBiasRoom * 4);
   }
   p.total = at;
   return p;
@@ -328,7 +353,7 @@ template <typename T> size_t workspace(int64_t V, int64_t H, int64_t N, int tran
   const Form f = form<T>(V, H, N);
   if (f == kMma) return mma_plan(V, H, N, trans, backward).total;
   if (f == kSmall) return small_plan<T>(V, H, N, trans, backward).total;
-  if (backward) return up((size_t)N * simt_piece<T>(V, N) * sizeof(T));
+  if (backward) return up((size_t)N * simt_piece<T>(V, N) * sizeof(T)) + up(kBiasRoom * sizeof(T));
   const int64_t tiles = (V + kTile - 1) / kTile;
   return up(4) + up((size_t)N * sizeof(T)) + 2 * up((size_t)tiles * N * sizeof(T));
 }
@@ -556,6 +581,15 @@ inline int linear_nll_fwd_mma(const Head<float>& h, float* total, int32_t* count
   return launch_status();
 }
 
+// db from rows of dS or of its sums over groups of instances
+template <typename T>
+void bias_gradient(const T* ds, int64_t ld, int64_t rows, int64_t J, T* db, T* parts, GradScale<T> g, cudaStream_t st) {
+  const int64_t k = bias_parts(rows, J), part = ceil_div(rows, k);
+  const dim3 grid((unsigned)ceil_div(J, 32), (unsigned)ceil_div(rows, part));
+  launch_chained(lnll_bias_kernel<T>, grid, 1024, 0, st, ds, ld, rows, J, part, grid.y > 1 ? parts : db, g);
+  if (grid.y > 1) launch_chained(lnll_sum_kernel<T>, (unsigned)ceil_div(J, 256), 256, 0, st, (const T*)parts, J, (int)grid.y, db, 0, g);
+}
+
 inline int linear_nll_bwd_mma(const Head<float>& h, const float* lse, GradScale<float> g, float* dw, float* db, float* dx, char* ws,
                               cudaStream_t st) {
   const MmaPlan p = mma_plan(h.V, h.H, h.N, h.trans, 1);
@@ -576,8 +610,7 @@ inline int linear_nll_bwd_mma(const Head<float>& h, const float* lse, GradScale<
       const MmaGradScores e1{exps, h.bias ? h.bias + v0 : nullptr, h.labels, lse, (__half*)(ws + p.ds), h.N, vp, p.dld, ds.plane, v0, dbp};
       if (int rc = mma_product(s.x, false, s.w, !h.trans, h.N, vp, h.H, 1, e1, st)) return rc;
     }
-    if (db)
-      launch_chained(lnll_bias_kernel<float>, (unsigned)ceil_div(vp, 32), 1024, 0, st, dbp, vp, ceil_div(h.N, p.s_parts > 1 ? kGradRows : kTM), vp, db + v0, g);
+    if (db) bias_gradient<float>(dbp, vp, ceil_div(h.N, p.s_parts > 1 ? kGradRows : kTM), vp, db + v0, (float*)(ws + p.bias), g, st);
     if (dx) {
       const int k = mma_parts(vp, p.x_parts);
       const MmaStore e2{exps, 0, k == 1 ? dx : parts, h.N, h.H, h.H, k == 1 ? 0 : h.N * h.H, k == 1 && v0 > 0, nullptr, g};
@@ -629,7 +662,7 @@ int linear_nll_bwd_small(const Head<T>& h, const T* lse, GradScale<T> g, T* dw, 
     const int64_t blocks = ceil_div(h.V, 1024);
     launch_chained(lnll_grad_kernel<T>, (unsigned)(blocks * h.N), 256, 0, st, ds, p.s_parts, h.bias, h.labels, lse, h.N, h.V, (uint32_t)blocks);
   }
-  if (db) launch_chained(lnll_bias_kernel<T>, (unsigned)ceil_div(h.V, 32), 1024, 0, st, ds, h.V, h.N, h.V, db, g);
+  if (db) bias_gradient<T>(ds, h.V, h.N, h.V, db, (T*)(ws + p.bias), g, st);
   const Matrix<T> m = weight_matrix(h);
   if (dx) {
     if (p.few) {
@@ -693,7 +726,7 @@ int linear_nll_bwd_pieces(const Head<T>& h, const T* lse, GradScale<T> g, T* dw,
     const Strided<T> w = h.weights(v0);
     simt_product<T>(Strided<T>{h.x, h.H, 1}, w, h.N, vp, h.H, h.H, nullptr,
                     GradScoresEpi<T>{h.bias ? h.bias + v0 : nullptr, h.labels, lse, ds, h.N, piece, v0}, st);
-    if (db) launch_chained(lnll_bias_kernel<T>, (unsigned)ceil_div(vp, 32), 1024, 0, st, ds, piece, h.N, vp, db + v0, g);
+    if (db) bias_gradient<T>(ds, piece, h.N, vp, db + v0, (T*)((char*)ws + up((size_t)h.N * piece * sizeof(T))), g, st);
     if (dx)
       simt_product<T>(Strided<T>{ds, piece, 1}, Strided<T>{w.p, w.sc, w.si}, h.N, h.H, vp, vp, nullptr, StoreEpi<T>{dx, h.H, v0 > 0, g}, st);
     if (dw && h.trans)

@@ -2,8 +2,9 @@
 //
 // A Float32 operand, scaled by a power of two that brings its largest magnitude into [2^14, 2^15), is
 // split into two fp16 terms, hi = fp16(x), lo = fp16(x - hi): together 22 bits, and never less than
-// 2^-25 of the scaled value's unit, so entries down to 2^-17 of the largest keep a relative error of
-// 2^-23.  A product takes three of the four partial products (lo*lo is below 2^-22 of it), which are
+// 2^-25 of the scaled value's unit, so entries down to 2^-16 of the largest keep a relative error of
+// 2^-23 (probabilities below 2^-16 in dS therefore do not; a third term would make a product of six instead
+// of three).  A product takes three of the four partial products (lo*lo is below 2^-22 of it), which are
 // exact in Float32; the tensor core adds them.  Its additions truncate: measured on sums of 1024 and 8192
 // products, an accumulator that takes n blocks of 32 summed indices comes out low by 0.75 n 2^-23 of its
 // value for terms of random signs (n = 4, 8, 16: 3.4e-7, 7.4e-7, 1.5e-6), about twice that for terms of
@@ -373,18 +374,20 @@ lnll_absmax_kernel(const float* __restrict__ w, int64_t n, const float* __restri
   uint32_t m = 0;
   for (int64_t c = (int64_t)blockIdx.x * kRun; c < n; c += (int64_t)gridDim.x * kRun)
     m = max(m, run_absmax<256>(w + c, (int)min((int64_t)kRun, n - c), threadIdx.x));
-  m = block_reduce(m, larger, 0u, red);
-  if (threadIdx.x == 0) part[blockIdx.x] = m;
-  m = 0;
+  uint32_t mx = 0;
   const int64_t runs = (H + kWarpRun - 1) / kWarpRun;
   for (int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); t < N * runs; t += (int64_t)gridDim.x * 8) {
     const int64_t i = t / runs, c = (t - i * runs) * kWarpRun;
     const bool used = __ldg(labels + i) != 0;          // does not hold up the loads
     const uint32_t v = run_absmax<32>(x + i * H + c, (int)min((int64_t)kWarpRun, H - c), threadIdx.x & 31);
-    m = used ? max(m, v) : m;
+    mx = used ? max(mx, v) : mx;
   }
   m = block_reduce(m, larger, 0u, red);
-  if (threadIdx.x == 0) part[kMaxBlocks + blockIdx.x] = m;
+  mx = block_reduce(mx, larger, 0u, red);
+  if (threadIdx.x == 0) {
+    part[blockIdx.x] = m;
+    part[kMaxBlocks + blockIdx.x] = mx;
+  }
 }
 
 // v = hi + lo in fp16 for two values; what is not finite goes to hi alone, so that an infinity is not NaN

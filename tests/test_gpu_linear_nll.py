@@ -38,6 +38,7 @@ class Case:
         g = torch.Generator(device="cuda")
         g.manual_seed(seed + 17 * V + 5 * H + N)
         self.V, self.H, self.N, self.dtype, self.trans = V, H, N, dtype, trans
+        self.ds_step = 0.0                  # absolute rounding of dS (without g)
         self.w = torch.randn((V, H), generator=g, device="cuda", dtype=dtype) * (std / math.sqrt(H))
         self.x = torch.randn((N, H), generator=g, device="cuda", dtype=dtype)
         self.b = torch.randn(V, generator=g, device="cuda", dtype=dtype) if bias else None
@@ -75,11 +76,12 @@ class Case:
         self.total, self.dtotal = float(per.sum()), float(dper.sum()) + 2 * u * float(per.abs().sum())
         self.count = int(used.sum())
         p = torch.exp(s - lse.unsqueeze(1))
-        e = p * (torch.expm1(ds + dlse.unsqueeze(1) + 8 * u) + 8 * u) + 2 * u * p
+        e = p * (torch.expm1(ds + dlse.unsqueeze(1) + 8 * u) + 8 * u) + 2 * u * p + self.ds_step
         p.scatter_add_(1, at, torch.full_like(lse, -1.0).unsqueeze(1))
         e.scatter_add_(1, at, torch.full_like(lse, 2 * u).unsqueeze(1))
         f = used.double().unsqueeze(1) * ((dy / self.count if self.count else 0.0) if average else dy)
-        p, e = p * f, e * f.abs() + 4 * u * (p * f).abs()
+        p, e = p * f, torch.where(f == 0, torch.zeros_like(e), e * f.abs() + 4 * u * (p * f).abs())     # skipped: exactly 0
+        self.p, self.top = p, 1 + float(torch.nan_to_num(s, neginf=0.0).abs().max())
         self.dx, self.ddx = p @ w, e @ w.abs() + gamma(V, u) * (p.abs() @ w.abs())
         self.dw, self.ddw = p.t() @ x, e.t() @ x.abs() + gamma(N, u) * (p.abs().t() @ x.abs())
         self.db, self.ddb = p.sum(0), e.sum(0) + gamma(N, u) * p.abs().sum(0)
@@ -371,3 +373,33 @@ def test_skipped_instances_may_hold_anything(K, dtype, trans, shape):
     for bad in (math.nan, math.inf, -math.inf, 1e30, torch.finfo(dtype).min):
         c.x[skip] = bad
         assert all(torch.equal(a, b) for a, b in zip(run(), want)), bad
+
+
+@pytest.mark.parametrize("shape", [(10, 5, 20000), (33, 7, 30001), (70, 3, 150000), (300, 2, 70000)], ids=str)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+def test_bias_gradient_over_many_instances(K, dtype, shape):
+    check(K, Case(*shape, dtype, False, True, True))
+
+
+@pytest.mark.parametrize("shape", [(4194240, 2, 5), (600001, 1, 33), (2, 4194240, 3), (3, 1048577, 40), (4, 3, 4194240), (5, 2, 4194240)], ids=str)
+@pytest.mark.parametrize("trans", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+def test_longest_axes(K, dtype, trans, shape):
+    """Each axis at its largest, few and many scores.  With millions of classes probabilities lie below 2^-16, and
+    the tensor-core form's own rounding of dS shows: p 2^14 is held as two fp16 numbers, whose second is a multiple
+    of fp16's smallest number 2^-24 (p < 2^-13 makes it that small), so p is off by half of that over 2^14, 2^-39."""
+    c = Case(*shape, dtype, trans, True, True)
+    V, H, N = shape
+    c.ds_step = 2.0 ** -39 if dtype == torch.float32 and (N * V > 2 ** 24 or V * H * N >= 2 ** 26) else 0.0
+    res, dw, dx, db = check(K, c)
+    # The worst order of millions of roundings says little, so also: they come with either sign, an error beyond
+    # 16 standard deviations of the longest sum's, sqrt(n) 2u of its largest value, is not rounding.
+    t = 16 * math.sqrt(max(shape)) * 2 * U[dtype] * c.top
+    used = c.labels != 0
+    assert float((res.lse.double() - c.lse)[used].abs().max() if bool(used.any()) else 0.0) <= t
+    # c.p holds the softmax minus one-hot; at the label the error is that of the softmax, at most t (|p - 1| + 1)
+    hot = torch.zeros_like(c.p).scatter_(1, (c.labels.long() - 1).clamp_min(0).unsqueeze(1), 1.0)
+    x, w, p = c.x.double().abs(), c.w.double().abs(), (c.p.abs() + (hot + c.ds_step) / max(c.count, 1)) * used.unsqueeze(1)
+    within(c.matrix(dw), c.dw, t * (p.t() @ x) + c.ds_step * x.sum(0), "dw")
+    within(dx.data.view(N, H), c.dx, t * (p @ w) + c.ds_step * w.sum(0) * used.unsqueeze(1), "dx")
+    within(db.data, c.db, t * p.sum(0) + c.ds_step, "db")

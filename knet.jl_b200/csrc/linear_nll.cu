@@ -174,13 +174,6 @@ template <typename T> struct Head {
 constexpr size_t kAlign = 256;
 inline size_t up(size_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
 
-// classes per piece of the backward: as many as keep dS within 64 MB, whole tiles
-template <typename T> int64_t simt_piece(int64_t V, int64_t N) {
-  int64_t v = (int64_t)((64u << 20) / sizeof(T)) / N / kTile * kTile;
-  if (v < kTile) v = kTile;
-  return v < V ? v : V;
-}
-
 constexpr int kPlanSMs = 148;
 
 // ---- plans; the tensor-core form (Float32) --------------------------------------------------------------
@@ -349,11 +342,51 @@ inline MmaPlan mma_plan(int64_t V, int64_t H, int64_t N, int trans, int backward
   return p;
 }
 
+// Tiles for the SMs: the parts of a sum of `len` (at least 64 long, at most 8) that leave the SMs idle least,
+// each SM taking its share of tiles * parts one after the other.
+inline void even_parts(int64_t tiles, int64_t len, int64_t bytes, int64_t& part, int& parts) {
+  int64_t most = (64 << 20) / (bytes + 1), best = 1;
+  most = most > 8 ? 8 : most;
+  most = most > len / 64 ? len / 64 : most;
+  double cost = 0;
+  for (int64_t k = 1; k <= most || k == 1; k++) {
+    const double c = (double)ceil_div(tiles * k, kPlanSMs) / k * (1.0 + 0.01 * k);
+    if (k == 1 || c < cost) {
+      cost = c;
+      best = k;
+    }
+  }
+  part = ceil_div(ceil_div(len, best), 64) * 64;
+  parts = (int)ceil_div(len, part);
+}
+// Float64 with many scores: pieces of equal size with at most 128 MB of dS
+struct PiecePlan {
+  int64_t piece, x_part, w_part;
+  int x_parts, w_parts;
+  size_t parts, bias, total;
+};
+template <typename T> PiecePlan piece_plan(int64_t V, int64_t H, int64_t N) {
+  PiecePlan p{};
+  int64_t most = (int64_t)((128u << 20) / sizeof(T)) / N / kTile;
+  most = most < 1 ? 1 : most;
+  const int64_t all = ceil_div(V, kTile);
+  p.piece = ceil_div(all, ceil_div(all, most)) * kTile;
+  p.piece = p.piece < V ? p.piece : V;
+  const int64_t nt = ceil_div(N, kTile), ht = ceil_div(H, kTile), vt = ceil_div(p.piece, kTile), sz = sizeof(T);
+  even_parts(nt * ht, p.piece, N * H * sz, p.x_part, p.x_parts);
+  even_parts(vt * ht, N, p.piece * H * sz, p.w_part, p.w_parts);
+  const size_t x = p.x_parts > 1 ? (size_t)p.x_parts * N * H * sz : 0, w = p.w_parts > 1 ? (size_t)p.w_parts * p.piece * H * sz : 0;
+  p.parts = up((size_t)N * p.piece * sz);
+  p.bias = p.parts + up(x > w ? x : w);
+  p.total = p.bias + up(kBiasRoom * sz);
+  return p;
+}
+
 template <typename T> size_t workspace(int64_t V, int64_t H, int64_t N, int trans, int backward) {
   const Form f = form<T>(V, H, N);
   if (f == kMma) return mma_plan(V, H, N, trans, backward).total;
   if (f == kSmall) return small_plan<T>(V, H, N, trans, backward).total;
-  if (backward) return up((size_t)N * simt_piece<T>(V, N) * sizeof(T)) + up(kBiasRoom * sizeof(T));
+  if (backward) return piece_plan<T>(V, H, N).total;
   const int64_t tiles = (V + kTile - 1) / kTile;
   return up(4) + up((size_t)N * sizeof(T)) + 2 * up((size_t)tiles * N * sizeof(T));
 }
@@ -368,6 +401,22 @@ void simt_product(Strided<T> a, Strided<T> b, int64_t I, int64_t J, int64_t C, i
   launch_chained(simt_product_kernel<T, false, Epi>, grid, kSimtThreads, 0, st, a, b, (const int32_t*)nullptr, (const int32_t*)nullptr, I, J, C,
                  c_part, done, epi);
 }
+// out (I x J, rows `ld` apart) = or += g * (parts, added in order)
+template <typename T>
+void sum_parts_to(const T* parts, int64_t I, int64_t J, int64_t ld, int count, T* out, int add, GradScale<T> g, cudaStream_t st) {
+  launch_chained(lnll_sum_kernel<T>, (unsigned)ceil_div(I * J, 256), 256, 0, st, parts, I * J, J, ld, count, out, add, g);
+}
+// out (I x J, rows `ld` apart) = or += g * sum_c A(i, c) B(j, c), through `parts` where the sum is cut
+template <typename T>
+void tile_product_out(Strided<T> a, Strided<T> b, int64_t I, int64_t J, int64_t C, int64_t c_part, int cuts, T* out, int64_t ld, int add,
+                      T* parts, GradScale<T> g, cudaStream_t st) {
+  if (cuts == 1) {
+    simt_product<T>(a, b, I, J, C, C, nullptr, StoreEpi<T>{out, ld, add, g}, st);
+  } else {
+    simt_product<T>(a, b, I, J, C, c_part, nullptr, PartsEpi<T>{parts}, st);
+    sum_parts_to<T>(parts, I, J, ld, cuts, out, add, g, st);
+  }
+}
 // dW's: the sum runs over the instances, of which the labels tell the skipped ones in the operand that is x
 template <typename T, typename Epi>
 void simt_product_dw(Strided<T> a, Strided<T> b, bool a_is_x, const int32_t* labels, int64_t I, int64_t J, int64_t N, int64_t c_part,
@@ -375,6 +424,16 @@ void simt_product_dw(Strided<T> a, Strided<T> b, bool a_is_x, const int32_t* lab
   const dim3 grid((unsigned)ceil_div(J, kTile), (unsigned)ceil_div(I, kTile), (unsigned)ceil_div(N, c_part));
   launch_chained(simt_product_kernel<T, true, Epi>, grid, kSimtThreads, 0, st, a, b, a_is_x ? labels : nullptr, a_is_x ? nullptr : labels, I, J, N,
                  c_part, (uint32_t*)nullptr, epi);
+}
+template <typename T>
+void tile_product_dw(Strided<T> a, Strided<T> b, bool a_is_x, const int32_t* labels, int64_t I, int64_t J, int64_t N, int64_t n_part, int cuts,
+                     T* out, int64_t ld, T* parts, GradScale<T> g, cudaStream_t st) {
+  if (cuts == 1) {
+    simt_product_dw<T>(a, b, a_is_x, labels, I, J, N, N, StoreEpi<T>{out, ld, 0, g}, st);
+  } else {
+    simt_product_dw<T>(a, b, a_is_x, labels, I, J, N, n_part, PartsEpi<T>{parts}, st);
+    sum_parts_to<T>(parts, I, J, ld, cuts, out, 0, g, st);
+  }
 }
 
 // packs of VEC elements are possible where base addresses and pitches are multiples of 16 bytes
@@ -587,7 +646,7 @@ void bias_gradient(const T* ds, int64_t ld, int64_t rows, int64_t J, T* db, T* p
   const int64_t k = bias_parts(rows, J), part = ceil_div(rows, k);
   const dim3 grid((unsigned)ceil_div(J, 32), (unsigned)ceil_div(rows, part));
   launch_chained(lnll_bias_kernel<T>, grid, 1024, 0, st, ds, ld, rows, J, part, grid.y > 1 ? parts : db, g);
-  if (grid.y > 1) launch_chained(lnll_sum_kernel<T>, (unsigned)ceil_div(J, 256), 256, 0, st, (const T*)parts, J, (int)grid.y, db, 0, g);
+  if (grid.y > 1) sum_parts_to<T>(parts, 1, J, J, (int)grid.y, db, 0, g, st);
 }
 
 inline int linear_nll_bwd_mma(const Head<float>& h, const float* lse, GradScale<float> g, float* dw, float* db, float* dx, char* ws,
@@ -615,7 +674,7 @@ inline int linear_nll_bwd_mma(const Head<float>& h, const float* lse, GradScale<
       const int k = mma_parts(vp, p.x_parts);
       const MmaStore e2{exps, 0, k == 1 ? dx : parts, h.N, h.H, h.H, k == 1 ? 0 : h.N * h.H, k == 1 && v0 > 0, nullptr, g};
       if (int rc = mma_product(ds, false, s.w, (bool)h.trans, h.N, h.H, vp, k, e2, st)) return rc;
-      if (k > 1) launch_chained(lnll_sum_kernel<float>, (unsigned)ceil_div(h.N * h.H, 256), 256, 0, st, parts, h.N * h.H, k, dx, v0 > 0, g);
+      if (k > 1) sum_parts_to<float>(parts, h.N, h.H, h.H, k, dx, v0 > 0, g, st);
     }
     if (dw) {
       const int k = mma_parts(h.N, p.w_parts);           // more than one only where one piece holds all classes
@@ -624,7 +683,7 @@ inline int linear_nll_bwd_mma(const Head<float>& h, const float* lse, GradScale<
       const MmaStore e3{exps, 1, k == 1 ? out : parts, I, J, h.trans ? h.H : h.V, k == 1 ? 0 : h.V * h.H, 0, nullptr, g};
       if (int rc = h.trans ? mma_product(ds, true, s.x, true, I, J, h.N, k, e3, st) : mma_product(s.x, true, ds, true, I, J, h.N, k, e3, st))
         return rc;
-      if (k > 1) launch_chained(lnll_sum_kernel<float>, (unsigned)ceil_div(h.V * h.H, 256), 256, 0, st, parts, h.V * h.H, k, dw, 0, g);
+      if (k > 1) sum_parts_to<float>(parts, I, J, J, k, dw, 0, g, st);
     }
   }
   return launch_status();
@@ -667,16 +726,10 @@ int linear_nll_bwd_small(const Head<T>& h, const T* lse, GradScale<T> g, T* dw, 
   if (dx) {
     if (p.few) {
       few_product<T>(!h.trans, m, ds, h.V, h.N, p.x_part, p.x_parts, nullptr, parts, st);
-      launch_chained(lnll_sum_kernel<T>, (unsigned)ceil_div(h.N * h.H, 256), 256, 0, st, parts, h.N * h.H, p.x_parts, dx, 0, g);
+      sum_parts_to<T>(parts, h.N, h.H, h.H, p.x_parts, dx, 0, g, st);
     } else {
       const Strided<T> w = h.weights(0);
-      const Strided<T> sd{ds, h.V, 1}, sw{w.p, w.sc, w.si};
-      if (p.x_parts == 1) {
-        simt_product<T>(sd, sw, h.N, h.H, h.V, h.V, nullptr, StoreEpi<T>{dx, h.H, 0, g}, st);
-      } else {
-        simt_product<T>(sd, sw, h.N, h.H, h.V, p.x_part, nullptr, PartsEpi<T>{parts}, st);
-        launch_chained(lnll_sum_kernel<T>, (unsigned)ceil_div(h.N * h.H, 256), 256, 0, st, parts, h.N * h.H, p.x_parts, dx, 0, g);
-      }
+      tile_product_out<T>(Strided<T>{ds, h.V, 1}, Strided<T>{w.p, w.sc, w.si}, h.N, h.H, h.V, p.x_part, p.x_parts, dx, h.H, 0, parts, g, st);
     }
   }
   if (dw) {
@@ -690,13 +743,7 @@ int linear_nll_bwd_small(const Head<T>& h, const T* lse, GradScale<T> g, T* dw, 
       if (aligned16(b, ldb) && aligned16(dw, C)) launch_chained(outer_kernel<T, VEC>, grid, 256, 0, st, a, lda, b, ldb, h.labels, h.N, R, C, dw, C, g);
       else launch_chained(outer_kernel<T, 1>, grid, 256, 0, st, a, lda, b, ldb, h.labels, h.N, R, C, dw, C, g);
     } else {
-      const Strided<T> sa{a, 1, lda}, sb{b, 1, ldb};
-      if (p.w_parts == 1) {
-        simt_product_dw<T>(sa, sb, !h.trans, h.labels, R, C, h.N, h.N, StoreEpi<T>{dw, C, 0, g}, st);
-      } else {
-        simt_product_dw<T>(sa, sb, !h.trans, h.labels, R, C, h.N, p.w_part, PartsEpi<T>{parts}, st);
-        launch_chained(lnll_sum_kernel<T>, (unsigned)ceil_div(R * C, 256), 256, 0, st, parts, R * C, p.w_parts, dw, 0, g);
-      }
+      tile_product_dw<T>(Strided<T>{a, 1, lda}, Strided<T>{b, 1, ldb}, !h.trans, h.labels, R, C, h.N, p.w_part, p.w_parts, dw, C, parts, g, st);
     }
   }
   return launch_status();
@@ -719,20 +766,19 @@ int linear_nll_fwd_pieces(const Head<T>& h, T* total, int32_t* count, T* lse, T*
 
 template <typename T>
 int linear_nll_bwd_pieces(const Head<T>& h, const T* lse, GradScale<T> g, T* dw, T* db, T* dx, char* ws, cudaStream_t st) {
-  const int64_t piece = simt_piece<T>(h.V, h.N);
-  T* ds = (T*)ws;
-  for (int64_t v0 = 0; v0 < h.V; v0 += piece) {
-    const int64_t vp = h.V - v0 < piece ? h.V - v0 : piece;
-    const Strided<T> w = h.weights(v0);
+  const PiecePlan p = piece_plan<T>(h.V, h.H, h.N);
+  T *ds = (T*)ws, *parts = (T*)(ws + p.parts);
+  for (int64_t v0 = 0; v0 < h.V; v0 += p.piece) {
+    const int64_t vp = h.V - v0 < p.piece ? h.V - v0 : p.piece;
+    const Strided<T> w = h.weights(v0), d{ds, 1, p.piece}, x{h.x, 1, h.H};
     simt_product<T>(Strided<T>{h.x, h.H, 1}, w, h.N, vp, h.H, h.H, nullptr,
-                    GradScoresEpi<T>{h.bias ? h.bias + v0 : nullptr, h.labels, lse, ds, h.N, piece, v0}, st);
-    if (db) bias_gradient<T>(ds, piece, h.N, vp, db + v0, (T*)((char*)ws + up((size_t)h.N * piece * sizeof(T))), g, st);
+                    GradScoresEpi<T>{h.bias ? h.bias + v0 : nullptr, h.labels, lse, ds, h.N, p.piece, v0}, st);
+    if (db) bias_gradient<T>(ds, p.piece, h.N, vp, db + v0, (T*)(ws + p.bias), g, st);
     if (dx)
-      simt_product<T>(Strided<T>{ds, piece, 1}, Strided<T>{w.p, w.sc, w.si}, h.N, h.H, vp, vp, nullptr, StoreEpi<T>{dx, h.H, v0 > 0, g}, st);
-    if (dw && h.trans)
-      simt_product_dw<T>(Strided<T>{ds, 1, piece}, Strided<T>{h.x, 1, h.H}, false, h.labels, vp, h.H, h.N, h.N, StoreEpi<T>{dw + v0 * h.H, h.H, 0, g}, st);
-    else if (dw)
-      simt_product_dw<T>(Strided<T>{h.x, 1, h.H}, Strided<T>{ds, 1, piece}, true, h.labels, h.H, vp, h.N, h.N, StoreEpi<T>{dw + v0, h.V, 0, g}, st);
+      tile_product_out<T>(Strided<T>{ds, p.piece, 1}, Strided<T>{w.p, w.sc, w.si}, h.N, h.H, vp, p.x_part, (int)ceil_div(vp, p.x_part), dx, h.H,
+                          v0 > 0, parts, g, st);
+    if (dw && h.trans) tile_product_dw<T>(d, x, false, h.labels, vp, h.H, h.N, p.w_part, p.w_parts, dw + v0 * h.H, h.H, parts, g, st);
+    else if (dw) tile_product_dw<T>(x, d, true, h.labels, h.H, vp, h.N, p.w_part, p.w_parts, dw + v0, h.V, parts, g, st);
   }
   return launch_status();
 }

@@ -216,7 +216,7 @@ template <typename T, int VEC> __device__ __forceinline__ Pack<T, VEC> ld_cached
 // parts[z part][n][row] = sum over a part of the columns of M(row, c) * y(n, c): a warp takes four
 // rows, its lanes the columns; the vectors come through L1.
 template <typename T, int NB, int VEC>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 2)
 row_dot_kernel(Matrix<T> m, const T* __restrict__ y, int64_t ldy, int64_t N, int64_t c_part, uint32_t* done, T* __restrict__ parts) {
   chain_begin();
   clear_done(done);
@@ -308,7 +308,7 @@ __device__ __forceinline__ void join_warps(T (&acc)[NB][4], T (*red)[NB][128]) {
 // its 8 warps share the rows; the vectors' entries come transposed through shared memory.
 constexpr int kColRows = 128;
 template <typename T, int NB, int VEC>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 2)
 col_sum_kernel(Matrix<T> m, const T* __restrict__ y, int64_t ldy, int64_t N, int64_t r_part, uint32_t* done, T* __restrict__ parts) {
   chain_begin();
   clear_done(done);
@@ -339,7 +339,7 @@ col_sum_kernel(Matrix<T> m, const T* __restrict__ y, int64_t ldy, int64_t N, int
     }
     __syncthreads();
     // rows warp, warp + 8, ... of the 128, UN at a time, the next batch in flight while one is used
-    constexpr int UN = NB >= 8 ? 4 : 8, BATCHES = kColRows / (8 * UN);
+    constexpr int UN = (NB >= 8 ? 4 : 8) / (sizeof(T) / 4), BATCHES = kColRows / (8 * UN);
     Pack<T, VEC> w[2][UN][Q];
     auto fetch = [&](Pack<T, VEC> (&to)[UN][Q], int batch) {
 #pragma unroll
@@ -583,15 +583,16 @@ lnll_grad_kernel(T* __restrict__ scores, int parts, const T* __restrict__ bias, 
     if (v0 + k * 256 < V) x[v0 + k * 256] = grad_score(t[k], hi, lo, lab, v0 + k * 256);
 }
 
-// out = g * (the parts, added in order)
+// out = g * (the parts, added in order), n numbers in rows of J, `ld` apart in `out`
 template <typename T>
 __global__ void __launch_bounds__(256)
-lnll_sum_kernel(const T* __restrict__ parts, int64_t n, int count, T* __restrict__ out, int add, GradScale<T> g) {
+lnll_sum_kernel(const T* __restrict__ parts, int64_t n, int64_t J, int64_t ld, int count, T* __restrict__ out, int add, GradScale<T> g) {
   chain_begin();
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= n) return;
   const T a = sum_parts(parts + i, n, count) * g.value();
-  out[i] = add ? out[i] + a : a;
+  const int64_t to = J == ld ? i : i / J * ld + i % J;
+  out[to] = add ? out[to] + a : a;
 }
 
 }  // namespace kn

@@ -204,9 +204,30 @@ template <typename T> Form form(int64_t V, int64_t H, int64_t N) {
   return fits && (double)V * H * N < (double)(1ll << 32) ? kSmall : kPieces;
 }
 
-// Parts of the summed axes of the three products in kSmall: no more CTAs than three per SM (tiles:
+// Parts (at most 8, of at least 64 terms) of the sums of `tiles` FP64 tiles that take the SMs the least time:
+// an SM gets ceil(tiles * parts / SMs) CTAs, one alone keeps its FP64 unit at about 0.6 of the rate of three, two
+// at 0.85, and writing and reading a part weighs as much as 40 terms.  Measured, loss and gradients:
+// 4645x1102, 318 instances 662 us with parts only below a round of three CTAs per SM, 605 us so.
+inline void even_parts(int64_t tiles, int64_t len, int64_t bytes, int64_t& part, int& parts) {
+  int64_t most = (64 << 20) / (bytes + 1), best = 1;
+  most = most > 8 ? 8 : most;
+  most = most > len / 64 ? len / 64 : most;
+  double cost = 0;
+  for (int64_t k = 1; k <= most || k == 1; k++) {
+    const int64_t n = ceil_div(tiles * k, kPlanSMs);
+    const double c = (double)n / k / (n == 1 ? 0.6 : n == 2 ? 0.85 : 1.0) * (1.0 + (k > 1 ? 40.0 * k / len : 0.0));
+    if (k == 1 || c < cost) {
+      cost = c;
+      best = k;
+    }
+  }
+  part = ceil_div(ceil_div(len, best), 64) * 64;
+  parts = (int)ceil_div(len, part);
+}
+// Parts of the summed axes of the three products in kSmall: no more CTAs than three per SM (Float32 tiles:
 // all run at once) or eight (few instances: the last round costs little), parts of at least 64 or
-// 128 terms, at most 64 parts.
+// 128 terms, at most 64 parts.  Float64 tiles, which the FP64 unit bounds, by even_parts where there is a
+// tile for every second SM.
 struct SmallPlan {
   int64_t few, s_part, x_part, w_part;         // few: by vectors, not tiles; lengths of the parts
   int s_parts, x_parts, w_parts;
@@ -217,6 +238,7 @@ template <typename T> SmallPlan small_plan(int64_t V, int64_t H, int64_t N, int 
   SmallPlan p{};
   p.few = N <= 4 * kFewInstances;
   auto cut = [&](int64_t ctas, int64_t len, int64_t unit, int64_t bytes, int64_t& part, int& parts) {
+    if (sizeof(T) == 8 && unit == 64 && ctas * 2 >= kPlanSMs) return even_parts(ctas, len, bytes, part, parts);
     int64_t k = unit == 64 ? 3 * kPlanSMs / ctas : ceil_div(8 * kPlanSMs, ctas);
     k = k > len / unit ? len / unit : k;
     k = k > 64 ? 64 : k;
@@ -342,23 +364,6 @@ inline MmaPlan mma_plan(int64_t V, int64_t H, int64_t N, int trans, int backward
   return p;
 }
 
-// Tiles for the SMs: the parts of a sum of `len` (at least 64 long, at most 8) that leave the SMs idle least,
-// each SM taking its share of tiles * parts one after the other.
-inline void even_parts(int64_t tiles, int64_t len, int64_t bytes, int64_t& part, int& parts) {
-  int64_t most = (64 << 20) / (bytes + 1), best = 1;
-  most = most > 8 ? 8 : most;
-  most = most > len / 64 ? len / 64 : most;
-  double cost = 0;
-  for (int64_t k = 1; k <= most || k == 1; k++) {
-    const double c = (double)ceil_div(tiles * k, kPlanSMs) / k * (1.0 + 0.01 * k);
-    if (k == 1 || c < cost) {
-      cost = c;
-      best = k;
-    }
-  }
-  part = ceil_div(ceil_div(len, best), 64) * 64;
-  parts = (int)ceil_div(len, part);
-}
 // Float64 with many scores: pieces of equal size with at most 128 MB of dS
 struct PiecePlan {
   int64_t piece, x_part, w_part;

@@ -341,7 +341,17 @@ col_sum_kernel(Matrix<T> m, const T* __restrict__ y, int64_t ldy, int64_t N, int
     // rows warp, warp + 8, ... of the 128, UN at a time, the next batch in flight while one is used
     constexpr int UN = (NB >= 8 ? 4 : 8) / (sizeof(T) / 4), BATCHES = kColRows / (8 * UN);
     Pack<T, VEC> w[2][UN][Q];
+    // all rows and columns inside: no bounds, one address per row
+    const bool full = j0 + 128 <= m.cols && rc + kColRows <= r_hi;
+    const T* from = m.p + (rc + warp) * m.pitch + j0 + lane * VEC;
     auto fetch = [&](Pack<T, VEC> (&to)[UN][Q], int batch) {
+      if (full) {
+#pragma unroll
+        for (int u = 0; u < UN; u++, from += 8 * m.pitch)
+#pragma unroll
+          for (int q = 0; q < Q; q++) to[u][q] = ld_stream<T, VEC>(from + q * 32 * VEC);
+        return;
+      }
 #pragma unroll
       for (int u = 0; u < UN; u++)
 #pragma unroll

@@ -194,9 +194,13 @@ constexpr size_t kBiasRoom = 2 * kPlanSMs * 32;
 //   kMma     Float32 beyond that
 //   kPieces  the rest (Float64 with many scores)
 // Few instances: kSmall reads W once per 8 instances, kMma about four times whatever their number (the
-// scale, the split, the product) and needs five launches.
+// scale, the split, the product) and needs five launches.  50257x1024, forward / with gradients, us, kSmall and kMma:
+// 8 instances 63 and 171 / 249 and 469, 16 instances 110 and 173 / 417 and 470, 24 instances 156 and 173 / 562 and
+// 478, 32 instances 208 and 175 / 729 and 471.
+// Work: FMA tiles and kMma with gradients: 300x256, 400 instances (2^25) 65 and 77 us, 500x512, 512 instances (2^27)
+// 94 and 85 us, 1000x512, 512 instances (2^28) 123 and 91 us.
 enum Form { kSmall, kMma, kPieces };
-constexpr int64_t kFewInstances = 8;
+constexpr int64_t kFewInstances = 16;
 template <typename T> Form form(int64_t V, int64_t H, int64_t N) {
   const bool fits = N * V <= (1 << 24);
   if (fits && N <= kFewInstances) return kSmall;
@@ -231,12 +235,12 @@ inline void even_parts(int64_t tiles, int64_t len, int64_t bytes, int64_t& part,
 struct SmallPlan {
   int64_t few, s_part, x_part, w_part;         // few: by vectors, not tiles; lengths of the parts
   int s_parts, x_parts, w_parts;
-  int64_t chunks;                              // of 2048 classes, where an instance has more than one
+  int64_t chunks;                              // of 2048 classes, where the statistics go by chunks
   size_t scores, parts, stats, bias, total;
 };
 template <typename T> SmallPlan small_plan(int64_t V, int64_t H, int64_t N, int trans, int backward) {
   SmallPlan p{};
-  p.few = N <= 4 * kFewInstances;
+  p.few = N <= 32;
   auto cut = [&](int64_t ctas, int64_t len, int64_t unit, int64_t bytes, int64_t& part, int& parts) {
     if (sizeof(T) == 8 && unit == 64 && ctas * 2 >= kPlanSMs) return even_parts(ctas, len, bytes, part, parts);
     int64_t k = unit == 64 ? 3 * kPlanSMs / ctas : ceil_div(8 * kPlanSMs, ctas);
@@ -262,7 +266,7 @@ template <typename T> SmallPlan small_plan(int64_t V, int64_t H, int64_t N, int 
   at += up((size_t)p.s_parts * N * V * sz);
   p.parts = at;
   p.stats = at;
-  p.chunks = V > kChunk ? ceil_div(V, kChunk) : 0;
+  p.chunks = V > 4 * kChunk ? ceil_div(V, kChunk) : 0;
   if (!backward && p.chunks) at += up((size_t)(2 * p.chunks + 1) * N * sz);
   if (backward) {
     const size_t x = (size_t)p.x_parts * N * H * sz, w = p.w_parts > 1 ? (size_t)p.w_parts * V * H * sz : 0;
@@ -332,7 +336,7 @@ inline MmaPlan mma_plan(int64_t V, int64_t H, int64_t N, int trans, int backward
     }
   }
   if (p.piece >= V) p.s_parts = (int)cut_sum(nt * all, H, N * V * 4);
-  p.chunks = V > kChunk ? ceil_div(V, kChunk) : 0;
+  p.chunks = V > 4 * kChunk ? ceil_div(V, kChunk) : 0;
   const int64_t vp = p.piece < V ? p.piece : V;
   // pitches of whole 128-byte lines: a box of 32 summed indices (64 bytes) then never straddles two sectors
   // (dx of 1000 classes, 8192 x 8192, with a pitch of 1000: 479 us)
@@ -539,12 +543,13 @@ int mma_product_cg(const Planes& a, bool a_mn, const Planes& b, bool b_mn, int64
   return (int)launch_chained_cluster(CG, mma_kernel<CG, Epi>, grid, kMmaThreads, kMmaSmem, st, am, bm, tl, epi);
 }
 
-// Pairs of CTAs need tiles of 256 rows: not where those would leave more than a seventh of the rows empty.
+// Pairs of CTAs are faster by a thirteenth (see linear_nll_mma.cuh) but need tiles of 256 rows: not where those
+// would add more to the rows (forward of 20000x1024: 850 instances in pairs 161 us, alone 150 us).
 template <typename Epi>
 int mma_product(const Planes& a, bool a_mn, const Planes& b, bool b_mn, int64_t I, int64_t J, int64_t C, int splits, const Epi& epi,
                 cudaStream_t st) {
   const int64_t one = ceil_div(I, kTM), two = 2 * ceil_div(I, 2 * kTM);
-  if (6 * two <= 7 * one) return mma_product_cg<2>(a, a_mn, b, b_mn, I, J, C, splits, epi, st);
+  if (13 * two <= 14 * one) return mma_product_cg<2>(a, a_mn, b, b_mn, I, J, C, splits, epi, st);
   return mma_product_cg<1>(a, a_mn, b, b_mn, I, J, C, splits, epi, st);
 }
 
@@ -601,19 +606,24 @@ inline int mma_scores(const Head<float>& h, const MmaPlan& p, const SplitState& 
   return mma_product(s.x, false, s.w, !h.trans, h.N, h.V, h.H, mma_parts(h.H, p.s_parts), epi, st);
 }
 
-// lse and loss from the parts of the scores
+// lse and loss from the parts of the scores: a warp per instance where there are many, or little to do (forward
+// of 1000x16, 4000 instances 30.0 us, with a CTA each 56.7; 500x64, 1000 instances 25.3 and 25.9), a CTA up to
+// 8192 classes (4000x64, 200 instances 24.8 us, in chunks 27.6), beyond that chunks of 2048 classes over all SMs
+// (50257x1024, one instance 40.4 us, by one CTA 60.0).  The chunks of up to 64 instances are joined by the CTA
+// that finishes last (50257x256, one instance 25.3 us, by a launch of its own 27.3; 5000x64, 64 instances 26.4
+// and 27.3).
 template <typename T>
 void statistics(const Head<T>& h, const T* scores, int parts, int64_t chunks, T* stats, T* total, int32_t* count, T* lse,
                 T* per_instance, uint32_t* done, cudaStream_t st) {
   if (chunks) {
     T *pm = stats + h.N, *ps = pm + chunks * h.N;
-    const bool few = h.N <= 16;
+    const bool few = h.N <= 64;
     launch_chained(lnll_chunks_kernel<T>, (unsigned)(chunks * h.N), 256, 0, st, scores, parts, h.bias, h.labels, h.N, h.V, (uint32_t)chunks, pm, ps,
                                                                    stats, lse, per_instance, total, count, few ? done : nullptr);
     if (!few)
       launch_chained(lnll_join_kernel<T>, (unsigned)ceil_div(h.N, 32), 1024, 0, st, pm, ps, stats, h.labels, h.N, h.V, chunks, lse, per_instance, total,
                                                                        count, done);
-  } else if (h.V <= 64 || (h.V <= 512 && h.N >= 2048)) {      // a warp per instance where there are many, or little to do
+  } else if (h.V <= 64 || (h.V <= 2048 && h.N >= 1024)) {
     launch_chained(lnll_rows_kernel<T, 32>, (unsigned)ceil_div(h.N, 8), 256, 0, st, scores, parts, h.bias, h.labels, h.N, h.V, lse, per_instance, total,
                                                                        count, done);
   } else {

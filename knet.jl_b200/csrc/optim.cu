@@ -353,7 +353,7 @@ int run_clip_factors(const knet_tensor_desc* table, int ntensors, int64_t total_
 // Squares are added in Float64 (a square of Float32 is exact there and neither overflows nor
 // vanishes), per chunk and then over the chunks in a fixed order by one CTA.  Bound by HBM: 402.75 M gradients
 // 231 us (6.97 TB/s), Adam with the factor behind it 1657 us (6.80 TB/s); 30 M in 301 arrays 25 us, Momentum 87 us,
-// from the end of the gradients, which the norm has left in L2 (90 us from their beginning).
+// from the end of the gradients, which the norm has left in L2.
 template <typename T>
 __global__ void __launch_bounds__(kOptThreads)
 gnorm_chunks_kernel(const knet_tensor_desc* __restrict__ table, int ntensors, double* __restrict__ partials) {

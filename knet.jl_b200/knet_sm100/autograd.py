@@ -494,7 +494,7 @@ def minimize_step(f, args, algo, parameters=None, gclip_global=0):
     `gclip_global` > 0 first clips the gradients to that norm taken over all of them."""
     from .train import gclip_global_, update_
     tape = diff(f, *args)
-    ps = parameters if parameters is not None else params(tape)
+    ps = list(parameters if parameters is not None else params(tape))        # walked twice
     if gclip_global:
         gclip_global_([_val(p.grad) for p in ps if p.grad is not None], gclip_global)
     for p in ps:

@@ -491,10 +491,22 @@ def _linear_nll_composed(w, x, b, res, trans, average, dy):
 def minimize_step(f, args, algo, parameters=None, gclip_global=0):
     """One iteration of `minimize(f, data, algo)` (src/train20/train.jl:22-36): differentiate
     f(args...), give every parameter a clone of `algo` on first sight, update!, return the loss.
-    `gclip_global` > 0 first clips the gradients to that norm taken over all of them."""
+    `gclip_global` > 0 first clips the gradients to that norm taken over all of them; no optimizer may
+    then clip array by array."""
     from .train import gclip_global_, update_
+
+    def clip_once(algos):
+        if gclip_global and any(getattr(a, "gclip", 0) for a in algos):
+            raise ValueError("clip by array (the optimizer's gclip) or by the global norm, not both")
+
+    if gclip_global and not gclip_global > 0:
+        raise ValueError("gclip_global must be positive")
+    ps = None if parameters is None else list(parameters)                     # walked more than once
+    clip_once([algo] + [p.opt for p in ps or ()])
     tape = diff(f, *args)
-    ps = list(parameters if parameters is not None else params(tape))        # walked twice
+    if ps is None:
+        ps = list(params(tape))
+        clip_once(p.opt for p in ps)
     if gclip_global:
         gclip_global_([_val(p.grad) for p in ps if p.grad is not None], gclip_global)
     for p in ps:

@@ -41,3 +41,31 @@ def test_parameters_may_be_a_generator(step):
     ps = params(autograd)
     assert autograd.minimize_step(None, (), train.SGD(lr=0.25), (p for p in ps), gclip_global=2.0) == 1.5
     assert calls == ["diff", ("clip", ["g0", "g2"], 2.0), ("update", "w0", "g0", 0.25), ("update", "w2", "g2", 0.25)]
+
+
+def test_clipping_by_array_and_by_the_global_norm_is_refused(step):
+    """As update_multi_ and MLP refuse it; nothing has been clipped or updated then, and what can be seen
+    before the function is differentiated is seen before."""
+    autograd, train, calls = step
+    ps = params(autograd)
+    with pytest.raises(ValueError, match="not both"):
+        autograd.minimize_step(None, (), train.SGD(gclip=1.0), ps, gclip_global=2.0)
+    ps[2].opt = train.Adam(gclip=0.5)
+    with pytest.raises(ValueError, match="not both"):
+        autograd.minimize_step(None, (), train.SGD(), iter(ps), gclip_global=2.0)
+    for bad in (-1.0, float("nan")):
+        with pytest.raises(ValueError, match="positive"):
+            autograd.minimize_step(None, (), train.SGD(), ps, gclip_global=bad)
+    assert calls == []
+    autograd.minimize_step(None, (), train.SGD(gclip=1.0), ps)                 # by array alone: as ever
+    assert [c[0] for c in calls[1:]] == ["update", "update"]
+
+
+def test_a_parameter_met_on_the_tape_with_its_own_clipping_is_refused(step, monkeypatch):
+    autograd, train, calls = step
+    ps = params(autograd)
+    ps[0].opt = train.SGD(gclip=1.0)
+    monkeypatch.setattr(autograd, "params", lambda tape: ps)
+    with pytest.raises(ValueError, match="not both"):
+        autograd.minimize_step(None, (), train.SGD(), gclip_global=2.0)
+    assert calls == ["diff"]

@@ -182,17 +182,31 @@ class MultiTensorPlan:
         first = arrays[0][0].data if isinstance(arrays[0][0], KnetArray) else arrays[0][0]
         self.table = torch.frombuffer(bytearray(raw), dtype=torch.uint8).to(first.device)      # beside its arrays
         self._keep = arrays
-        held = [(host[i].p[1], host[i].n) for i in range(n) if host[i].p[1] and host[i].n]
-        self.repeated = len(set(held)) < len(held)
+        held = sorted((host[i].p[1], host[i].n) for i in range(n) if host[i].p[1] and host[i].n)
+        size = first.element_size()
+        self.repeated = any(p + k * size > q for (p, k), (q, _) in zip(held, held[1:]))      # some gradients share memory
         self.clip_partials = self.clip_factors = None      # scratch of the fused gradient clipping
 
 
+def _disjoint(arrays):
+    """1-D views that hold every element of `arrays` once, whatever the arrays share."""
+    views, end = [], 0
+    for a in sorted((a.view(-1) for a in arrays if a.numel()), key=lambda a: (a.data_ptr(), -a.numel())):
+        size, done = a.element_size(), max(end - a.data_ptr(), 0)
+        if done % size:
+            raise ValueError("gradients overlap by part of an element")
+        if done < a.numel() * size:
+            views.append(a[done // size:])
+            end = a.data_ptr() + a.numel() * size
+    return views
+
+
 def _one_plan(grads):
-    """(plan over all gradients, plan over each buffer once).  A plan is taken as it is and must not
-    hold a gradient twice; a list may (two parameters whose gradient is one array)."""
+    """(plan over all gradients, plan over each element once).  A plan is taken as it is and its gradients
+    must not share memory; those of a list may (two parameters whose gradient is one array, or part of it)."""
     if isinstance(grads, MultiTensorPlan):
         if grads.repeated:
-            raise ValueError("the plan holds a gradient array twice")
+            raise ValueError("gradients of the plan share memory")
         return grads, grads
     arrays = [g.data if isinstance(g, KnetArray) else g for g in grads]
     if not arrays:
@@ -203,9 +217,8 @@ def _one_plan(grads):
             raise TypeError("gradients must be contiguous GPU arrays")
         if a.dtype != arrays[0].dtype or a.device != arrays[0].device:
             raise TypeError("gradients of one norm must share an element type and a device")
-    once = list({(a.data_ptr(), a.numel()): a for a in arrays}.values())
     plan = MultiTensorPlan([(a, a) for a in arrays])
-    return plan, plan if len(once) == len(arrays) else MultiTensorPlan([(a, a) for a in once])
+    return plan, MultiTensorPlan([(a, a) for a in _disjoint(arrays)]) if plan.repeated else plan
 
 
 def _global_norm(plan, gclip, gscale):
@@ -237,7 +250,8 @@ def gclip_global_(grads, gclip, gscale=1.0):
     """Clip by the norm of all gradients: multiply every one in place by gclip / norm when
     norm = gnorm(grads, gscale) exceeds gclip (gclip! does so array by array,
     src/train20/update.jl:572-583).  Returns the norm before clipping, on the device; nothing
-    waits for it.  A norm that is NaN leaves the gradients as they are."""
+    waits for it.  A norm that is NaN leaves the gradients as they are.  What arrays of a list share
+    counts in the norm of each and is multiplied once; a plan whose gradients share memory is refused."""
     if not gclip > 0:
         raise ValueError("gclip must be positive")
     plan, once = _one_plan(grads)

@@ -69,3 +69,40 @@ def test_a_parameter_met_on_the_tape_with_its_own_clipping_is_refused(step, monk
     with pytest.raises(ValueError, match="not both"):
         autograd.minimize_step(None, (), train.SGD(), gclip_global=2.0)
     assert calls == ["diff"]
+
+
+def cover(views):
+    """how often each element of the buffer behind `views` is scaled"""
+    import torch
+    from knet_sm100 import train
+    buf = torch.zeros(40)
+    for v in train._disjoint([buf[a:b] for a, b in views]):
+        v += 1
+    return buf
+
+
+@pytest.mark.parametrize("views", [[(0, 10), (5, 15)], [(5, 15), (0, 10), (0, 10)], [(0, 30), (3, 9), (8, 31)], [(0, 10), (10, 20)],
+                                   [(7, 7), (3, 9), (3, 5), (4, 12), (30, 40)]], ids=str)
+def test_overlapping_gradients_are_scaled_once(views):
+    """Views of one buffer that share some of their elements: each of those is multiplied once, by one CTA."""
+    want = [float(any(a <= i < b for a, b in views)) for i in range(40)]
+    assert cover(views).tolist() == want
+
+
+def test_arrays_that_share_part_of_an_element_are_refused():
+    import torch
+    from knet_sm100 import train
+    raw = torch.zeros(64, dtype=torch.uint8)
+    with pytest.raises(ValueError, match="overlap"):
+        train._disjoint([raw[0:32].view(torch.float32), raw[18:50].view(torch.int16)[1:9]])
+
+
+@pytest.mark.parametrize("views,shared", [([(0, 10), (5, 15)], True), ([(5, 15), (0, 30), (38, 39)], True), ([(0, 10), (10, 20)], False),
+                                          ([(0, 10), (0, 10)], True), ([(0, 10), (4, 4)], False)], ids=str)
+def test_a_plan_knows_whether_its_gradients_overlap(views, shared):
+    """In a plan, whose table is used as it is, overlapping gradients cannot be clipped in place."""
+    import torch
+    from knet_sm100 import train
+    buf = torch.zeros(40)
+    plan = train.MultiTensorPlan([(torch.zeros(b - a), buf[a:b]) for a, b in views])
+    assert plan.repeated == shared

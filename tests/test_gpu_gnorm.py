@@ -228,3 +228,18 @@ def test_refusals(K):
     with pytest.raises(TypeError):
         K.gnorm([torch.ones(4, 4, device="cuda").t()[1:]])
     assert float(K.gnorm([])) == 0.0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+def test_overlapping_views_are_scaled_once(K, dtype):
+    """Views that share part of their elements: each listed array counts in the norm, each element is
+    multiplied once."""
+    host, buf, (g,) = flat_set([50_000], dtype, 3)
+    views = [g[20_000:], g[:30_000], K.KnetArray(g[100:200])]
+    want = exact_norm([host[0][20_000:], host[0][:30_000], host[0][100:200]], 1.0)
+    norm = K.gclip_global_(views, want / 8)
+    assert near(norm, want, [host[0], host[0]])
+    factor = (want / 8) / float(norm)
+    np.testing.assert_array_equal(g.cpu().numpy(), (factor * host[0].astype(np.float64)).astype(NPDT[dtype]))
+    with pytest.raises(ValueError):
+        K.gclip_global_(K.MultiTensorPlan([(v, v) for v in (g[20_000:], g[:30_000])]), 1.0)

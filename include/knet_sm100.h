@@ -525,7 +525,9 @@ KNET_BOTH_TYPES(KNET_DECL_MULTI, multi)
  * gnorm:        *norm = |gscale| * sqrt(sum over all tensors of g^2), in Float64.
  * gclip_global: the same norm, and *factor = gclip / norm when norm > gclip, else 1 (also for a
  *               NaN norm); gclip > 0.  Both take two launches and add in a fixed order;
- *               `partials` is scratch of total_chunks doubles.
+ *               `partials` is scratch of total_chunks doubles.  Finite Float64 gradients whose
+ *               squares leave the type's range count too; where the norm itself does, *norm is
+ *               inf and *factor still what brings the gradients to gclip.
  * gclip_apply:  g = lmul!(*factor, g) on every tensor; a factor of 1 touches nothing.
  * _gc updates:  as the multi-tensor updates above with g replaced on load by lmul!(*factor, g);
  *               adam_multi_gcg also reads its bias corrections from device memory (see

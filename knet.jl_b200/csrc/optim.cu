@@ -354,6 +354,12 @@ int run_clip_factors(const knet_tensor_desc* table, int ntensors, int64_t total_
 // vanishes), per chunk and then over the chunks in a fixed order by one CTA.  Bound by HBM: 402.75 M gradients
 // 231 us (6.97 TB/s), Adam with the factor behind it 1657 us (6.80 TB/s); 30 M in 301 arrays 25 us, Momentum 87 us,
 // from the end of the gradients, which the norm has left in L2.
+//
+// Squares of Float64 may do both.  A chunk whose sum leaves [2^-900, 2^960] is read again, times 2^-600 or 2^600
+// (its largest entry is then above 2^473 or below 2^-450, so what the scale takes below the range is nothing
+// beside it), and leaves minus its norm times 2^-20 or 2^20: the sign tells the finishing kernel, the factor keeps
+// a norm of 8192 of the type's largest or smallest numbers inside the range.
+constexpr double kSumLow = 0x1p-900, kSumHigh = 0x1p960;
 template <typename T>
 __global__ void __launch_bounds__(kOptThreads)
 gnorm_chunks_kernel(const knet_tensor_desc* __restrict__ table, int ntensors, double* __restrict__ partials) {
@@ -367,6 +373,16 @@ gnorm_chunks_kernel(const knet_tensor_desc* __restrict__ table, int ntensors, do
   double acc = 0.0;
   segment_visit<T>(g, cnt, threadIdx.x, kOptThreads, [&](T v, uint32_t) { acc = ::fma((double)v, (double)v, acc); });
   acc = block_reduce(acc, [](double a, double b) { return a + b; }, 0.0, red);
+  if constexpr (sizeof(T) == 8) {
+    if (!(acc >= kSumLow && acc <= kSumHigh)) {      // the same in every thread; NaN too
+      const bool low = acc < kSumLow;
+      const double s = low ? 0x1p600 : 0x1p-600;
+      acc = 0.0;
+      segment_visit<T>(g, cnt, threadIdx.x, kOptThreads, [&](T v, uint32_t) { acc = ::fma(v * s, v * s, acc); });
+      acc = block_reduce(acc, [](double a, double b) { return a + b; }, 0.0, red);
+      if (acc > 0 && acc < CUDART_INF) acc = -::sqrt(acc) * (low ? 0x1p-580 : 0x1p580);      // 0, inf and NaN as they are
+    }
+  }
   if (threadIdx.x == 0) partials[blockIdx.x] = acc;
 }
 
@@ -376,12 +392,30 @@ gnorm_finish_kernel(const double* __restrict__ partials, int64_t total_chunks, d
   chain_begin();
   __shared__ double red[32];
   double acc = 0.0;
-  for (int64_t c = threadIdx.x; c < total_chunks; c += 1024) acc += partials[c];
+  bool some = false, large = false, small = false;
+  for (int64_t c = threadIdx.x; c < total_chunks; c += 1024) {
+    const double p = partials[c];
+    if (p < 0) (p < -1.0 ? large : small) = true;
+    else {
+      some |= p != 0;
+      acc += p;
+    }
+  }
+  double s = 1.0;                                    // the squares of s * g are what is added
+  if (__syncthreads_or(large)) s = 0x1p-600;
+  else if (__syncthreads_or(small) && !__syncthreads_or(some)) s = 0x1p600;
+  if (__syncthreads_or(large || small)) {
+    acc = acc * s * s;
+    for (int64_t c = threadIdx.x; c < total_chunks; c += 1024) {
+      const double p = partials[c], v = p * (p < -1.0 ? 0x1p20 * s : 0x1p-20 * s);
+      if (p < 0) acc = ::fma(v, v, acc);
+    }
+  }
   acc = block_reduce(acc, [](double a, double b) { return a + b; }, 0.0, red);
   if (threadIdx.x == 0) {
-    const double nrm = ::sqrt(acc) * fabs(gscale);
+    const double scaled = ::sqrt(acc) * fabs(gscale), nrm = scaled / s;
     if (norm) *norm = nrm;
-    if (factor) *factor = nrm > gclip ? gclip / nrm : 1.0;
+    if (factor) *factor = nrm > gclip ? gclip * s / scaled : 1.0;      // also where the norm itself is beyond the type
   }
 }
 

@@ -243,3 +243,37 @@ def test_overlapping_views_are_scaled_once(K, dtype):
     np.testing.assert_array_equal(g.cpu().numpy(), (factor * host[0].astype(np.float64)).astype(NPDT[dtype]))
     with pytest.raises(ValueError):
         K.gclip_global_(K.MultiTensorPlan([(v, v) for v in (g[20_000:], g[:30_000])]), 1.0)
+
+
+@pytest.mark.parametrize("off", [0, 1])
+@pytest.mark.parametrize("stds", [(1e200, 1e200), (1e-200, 1e-200), (1e-309, 1e-309), (1e200, 1.0), (1.0, 1e-200), (1e-200, 1e-165),
+                                  (1e-200, 1e-136), (1e152, 1e150), (1e200, 1e-200), (1e-200, 0.0)], ids=str)
+def test_float64_squares_beyond_the_range(K, stds, off):
+    """Finite gradients whose squares overflow or vanish in Float64, alone and beside ordinary arrays.  The root
+    per chunk and its square add two roundings to each term, within the bound's 16."""
+    sizes = [20_000, 9_000, 3]
+    host, _, g = flat_set(sizes, torch.float64, off, std=1.0)
+    for a, h, s in zip(g, host, stds + stds[:1]):
+        h *= s
+        a.copy_(torch.from_numpy(h).cuda())
+    want = np.sqrt(sum((h.astype(np.longdouble) ** 2).sum() for h in host))       # 15 bits of exponent
+    assert abs(float(K.gnorm(g)) - want) <= (sum(sizes) + 16) * 2.0 ** -53 * want
+    norm = float(K.gclip_global_(g, float(want / 4)))
+    for a, h in zip(g, host):
+        np.testing.assert_array_equal(a.cpu().numpy(), (float(want / 4) / norm) * h)
+
+
+def test_a_norm_beyond_float64(K):
+    """Entries near the type's largest: their norm is inf, the clipped gradients have the norm asked for."""
+    n = 30_000
+    g = [torch.full((n,), 1.5e308, dtype=torch.float64, device="cuda"), torch.full((100,), -1.0, dtype=torch.float64, device="cuda")]
+    assert float(K.gnorm(g)) == np.inf and abs(float(K.gnorm(g, 2.0 ** -20)) / (1.5e308 * 2.0 ** -20 * n ** 0.5) - 1) < 1e-11
+    assert float(K.gclip_global_(g, 3.0)) == np.inf
+    # a factor of about 2^-1031 has 43 bits left
+    assert bool(((g[0] * n ** 0.5 / 3.0 - 1).abs() < 2.0 ** -41).all()) and bool((g[1].abs() < 1e-300).all())
+    zero = [torch.zeros(20_000, dtype=torch.float64, device="cuda")]
+    assert float(K.gclip_global_(zero, 1.0)) == 0 and not zero[0].any()
+    zero[0][7] = float("inf")
+    assert float(K.gnorm(zero)) == np.inf
+    zero[0][8] = float("nan")
+    assert np.isnan(float(K.gnorm(zero)))

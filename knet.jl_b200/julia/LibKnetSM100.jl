@@ -244,14 +244,25 @@ end
 Base.close(c::DpComm) = (check(ccall((:knet_dp_destroy, libknet8), Cint, (Ptr{Cvoid},), c.handle), :knet_dp_destroy); nothing)
 
 # ---- nll of a linear layer without its score matrix, clipping by the norm of all gradients --------------
+# (V, H, N) of scores = W*x .+ b; the library reads as far as these say, so every array is held against them
+function head_sizes(w, x, labels, b, trans)
+    ndims(w) == 2 || throw(DimensionMismatch("w must be a matrix"))
+    V, H = trans ? (size(w, 2), size(w, 1)) : size(w)
+    H > 0 && size(x, 1) == H || throw(DimensionMismatch("x has $(size(x, 1)) features, w $H"))
+    N = div(length(x), H)
+    length(labels) == N || throw(DimensionMismatch("one label per instance is needed"))
+    b === nothing || length(b) == V || throw(DimensionMismatch("b has $(length(b)) entries for $V classes"))
+    (V, H, N)
+end
+
 for (T, S) in ((Float32, "32"), (Float64, "64"))
     wsf, fwd, bwd = Symbol("knet_linear_nll_workspace_", S), Symbol("knet_linear_nll_fwd_", S), Symbol("knet_linear_nll_bwd_", S)
     gcl, app = Symbol("knet_gclip_global_", S), Symbol("knet_gclip_apply_", S)
     @eval begin
         # nll(W*x .+ b, labels), W (V,H) or, with trans, (H,V); b may be nothing.  Returns total, count
         # and the lse pair that the backward call needs; nothing waits for the device.
-        function linear_nll(w::DevArray{$T}, x::DevArray{$T}, labels::CuArray{Int32}; b=nothing, trans=false)
-            H = size(x, 1); N = div(length(x), H); V = div(length(w), H)
+        function linear_nll(w::DevArray{$T}, x::DevArray{$T}, labels::CuArray{Int32}; b::Union{Nothing,DevArray{$T}}=nothing, trans=false)
+            V, H, N = head_sizes(w, x, labels, b, trans)
             ws = CuArray{UInt8}(undef, ccall(($(QuoteNode(wsf)), libknet8), Csize_t, (Int64, Int64, Int64, Cint), V, H, N, 0))
             total = CuArray{$T}(undef, 1); count = CuArray{Int32}(undef, 1)
             lse = CuArray{$T}(undef, 2N + 2); per = CuArray{$T}(undef, N)
@@ -262,9 +273,10 @@ for (T, S) in ((Float32, "32"), (Float64, "64"))
                         CUDA.stream()), $(QuoteNode(fwd)))
             (total, count, lse)
         end
-        function linear_nll_back(w::DevArray{$T}, x::DevArray{$T}, labels::CuArray{Int32}, lse, count, dy; b=nothing, trans=false,
-                                 average=true)
-            H = size(x, 1); N = div(length(x), H); V = div(length(w), H)
+        function linear_nll_back(w::DevArray{$T}, x::DevArray{$T}, labels::CuArray{Int32}, lse::CuArray{$T}, count::CuArray{Int32}, dy;
+                                 b::Union{Nothing,DevArray{$T}}=nothing, trans=false, average=true)
+            V, H, N = head_sizes(w, x, labels, b, trans)
+            length(lse) == 2N + 2 && length(count) == 1 || throw(DimensionMismatch("the forward result belongs to other arrays"))
             ws = CuArray{UInt8}(undef, ccall(($(QuoteNode(wsf)), libknet8), Csize_t, (Int64, Int64, Int64, Cint), V, H, N, 1))
             dw = similar(w); dx = similar(x); db = b === nothing ? nothing : similar(b)
             check(ccall(($(QuoteNode(bwd)), libknet8), Cint,

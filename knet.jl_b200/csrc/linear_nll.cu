@@ -269,7 +269,7 @@ template <typename T> SmallPlan small_plan(int64_t V, int64_t H, int64_t N, int 
   p.chunks = V > 4 * kChunk ? ceil_div(V, kChunk) : 0;
   if (!backward && p.chunks) at += up((size_t)(2 * p.chunks + 1) * N * sz);
   if (backward) {
-    const size_t x = (size_t)p.x_parts * N * H * sz, w = p.w_parts > 1 ? (size_t)p.w_parts * V * H * sz : 0;
+    const size_t x = p.few || p.x_parts > 1 ? (size_t)p.x_parts * N * H * sz : 0, w = p.w_parts > 1 ? (size_t)p.w_parts * V * H * sz : 0;
     at += up(x > w ? x : w);
     p.bias = at;
     at += up(kBiasRoom * sz);

@@ -64,3 +64,10 @@ def test_global_norm_arguments(lib):
         assert getattr(lib, f"knet_sgd_multi_gc_{S}")(P, 1, 1, 0.1, 1.0, None, None) == -1
         assert getattr(lib, f"knet_adam_multi_gc_{S}")(P, 1, 1, 0.1, 0.9, 0.99, 1e-8, 0, 1.0, P, None) == -1
         assert getattr(lib, f"knet_adam_multi_gcg_{S}")(P, 1, 1, 0.1, 0.9, 0.99, 1e-8, None, 1.0, P, None) == -1
+
+
+def test_workspace_holds_no_room_that_nothing_uses(lib):
+    """Few classes, many instances: dx is written where it belongs, not by way of the workspace."""
+    scores = 10 * 100_000
+    assert lib.knet_linear_nll_workspace_64(10, 4096, 100_000, 1) < 2 * 8 * scores + (64 << 20) + (1 << 20)
+    assert lib.knet_linear_nll_workspace_32(10, 64, 100_000, 1) < 4 * scores + (1 << 20)

@@ -84,9 +84,9 @@ template <typename T> struct GradScoresEpi {
 // sums relative to it, added in Float64 (8 warps took 25 us for 197 tiles of 4096 instances).
 template <typename T>
 __global__ void __launch_bounds__(1024)
-lnll_join_kernel(const T* __restrict__ part_m, const T* __restrict__ part_s, const T* __restrict__ label_score,
-                 const int32_t* __restrict__ labels, int64_t N, int64_t V, int64_t tiles, T* __restrict__ lse,
-                 T* __restrict__ per_instance, T* __restrict__ total, int32_t* __restrict__ count, uint32_t* __restrict__ done) {
+lnll_join_kernel(const T* part_m, const T* part_s, const T* label_score,
+                 const int32_t* labels, int64_t N, int64_t V, int64_t tiles, T* lse,
+                 T* per_instance, T* total, int32_t* count, uint32_t* done) {
   chain_begin();
   __shared__ T sm[32][32];
   __shared__ double ss[32][32];
@@ -131,7 +131,7 @@ template <typename T> __global__ void lnll_none_kernel(T* total, int32_t* count)
 // parts of `rows` instances, the plain sums of each go to parts[part][j].
 template <typename T>
 __global__ void __launch_bounds__(1024)
-lnll_bias_kernel(const T* __restrict__ ds, int64_t ld, int64_t N, int64_t J, int64_t rows, T* __restrict__ out, GradScale<T> g) {
+lnll_bias_kernel(const T* ds, int64_t ld, int64_t N, int64_t J, int64_t rows, T* out, GradScale<T> g) {
   chain_begin();
   __shared__ T part[32][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;

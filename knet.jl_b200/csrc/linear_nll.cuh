@@ -38,7 +38,7 @@ template <typename T> struct GradScale {
   T dy;
   __device__ __forceinline__ T value() const {
     if (!count) return dy;
-    const int32_t c = __ldg(count);
+    const int32_t c = *count;
     return c > 0 ? dy / (T)c : (T)0;
   }
 };
@@ -68,13 +68,13 @@ __device__ __forceinline__ void load_scores(T (&t)[K], const T* x, int64_t v, in
   if (bias) {
 #pragma unroll
     for (int k = 0; k < K; k++)
-      if (v + k * STEP < V) t[k] += __ldg(bias + v + k * STEP);
+      if (v + k * STEP < V) t[k] += bias[v + k * STEP];
   }
 }
 
 // total and count over the instances in a fixed order, by one CTA
 template <typename T, int THREADS>
-__device__ __forceinline__ void add_losses(const T* per_instance, const int32_t* __restrict__ labels, int64_t N, T* total, int32_t* count) {
+__device__ __forceinline__ void add_losses(const T* per_instance, const int32_t* labels, int64_t N, T* total, int32_t* count) {
   __shared__ double sd[32];
   __shared__ int sc[32];
   double a = 0.0;
@@ -85,7 +85,7 @@ __device__ __forceinline__ void add_losses(const T* per_instance, const int32_t*
 #pragma unroll
     for (int k = 0; k < 8; k++) {
       const int64_t n = n0 + (int64_t)k * THREADS;
-      l[k] = n < N ? __ldg(labels + n) : 0;
+      l[k] = n < N ? labels[n] : 0;
       v[k] = n < N ? __ldcg(per_instance + n) : (T)0;
     }
 #pragma unroll
@@ -104,7 +104,7 @@ __device__ __forceinline__ void add_losses(const T* per_instance, const int32_t*
 }
 // the same by the last CTA of the grid to get here; `done` counts them
 template <typename T, int THREADS>
-__device__ __forceinline__ void last_adds_losses(const T* per_instance, const int32_t* __restrict__ labels, int64_t N, T* total,
+__device__ __forceinline__ void last_adds_losses(const T* per_instance, const int32_t* labels, int64_t N, T* total,
                                                  int32_t* count, uint32_t* done) {
   __shared__ uint32_t last;
   __threadfence();

@@ -357,7 +357,7 @@ template <int LANES> __device__ __forceinline__ uint32_t run_absmax(const float*
   float4 v[8];
 #pragma unroll
   for (int u = 0; u < 8; u++)
-    if (t + u * LANES < nv) v[u] = __ldg(q + t + u * LANES);
+    if (t + u * LANES < nv) v[u] = q[t + u * LANES];
 #pragma unroll
   for (int u = 0; u < 8; u++)
     if (t + u * LANES < nv) { take(v[u].x); take(v[u].y); take(v[u].z); take(v[u].w); }
@@ -366,8 +366,8 @@ template <int LANES> __device__ __forceinline__ uint32_t run_absmax(const float*
   return m;
 }
 __global__ void __launch_bounds__(256)
-lnll_absmax_kernel(const float* __restrict__ w, int64_t n, const float* __restrict__ x, const int32_t* __restrict__ labels, int64_t N,
-                   int64_t H, uint32_t* __restrict__ part) {
+lnll_absmax_kernel(const float* w, int64_t n, const float* x, const int32_t* labels, int64_t N,
+                   int64_t H, uint32_t* part) {
   chain_begin();
   __shared__ uint32_t red[32];
   auto larger = [](uint32_t a, uint32_t b) { return max(a, b); };
@@ -378,7 +378,7 @@ lnll_absmax_kernel(const float* __restrict__ w, int64_t n, const float* __restri
   const int64_t runs = (H + kWarpRun - 1) / kWarpRun;
   for (int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); t < N * runs; t += (int64_t)gridDim.x * 8) {
     const int64_t i = t / runs, c = (t - i * runs) * kWarpRun;
-    const bool used = __ldg(labels + i) != 0;          // does not hold up the loads
+    const bool used = labels[i] != 0;          // does not hold up the loads
     const uint32_t v = run_absmax<32>(x + i * H + c, (int)min((int64_t)kWarpRun, H - c), threadIdx.x & 31);
     mx = used ? max(mx, v) : mx;
   }
@@ -408,14 +408,14 @@ __device__ __forceinline__ void load8(const float* row, int64_t c, int64_t cols,
   const int off = (int)(((uintptr_t)row >> 2) & 3);
   if (c - off >= 0 && c - off + (off ? 12 : 8) <= cols) {
     const float4* q = reinterpret_cast<const float4*>(row + c - off);
-    const float4 a = __ldg(q), b = __ldg(q + 1);
-    const float4 d = off ? __ldg(q + 2) : b;
+    const float4 a = q[0], b = q[1];
+    const float4 d = off ? q[2] : b;
     const float t[12] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, d.x, d.y, d.z, d.w};
 #pragma unroll
     for (int k = 0; k < 8; k++) v[k] = off == 0 ? t[k] : off == 1 ? t[k + 1] : off == 2 ? t[k + 2] : t[k + 3];
   } else {
 #pragma unroll
-    for (int k = 0; k < 8; k++) v[k] = c + k < cols ? __ldg(row + c + k) : 0.0f;
+    for (int k = 0; k < 8; k++) v[k] = c + k < cols ? row[c + k] : 0.0f;
   }
 }
 
@@ -424,8 +424,8 @@ __device__ __forceinline__ void load8(const float* row, int64_t c, int64_t cols,
 // backward, from what the forward left (`given`).  In a skipped instance (label 0), which the scale does not
 // regard, whatever has no fp16 value becomes 0: its dS is 0, which times infinity would be NaN in dW.
 __global__ void __launch_bounds__(256)
-lnll_split_kernel(SplitJob a, SplitJob b, uint32_t blocks_a, const uint32_t* __restrict__ part, uint32_t parts,
-                  const float* __restrict__ given, float* __restrict__ saved, int* __restrict__ exps) {
+lnll_split_kernel(SplitJob a, SplitJob b, uint32_t blocks_a, const uint32_t* part, uint32_t parts,
+                  const float* given, float* saved, int* exps) {
   chain_begin();
   __shared__ uint32_t red[32];
   const bool second = blockIdx.x >= blocks_a;
@@ -451,7 +451,7 @@ lnll_split_kernel(SplitJob a, SplitJob b, uint32_t blocks_a, const uint32_t* __r
   for (int64_t g = total - 1 - ((int64_t)(blockIdx.x - first) * 256 + threadIdx.x); g >= 0; g -= (int64_t)nb * 256) {
     const int64_t r = g / groups, c = (g - r * groups) * 8;
     float v[8];
-    const bool skipped = j.labels && __ldg(j.labels + r) == 0;
+    const bool skipped = j.labels && j.labels[r] == 0;
     load8(j.src + r * j.pitch, c, j.cols, v);
 #pragma unroll
     for (int k = 0; k < 8; k++) {
@@ -482,7 +482,7 @@ __device__ __forceinline__ float exp2_approx(float t) {
 // the bias of the tile's classes into shared memory, 0 without one and past the last class
 __device__ __forceinline__ void stage_bias(const float* bias, int64_t j0, int64_t J, float* to) {
   const int col = threadIdx.x;
-  if (col < kTN) to[col] = bias && j0 + col < J ? __ldg(bias + j0 + col) : 0.0f;
+  if (col < kTN) to[col] = bias && j0 + col < J ? bias[j0 + col] : 0.0f;
 }
 
 // i = instance, j = class: maximum and sum of exponentials of the tile's 256 classes per instance
@@ -627,8 +627,8 @@ struct MmaGradScores {
   __device__ __forceinline__ void operator()(float2 (&acc)[32], const TileAt& at) const {
     const Unscale us = unscale(exps[0] + exps[1], at.gain);
     const bool live = at.i < N;
-    const int32_t label = live ? __ldg(labels + at.i) : 0;    // rows past the last instance act as skipped
-    const float hi = live ? __ldg(lse + at.i) : 0.0f, lo = live ? __ldg(lse + N + at.i) : 0.0f;
+    const int32_t label = live ? labels[at.i] : 0;    // rows past the last instance act as skipped
+    const float hi = live ? lse[at.i] : 0.0f, lo = live ? lse[N + at.i] : 0.0f;
     const float2 ua = both(us.a), ub = both(us.b), nhi = both(-hi), nlo = both(-lo), l2e = both(kLog2e), scale = both((float)(1 << kGradExp));
     const int64_t hit64 = (int64_t)label - 1 - v0 - at.j0;
     const int hit = hit64 >= 0 && hit64 < 64 ? (int)hit64 : -1;
@@ -767,9 +767,9 @@ struct MmaStore {
 // dS in two fp16 planes from the parts of the scores, with its sums over groups of 8 instances
 constexpr int kGradRows = 8;
 __global__ void __launch_bounds__(256)
-lnll_grad_planes_kernel(const float* __restrict__ scores, int parts, const float* __restrict__ bias, const int32_t* __restrict__ labels,
-                        const float* __restrict__ lse, int64_t N, int64_t V, __half* __restrict__ ds, int64_t ld, int64_t plane,
-                        float* __restrict__ db_part) {
+lnll_grad_planes_kernel(const float* scores, int parts, const float* bias, const int32_t* labels,
+                        const float* lse, int64_t N, int64_t V, __half* ds, int64_t ld, int64_t plane,
+                        float* db_part) {
   chain_begin();
   const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x, n0 = (int64_t)blockIdx.y * kGradRows;
   if (v >= ld) return;

@@ -59,7 +59,7 @@ template <typename T, bool MASK> struct TileCopy {
   }
   __device__ __forceinline__ void look(int k, int64_t left) {
 #pragma unroll
-    for (int r = 0; r < PER; r++) used[r] = !labels || (c[r] < left && __ldg(labels + (int64_t)k * S + c[r]) != 0);
+    for (int r = 0; r < PER; r++) used[r] = !labels || (c[r] < left && labels[(int64_t)k * S + c[r]] != 0);
   }
   // step k into `stage`; `left` summed indices remain from its first on
   __device__ __forceinline__ void start(T* stage, int k, int64_t left) {
@@ -220,7 +220,7 @@ template <typename T, int VEC> __device__ __forceinline__ Pack<T, VEC> ld_cached
 // one vector 33 us (6.2 TB/s), eight 54 us, where the vectors' loads and 8 FMAs per element show.
 template <typename T, int NB, int VEC>
 __global__ void __launch_bounds__(256, 2)
-row_dot_kernel(Matrix<T> m, const T* __restrict__ y, int64_t ldy, int64_t N, int64_t c_part, uint32_t* done, T* __restrict__ parts) {
+row_dot_kernel(Matrix<T> m, const T* y, int64_t ldy, int64_t N, int64_t c_part, uint32_t* done, T* parts) {
   chain_begin();
   clear_done(done);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -314,7 +314,7 @@ __device__ __forceinline__ void join_warps(T (&acc)[NB][4], T (*red)[NB][128]) {
 constexpr int kColRows = 128;
 template <typename T, int NB, int VEC>
 __global__ void __launch_bounds__(256, 2)
-col_sum_kernel(Matrix<T> m, const T* __restrict__ y, int64_t ldy, int64_t N, int64_t r_part, uint32_t* done, T* __restrict__ parts) {
+col_sum_kernel(Matrix<T> m, const T* y, int64_t ldy, int64_t N, int64_t r_part, uint32_t* done, T* parts) {
   chain_begin();
   clear_done(done);
   constexpr int Q = 4 / VEC;                       // packs per thread: 4 columns
@@ -406,8 +406,8 @@ col_sum_kernel(Matrix<T> m, const T* __restrict__ y, int64_t ldy, int64_t N, int
 // Skipped instances (label 0) are passed over: 0 times what a padded batch holds there may be NaN.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
-outer_kernel(const T* __restrict__ a, int64_t lda, const T* __restrict__ b, int64_t ldb, const int32_t* __restrict__ labels, int64_t N,
-             int64_t R, int64_t C, T* __restrict__ out, int64_t ld, GradScale<T> g) {
+outer_kernel(const T* a, int64_t lda, const T* b, int64_t ldb, const int32_t* labels, int64_t N,
+             int64_t R, int64_t C, T* out, int64_t ld, GradScale<T> g) {
   chain_begin();
   constexpr int Q = 4 / VEC, NB = 8;
   __shared__ __align__(16) T as[NB][64];
@@ -428,7 +428,7 @@ outer_kernel(const T* __restrict__ a, int64_t lda, const T* __restrict__ b, int6
 #pragma unroll
     for (int n = 0; n < NB; n++) {
       if (n0 + n >= N) break;
-      if (__ldg(labels + n0 + n) == 0) continue;
+      if (labels[n0 + n] == 0) continue;
       T av[8];
 #pragma unroll
       for (int r = 0; r < 8; r++) av[r] = as[n][warp * 8 + r];
@@ -469,9 +469,9 @@ outer_kernel(const T* __restrict__ a, int64_t lda, const T* __restrict__ b, int6
 // that ran before set it to 0).
 template <typename T, int GROUP>
 __global__ void __launch_bounds__(GROUP < 256 ? 256 : GROUP)
-lnll_rows_kernel(const T* __restrict__ scores, int parts, const T* __restrict__ bias, const int32_t* __restrict__ labels, int64_t N,
-                 int64_t V, T* __restrict__ lse, T* __restrict__ per_instance, T* __restrict__ total, int32_t* __restrict__ count,
-                 uint32_t* __restrict__ done) {
+lnll_rows_kernel(const T* scores, int parts, const T* bias, const int32_t* labels, int64_t N,
+                 int64_t V, T* lse, T* per_instance, T* total, int32_t* count,
+                 uint32_t* done) {
   chain_begin();
   constexpr int THREADS = GROUP < 256 ? 256 : GROUP;
   constexpr int KEEP = 8;                      // scores in flight per thread; the first ones stay in registers
@@ -526,10 +526,10 @@ lnll_rows_kernel(const T* __restrict__ scores, int parts, const T* __restrict__ 
 constexpr int kChunk = 2048;
 template <typename T>
 __global__ void __launch_bounds__(256)
-lnll_chunks_kernel(const T* __restrict__ scores, int parts, const T* __restrict__ bias, const int32_t* __restrict__ labels, int64_t N,
-                   int64_t V, uint32_t chunks, T* __restrict__ part_m, T* __restrict__ part_s, T* __restrict__ label_score,
-                   T* __restrict__ lse, T* __restrict__ per_instance, T* __restrict__ total, int32_t* __restrict__ count,
-                   uint32_t* __restrict__ done) {
+lnll_chunks_kernel(const T* scores, int parts, const T* bias, const int32_t* labels, int64_t N,
+                   int64_t V, uint32_t chunks, T* part_m, T* part_s, T* label_score,
+                   T* lse, T* per_instance, T* total, int32_t* count,
+                   uint32_t* done) {
   chain_begin();
   __shared__ T red[32];
   __shared__ uint32_t last;
@@ -584,8 +584,8 @@ lnll_chunks_kernel(const T* __restrict__ scores, int parts, const T* __restrict_
 // dS (without g) over the first part of the scores; `blocks` CTAs per instance
 template <typename T>
 __global__ void __launch_bounds__(256)
-lnll_grad_kernel(T* __restrict__ scores, int parts, const T* __restrict__ bias, const int32_t* __restrict__ labels,
-                 const T* __restrict__ lse, int64_t N, int64_t V, uint32_t blocks) {
+lnll_grad_kernel(T* scores, int parts, const T* bias, const int32_t* labels,
+                 const T* lse, int64_t N, int64_t V, uint32_t blocks) {
   chain_begin();
   const int64_t n = blockIdx.x / blocks;
   const T hi = lse[n], lo = lse[N + n];
@@ -602,7 +602,7 @@ lnll_grad_kernel(T* __restrict__ scores, int parts, const T* __restrict__ bias, 
 // out = g * (the parts, added in order), n numbers in rows of J, `ld` apart in `out`
 template <typename T>
 __global__ void __launch_bounds__(256)
-lnll_sum_kernel(const T* __restrict__ parts, int64_t n, int64_t J, int64_t ld, int count, T* __restrict__ out, int add, GradScale<T> g) {
+lnll_sum_kernel(const T* parts, int64_t n, int64_t J, int64_t ld, int count, T* out, int add, GradScale<T> g) {
   chain_begin();
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= n) return;

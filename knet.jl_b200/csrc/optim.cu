@@ -120,8 +120,8 @@ template <typename T> struct AdamDevF {
 template <typename F> __device__ __forceinline__ const F& resolve(const F& f) { return f; }
 template <typename T> __device__ __forceinline__ AdamF<T> resolve(const AdamDevF<T>& d) {
   AdamF<T> f = d.f;
-  f.b1t = __ldg(d.bias_corr);
-  f.b2t = __ldg(d.bias_corr + 1);
+  f.b1t = d.bias_corr[0];
+  f.b2t = d.bias_corr[1];
   return f;
 }
 
@@ -362,7 +362,7 @@ int run_clip_factors(const knet_tensor_desc* table, int ntensors, int64_t total_
 constexpr double kSumLow = 0x1p-900, kSumHigh = 0x1p960;
 template <typename T>
 __global__ void __launch_bounds__(kOptThreads)
-gnorm_chunks_kernel(const knet_tensor_desc* __restrict__ table, int ntensors, double* __restrict__ partials) {
+gnorm_chunks_kernel(const knet_tensor_desc* table, int ntensors, double* partials) {
   chain_begin();
   __shared__ int s_t;
   __shared__ double red[32];
@@ -387,8 +387,8 @@ gnorm_chunks_kernel(const knet_tensor_desc* __restrict__ table, int ntensors, do
 }
 
 __global__ void __launch_bounds__(1024)
-gnorm_finish_kernel(const double* __restrict__ partials, int64_t total_chunks, double gclip, double gscale,
-                    double* __restrict__ norm, double* __restrict__ factor) {
+gnorm_finish_kernel(const double* partials, int64_t total_chunks, double gclip, double gscale,
+                    double* norm, double* factor) {
   chain_begin();
   __shared__ double red[32];
   double acc = 0.0;
@@ -427,7 +427,7 @@ template <typename T> struct ScaleF {
 };
 template <typename T>
 __global__ void __launch_bounds__(kOptThreads)
-gclip_apply_kernel(const knet_tensor_desc* __restrict__ table, int ntensors, const double* __restrict__ factor) {
+gclip_apply_kernel(const knet_tensor_desc* table, int ntensors, const double* factor) {
   chain_begin();
   __shared__ int s_t;
   const double f = *factor;
@@ -441,7 +441,7 @@ gclip_apply_kernel(const knet_tensor_desc* __restrict__ table, int ntensors, con
 // an update whose gradients are all multiplied by the same device-side factor
 template <typename T, typename F0>
 __global__ void __launch_bounds__(kOptThreads)
-opt_gclip_kernel(F0 f0, const knet_tensor_desc* __restrict__ table, int ntensors, const double* __restrict__ factor) {
+opt_gclip_kernel(F0 f0, const knet_tensor_desc* table, int ntensors, const double* factor) {
   chain_begin();
   const auto f = resolve(f0);
   typedef typename std::remove_cv<typename std::remove_reference<decltype(f)>::type>::type F;

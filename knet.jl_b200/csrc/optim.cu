@@ -370,19 +370,18 @@ gnorm_chunks_kernel(const knet_tensor_desc* table, int ntensors, double* partial
   const int64_t start = ((int64_t)blockIdx.x - d.first_chunk) * KNET_MULTI_CHUNK;
   const uint32_t cnt = start < d.n ? (uint32_t)min((int64_t)KNET_MULTI_CHUNK, d.n - start) : 0u;
   const T* g = reinterpret_cast<const T*>(d.p[1]) + start;
-  double acc = 0.0;
-  segment_visit<T>(g, cnt, threadIdx.x, kOptThreads, [&](T v, uint32_t) { acc = ::fma((double)v, (double)v, acc); });
-  acc = block_reduce(acc, [](double a, double b) { return a + b; }, 0.0, red);
-  if constexpr (sizeof(T) == 8) {
-    if (!(acc >= kSumLow && acc <= kSumHigh)) {      // the same in every thread; NaN too
-      const bool low = acc < kSumLow;
-      const double s = low ? 0x1p600 : 0x1p-600;
-      acc = 0.0;
-      segment_visit<T>(g, cnt, threadIdx.x, kOptThreads, [&](T v, uint32_t) { acc = ::fma(v * s, v * s, acc); });
-      acc = block_reduce(acc, [](double a, double b) { return a + b; }, 0.0, red);
-      if (acc > 0 && acc < CUDART_INF) acc = -::sqrt(acc) * (low ? 0x1p-580 : 0x1p580);      // 0, inf and NaN as they are
-    }
+  double acc, s = 1.0;
+  for (;;) {                                         // a second time where need be; one copy of the loop, no call
+    acc = 0.0;
+    segment_visit<T>(g, cnt, threadIdx.x, kOptThreads, [&](T v, uint32_t) {
+      const double t = sizeof(T) == 8 ? v * s : (double)v;
+      acc = ::fma(t, t, acc);
+    });
+    acc = block_reduce(acc, [](double a, double b) { return a + b; }, 0.0, red);
+    if (sizeof(T) == 4 || s != 1.0 || (acc >= kSumLow && acc <= kSumHigh)) break;      // the same in every thread
+    s = acc < kSumLow ? 0x1p600 : 0x1p-600;
   }
+  if (s != 1.0 && acc > 0 && acc < CUDART_INF) acc = -::sqrt(acc) * (s > 1.0 ? 0x1p-580 : 0x1p580);      // 0, inf and NaN as they are
   if (threadIdx.x == 0) partials[blockIdx.x] = acc;
 }
 
@@ -391,20 +390,17 @@ gnorm_finish_kernel(const double* partials, int64_t total_chunks, double gclip, 
                     double* norm, double* factor) {
   chain_begin();
   __shared__ double red[32];
-  double acc = 0.0;
-  bool some = false, large = false, small = false;
+  __shared__ int flags[32];
+  double acc = 0.0, s = 1.0;                         // squares of s * g are added
+  int tags = 0;                                      // 1: a sum other than 0, 2: a small chunk's norm, 4: a large one's
   for (int64_t c = threadIdx.x; c < total_chunks; c += 1024) {
     const double p = partials[c];
-    if (p < 0) (p < -1.0 ? large : small) = true;
-    else {
-      some |= p != 0;
-      acc += p;
-    }
+    tags |= p < -1.0 ? 4 : p < 0 ? 2 : p != 0 ? 1 : 0;
+    acc += p < 0 ? 0.0 : p;
   }
-  double s = 1.0;                                    // the squares of s * g are what is added
-  if (__syncthreads_or(large)) s = 0x1p-600;
-  else if (__syncthreads_or(small) && !__syncthreads_or(some)) s = 0x1p600;
-  if (__syncthreads_or(large || small)) {
+  if (__syncthreads_or(tags > 1)) {
+    tags = block_reduce(tags, [](int a, int b) { return a | b; }, 0, flags);
+    s = tags & 4 ? 0x1p-600 : tags & 1 ? 1.0 : 0x1p600;
     acc = acc * s * s;
     for (int64_t c = threadIdx.x; c < total_chunks; c += 1024) {
       const double p = partials[c], v = p * (p < -1.0 ? 0x1p20 * s : 0x1p-20 * s);

@@ -290,7 +290,7 @@ struct MmaPlan {
   int64_t piece, wld, xld, dld;        // classes per piece; row pitches of split w, x and dS (elements)
   int s_parts, x_parts, w_parts;
   int64_t chunks;                      // of 2048 classes, where the scores are in the workspace (s_parts > 1)
-  size_t exps, absmax, xs, ws, label, part_m, part_s, scores, ds, parts, db, bias, total;
+  size_t done, absmax, xs, ws, xmag, wmag, label, part_m, part_s, scores, maxima, ds, dx_ds, dw_ds, parts, db, bias, total;
 };
 
 inline int64_t cut_sum(int64_t tiles, int64_t len, int64_t bytes) {
@@ -348,17 +348,22 @@ inline MmaPlan mma_plan(int64_t V, int64_t H, int64_t N, int trans, int backward
     where = at;
     at += up(bytes);
   };
-  put(p.exps, 16);
+  put(p.done, 16);
   put(p.absmax, 2 * kMaxBlocks * 4);
   put(p.xs, (size_t)N * p.xld * 4);
   put(p.ws, (size_t)(trans ? vp : H) * p.wld * 4);
+  put(p.xmag, (size_t)N * 4);
+  put(p.wmag, (size_t)vp * 4);
   if (p.s_parts > 1) put(p.scores, (size_t)p.s_parts * N * V * 4);
   if (!backward) {
     put(p.label, (size_t)N * 4);
     put(p.part_m, (size_t)(p.s_parts > 1 ? p.chunks : all) * N * 4);
     put(p.part_s, (size_t)(p.s_parts > 1 ? p.chunks : all) * N * 4);
   } else {
+    put(p.maxima, (size_t)(N + vp) * 4);
     put(p.ds, (size_t)N * p.dld * 4);
+    put(p.dx_ds, (size_t)N * p.dld * 4);
+    put(p.dw_ds, (size_t)N * p.dld * 4);
     const size_t x = p.x_parts > 1 ? (size_t)p.x_parts * N * H * 4 : 0, w = p.w_parts > 1 ? (size_t)p.w_parts * V * H * 4 : 0;
     put(p.parts, x > w ? x : w);
     put(p.db, (size_t)ceil_div(N, kGradRows) * vp * 4);
@@ -566,9 +571,10 @@ inline unsigned scale_operands(const Head<float>& h, const MmaPlan& p, char* ws,
 // w's classes [v0, v0 + vp) and, with the first piece, x in two planes; see lnll_split_kernel for the scales
 struct SplitState {
   Planes w, x;
+  const uint32_t *wmag, *xmag;
 };
 inline SplitState split_operands(const Head<float>& h, const MmaPlan& p, char* ws, int64_t v0, int64_t vp, unsigned parts,
-                                 const float* given, float* saved, cudaStream_t st) {
+                                 const float* given, float* saved, uint32_t* zeros, int64_t nzeros, cudaStream_t st) {
   SplitJob w, x;
   w.src = h.trans ? h.w + v0 * h.H : h.w + v0;
   w.rows = h.trans ? vp : h.H;
@@ -578,6 +584,8 @@ inline SplitState split_operands(const Head<float>& h, const MmaPlan& p, char* w
   w.ld = p.wld;
   w.plane = w.rows * p.wld;
   w.labels = nullptr;
+  w.mag = (uint32_t*)(ws + p.wmag);
+  w.mags = vp;
   x.src = h.x;
   x.rows = h.N;
   x.cols = x.pitch = h.H;
@@ -585,11 +593,12 @@ inline SplitState split_operands(const Head<float>& h, const MmaPlan& p, char* w
   x.ld = p.xld;
   x.plane = x.rows * p.xld;
   x.labels = h.labels;
-  const SplitState s{Planes{w.dst, w.rows, w.cols, w.ld, w.plane}, Planes{x.dst, x.rows, x.cols, x.ld, x.plane}};
+  x.mag = (uint32_t*)(ws + p.xmag);
+  x.mags = h.N;
+  const SplitState s{Planes{w.dst, w.rows, w.cols, w.ld, w.plane}, Planes{x.dst, x.rows, x.cols, x.ld, x.plane}, w.mag, x.mag};
   const int64_t bw = ceil_div(w.rows * ceil_div(w.cols, 8), 1024), bx = v0 ? 0 : ceil_div(x.rows * ceil_div(x.cols, 8), 1024);
   const unsigned na = (unsigned)(bw < 8192 ? bw : 8192), nb = (unsigned)(bx < 8192 ? bx : 8192);
-  launch_chained(lnll_split_kernel, na + nb, 256, 0, st, w, x, na, (const uint32_t*)(ws + p.absmax), parts, given, saved,
-                 (int*)(ws + p.exps));
+  launch_chained(lnll_split_kernel, na + nb, 256, 0, st, w, x, na, (const uint32_t*)(ws + p.absmax), parts, given, saved, zeros, nzeros);
   return s;
 }
 
@@ -600,9 +609,8 @@ inline int mma_parts(int64_t C, int parts) {
   return (int)ceil_div(blocks, ceil_div(blocks, k));
 }
 // parts of the scores of all classes
-inline int mma_scores(const Head<float>& h, const MmaPlan& p, const SplitState& s, float* scores, uint32_t* done, char* ws,
-                      cudaStream_t st) {
-  const MmaStore epi{(const int*)(ws + p.exps), 2, scores, h.N, h.V, h.V, h.N * h.V, 0, done, GradScale<float>{nullptr, 1.0f}};
+inline int mma_scores(const Head<float>& h, const MmaPlan& p, const SplitState& s, float* scores, uint32_t* done, cudaStream_t st) {
+  const MmaStore epi{s.xmag, s.wmag, scores, h.N, h.V, h.V, h.N * h.V, 0, done, GradScale<float>{nullptr, 1.0f}};
   return mma_product(s.x, false, s.w, !h.trans, h.N, h.V, h.H, mma_parts(h.H, p.s_parts), epi, st);
 }
 
@@ -636,18 +644,18 @@ inline int linear_nll_fwd_mma(const Head<float>& h, float* total, int32_t* count
   const MmaPlan p = mma_plan(h.V, h.H, h.N, h.trans, 0);
   const int64_t all = ceil_div(h.V, kTN);
   const unsigned parts = scale_operands(h, p, ws, st);
-  uint32_t* done = (uint32_t*)(ws + p.exps) + 2;
+  uint32_t* done = (uint32_t*)(ws + p.done);
   float *label = (float*)(ws + p.label), *pm = (float*)(ws + p.part_m), *ps = (float*)(ws + p.part_s);
   for (int64_t v0 = 0; v0 < h.V; v0 += p.piece) {
     const int64_t vp = h.V - v0 < p.piece ? h.V - v0 : p.piece;
-    const SplitState s = split_operands(h, p, ws, v0, vp, parts, nullptr, lse + 2 * h.N, st);
+    const SplitState s = split_operands(h, p, ws, v0, vp, parts, nullptr, lse + 2 * h.N, nullptr, 0, st);
     if (p.s_parts > 1) {      // one piece
       float* scores = (float*)(ws + p.scores);
-      if (int rc = mma_scores(h, p, s, scores, done, ws, st)) return rc;
+      if (int rc = mma_scores(h, p, s, scores, done, st)) return rc;
       statistics<float>(h, scores, mma_parts(h.H, p.s_parts), p.chunks, label, total, count, lse, per_instance, done, st);
       return launch_status();
     }
-    const MmaStats epi{(const int*)(ws + p.exps), h.bias ? h.bias + v0 : nullptr, h.labels, pm, ps, label, done, h.N, vp, v0, v0 / kTN};
+    const MmaStats epi{s.xmag, s.wmag, h.bias ? h.bias + v0 : nullptr, h.labels, pm, ps, label, done, h.N, vp, v0, v0 / kTN};
     if (int rc = mma_product(s.x, false, s.w, !h.trans, h.N, vp, h.H, 1, epi, st)) return rc;
   }
   launch_chained(lnll_join_kernel<float>, (unsigned)ceil_div(h.N, 32), 1024, 0, st, pm, ps, label, h.labels, h.N, h.V, all, lse, per_instance, total,
@@ -667,36 +675,40 @@ void bias_gradient(const T* ds, int64_t ld, int64_t rows, int64_t J, T* db, T* p
 inline int linear_nll_bwd_mma(const Head<float>& h, const float* lse, GradScale<float> g, float* dw, float* db, float* dx, char* ws,
                               cudaStream_t st) {
   const MmaPlan p = mma_plan(h.V, h.H, h.N, h.trans, 1);
-  const int* exps = (const int*)(ws + p.exps);
-  float* parts = (float*)(ws + p.parts);
-  float* dbp = db ? (float*)(ws + p.db) : nullptr;
+  float *parts = (float*)(ws + p.parts), *ds = (float*)(ws + p.ds), *dbp = db ? (float*)(ws + p.db) : nullptr;
+  uint32_t *rowmax = (uint32_t*)(ws + p.maxima), *colmax = rowmax + h.N;
   for (int64_t v0 = 0; v0 < h.V; v0 += p.piece) {
     const int64_t vp = h.V - v0 < p.piece ? h.V - v0 : p.piece;
-    const SplitState s = split_operands(h, p, ws, v0, vp, 0, lse + 2 * h.N, nullptr, st);
-    const Planes ds{(__half*)(ws + p.ds), h.N, vp, p.dld, h.N * p.dld};
+    const SplitState s = split_operands(h, p, ws, v0, vp, 0, lse + 2 * h.N, nullptr, rowmax, h.N + vp, st);
     if (p.s_parts > 1) {
       float* scores = (float*)(ws + p.scores);
-      if (int rc = mma_scores(h, p, s, scores, nullptr, ws, st)) return rc;
-      const dim3 grid((unsigned)ceil_div(p.dld, 256), (unsigned)ceil_div(h.N, kGradRows));
-      launch_chained(lnll_grad_planes_kernel, grid, 256, 0, st, scores, mma_parts(h.H, p.s_parts), h.bias, h.labels, lse, h.N, h.V, (__half*)(ws + p.ds),
-                                                    p.dld, ds.plane, dbp);
+      if (int rc = mma_scores(h, p, s, scores, nullptr, st)) return rc;
+      const dim3 grid((unsigned)ceil_div(h.V, 256), (unsigned)ceil_div(h.N, kGradRows));
+      launch_chained(lnll_grad_scores_kernel, grid, 256, 0, st, scores, mma_parts(h.H, p.s_parts), h.bias, h.labels, lse, s.xmag, s.wmag, h.N, h.V,
+                     ds, p.dld, rowmax, colmax, dbp);
     } else {
-      const MmaGradScores e1{exps, h.bias ? h.bias + v0 : nullptr, h.labels, lse, (__half*)(ws + p.ds), h.N, vp, p.dld, ds.plane, v0, dbp};
+      const MmaGradScores e1{s.xmag, s.wmag, h.bias ? h.bias + v0 : nullptr, h.labels, lse, ds, h.N, vp, p.dld, v0, rowmax, colmax, dbp};
       if (int rc = mma_product(s.x, false, s.w, !h.trans, h.N, vp, h.H, 1, e1, st)) return rc;
     }
     if (db) bias_gradient<float>(dbp, vp, ceil_div(h.N, p.s_parts > 1 ? kGradRows : kTM), vp, db + v0, (float*)(ws + p.bias), g, st);
+    if (!dx && !dw) continue;
+    const int64_t plane = h.N * p.dld;
+    const Planes for_dx{(__half*)(ws + p.dx_ds), h.N, vp, p.dld, plane}, for_dw{(__half*)(ws + p.dw_ds), h.N, vp, p.dld, plane};
+    launch_chained(lnll_grad_planes_kernel, dim3((unsigned)ceil_div(vp, 256), (unsigned)ceil_div(h.N, 64)), 256, 0, st, ds, p.dld, h.N, vp, s.xmag,
+                   s.wmag, rowmax, colmax, dx ? (__half*)for_dx.p : nullptr, dw ? (__half*)for_dw.p : nullptr, plane);
     if (dx) {
       const int k = mma_parts(vp, p.x_parts);
-      const MmaStore e2{exps, 0, k == 1 ? dx : parts, h.N, h.H, h.H, k == 1 ? 0 : h.N * h.H, k == 1 && v0 > 0, nullptr, g};
-      if (int rc = mma_product(ds, false, s.w, (bool)h.trans, h.N, h.H, vp, k, e2, st)) return rc;
+      const MmaStore e2{rowmax, nullptr, k == 1 ? dx : parts, h.N, h.H, h.H, k == 1 ? 0 : h.N * h.H, k == 1 && v0 > 0, nullptr, g};
+      if (int rc = mma_product(for_dx, false, s.w, (bool)h.trans, h.N, h.H, vp, k, e2, st)) return rc;
       if (k > 1) sum_parts_to<float>(parts, h.N, h.H, h.H, k, dx, v0 > 0, g, st);
     }
     if (dw) {
       const int k = mma_parts(h.N, p.w_parts);           // more than one only where one piece holds all classes
       const int64_t I = h.trans ? vp : h.H, J = h.trans ? h.H : vp;
       float* out = h.trans ? dw + v0 * h.H : dw + v0;
-      const MmaStore e3{exps, 1, k == 1 ? out : parts, I, J, h.trans ? h.H : h.V, k == 1 ? 0 : h.V * h.H, 0, nullptr, g};
-      if (int rc = h.trans ? mma_product(ds, true, s.x, true, I, J, h.N, k, e3, st) : mma_product(s.x, true, ds, true, I, J, h.N, k, e3, st))
+      const MmaStore e3{h.trans ? colmax : nullptr, h.trans ? nullptr : colmax, k == 1 ? out : parts, I, J, h.trans ? h.H : h.V,
+                        k == 1 ? 0 : h.V * h.H, 0, nullptr, g};
+      if (int rc = h.trans ? mma_product(for_dw, true, s.x, true, I, J, h.N, k, e3, st) : mma_product(s.x, true, for_dw, true, I, J, h.N, k, e3, st))
         return rc;
       if (k > 1) sum_parts_to<float>(parts, I, J, J, k, dw, 0, g, st);
     }

@@ -42,14 +42,13 @@ template <int CG> constexpr uint32_t kStageB = 2 * (kTN / CG) * kBK * 2;
 template <int CG> constexpr uint32_t kStageBytes = kStageA + kStageB<CG>;
 template <int CG> constexpr uint32_t kStages = CG == 1 ? 4 : 6;
 constexpr int kMaxStages = 6;
-constexpr int kGradExp = 14;                            // dS lies in [-1, 1]
 
 struct MmaShared {
   uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2], drain;
   uint32_t tmem;
   int gave_up;
   float2 stat[2][4][kTM];                               // per tile parity, column quarter and row
-  __align__(16) float bias[2][kTN];                     // per tile parity
+  __align__(16) float bias[2][kTN], mag[2][kTN];        // per tile parity
   float colsum[4][kTN];
 };
 constexpr size_t kMmaSmem = 1024 + (size_t)kStages<1> * kStageBytes<1> + sizeof(MmaShared);
@@ -272,7 +271,7 @@ mma_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUt
     for (uint32_t t = worker; t < tiles && ok; t += workers, turn++) {
       const uint32_t it = t % tl.i_tiles, r = t / tl.i_tiles, jt = r % tl.j_tiles, sp = r / tl.j_tiles;
       const uint32_t k0 = sp * tl.blocks_per_split, k1 = min(k0 + tl.blocks_per_split, tl.blocks);
-      epi.stage((int64_t)jt * kTN, sh->bias[turn & 1]);  // read after the barrier below
+      epi.stage((int64_t)jt * kTN, sh, turn & 1);        // read after the barrier below
       float2 acc[32];                                   // 64 columns
 #pragma unroll
       for (int e = 0; e < 32; e++) acc[e] = both(0.0f);
@@ -314,19 +313,24 @@ mma_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUt
 }
 
 // ---- scaling ------------------------------------------------------------------------------------------
-// exps[0] = exponent of w, exps[1] = exponent of x: both were multiplied by 2^exp.  2^126 is the largest
-// factor: data below 2^-112 stays below 2^14, with terms as fine as before.
+// An operand's row is multiplied by 2^14 / m, m being the power of two at or below its largest finite magnitude
+// (2^-112 at least: data below it stays below 2^14, with terms as fine as before).  Arrays keep that
+// magnitude's bits, 0 for a row of zeros.
+__device__ __forceinline__ float magnitude(uint32_t max_bits) { return __uint_as_float(max(max_bits & 0x7f800000u, 15u << 23)); }
+__device__ __forceinline__ float scale_of(float m) { return __uint_as_float((268u << 23) - __float_as_uint(m)); }
 __device__ __forceinline__ float power2(int e) { return __int_as_float((127 + e) << 23); }
-__device__ __forceinline__ int scale_exponent(uint32_t max_bits) {
-  return max_bits ? min(126, 14 - ilogbf(__uint_as_float(max_bits))) : 0;
+__device__ __forceinline__ uint32_t finite_bits(float v) {
+  const uint32_t u = __float_as_uint(v) & 0x7fffffffu;
+  return u < 0x7f800000u ? u : 0u;
 }
-// 2^-e in two factors (the exponents of two operands add up to -226 .. 252)
+// A sum of products of two such operands times 2^-28, the row's m and the column's: acc * a * column * b, in an
+// order in which no step leaves the range unless the result does (m is 2^-112 .. 2^127).
 struct Unscale {
   float a, b;
 };
-__device__ __forceinline__ Unscale unscale(int e, float gain = 1.0f) {
-  const int h = e / 2;
-  return Unscale{gain * power2(-h), power2(-(e - h))};
+__device__ __forceinline__ Unscale unscale(float m, float gain) {
+  const int e = (int)(__float_as_uint(m) >> 23) - 127, h = e / 2;
+  return Unscale{gain * power2(h - 28), power2(e - h)};
 }
 
 struct SplitJob {
@@ -335,6 +339,8 @@ struct SplitJob {
   __half* dst;                 // two planes of rows x ld
   int64_t ld, plane;
   const int32_t* labels;       // of the rows, or null: see lnll_split_kernel
+  uint32_t* mag;               // per instance or class
+  int64_t mags;
 };
 constexpr int kMaxBlocks = 592;                         // absmax blocks: 4 per SM
 
@@ -345,10 +351,7 @@ constexpr int kRun = 8192, kWarpRun = 1024;
 // len <= 32 * LANES values from p on, by LANES threads of which this is number t
 template <int LANES> __device__ __forceinline__ uint32_t run_absmax(const float* p, int len, int t) {
   uint32_t m = 0;
-  auto take = [&](float v) {
-    const uint32_t u = __float_as_uint(v) & 0x7fffffffu;
-    m = max(m, u < 0x7f800000u ? u : 0u);
-  };
+  auto take = [&](float v) { m = max(m, finite_bits(v)); };
   int head = (int)(((16 - ((uintptr_t)p & 15)) & 15) / 4);
   if (head > len) head = len;
   const int nv = (len - head) / 4;
@@ -420,31 +423,29 @@ __device__ __forceinline__ void load8(const float* row, int64_t c, int64_t cols,
 }
 
 // Both operands into their two planes; rows are shared out over blocks, 8 columns per thread and turn.
-// The exponents come from the maxima in `part` (and are left in `saved` for the backward) or, in the
+// The magnitudes come from the maxima in `part` (and are left in `saved` for the backward) or, in the
 // backward, from what the forward left (`given`).  In a skipped instance (label 0), which the scale does not
 // regard, whatever has no fp16 value becomes 0: its dS is 0, which times infinity would be NaN in dW.
+// Maxima of dS's rows and columns, which the kernel that follows takes, begin at 0.
 __global__ void __launch_bounds__(256)
 lnll_split_kernel(SplitJob a, SplitJob b, uint32_t blocks_a, const uint32_t* part, uint32_t parts,
-                  const float* given, float* saved, int* exps) {
+                  const float* given, float* saved, uint32_t* zeros, int64_t nzeros) {
   chain_begin();
   __shared__ uint32_t red[32];
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < nzeros; i += (int64_t)gridDim.x * 256) zeros[i] = 0;
   const bool second = blockIdx.x >= blocks_a;
   const SplitJob j = second ? b : a;
-  int e;
+  uint32_t m = 0;
   if (given) {
-    e = max(-113, min(126, (int)given[second]));
+    m = __float_as_uint(given[second]);
   } else {
-    uint32_t m = 0;
     for (uint32_t k = threadIdx.x; k < parts; k += 256) m = max(m, part[(second ? kMaxBlocks : 0) + k]);
     m = block_reduce(m, [](uint32_t x, uint32_t y) { return max(x, y); }, 0u, red);
-    e = scale_exponent(m);
   }
   const uint32_t first = second ? blocks_a : 0, nb = (second ? gridDim.x - blocks_a : blocks_a);
-  if (blockIdx.x == first && threadIdx.x == 0) {
-    exps[second] = e;
-    if (saved) saved[second] = (float)e;
-  }
-  const float f = power2(e);
+  if (blockIdx.x == first && threadIdx.x == 0 && saved) saved[second] = __uint_as_float(m);
+  for (int64_t i = (int64_t)(blockIdx.x - first) * 256 + threadIdx.x; i < j.mags; i += (int64_t)nb * 256) j.mag[i] = m;
+  const float f = scale_of(magnitude(m));
   const int64_t groups = (j.cols + 7) / 8;               // the pitch ld is a multiple of 8
   const int64_t total = groups * j.rows;
   // from the end: what the maximum's pass read last is still in L2
@@ -479,38 +480,40 @@ __device__ __forceinline__ float exp2_approx(float t) {
   return y;
 }
 
-// the bias of the tile's classes into shared memory, 0 without one and past the last class
-__device__ __forceinline__ void stage_bias(const float* bias, int64_t j0, int64_t J, float* to) {
-  const int col = threadIdx.x;
-  if (col < kTN) to[col] = bias && j0 + col < J ? bias[j0 + col] : 0.0f;
+// the bias (0 without one) and the magnitudes (1 without them) of the tile's columns into shared memory
+__device__ __forceinline__ void stage_columns(const float* bias, const uint32_t* mag, int64_t j0, int64_t J, MmaShared* sh, int turn) {
+  const int col = threadIdx.x & (kTN - 1);
+  if (threadIdx.x < kTN) sh->bias[turn][col] = bias && j0 + col < J ? bias[j0 + col] : 0.0f;
+  else sh->mag[turn][col] = mag && j0 + col < J ? magnitude(mag[j0 + col]) : 1.0f;
 }
 
 // i = instance, j = class: maximum and sum of exponentials of the tile's 256 classes per instance
 struct MmaStats {
-  const int* exps;
+  const uint32_t *xmag, *wmag;
   const float* bias;
   const int32_t* labels;
   float *part_m, *part_s, *label_score;
   uint32_t* done;              // counter of the joining kernel that follows
   int64_t N, J;                // instances, classes of this launch
   int64_t v0, tile0;           // first class and first tile of this launch
-  __device__ __forceinline__ void stage(int64_t j0, float* to) const {
+  __device__ __forceinline__ void stage(int64_t j0, MmaShared* sh, int turn) const {
     clear_done(done);
-    stage_bias(bias, j0, J, to);
+    stage_columns(bias, wmag, j0, J, sh, turn);
   }
   __device__ __forceinline__ void operator()(float2 (&acc)[32], const TileAt& at) const {
-    const Unscale us = unscale(exps[0] + exps[1], at.gain);
     const bool live = at.i < N;
+    const Unscale us = unscale(live ? magnitude(xmag[at.i]) : 1.0f, at.gain);
     const int64_t lab = live ? (int64_t)labels[at.i] - 1 - v0 - at.j0 : -1;
     const float4* bs = reinterpret_cast<const float4*>(at.sh->bias[at.turn & 1] + at.quarter * 64);
+    const float4* ms = reinterpret_cast<const float4*>(at.sh->mag[at.turn & 1] + at.quarter * 64);
     float m = -CUDART_INF_F;
     const int in = (int)min((int64_t)64, J - at.j0);        // columns that are classes
     const float2 ua = both(us.a), ub = both(us.b);
 #pragma unroll
     for (int g = 0; g < 16; g++) {
-      const float4 b = bs[g];
-      acc[2 * g] = fma2(mul2(acc[2 * g], ua), ub, make_float2(b.x, b.y));
-      acc[2 * g + 1] = fma2(mul2(acc[2 * g + 1], ua), ub, make_float2(b.z, b.w));
+      const float4 b = bs[g], c = ms[g];
+      acc[2 * g] = fma2(mul2(mul2(acc[2 * g], ua), make_float2(c.x, c.y)), ub, make_float2(b.x, b.y));
+      acc[2 * g + 1] = fma2(mul2(mul2(acc[2 * g + 1], ua), make_float2(c.z, c.w)), ub, make_float2(b.z, b.w));
     }
     if (in < 64) {
 #pragma unroll
@@ -558,22 +561,6 @@ struct MmaStats {
   }
 };
 
-// 32 values per lane -> the sums over the 32 lanes of column `lane`
-__device__ __forceinline__ float lane_sum(float (&v)[32]) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const bool up = lane & o;
-#pragma unroll
-    for (int k = 0; k < 16; k++)
-      if (k < o) {
-        const float send = up ? v[k] : v[k + o], keep = up ? v[k + o] : v[k];
-        v[k] = keep + __shfl_xor_sync(0xffffffffu, send, o);
-      }
-  }
-  return v[0];
-}
-
 // Eight lanes that hold one row of eight 16-byte groups each (32 words) exchange them so that lane r
 // (of the eight) holds group r of all eight rows: stores then cover 128 contiguous bytes per row
 // instead of 16 bytes in each of 32 lines.
@@ -613,95 +600,104 @@ __device__ __forceinline__ void transpose32(uint32_t (&w)[32]) {
   }
 }
 
-// i = instance, j = class of the piece: dS without g in two fp16 planes, and its sums over the tile's
-// instances for the bias gradient
+// i = instance, j = class of the piece: dS without g, and what the products that follow need to scale it:
+// of each instance the largest |dS| times its class's magnitude (as dS meets W in dx), of each class the largest
+// |dS| times its instance's (as it meets x in dW); maxima do not depend on the order of the atomics.  Also dS's sums
+// over the tile's instances for the bias gradient.
 struct MmaGradScores {
-  const int* exps;
+  const uint32_t *xmag, *wmag;
   const float* bias;           // of the piece's first class
   const int32_t* labels;
   const float* lse;            // N rounded values, N remainders
-  __half* ds;                  // [2][N][ld]
-  int64_t N, J, ld, plane, v0;
+  float* ds;                   // [N][ld], ld a multiple of 64
+  int64_t N, J, ld, v0;
+  uint32_t *rowmax, *colmax;
   float* db_part;              // [instance tile][J] or null
-  __device__ __forceinline__ void stage(int64_t j0, float* to) const { stage_bias(bias, j0, J, to); }
+  __device__ __forceinline__ void stage(int64_t j0, MmaShared* sh, int turn) const { stage_columns(bias, wmag, j0, J, sh, turn); }
   __device__ __forceinline__ void operator()(float2 (&acc)[32], const TileAt& at) const {
-    const Unscale us = unscale(exps[0] + exps[1], at.gain);
     const bool live = at.i < N;
-    const int32_t label = live ? labels[at.i] : 0;    // rows past the last instance act as skipped
+    const float mine = live ? magnitude(xmag[at.i]) : 1.0f;
+    const Unscale us = unscale(mine, at.gain);
+    const int32_t label = live ? labels[at.i] : 0;            // rows past the last instance act as skipped
     const float hi = live ? lse[at.i] : 0.0f, lo = live ? lse[N + at.i] : 0.0f;
-    const float2 ua = both(us.a), ub = both(us.b), nhi = both(-hi), nlo = both(-lo), l2e = both(kLog2e), scale = both((float)(1 << kGradExp));
+    const float2 ua = both(us.a), ub = both(us.b), nhi = both(-hi), nlo = both(-lo), l2e = both(kLog2e);
     const int64_t hit64 = (int64_t)label - 1 - v0 - at.j0;
     const int hit = hit64 >= 0 && hit64 < 64 ? (int)hit64 : -1;
     const int in = (int)max((int64_t)0, min((int64_t)64, J - at.j0));
-    const float4* bs = reinterpret_cast<const float4*>(at.sh->bias[at.turn & 1] + at.quarter * 64);
     const int lane = threadIdx.x & 31, r8 = lane & 7;
     const int64_t row0 = at.i - lane + (lane & ~7);           // first of the eight rows of this lane's group
-    const int64_t col = at.j0 + r8 * 8;                       // after the exchange: 8 classes of each of the eight rows
-    __half* out = ds + row0 * ld + col;
+    float* out = ds + row0 * ld + at.j0 + 4 * r8;
+    uint32_t* top = colmax + at.j0 + 4 * r8;
+    const int rows = (int)max((int64_t)0, min((int64_t)8, N - row0));
+    float rm = 0.0f;                                          // fmaxf passes over NaN
 #pragma unroll
-    for (int g = 0; g < 16; g++) {
-      const float4 b4 = bs[g];
-#pragma unroll
-      for (int k = 0; k < 2; k++) {
-        float2& d = acc[2 * g + k];
-        const float2 s = fma2(mul2(d, ua), ub, k ? make_float2(b4.z, b4.w) : make_float2(b4.x, b4.y));
-        const float2 t = mul2(add2(add2(s, nhi), nlo), l2e);
-        const float2 p = mul2(make_float2(exp2_approx(t.x), exp2_approx(t.y)), scale);
-        d = label == 0 ? both(0.0f) : p;
-      }
-    }
-    if (hit >= 0) {
-#pragma unroll
-      for (int e = 0; e < 32; e++) {
-        if (hit == 2 * e) acc[e].x -= (float)(1 << kGradExp);
-        if (hit == 2 * e + 1) acc[e].y -= (float)(1 << kGradExp);
-      }
-    }
-    if (in < 64) {
-#pragma unroll
-      for (int e = 0; e < 32; e++) {
-        if (2 * e >= in) acc[e].x = 0.0f;
-        if (2 * e + 1 >= in) acc[e].y = 0.0f;
-      }
-    }
-    if (db_part) {
-#pragma unroll
-      for (int half = 0; half < 2; half++) {
-        float v[32];
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-          v[2 * e] = acc[16 * half + e].x;
-          v[2 * e + 1] = acc[16 * half + e].y;
-        }
-        at.sh->colsum[at.row >> 5][at.quarter * 64 + half * 32 + lane] = lane_sum(v);
-      }
-    }
-#pragma unroll
-    for (int pl = 0; pl < 2; pl++) {
+    for (int h = 0; h < 2; h++) {                             // 32 columns at a time, which the registers hold
+      const float4* bs = reinterpret_cast<const float4*>(at.sh->bias[at.turn & 1] + at.quarter * 64 + 32 * h);
+      const float4* ms = reinterpret_cast<const float4*>(at.sh->mag[at.turn & 1] + at.quarter * 64 + 32 * h);
+      const int hit_h = hit - 32 * h, in_h = in - 32 * h;
       uint32_t w[32];
 #pragma unroll
-      for (int k = 0; k < 32; k++) {
-        __half2 h = __floats2half2_rn(acc[k].x, acc[k].y);
-        if (pl) {
-          const float2 f = __half22float2(h);
-          h = __floats2half2_rn(acc[k].x - f.x, acc[k].y - f.y);
+      for (int g = 0; g < 8; g++) {
+        asm volatile("" ::: "memory");                        // no loads of later columns before this one is done with
+        const float4 b4 = bs[g], m4 = ms[g];
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          const float2 c = k ? make_float2(m4.z, m4.w) : make_float2(m4.x, m4.y);
+          const float2 s = fma2(mul2(mul2(acc[16 * h + 2 * g + k], ua), c), ub, k ? make_float2(b4.z, b4.w) : make_float2(b4.x, b4.y));
+          const float2 t = mul2(add2(add2(s, nhi), nlo), l2e);
+          float2 d = label == 0 ? both(0.0f) : make_float2(exp2_approx(t.x), exp2_approx(t.y));
+          const int e = 4 * g + 2 * k;
+          if (hit_h == e) d.x -= 1.0f;
+          if (hit_h == e + 1) d.y -= 1.0f;
+          if (e >= in_h) d.x = 0.0f;
+          if (e + 1 >= in_h) d.y = 0.0f;
+          const float2 r = mul2(d, c);
+          rm = fmaxf(rm, fmaxf(fabsf(r.x), fabsf(r.y)));
+          w[e] = __float_as_uint(d.x);
+          w[e + 1] = __float_as_uint(d.y);
         }
-        w[k] = *reinterpret_cast<const uint32_t*>(&h);
       }
-      transpose8(w);
+      transpose8(w);                                          // now four classes of each of the eight rows
+      const int left = in_h - 4 * r8;                         // classes of the four
 #pragma unroll
       for (int q = 0; q < 8; q++)
-        if (col < J && row0 + q < N)                           // ld is a multiple of 8
-          *reinterpret_cast<uint4*>(out + pl * plane + q * ld) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+        if (q < rows && left > 0) *reinterpret_cast<uint4*>(out + q * ld + 32 * h) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+      if (db_part) {
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          float cs = 0.0f;
+#pragma unroll
+          for (int q = 0; q < 8; q++) cs += __uint_as_float(w[4 * q + c]);
+#pragma unroll
+          for (int o = 8; o < 32; o <<= 1) cs += __shfl_xor_sync(0xffffffffu, cs, o);
+          if (lane < 8) at.sh->colsum[at.row >> 5][at.quarter * 64 + 32 * h + 4 * r8 + c] = cs;
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 8; q++) {
+        const float mx = __shfl_sync(0xffffffffu, mine, (lane & ~7) + q);
+#pragma unroll
+        for (int c = 0; c < 4; c++) w[4 * q + c] = __float_as_uint(fabsf(__uint_as_float(w[4 * q + c]) * mx));
+      }
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        float cm = 0.0f;
+#pragma unroll
+        for (int q = 0; q < 8; q++) cm = fmaxf(cm, __uint_as_float(w[4 * q + c]));
+#pragma unroll
+        for (int o = 8; o < 32; o <<= 1) cm = fmaxf(cm, __shfl_xor_sync(0xffffffffu, cm, o));
+        if (lane < 8 && c < left && cm > 0.0f) atomicMax(top + 32 * h + c, __float_as_uint(cm));
+      }
     }
+    if (live && rm > 0.0f) atomicMax(rowmax + at.i, __float_as_uint(rm));
     if (db_part) {
       epi_sync();
       const int c = threadIdx.x;
       if (c < kTN) {
         const int64_t j = (int64_t)at.jt * kTN + c;
         if (j < J && (int64_t)at.it * kTM < N)                // a pair's second tile may lie past the last instance
-          db_part[(int64_t)at.it * J + j] = ((at.sh->colsum[0][c] + at.sh->colsum[1][c]) +
-                                             (at.sh->colsum[2][c] + at.sh->colsum[3][c])) * (1.0f / (1 << kGradExp));
+          db_part[(int64_t)at.it * J + j] =
+              (at.sh->colsum[0][c] + at.sh->colsum[1][c]) + (at.sh->colsum[2][c] + at.sh->colsum[3][c]);
       }
     }
   }
@@ -709,16 +705,19 @@ struct MmaGradScores {
 
 // out(i, j) = or += g * acc; with several parts of the summed axis the plain sums go to `out` + part
 struct MmaStore {
-  const int* exps;
-  int which;                   // the operand beside dS: 0 w, 1 x; 2: the product of w and x, without dS
+  const uint32_t *row, *col;   // magnitudes of the result's rows and columns, null where there are none
   float* out;
   int64_t I, J, ld, part;      // part: elements between the parts' results (0: there is one)
   int add;
   uint32_t* done;              // counter of the statistics kernel that follows, or null
   GradScale<float> g;
-  __device__ __forceinline__ void stage(int64_t, float*) const { clear_done(done); }
+  __device__ __forceinline__ void stage(int64_t j0, MmaShared* sh, int turn) const {
+    clear_done(done);
+    stage_columns(nullptr, col, j0, J, sh, turn);
+  }
   __device__ __forceinline__ void operator()(float2 (&acc)[32], const TileAt& at) const {
-    const Unscale us = unscale(which == 2 ? exps[0] + exps[1] : exps[which] + kGradExp, at.gain);
+    const Unscale us = unscale(row && at.i < I ? magnitude(row[at.i]) : 1.0f, at.gain);
+    const float4* ms = reinterpret_cast<const float4*>(at.sh->mag[at.turn & 1] + at.quarter * 64);
     const float f = part ? 1.0f : g.value();
     const int lane = threadIdx.x & 31, r8 = lane & 7;
     const int64_t row0 = at.i - lane + (lane & ~7);
@@ -729,7 +728,9 @@ struct MmaStore {
       uint32_t w[32];
 #pragma unroll
       for (int e = 0; e < 16; e++) {
-        const float2 v = mul2(mul2(mul2(acc[16 * h + e], both(us.a)), both(us.b)), both(f));
+        const float4 m4 = ms[8 * h + e / 2];
+        const float2 c = e & 1 ? make_float2(m4.z, m4.w) : make_float2(m4.x, m4.y);
+        const float2 v = mul2(mul2(mul2(mul2(acc[16 * h + e], both(us.a)), c), both(us.b)), both(f));
         w[2 * e] = __float_as_uint(v.x);
         w[2 * e + 1] = __float_as_uint(v.y);
       }
@@ -764,17 +765,16 @@ struct MmaStore {
   }
 };
 
-// dS in two fp16 planes from the parts of the scores, with its sums over groups of 8 instances
+// The same dS, maxima and sums over groups of 8 instances from the parts of the scores
 constexpr int kGradRows = 8;
 __global__ void __launch_bounds__(256)
-lnll_grad_planes_kernel(const float* scores, int parts, const float* bias, const int32_t* labels,
-                        const float* lse, int64_t N, int64_t V, __half* ds, int64_t ld, int64_t plane,
+lnll_grad_scores_kernel(const float* scores, int parts, const float* bias, const int32_t* labels, const float* lse, const uint32_t* xmag,
+                        const uint32_t* wmag, int64_t N, int64_t V, float* ds, int64_t ld, uint32_t* rowmax, uint32_t* colmax,
                         float* db_part) {
   chain_begin();
   const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x, n0 = (int64_t)blockIdx.y * kGradRows;
-  if (v >= ld) return;
-  const float b = bias && v < V ? bias[v] : 0.0f;
-  float t[kGradRows], sum = 0.0f;
+  const float b = bias && v < V ? bias[v] : 0.0f, mw = v < V ? magnitude(wmag[v]) : 0.0f;
+  float t[kGradRows], sum = 0.0f, cm = 0.0f;
 #pragma unroll
   for (int k = 0; k < kGradRows; k++) t[k] = v < V && n0 + k < N ? scores[(n0 + k) * V + v] : 0.0f;
   for (int p = 1; p < parts; p++) {
@@ -788,12 +788,55 @@ lnll_grad_planes_kernel(const float* scores, int parts, const float* bias, const
     if (n >= N) break;
     const float d = v < V ? grad_score(t[k] + b, lse[n], lse[N + n], labels[n], v) : 0.0f;
     sum += d;
-    uint32_t h, l;
-    split_pair(d * (float)(1 << kGradExp), 0.0f, h, l);
-    ds[n * ld + v] = __ushort_as_half((unsigned short)h);
-    ds[plane + n * ld + v] = __ushort_as_half((unsigned short)l);
+    if (v < V) ds[n * ld + v] = d;
+    cm = fmaxf(cm, fabsf(d * magnitude(xmag[n])));
+    const float rm = warp_reduce(fmaxf(0.0f, fabsf(d * mw)), [](float x, float y) { return fmaxf(x, y); });
+    if ((threadIdx.x & 31) == 0 && rm > 0.0f) atomicMax(rowmax + n, __float_as_uint(rm));
   }
+  if (v < V && cm > 0.0f) atomicMax(colmax + v, __float_as_uint(cm));
   if (db_part && v < V) db_part[(int64_t)blockIdx.y * V + v] = sum;
+}
+
+// dS (rows `ld` apart) as the operands of dx and of dW, two planes each (either may be null): times its class's
+// magnitude and scaled by the instance's maximum, times its instance's magnitude and scaled by the class's.  One row
+// of dx, or one class of dW, then keeps its terms to 2^-39 of the largest of them, whatever the others hold.  A warp
+// takes 256 classes of an instance, a CTA 64 instances.
+__global__ void __launch_bounds__(256)
+lnll_grad_planes_kernel(const float* ds, int64_t ld, int64_t N, int64_t J, const uint32_t* xmag, const uint32_t* wmag, const uint32_t* rowmax,
+                        const uint32_t* colmax, __half* for_dx, __half* for_dw, int64_t plane) {
+  chain_begin();
+  const int64_t c = (int64_t)blockIdx.x * 256 + (threadIdx.x & 31) * 8, n0 = (int64_t)blockIdx.y * 64 + (threadIdx.x >> 5);
+  if (c >= J) return;
+  float mw[8], sw[8];
+#pragma unroll
+  for (int k = 0; k < 8; k++) {
+    mw[k] = c + k < J ? magnitude(wmag[c + k]) : 0.0f;
+    sw[k] = c + k < J ? scale_of(magnitude(colmax[c + k])) : 0.0f;
+  }
+#pragma unroll 4
+  for (int r = 0; r < 64; r += 8) {
+    const int64_t n = n0 + r;
+    if (n >= N) break;
+    const float4 a = *reinterpret_cast<const float4*>(ds + n * ld + c), b = *reinterpret_cast<const float4*>(ds + n * ld + c + 4);
+    const float d[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    const float mx = magnitude(xmag[n]), sx = scale_of(magnitude(rowmax[n]));
+    uint4 hi, lo;
+    uint32_t *h = &hi.x, *l = &lo.x;
+    if (for_dx) {
+#pragma unroll
+      for (int k = 0; k < 8; k += 2)
+        split_pair(c + k < J ? d[k] * mw[k] * sx : 0.0f, c + k + 1 < J ? d[k + 1] * mw[k + 1] * sx : 0.0f, h[k / 2], l[k / 2]);
+      *reinterpret_cast<uint4*>(for_dx + n * ld + c) = hi;
+      *reinterpret_cast<uint4*>(for_dx + plane + n * ld + c) = lo;
+    }
+    if (for_dw) {
+#pragma unroll
+      for (int k = 0; k < 8; k += 2)
+        split_pair(c + k < J ? d[k] * mx * sw[k] : 0.0f, c + k + 1 < J ? d[k + 1] * mx * sw[k + 1] : 0.0f, h[k / 2], l[k / 2]);
+      *reinterpret_cast<uint4*>(for_dw + n * ld + c) = hi;
+      *reinterpret_cast<uint4*>(for_dw + plane + n * ld + c) = lo;
+    }
+  }
 }
 
 }  // namespace kn

@@ -350,9 +350,8 @@ KNET_BOTH_TYPES(KNET_DECL_NLL, nll)
  * (transW 1: the embedding matrix of a tied model), x (H,N), b of V or NULL; labels 1-based
  * Int32, 0 = skip the instance, anything outside 0..V makes the loss NaN.  All column-major.
  * fwd: *total = sum over used instances of lse - s[label], *count = instances used,
- *      per_instance of N their terms (0 when skipped); lse of 2N + 2: log sum_v exp(s_vn)
- *      rounded, then what the rounding left, then the scales of W and x.  bwd reads all of it and
- *      takes the same W, x, b and sizes.
+ *      per_instance of N their terms (0 when skipped); lse of 2N: log sum_v exp(s_vn) rounded,
+ *      then what the rounding left.  bwd reads all of it and takes the same W, x, b and sizes.
  * bwd: with g = dy (average 0) or dy / *count (average 1; *count 0 gives g = 0),
  *      dx (H,N) = W' dS, dW (as W) = dS x', db (V) = sum over n of dS, where
  *      dS = (softmax - onehot) g, 0 on skipped instances.  Any of dw, db, dx may be NULL; they
@@ -362,10 +361,11 @@ KNET_BOTH_TYPES(KNET_DECL_NLL, nll)
  * instance is fine, an instance with every class masked gives NaN, as the composed form does.
  * An infinity or a NaN in W or x may make every score that it enters NaN.  What x holds in a
  * skipped instance reaches neither the loss nor a gradient (its lse is then of no use).
- * Large Float32 products (V*H*N from 2^26, or more than 2^24 scores) hold W, x (used instances)
- * to 2^-39 of the largest magnitude of each and dS without g to 2^-39: as exact as Float32
- * arithmetic for entries down to 2^-16 of the largest (of 1), less so below; a dW of a class whose
- * probabilities are all about 2^-28 has 2^-11 of relative error per term.
+ * Large Float32 products (V*H*N from 2^26, or more than 2^24 scores) hold every class of W and every
+ * instance of x to 2^-39 of the largest magnitude in it, and the terms of a row of dx or of a class
+ * of dW to 2^-39 of the largest of them: as exact as Float32 arithmetic for entries down to 2^-16
+ * of that largest one, less so below; what other instances and classes hold does not matter.
+ * Products whose terms all have one sign come out up to 1e-6 of their value low.
  * Up to 2^24 scores may pass through the workspace where that is faster.
  * workspace: at least knet_linear_nll_workspace_S(V, H, N, backward) bytes (0 for sizes that the
  * entry points refuse), 256-byte aligned; calls that share one must be ordered on one stream.

@@ -279,7 +279,7 @@ template <typename T> SmallPlan small_plan(int64_t V, int64_t H, int64_t N, int 
 }
 
 // Pieces of the vocabulary and parts of the products' sums.  Workspace bounds: 256 MB of split weights in
-// the forward; 128 MB of dS and 192 MB of split weights in the backward.  Within them the backward takes
+// the forward; 128 MB of dS, twice as much of its split forms and 192 MB of split weights in the backward.  Within them the backward takes
 // the piece with the fewest waves of tiles over its three products (a product's tiles are 128 x 256, a
 // pair's two of them, and its time is proportional to the summed length), charging each piece for its
 // launches.  Only the smallest piece of each number of pieces is tried: for four million classes that takes the host
@@ -290,7 +290,7 @@ struct MmaPlan {
   int64_t piece, wld, xld, dld;        // classes per piece; row pitches of split w, x and dS (elements)
   int s_parts, x_parts, w_parts;
   int64_t chunks;                      // of 2048 classes, where the scores are in the workspace (s_parts > 1)
-  size_t done, absmax, xs, ws, xmag, wmag, label, part_m, part_s, scores, maxima, ds, dx_ds, dw_ds, parts, db, bias, total;
+  size_t done, xs, ws, xmag, wmag, label, part_m, part_s, scores, maxima, ds, dx_ds, dw_ds, parts, db, bias, total;
 };
 
 inline int64_t cut_sum(int64_t tiles, int64_t len, int64_t bytes) {
@@ -349,7 +349,6 @@ inline MmaPlan mma_plan(int64_t V, int64_t H, int64_t N, int trans, int backward
     at += up(bytes);
   };
   put(p.done, 16);
-  put(p.absmax, 2 * kMaxBlocks * 4);
   put(p.xs, (size_t)N * p.xld * 4);
   put(p.ws, (size_t)(trans ? vp : H) * p.wld * 4);
   put(p.xmag, (size_t)N * 4);
@@ -558,23 +557,33 @@ int mma_product(const Planes& a, bool a_mn, const Planes& b, bool b_mn, int64_t 
   return mma_product_cg<1>(a, a_mn, b, b_mn, I, J, C, splits, epi, st);
 }
 
-// the largest magnitudes of w and x, one value per block of each
-inline unsigned scale_operands(const Head<float>& h, const MmaPlan& p, char* ws, cudaStream_t st) {
-  const int64_t want = ceil_div(h.V * h.H + h.N * h.H, 4096);
-  const unsigned blocks = (unsigned)(want < kMaxBlocks ? want : kMaxBlocks);
-  // an ordinary launch: placed under the tail of another kernel, its equal shares would land unevenly on the
-  // SMs (32000x4096 n512, where it ran once per piece: 2.20 against 2.10 ms)
-  lnll_absmax_kernel<<<blocks, 256, 0, st>>>(h.w, h.V * h.H, h.x, h.labels, h.N, h.H, (uint32_t*)(ws + p.absmax));
-  return blocks;
-}
-
-// w's classes [v0, v0 + vp) and, with the first piece, x in two planes; see lnll_split_kernel for the scales
+// W's classes [v0, v0 + vp) and, with the first piece, x in two planes, each class and each instance with a scale
+// of its own
 struct SplitState {
   Planes w, x;
   const uint32_t *wmag, *xmag;
 };
-inline SplitState split_operands(const Head<float>& h, const MmaPlan& p, char* ws, int64_t v0, int64_t vp, unsigned parts,
-                                 const float* given, float* saved, uint32_t* zeros, int64_t nzeros, cudaStream_t st) {
+template <int GROUP, int LANES>
+void split_cols_launch(const SplitJob& w, const SplitJob& x, int64_t blocks_x, uint32_t* zeros, int64_t nzeros, cudaStream_t st) {
+  uint32_t ctas = 1;
+  while (ctas < kSplitCtas && w.rows >= 64 * (int64_t)ctas) ctas *= 2;
+  const int64_t bw = ceil_div(w.cols, 8 * LANES) * ctas, bx = ceil_div(blocks_x, ctas) * ctas;
+  launch_chained_cluster(ctas, lnll_split_cols_kernel<GROUP, LANES>, (unsigned)(bw + bx), 256, 0, st, w, x, (uint32_t)bw, ctas, zeros, nzeros);
+}
+template <int GROUP>
+void split_launch(bool rows, const SplitJob& w, const SplitJob& x, bool with_x, uint32_t* zeros, int64_t nzeros, cudaStream_t st) {
+  const int64_t per = 256 / GROUP, bx = with_x ? ceil_div(x.rows, per) : 0;
+  if (rows) {
+    const int64_t bw = ceil_div(w.rows, per);
+    launch_chained(lnll_split_rows_kernel<GROUP>, (unsigned)(bw + bx), 256, 0, st, w, x, (uint32_t)bw, zeros, nzeros);
+  } else if (ceil_div(w.cols, 256) * kSplitCtas >= 2 * kPlanSMs) {
+    split_cols_launch<GROUP, 32>(w, x, bx, zeros, nzeros, st);
+  } else {                   // 64 classes to a cluster where 256 would make less than two CTAs per SM
+    split_cols_launch<GROUP, 8>(w, x, bx, zeros, nzeros, st);
+  }
+}
+inline SplitState split_operands(const Head<float>& h, const MmaPlan& p, char* ws, int64_t v0, int64_t vp, uint32_t* zeros, int64_t nzeros,
+                                 cudaStream_t st) {
   SplitJob w, x;
   w.src = h.trans ? h.w + v0 * h.H : h.w + v0;
   w.rows = h.trans ? vp : h.H;
@@ -585,7 +594,6 @@ inline SplitState split_operands(const Head<float>& h, const MmaPlan& p, char* w
   w.plane = w.rows * p.wld;
   w.labels = nullptr;
   w.mag = (uint32_t*)(ws + p.wmag);
-  w.mags = vp;
   x.src = h.x;
   x.rows = h.N;
   x.cols = x.pitch = h.H;
@@ -594,12 +602,11 @@ inline SplitState split_operands(const Head<float>& h, const MmaPlan& p, char* w
   x.plane = x.rows * p.xld;
   x.labels = h.labels;
   x.mag = (uint32_t*)(ws + p.xmag);
-  x.mags = h.N;
-  const SplitState s{Planes{w.dst, w.rows, w.cols, w.ld, w.plane}, Planes{x.dst, x.rows, x.cols, x.ld, x.plane}, w.mag, x.mag};
-  const int64_t bw = ceil_div(w.rows * ceil_div(w.cols, 8), 1024), bx = v0 ? 0 : ceil_div(x.rows * ceil_div(x.cols, 8), 1024);
-  const unsigned na = (unsigned)(bw < 8192 ? bw : 8192), nb = (unsigned)(bx < 8192 ? bx : 8192);
-  launch_chained(lnll_split_kernel, na + nb, 256, 0, st, w, x, na, (const uint32_t*)(ws + p.absmax), parts, given, saved, zeros, nzeros);
-  return s;
+  // threads per row of up to 32 features each
+  if (h.H <= 256) split_launch<8>(h.trans, w, x, v0 == 0, zeros, nzeros, st);
+  else if (h.H <= 1024) split_launch<32>(h.trans, w, x, v0 == 0, zeros, nzeros, st);
+  else split_launch<256>(h.trans, w, x, v0 == 0, zeros, nzeros, st);
+  return SplitState{Planes{w.dst, w.rows, w.cols, w.ld, w.plane}, Planes{x.dst, x.rows, x.cols, x.ld, x.plane}, w.mag, x.mag};
 }
 
 // how many parts a sum of C terms really has (each has work, in blocks of 32)
@@ -643,12 +650,11 @@ inline int linear_nll_fwd_mma(const Head<float>& h, float* total, int32_t* count
                               cudaStream_t st) {
   const MmaPlan p = mma_plan(h.V, h.H, h.N, h.trans, 0);
   const int64_t all = ceil_div(h.V, kTN);
-  const unsigned parts = scale_operands(h, p, ws, st);
   uint32_t* done = (uint32_t*)(ws + p.done);
   float *label = (float*)(ws + p.label), *pm = (float*)(ws + p.part_m), *ps = (float*)(ws + p.part_s);
   for (int64_t v0 = 0; v0 < h.V; v0 += p.piece) {
     const int64_t vp = h.V - v0 < p.piece ? h.V - v0 : p.piece;
-    const SplitState s = split_operands(h, p, ws, v0, vp, parts, nullptr, lse + 2 * h.N, nullptr, 0, st);
+    const SplitState s = split_operands(h, p, ws, v0, vp, nullptr, 0, st);
     if (p.s_parts > 1) {      // one piece
       float* scores = (float*)(ws + p.scores);
       if (int rc = mma_scores(h, p, s, scores, done, st)) return rc;
@@ -679,7 +685,7 @@ inline int linear_nll_bwd_mma(const Head<float>& h, const float* lse, GradScale<
   uint32_t *rowmax = (uint32_t*)(ws + p.maxima), *colmax = rowmax + h.N;
   for (int64_t v0 = 0; v0 < h.V; v0 += p.piece) {
     const int64_t vp = h.V - v0 < p.piece ? h.V - v0 : p.piece;
-    const SplitState s = split_operands(h, p, ws, v0, vp, 0, lse + 2 * h.N, nullptr, rowmax, h.N + vp, st);
+    const SplitState s = split_operands(h, p, ws, v0, vp, rowmax, h.N + vp, st);
     if (p.s_parts > 1) {
       float* scores = (float*)(ws + p.scores);
       if (int rc = mma_scores(h, p, s, scores, nullptr, st)) return rc;
@@ -694,7 +700,7 @@ inline int linear_nll_bwd_mma(const Head<float>& h, const float* lse, GradScale<
     if (!dx && !dw) continue;
     const int64_t plane = h.N * p.dld;
     const Planes for_dx{(__half*)(ws + p.dx_ds), h.N, vp, p.dld, plane}, for_dw{(__half*)(ws + p.dw_ds), h.N, vp, p.dld, plane};
-    launch_chained(lnll_grad_planes_kernel, dim3((unsigned)ceil_div(vp, 256), (unsigned)ceil_div(h.N, 64)), 256, 0, st, ds, p.dld, h.N, vp, s.xmag,
+    launch_chained(lnll_grad_planes_kernel, dim3((unsigned)ceil_div(h.N, kPlaneRows), (unsigned)ceil_div(vp, 256)), 256, 0, st, ds, p.dld, h.N, vp, s.xmag,
                    s.wmag, rowmax, colmax, dx ? (__half*)for_dx.p : nullptr, dw ? (__half*)for_dw.p : nullptr, plane);
     if (dx) {
       const int k = mma_parts(vp, p.x_parts);

@@ -1,17 +1,20 @@
 // Float32 products of the linear-layer cross entropy on the tensor cores.
 //
-// A Float32 operand, scaled by a power of two that brings its largest magnitude into [2^14, 2^15), is
-// split into two fp16 terms, hi = fp16(x), lo = fp16(x - hi): together 22 bits, and never less than
-// 2^-25 of the scaled value's unit, so entries down to 2^-16 of the largest keep a relative error of
-// 2^-23 (probabilities below 2^-16 in dS therefore do not; a third term would make a product of six instead
-// of three).  A product takes three of the four partial products (lo*lo is below 2^-22 of it), which are
+// A row of a Float32 operand (a class of W, an instance of x), scaled by a power of two that brings its largest
+// magnitude into [2^14, 2^15), is split into two fp16 terms, hi = fp16(v), lo = fp16(v - hi): together 22 bits,
+// and never less than 2^-25 of the scaled value's unit, so entries down to 2^-16 of the row's largest keep a relative
+// error of 2^-23.  The row has its own scale, undone in the epilogue, so that a large instance or class costs no
+// other one its bits.  dS is kept in Float32 and split twice: for dx = W' dS with a scale per instance, for
+// dW = dS x' with one per class, the scales of W's classes and x's instances taken into it, since the sums run over
+// those.  (Terms of every magnitude, three in bf16, would make a product of six partial ones.)
+// A product takes three of the four partial products (lo*lo is below 2^-22 of it), which are
 // exact in Float32; the tensor core adds them.  Its additions truncate: measured on sums of 1024 and 8192
 // products, an accumulator that takes n blocks of 32 summed indices comes out low by 0.75 n 2^-23 of its
 // value for terms of random signs (n = 4, 8, 16: 3.4e-7, 7.4e-7, 1.5e-6), about twice that for terms of
 // one sign.  The accumulator in TMEM therefore takes 256 summed indices, the chunks are added in registers
 // with rounding to nearest, and the epilogue multiplies by 1 + 0.75 n 2^-23, which leaves a relative error
-// of 5e-7 to 8e-7 in a product.  (Chunks of 128 halve the error; 256 give the epilogue 10 us instead of 5
-// before the tensor core has to wait for it: dS of 4608 classes x 4096 instances 123 -> 112 us.)
+// of 5e-7 to 8e-7 in a product and leaves one of terms of one sign up to 9e-7 low.  (Chunks of 128 halve the error;
+// 256 give the epilogue 10 us instead of 5 before the tensor core has to wait for it.)
 //
 // A CTA owns a 128 x 256 tile of the result, or a pair of CTAs (a cluster) one of 256 x 256.  Warp 16 loads
 // the operands with TMA into a ring of stages of 32 summed indices (both planes of 128 rows of A and of 256
@@ -338,60 +341,9 @@ struct SplitJob {
   int64_t rows, cols, pitch;
   __half* dst;                 // two planes of rows x ld
   int64_t ld, plane;
-  const int32_t* labels;       // of the rows, or null: see lnll_split_kernel
-  uint32_t* mag;               // per instance or class
-  int64_t mags;
+  const int32_t* labels;       // of the rows, or null: see split_rows
+  uint32_t* mag;               // largest finite magnitude per instance or class
 };
-constexpr int kMaxBlocks = 592;                         // absmax blocks: 4 per SM
-
-// Largest finite magnitude of each of two arrays, one value per block and array.  W, contiguous, goes to
-// the blocks in turns of 8192 elements; x goes to the warps, 1024 elements of one instance at a time, and
-// a skipped instance (label 0) does not count: a padded batch may hold anything there.
-constexpr int kRun = 8192, kWarpRun = 1024;
-// len <= 32 * LANES values from p on, by LANES threads of which this is number t
-template <int LANES> __device__ __forceinline__ uint32_t run_absmax(const float* p, int len, int t) {
-  uint32_t m = 0;
-  auto take = [&](float v) { m = max(m, finite_bits(v)); };
-  int head = (int)(((16 - ((uintptr_t)p & 15)) & 15) / 4);
-  if (head > len) head = len;
-  const int nv = (len - head) / 4;
-  if (t < head) take(p[t]);
-  const float4* q = reinterpret_cast<const float4*>(p + head);
-  float4 v[8];
-#pragma unroll
-  for (int u = 0; u < 8; u++)
-    if (t + u * LANES < nv) v[u] = q[t + u * LANES];
-#pragma unroll
-  for (int u = 0; u < 8; u++)
-    if (t + u * LANES < nv) { take(v[u].x); take(v[u].y); take(v[u].z); take(v[u].w); }
-  const int tail = head + nv * 4 + t;
-  if (tail < len) take(p[tail]);
-  return m;
-}
-__global__ void __launch_bounds__(256)
-lnll_absmax_kernel(const float* w, int64_t n, const float* x, const int32_t* labels, int64_t N,
-                   int64_t H, uint32_t* part) {
-  chain_begin();
-  __shared__ uint32_t red[32];
-  auto larger = [](uint32_t a, uint32_t b) { return max(a, b); };
-  uint32_t m = 0;
-  for (int64_t c = (int64_t)blockIdx.x * kRun; c < n; c += (int64_t)gridDim.x * kRun)
-    m = max(m, run_absmax<256>(w + c, (int)min((int64_t)kRun, n - c), threadIdx.x));
-  uint32_t mx = 0;
-  const int64_t runs = (H + kWarpRun - 1) / kWarpRun;
-  for (int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); t < N * runs; t += (int64_t)gridDim.x * 8) {
-    const int64_t i = t / runs, c = (t - i * runs) * kWarpRun;
-    const bool used = labels[i] != 0;          // does not hold up the loads
-    const uint32_t v = run_absmax<32>(x + i * H + c, (int)min((int64_t)kWarpRun, H - c), threadIdx.x & 31);
-    mx = used ? max(mx, v) : mx;
-  }
-  m = block_reduce(m, larger, 0u, red);
-  mx = block_reduce(mx, larger, 0u, red);
-  if (threadIdx.x == 0) {
-    part[blockIdx.x] = m;
-    part[kMaxBlocks + blockIdx.x] = mx;
-  }
-}
 
 // v = hi + lo in fp16 for two values; what is not finite goes to hi alone, so that an infinity is not NaN
 __device__ __forceinline__ void split_pair(float v0, float v1, uint32_t& hi, uint32_t& lo) {
@@ -405,67 +357,218 @@ __device__ __forceinline__ void split_pair(float v0, float v1, uint32_t& hi, uin
   lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
-// Eight consecutive floats of a row that starts at any alignment: aligned 16-byte loads that lie inside the
-// row, shifted by the row's offset in a line; single loads at its ends.
-__device__ __forceinline__ void load8(const float* row, int64_t c, int64_t cols, float (&v)[8]) {
-  const int off = (int)(((uintptr_t)row >> 2) & 3);
-  if (c - off >= 0 && c - off + (off ? 12 : 8) <= cols) {
-    const float4* q = reinterpret_cast<const float4*>(row + c - off);
-    const float4 a = q[0], b = q[1];
-    const float4 d = off ? q[2] : b;
+// Eight consecutive floats at p, of which `left` are inside the row (0 past its end).  OFF 0..3: p lies OFF floats past a
+// multiple of 16 bytes and the aligned 16-byte words around the eight are inside the row; the shift is the same for
+// all rows that a thread walks, so it is a constant here.  OFF 4: single loads.
+template <int OFF> __device__ __forceinline__ void load_at(const float* p, int64_t left, float (&v)[8]) {
+  if constexpr (OFF < 4) {
+    const float4* q = reinterpret_cast<const float4*>(p - OFF);
+    const float4 a = q[0], b = q[1], d = OFF ? q[2] : b;
     const float t[12] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, d.x, d.y, d.z, d.w};
 #pragma unroll
-    for (int k = 0; k < 8; k++) v[k] = off == 0 ? t[k] : off == 1 ? t[k + 1] : off == 2 ? t[k + 2] : t[k + 3];
+    for (int k = 0; k < 8; k++) v[k] = t[k + OFF];
   } else {
 #pragma unroll
-    for (int k = 0; k < 8; k++) v[k] = c + k < cols ? row[c + k] : 0.0f;
+    for (int k = 0; k < 8; k++) v[k] = k < left ? p[k] : 0.0f;
+  }
+}
+__device__ __forceinline__ int offset_of(const float* p) { return (int)(((uintptr_t)p >> 2) & 3); }
+__device__ __forceinline__ bool words_inside(int off, int64_t c, int64_t cols) { return c - off >= 0 && c - off + (off ? 12 : 8) <= cols; }
+
+// 8 values times their scales in two planes; the pitch is a multiple of 8
+__device__ __forceinline__ void store_split(const SplitJob& j, int64_t r, int64_t c, const float (&v)[8]) {
+  uint4 hi, lo;
+  split_pair(v[0], v[1], hi.x, lo.x);
+  split_pair(v[2], v[3], hi.y, lo.y);
+  split_pair(v[4], v[5], hi.z, lo.z);
+  split_pair(v[6], v[7], hi.w, lo.w);
+  *reinterpret_cast<uint4*>(j.dst + r * j.ld + c) = hi;
+  *reinterpret_cast<uint4*>(j.dst + j.plane + r * j.ld + c) = lo;
+}
+
+// x, or W whose classes are rows: GROUP threads take a row, read it (up to 32 values per thread stay in registers,
+// what is longer comes from L1 the second time) and scale it by its own maximum.  In a skipped instance
+// (label 0) whatever has no fp16 value becomes 0: its dS is 0, which times infinity would be NaN in dW.
+template <int GROUP, int OFF>
+__device__ __forceinline__ void split_row(const SplitJob& j, int64_t r, bool live, uint32_t* red) {
+  constexpr int KEEP = 4;
+  const int t = threadIdx.x % GROUP;
+  const float* row = j.src + r * j.pitch;
+  const bool skipped = j.labels && j.labels[r] == 0;
+  const bool kept = j.cols <= KEEP * GROUP * 8;
+  auto load = [&](int64_t c, float (&v)[8]) {
+    if (words_inside(OFF, c, j.cols)) load_at<OFF>(row + c, 8, v);
+    else load_at<4>(row + c, j.cols - c, v);
+  };
+  float v[KEEP][8];
+  uint32_t m = 0;
+  for (int64_t c0 = t * 8; c0 < j.cols; c0 += KEEP * GROUP * 8) {
+#pragma unroll
+    for (int k = 0; k < KEEP; k++)
+      if (c0 + k * GROUP * 8 < j.cols) load(c0 + k * GROUP * 8, v[k]);
+#pragma unroll
+    for (int k = 0; k < KEEP; k++)
+      if (c0 + k * GROUP * 8 < j.cols) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) m = max(m, finite_bits(v[k][e]));
+      }
+  }
+  if constexpr (GROUP == 256) {
+    m = block_reduce(m, [](uint32_t a, uint32_t b) { return max(a, b); }, 0u, red);
+  } else {      // rows of a warp may take different branches of the caller
+    const uint32_t mask = GROUP == 32 ? 0xffffffffu : ((1u << GROUP) - 1) << (threadIdx.x & 31 & ~(GROUP - 1));
+#pragma unroll
+    for (int o = GROUP / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(mask, m, o));
+  }
+  if (!live) return;
+  if (t == 0) j.mag[r] = m;
+  const float f = scale_of(magnitude(m));
+  for (int64_t c0 = t * 8; c0 < j.cols; c0 += KEEP * GROUP * 8)
+#pragma unroll
+    for (int k = 0; k < KEEP; k++) {
+      const int64_t c = c0 + k * GROUP * 8;
+      if (c >= j.cols) break;
+      if (!kept) load(c, v[k]);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        v[k][e] *= f;
+        if (skipped && !(fabsf(v[k][e]) <= 65504.0f)) v[k][e] = 0.0f;
+      }
+      store_split(j, r, c, v[k]);
+    }
+}
+template <int GROUP> __device__ __forceinline__ void split_rows(const SplitJob& j, int64_t block, uint32_t* red) {
+  if (block * (256 / GROUP) >= j.rows) return;           // the whole CTA
+  const int64_t at = block * (256 / GROUP) + threadIdx.x / GROUP;
+  const bool live = at < j.rows;
+  const int64_t r = live ? at : j.rows - 1;
+  switch (offset_of(j.src + r * j.pitch)) {              // one row per CTA where it has barriers
+    case 0: return split_row<GROUP, 0>(j, r, live, red);
+    case 1: return split_row<GROUP, 1>(j, r, live, red);
+    case 2: return split_row<GROUP, 2>(j, r, live, red);
+    default: return split_row<GROUP, 3>(j, r, live, red);
   }
 }
 
-// Both operands into their two planes; rows are shared out over blocks, 8 columns per thread and turn.
-// The magnitudes come from the maxima in `part` (and are left in `saved` for the backward) or, in the
-// backward, from what the forward left (`given`).  In a skipped instance (label 0), which the scale does not
-// regard, whatever has no fp16 value becomes 0: its dS is 0, which times infinity would be NaN in dW.
-// Maxima of dS's rows and columns, which the kernel that follows takes, begin at 0.
-__global__ void __launch_bounds__(256)
-lnll_split_kernel(SplitJob a, SplitJob b, uint32_t blocks_a, const uint32_t* part, uint32_t parts,
-                  const float* given, float* saved, uint32_t* zeros, int64_t nzeros) {
+// maxima of dS's rows and columns, which a kernel that follows takes, begin at 0
+__device__ __forceinline__ void clear(uint32_t* zeros, int64_t n) {
+  const int64_t blocks = (int64_t)gridDim.x * gridDim.y, b = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+  for (int64_t i = b * 256 + threadIdx.x; i < n; i += blocks * 256) zeros[i] = 0;
+}
+
+// x and W whose classes are rows: the first blocks take W, the others x
+template <int GROUP>
+__global__ void __launch_bounds__(256, 4)
+lnll_split_rows_kernel(SplitJob w, SplitJob x, uint32_t blocks_w, uint32_t* zeros, int64_t nzeros) {
   chain_begin();
   __shared__ uint32_t red[32];
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < nzeros; i += (int64_t)gridDim.x * 256) zeros[i] = 0;
-  const bool second = blockIdx.x >= blocks_a;
-  const SplitJob j = second ? b : a;
-  uint32_t m = 0;
-  if (given) {
-    m = __float_as_uint(given[second]);
-  } else {
-    for (uint32_t k = threadIdx.x; k < parts; k += 256) m = max(m, part[(second ? kMaxBlocks : 0) + k]);
-    m = block_reduce(m, [](uint32_t x, uint32_t y) { return max(x, y); }, 0u, red);
-  }
-  const uint32_t first = second ? blocks_a : 0, nb = (second ? gridDim.x - blocks_a : blocks_a);
-  if (blockIdx.x == first && threadIdx.x == 0 && saved) saved[second] = __uint_as_float(m);
-  for (int64_t i = (int64_t)(blockIdx.x - first) * 256 + threadIdx.x; i < j.mags; i += (int64_t)nb * 256) j.mag[i] = m;
-  const float f = scale_of(magnitude(m));
-  const int64_t groups = (j.cols + 7) / 8;               // the pitch ld is a multiple of 8
-  const int64_t total = groups * j.rows;
-  // from the end: what the maximum's pass read last is still in L2
-  for (int64_t g = total - 1 - ((int64_t)(blockIdx.x - first) * 256 + threadIdx.x); g >= 0; g -= (int64_t)nb * 256) {
-    const int64_t r = g / groups, c = (g - r * groups) * 8;
-    float v[8];
-    const bool skipped = j.labels && j.labels[r] == 0;
-    load8(j.src + r * j.pitch, c, j.cols, v);
+  clear(zeros, nzeros);
+  if (blockIdx.x >= blocks_w) split_rows<GROUP>(x, blockIdx.x - blocks_w, red);
+  else split_rows<GROUP>(w, blockIdx.x, red);
+}
+
+// W whose classes are columns: a cluster of CTAs takes 8 * LANES of them, each CTA a share of the rows (the features)
+// and a thread eight classes.  The maxima of the shares meet through the cluster's shared memory; the second read
+// of a share, from its end, finds part of it in L1 and most in L2.
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+constexpr int kSplitCtas = 8;
+template <int STEP, int OFF>
+__device__ __forceinline__ void col_maxima(const SplitJob& w, int64_t c, int64_t r0, int64_t hi, uint32_t (&m)[8]) {
+  constexpr int UN = 2;
+  for (int64_t r = r0; r < hi; r += STEP * UN) {
+    float v[UN][8];
 #pragma unroll
-    for (int k = 0; k < 8; k++) {
-      v[k] *= f;
-      if (skipped && !(fabsf(v[k]) <= 65504.0f)) v[k] = 0.0f;
+    for (int u = 0; u < UN; u++)
+      if (r + STEP * u < hi) load_at<OFF>(w.src + (r + STEP * u) * w.pitch + c, w.cols - c, v[u]);
+#pragma unroll
+    for (int u = 0; u < UN; u++)
+      if (r + STEP * u < hi) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) m[e] = max(m[e], finite_bits(v[u][e]));
+      }
+  }
+}
+template <int STEP, int OFF>
+__device__ __forceinline__ void col_split(const SplitJob& w, int64_t c, int64_t r0, int64_t hi, const float (&f)[8]) {
+  constexpr int UN = 2;
+  for (int64_t r = r0 + (hi - 1 - r0) / STEP * STEP; r >= r0; r -= STEP * UN) {
+    float v[UN][8];
+#pragma unroll
+    for (int u = 0; u < UN; u++)
+      if (r - STEP * u >= r0) load_at<OFF>(w.src + (r - STEP * u) * w.pitch + c, w.cols - c, v[u]);
+#pragma unroll
+    for (int u = 0; u < UN; u++)
+      if (r - STEP * u >= r0) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[u][e] *= f[e];
+        store_split(w, r - STEP * u, c, v[u]);
+      }
+  }
+}
+// the clusters of the first blocks take W, the other blocks x
+template <int GROUP, int LANES>
+__global__ void __launch_bounds__(256, 4)
+lnll_split_cols_kernel(SplitJob w, SplitJob x, uint32_t blocks_w, uint32_t ctas, uint32_t* zeros, int64_t nzeros) {
+  chain_begin();
+  clear(zeros, nzeros);
+  constexpr int COLS = LANES * 8, STEP = 256 / LANES;    // a multiple of 4, so that a thread's rows have one offset
+  __shared__ uint32_t part[8][COLS], mine[COLS], all[COLS];
+  if (blockIdx.x >= blocks_w) return split_rows<GROUP>(x, blockIdx.x - blocks_w, mine);
+  const uint32_t rank = ctas > 1 ? cluster_rank() : 0;
+  const int64_t g0 = (int64_t)(blockIdx.x / ctas) * COLS, share = (w.rows + ctas - 1) / ctas;
+  const int64_t lo = rank * share, hi = min(w.rows, lo + share);
+  const int lane = threadIdx.x % LANES;
+  const int64_t c = g0 + lane * 8, r0 = lo + threadIdx.x / LANES;
+  const bool in = c < w.cols && r0 < hi;
+  const int off = in ? offset_of(w.src + r0 * w.pitch + c) : 0, how = words_inside(off, c, w.cols) ? off : 4;
+  uint32_t m[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (in) switch (how) {
+      case 0: col_maxima<STEP, 0>(w, c, r0, hi, m); break;
+      case 1: col_maxima<STEP, 1>(w, c, r0, hi, m); break;
+      case 2: col_maxima<STEP, 2>(w, c, r0, hi, m); break;
+      case 3: col_maxima<STEP, 3>(w, c, r0, hi, m); break;
+      default: col_maxima<STEP, 4>(w, c, r0, hi, m);
     }
-    uint4 hi, lo;
-    split_pair(v[0], v[1], hi.x, lo.x);
-    split_pair(v[2], v[3], hi.y, lo.y);
-    split_pair(v[4], v[5], hi.z, lo.z);
-    split_pair(v[6], v[7], hi.w, lo.w);
-    *reinterpret_cast<uint4*>(j.dst + r * j.ld + c) = hi;
-    *reinterpret_cast<uint4*>(j.dst + j.plane + r * j.ld + c) = lo;
+  __syncwarp();
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+#pragma unroll
+    for (int o = LANES; o < 32; o <<= 1) m[e] = max(m[e], __shfl_xor_sync(0xffffffffu, m[e], o));
+    if ((threadIdx.x & 31) < LANES) part[threadIdx.x >> 5][lane * 8 + e] = m[e];
+  }
+  __syncthreads();
+  if (threadIdx.x < COLS) {
+    uint32_t a = 0;
+#pragma unroll
+    for (int k = 0; k < 8; k++) a = max(a, part[k][threadIdx.x]);
+    mine[threadIdx.x] = a;
+    all[threadIdx.x] = a;
+  }
+  if (ctas > 1) {
+    cluster_barrier();
+    if (threadIdx.x < COLS) {
+      uint32_t a = 0;
+      for (uint32_t k = 0; k < ctas; k++) a = max(a, ld_cluster_u32(mapa_u32(&mine[threadIdx.x], k)));
+      all[threadIdx.x] = a;
+    }
+    cluster_barrier();                                   // no CTA leaves while another reads its share
+  }
+  __syncthreads();
+  if (rank == 0 && threadIdx.x < COLS && g0 + threadIdx.x < w.cols) w.mag[g0 + threadIdx.x] = all[threadIdx.x];
+  if (!in) return;
+  float f[8];
+#pragma unroll
+  for (int e = 0; e < 8; e++) f[e] = scale_of(magnitude(all[lane * 8 + e]));
+  switch (how) {
+    case 0: return col_split<STEP, 0>(w, c, r0, hi, f);
+    case 1: return col_split<STEP, 1>(w, c, r0, hi, f);
+    case 2: return col_split<STEP, 2>(w, c, r0, hi, f);
+    case 3: return col_split<STEP, 3>(w, c, r0, hi, f);
+    default: return col_split<STEP, 4>(w, c, r0, hi, f);
   }
 }
 
@@ -473,6 +576,9 @@ lnll_split_kernel(SplitJob a, SplitJob b, uint32_t blocks_a, const uint32_t* par
 // A thread holds 64 columns of one row.  The epilogue has to stay below the time of two chunks, about
 // 12 000 clocks: the tensor core runs ahead by that much and then waits.
 constexpr float kLog2e = 1.4426950408889634f;
+
+// 2^t, t = (s - lse) log2 e rounded: relative error |t| 2^-24 ln 2 and 2^-22 of the instruction, beside what the
+// rounding of the scores themselves, |s| 2^-24, does to any exponential of them
 
 __device__ __forceinline__ float exp2_approx(float t) {
   float y;
@@ -800,12 +906,13 @@ lnll_grad_scores_kernel(const float* scores, int parts, const float* bias, const
 // dS (rows `ld` apart) as the operands of dx and of dW, two planes each (either may be null): times its class's
 // magnitude and scaled by the instance's maximum, times its instance's magnitude and scaled by the class's.  One row
 // of dx, or one class of dW, then keeps its terms to 2^-39 of the largest of them, whatever the others hold.  A warp
-// takes 256 classes of an instance, a CTA 64 instances.
+// takes 256 classes of an instance, a CTA 32 instances; from the last classes, which are still in L2.
+constexpr int kPlaneRows = 32;
 __global__ void __launch_bounds__(256)
 lnll_grad_planes_kernel(const float* ds, int64_t ld, int64_t N, int64_t J, const uint32_t* xmag, const uint32_t* wmag, const uint32_t* rowmax,
                         const uint32_t* colmax, __half* for_dx, __half* for_dw, int64_t plane) {
   chain_begin();
-  const int64_t c = (int64_t)blockIdx.x * 256 + (threadIdx.x & 31) * 8, n0 = (int64_t)blockIdx.y * 64 + (threadIdx.x >> 5);
+  const int64_t c = (int64_t)(gridDim.y - 1 - blockIdx.y) * 256 + (threadIdx.x & 31) * 8, n0 = (int64_t)blockIdx.x * kPlaneRows + (threadIdx.x >> 5);
   if (c >= J) return;
   float mw[8], sw[8];
 #pragma unroll
@@ -813,8 +920,8 @@ lnll_grad_planes_kernel(const float* ds, int64_t ld, int64_t N, int64_t J, const
     mw[k] = c + k < J ? magnitude(wmag[c + k]) : 0.0f;
     sw[k] = c + k < J ? scale_of(magnitude(colmax[c + k])) : 0.0f;
   }
-#pragma unroll 4
-  for (int r = 0; r < 64; r += 8) {
+#pragma unroll
+  for (int r = 0; r < kPlaneRows; r += 8) {
     const int64_t n = n0 + r;
     if (n >= N) break;
     const float4 a = *reinterpret_cast<const float4*>(ds + n * ld + c), b = *reinterpret_cast<const float4*>(ds + n * ld + c + 4);

@@ -265,7 +265,7 @@ for (T, S) in ((Float32, "32"), (Float64, "64"))
             V, H, N = head_sizes(w, x, labels, b, trans)
             ws = CuArray{UInt8}(undef, ccall(($(QuoteNode(wsf)), libknet8), Csize_t, (Int64, Int64, Int64, Cint), V, H, N, 0))
             total = CuArray{$T}(undef, 1); count = CuArray{Int32}(undef, 1)
-            lse = CuArray{$T}(undef, 2N + 2); per = CuArray{$T}(undef, N)
+            lse = CuArray{$T}(undef, 2N); per = CuArray{$T}(undef, N)
             check(ccall(($(QuoteNode(fwd)), libknet8), Cint,
                         (CuPtr{$T}, Cint, CuPtr{$T}, CuPtr{$T}, CuPtr{Int32}, Int64, Int64, Int64, CuPtr{$T}, CuPtr{Int32},
                          CuPtr{$T}, CuPtr{$T}, CuPtr{UInt8}, Csize_t, CUDA.CUstream),
@@ -276,7 +276,7 @@ for (T, S) in ((Float32, "32"), (Float64, "64"))
         function linear_nll_back(w::DevArray{$T}, x::DevArray{$T}, labels::CuArray{Int32}, lse::CuArray{$T}, count::CuArray{Int32}, dy;
                                  b::Union{Nothing,DevArray{$T}}=nothing, trans=false, average=true)
             V, H, N = head_sizes(w, x, labels, b, trans)
-            length(lse) == 2N + 2 && length(count) == 1 || throw(DimensionMismatch("the forward result belongs to other arrays"))
+            length(lse) == 2N && length(count) == 1 || throw(DimensionMismatch("the forward result belongs to other arrays"))
             ws = CuArray{UInt8}(undef, ccall(($(QuoteNode(wsf)), libknet8), Csize_t, (Int64, Int64, Int64, Cint), V, H, N, 1))
             dw = similar(w); dx = similar(x); db = b === nothing ? nothing : similar(b)
             check(ccall(($(QuoteNode(bwd)), libknet8), Cint,

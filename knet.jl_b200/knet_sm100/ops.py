@@ -374,7 +374,7 @@ def nll_back(scores, labels, dims=1, average=True, dy=1.0, count=None):
 
 class LinearNllResult(NllResult):
     """Device-side result of linear_nll_device: NllResult plus `saved`, what the backward pass reads: log
-    sum exp per instance as its rounded value (`lse`) and the remainder of that rounding, and two scales."""
+    sum exp per instance as its rounded value (`lse`) and the remainder of that rounding."""
 
     def __init__(self, total, count, per_instance, labels, saved):
         super().__init__(total, count, per_instance, labels)
@@ -382,7 +382,7 @@ class LinearNllResult(NllResult):
 
     @property
     def lse(self):
-        return self.saved[:self.saved.numel() // 2 - 1]
+        return self.saved[:self.saved.numel() // 2]
 
 
 def _head_sizes(w, x, b, trans):
@@ -422,7 +422,7 @@ def linear_nll_device(w, x, labels, b=None, trans=False):
         total = torch.empty(1, dtype=dt, device=dev)
         count = torch.empty(1, dtype=torch.int32, device=dev)
         per = torch.empty(max(N, 1), dtype=dt, device=dev)
-        lse = torch.empty(2 * N + 2, dtype=dt, device=dev)
+        lse = torch.empty(2 * N, dtype=dt, device=dev)
         size = getattr(libknet, f"knet_linear_nll_workspace_{S}")(V, H, N, 0)
         ws = torch.empty(max(size, 1), dtype=torch.uint8, device=dev)
         knet(f"knet_linear_nll_fwd_{S}", _address(w), 1 if trans else 0, _address(b), _address(x), lab.data_ptr(), V, H, N,

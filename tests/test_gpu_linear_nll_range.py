@@ -27,3 +27,131 @@ def test_classes_that_are_never_hit(K, trans, shape):
     _, dw, _, db = check(K, c)
     for k in range(5):
         assert bool(c.matrix(dw)[c.V // 3 + k::8].any()) and bool((db.data[c.V // 3 + k::8] > 0).all())
+
+
+class Wide(Case):
+    """A Case whose instance `big` and class `masked` have values 2^k times the others'.  Instance `big` is 2^k times
+    the weights of class `top`, whose score in it is then far above any other; class `masked` has the score -4 * 2^k
+    in every instance, of which its remaining weights move a tenth.  Their shares of the softmax are exactly 1 and 0
+    and do not feel the rounding of those scores."""
+
+    def __init__(self, V, H, N, trans, bias, k):
+        super().__init__(V, H, N, torch.float32, trans, bias, True)
+        self.big, self.masked, self.top = N // 2, V // 2, 3
+        s = 2.0 ** k
+        self.x[:, 1] = 1.0
+        self.w[self.masked] *= s * 0.05
+        self.w[self.masked, 1] = -4.0 * s
+        self.w[self.top, 1] = 1.0                                     # so that the two meet with the score -4 * 4^k
+        self.x[self.big] = self.w[self.top] * s
+        self.labels[self.big] = 1
+        self.labels[self.labels == self.masked + 1] = 1
+        self.labels[1] = self.masked + 1                              # one instance is labelled with it: a loss of about 4 * 2^k
+
+    def solve(self):
+        u, V, H, N = U[self.dtype], self.V, self.H, self.N
+        w, x = self.w.double(), self.x.double()
+        b = torch.zeros(V, device="cuda", dtype=torch.float64) if self.b is None else self.b.double()
+        s = x @ w.t() + b
+        ds = gamma(H, u) * (x.abs() @ w.abs().t()) + 2 * u * (s.abs() + b.abs())
+        lse = torch.logsumexp(s, 1)
+        p = torch.exp(s - lse.unsqueeze(1))
+        sure = (p == 0) | (p == 1)                                     # beyond any rounding, as is checked here:
+        gap = (s - s.max(1, keepdim=True).values).abs()
+        alone = torch.zeros_like(sure)
+        alone[self.big] = True
+        alone[:, self.masked] = True
+        assert bool(sure[alone].all())
+        far = gap - ds - ds.gather(1, s.argmax(1, keepdim=True))
+        assert bool((far[alone & (p == 0)] > 200).all())
+        de = torch.where(alone, torch.zeros_like(ds), ds)              # what reaches the softmax
+        dlse = de.max(1).values + (V / 64 + 40) * 2 * u
+        used = self.labels != 0
+        at = (self.labels.long() - 1).clamp_min(0).unsqueeze(1)
+        top = ds.gather(1, s.argmax(1, keepdim=True)).squeeze(1)
+        per = torch.where(used, lse - s.gather(1, at).squeeze(1), torch.zeros_like(lse))
+        self.lse, self.dlse = lse, dlse + torch.maximum(top, dlse) + 2 * u * lse.abs()
+        self.per, self.dper = per, torch.where(used, self.dlse + ds.gather(1, at).squeeze(1) + 2 * u * per.abs(), torch.zeros_like(lse))
+        e = p * (torch.expm1(de + dlse.unsqueeze(1) + 8 * u) + 8 * u) + 2 * u * p
+        p = p.scatter_add(1, at, torch.full_like(lse, -1.0).unsqueeze(1))
+        e = e.scatter_add(1, at, torch.full_like(lse, 2 * u).unsqueeze(1))
+        f = used.double().unsqueeze(1) / int(used.sum())
+        p, e = p * f, e * f + 4 * u * (p * f).abs()
+        self.p = p
+        self.dx, self.ddx = p @ w, e @ w.abs() + gamma(V, u) * (p.abs() @ w.abs())
+        self.dw, self.ddw = p.t() @ x, e.t() @ x.abs() + gamma(N, u) * (p.abs().t() @ x.abs())
+        self.db, self.ddb = p.sum(0), e.sum(0) + gamma(N, u) * p.abs().sum(0)
+        return self
+
+
+@pytest.mark.parametrize("k", [20, 40, 60])
+@pytest.mark.parametrize("trans", [False, True])
+@pytest.mark.parametrize("shape", FORMS, ids=str)
+def test_one_instance_and_one_class_far_above_the_others(K, trans, shape, k):
+    """A finite outlier reaches its own instance or class only: the losses, lse, dx of the other instances and dW, db
+    of the other classes are as exact as without it."""
+    c = Wide(*shape, trans, shape[0] % 2 == 0, k).solve()
+    kw, kx, kb = c.arrays(K)
+    res = K.ops.linear_nll_device(kw, kx, c.labels, b=kb, trans=trans)
+    dw, dx, db = K.ops.linear_nll_back(kw, kx, res, b=kb, trans=trans)
+    within(res.lse, c.lse, c.dlse, "lse")
+    within(res.per_instance[:c.N], c.per, c.dper, "per_instance")
+    others = torch.ones(c.N, dtype=torch.bool, device="cuda")
+    others[[c.big, 1]] = False
+    loss = res.per_instance[:c.N].double()
+    assert float((loss - c.per)[others].abs().max()) < 1e-2
+    within(dx.data.view(c.N, c.H), c.dx, c.ddx, "dx")
+    within(c.matrix(dw), c.dw, c.ddw, "dw")
+    if db is not None:
+        within(db.data, c.db, c.ddb, "db")
+
+
+@pytest.mark.parametrize("trans", [False, True])
+@pytest.mark.parametrize("shape", [(1000, 256, 300), (3001, 515, 700), (1000, 2100, 300), (2000, 9000, 130)], ids=str)
+def test_magnitudes_of_every_size(K, trans, shape):
+    """Each instance and each class with a power of two of its own: instances from 2^-39 to 2, classes from 2^-30
+    to 4."""
+    c = Case(*shape, torch.float32, trans, True, True)
+    c.w *= 2.0 ** -torch.arange(c.V, device="cuda").remainder(33).sub(2).float().unsqueeze(1)
+    c.x *= 2.0 ** -torch.arange(c.N, device="cuda").remainder(41).sub(1).float().unsqueeze(1)
+    check(K, c)
+
+
+@pytest.mark.parametrize("trans", [False, True])
+@pytest.mark.parametrize("scales", [(2.0 ** 100, 2.0 ** -110), (2.0 ** -100, 2.0 ** 110), (2.0 ** -120, 2.0 ** 100), (2.0 ** 124, 2.0 ** -126)],
+                         ids=str)
+def test_magnitudes_at_the_ends_of_the_type(K, trans, scales):
+    """Scores far below the type's largest value from operands close to it and to its smallest."""
+    c = Case(1000, 256, 300, torch.float32, trans, False, True, std=0.5)
+    c.w *= scales[0]
+    c.x *= scales[1]
+    kw, kx, _ = c.arrays(K)
+    res = K.ops.linear_nll_device(kw, kx, c.labels, trans=trans)
+    c.solve()
+    within(res.lse, c.lse, c.dlse, "lse")
+    within(res.per_instance[:c.N], c.per, c.dper, "per_instance")
+
+
+@pytest.mark.parametrize("trans", [False, True])
+@pytest.mark.parametrize("shape", [(1000, 1024, 300), (3001, 2048, 700), (20000, 256, 2000)], ids=str)
+def test_terms_of_one_sign(K, trans, shape):
+    """Operands without negative entries, as after relu: every truncated addition of the tensor core then errs in
+    the same direction.  An accumulator takes 8 blocks of 32 summed indices, 3 products of 2 steps each, so at most 48
+    additions that each lose less than 2^-23 of the sum, of which the epilogue gives back 6 * 2^-23; what the split
+    leaves out is 3 * 2^-22 and the additions of chunks in Float32 lose n / 256 times 2^-24: below 2^-17 of the
+    sum, far inside gamma(n) from n = 256 on.  The scores here are shifted so that the softmax is not one-hot."""
+    c = Case(*shape, torch.float32, trans, True, True)
+    c.w.abs_()
+    c.x.abs_()
+    c.w *= 0.25
+    res, dw, dx, db = check(K, c)
+    # lse within 2^-17 of the scores' size, the gradients within that of the sums of absolute values and
+    # what the error of the scores, at most 2 * 2^-17 of them, does to the probabilities
+    t = 2.0 ** -17
+    top = float((c.x.double() @ c.w.double().t()).max()) + float(c.b.abs().max())
+    used = c.labels != 0
+    assert float((res.lse.double() - c.lse)[used].abs().max()) <= t * top
+    hot = torch.zeros_like(c.p).scatter_(1, (c.labels.long() - 1).clamp_min(0).unsqueeze(1), 1.0 / c.count) * used.unsqueeze(1)
+    p = c.p.abs() + hot
+    within(c.matrix(dw), c.dw, t * (2 * top + 2) * (p.t() @ c.x.double()), "dw")
+    within(dx.data.view(c.N, c.H), c.dx, t * (2 * top + 2) * (p @ c.w.double()), "dx")

@@ -17,7 +17,7 @@ def test_linear_nll_compares_sizes_before_the_call():
     for name in ("linear_nll", "linear_nll_back"):
         body = method(name)
         assert body.index("head_sizes(w, x, labels, b, trans)") < body.index("ccall")
-    assert "length(lse) == 2N + 2" in method("linear_nll_back") and "length(count) == 1" in method("linear_nll_back")
+    assert "length(lse) == 2N " in method("linear_nll_back") and "length(count) == 1" in method("linear_nll_back")
     sizes = method("head_sizes")
     for what in ("ndims(w) == 2", "size(x, 1) == H", "length(labels) == N", "length(b) == V"):
         assert what in sizes

@@ -285,7 +285,7 @@ template <typename T> SmallPlan small_plan(int64_t V, int64_t H, int64_t N, int 
 // launches.  Only the smallest piece of each number of pieces is tried: for four million classes that takes the host
 // 10 us, every size of a piece 0.7 ms.  Where a
 // product has tiles for less than half of the SMs, its sum is cut into parts of at least 128 (a chunk);
-// the scores only if they fit 64 MB with their parts, dW only if there is one piece.
+// the scores only if all of them fit 64 MB with their parts, dW only if there is one piece.
 struct MmaPlan {
   int64_t piece, wld, xld, dld;        // classes per piece; row pitches of split w, x and dS (elements)
   int s_parts, x_parts, w_parts;
@@ -305,11 +305,12 @@ inline MmaPlan mma_plan(int64_t V, int64_t H, int64_t N, int trans, int backward
   MmaPlan p{};
   const int64_t all = ceil_div(V, kTN), nt = ceil_div(N, kTM), hj = ceil_div(H, kTN), hi = ceil_div(H, kTM);
   p.s_parts = p.x_parts = p.w_parts = 1;
-  if (!backward) {
-    int64_t m = (int64_t)(256u << 20) / 4 / (ceil_div(H, 64) * 64) / kTN;
-    m = m < 1 ? 1 : m;
-    p.piece = kTN * ceil_div(all, ceil_div(all, m));
-  } else {
+  int64_t most = (int64_t)(256u << 20) / 4 / (ceil_div(H, 64) * 64) / kTN;
+  most = most < 1 ? 1 : most;
+  p.piece = kTN * ceil_div(all, ceil_div(all, most));      // of the forward
+  // the backward's scores are the forward's bit for bit, summed in the same parts, whatever its own pieces
+  if (p.piece >= V) p.s_parts = (int)cut_sum(nt * all, H, N * V * 4);
+  if (backward) {
     // the largest piece within the bounds, then the smallest piece of each number of pieces
     const int64_t row = ceil_div(H, 64) * 64 * 4 * kTN, most_ds = (128ll << 20) / (kTN * N * 4), most_w = (192ll << 20) / row;
     int64_t m = most_ds < most_w ? most_ds : most_w;
@@ -335,7 +336,6 @@ inline MmaPlan mma_plan(int64_t V, int64_t H, int64_t N, int trans, int backward
       m--;
     }
   }
-  if (p.piece >= V) p.s_parts = (int)cut_sum(nt * all, H, N * V * 4);
   p.chunks = V > 4 * kChunk ? ceil_div(V, kChunk) : 0;
   const int64_t vp = p.piece < V ? p.piece : V;
   // pitches of whole 128-byte lines: a box of 32 summed indices (64 bytes) then never straddles two sectors
@@ -353,7 +353,7 @@ inline MmaPlan mma_plan(int64_t V, int64_t H, int64_t N, int trans, int backward
   put(p.ws, (size_t)(trans ? vp : H) * p.wld * 4);
   put(p.xmag, (size_t)N * 4);
   put(p.wmag, (size_t)vp * 4);
-  if (p.s_parts > 1) put(p.scores, (size_t)p.s_parts * N * V * 4);
+  if (p.s_parts > 1) put(p.scores, (size_t)p.s_parts * N * vp * 4);
   if (!backward) {
     put(p.label, (size_t)N * 4);
     put(p.part_m, (size_t)(p.s_parts > 1 ? p.chunks : all) * N * 4);
@@ -615,10 +615,10 @@ inline int mma_parts(int64_t C, int parts) {
   const int64_t k = parts < blocks ? parts : blocks;
   return (int)ceil_div(blocks, ceil_div(blocks, k));
 }
-// parts of the scores of all classes
-inline int mma_scores(const Head<float>& h, const MmaPlan& p, const SplitState& s, float* scores, uint32_t* done, cudaStream_t st) {
-  const MmaStore epi{s.xmag, s.wmag, scores, h.N, h.V, h.V, h.N * h.V, 0, done, GradScale<float>{nullptr, 1.0f}};
-  return mma_product(s.x, false, s.w, !h.trans, h.N, h.V, h.H, mma_parts(h.H, p.s_parts), epi, st);
+// parts of the scores of a piece's classes
+inline int mma_scores(const Head<float>& h, const MmaPlan& p, const SplitState& s, int64_t vp, float* scores, uint32_t* done, cudaStream_t st) {
+  const MmaStore epi{s.xmag, s.wmag, scores, h.N, vp, vp, h.N * vp, 0, done, GradScale<float>{nullptr, 1.0f}};
+  return mma_product(s.x, false, s.w, !h.trans, h.N, vp, h.H, mma_parts(h.H, p.s_parts), epi, st);
 }
 
 // lse and loss from the parts of the scores: a warp per instance where there are many, or little to do (forward
@@ -657,7 +657,7 @@ inline int linear_nll_fwd_mma(const Head<float>& h, float* total, int32_t* count
     const SplitState s = split_operands(h, p, ws, v0, vp, nullptr, 0, st);
     if (p.s_parts > 1) {      // one piece
       float* scores = (float*)(ws + p.scores);
-      if (int rc = mma_scores(h, p, s, scores, done, st)) return rc;
+      if (int rc = mma_scores(h, p, s, vp, scores, done, st)) return rc;
       statistics<float>(h, scores, mma_parts(h.H, p.s_parts), p.chunks, label, total, count, lse, per_instance, done, st);
       return launch_status();
     }
@@ -688,10 +688,10 @@ inline int linear_nll_bwd_mma(const Head<float>& h, const float* lse, GradScale<
     const SplitState s = split_operands(h, p, ws, v0, vp, rowmax, h.N + vp, st);
     if (p.s_parts > 1) {
       float* scores = (float*)(ws + p.scores);
-      if (int rc = mma_scores(h, p, s, scores, nullptr, st)) return rc;
-      const dim3 grid((unsigned)ceil_div(h.V, 256), (unsigned)ceil_div(h.N, kGradRows));
-      launch_chained(lnll_grad_scores_kernel, grid, 256, 0, st, scores, mma_parts(h.H, p.s_parts), h.bias, h.labels, lse, s.xmag, s.wmag, h.N, h.V,
-                     ds, p.dld, rowmax, colmax, dbp);
+      if (int rc = mma_scores(h, p, s, vp, scores, nullptr, st)) return rc;
+      const dim3 grid((unsigned)ceil_div(vp, 256), (unsigned)ceil_div(h.N, kGradRows));
+      launch_chained(lnll_grad_scores_kernel, grid, 256, 0, st, scores, mma_parts(h.H, p.s_parts), h.bias ? h.bias + v0 : nullptr, h.labels, lse,
+                     s.xmag, s.wmag, h.N, vp, v0, ds, p.dld, rowmax, colmax, dbp);
     } else {
       const MmaGradScores e1{s.xmag, s.wmag, h.bias ? h.bias + v0 : nullptr, h.labels, lse, ds, h.N, vp, p.dld, v0, rowmax, colmax, dbp};
       if (int rc = mma_product(s.x, false, s.w, !h.trans, h.N, vp, h.H, 1, e1, st)) return rc;

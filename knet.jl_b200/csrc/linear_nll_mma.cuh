@@ -871,11 +871,11 @@ struct MmaStore {
   }
 };
 
-// The same dS, maxima and sums over groups of 8 instances from the parts of the scores
+// The same dS, maxima and sums over groups of 8 instances from the parts of the scores of V classes from v0 on
 constexpr int kGradRows = 8;
 __global__ void __launch_bounds__(256)
 lnll_grad_scores_kernel(const float* scores, int parts, const float* bias, const int32_t* labels, const float* lse, const uint32_t* xmag,
-                        const uint32_t* wmag, int64_t N, int64_t V, float* ds, int64_t ld, uint32_t* rowmax, uint32_t* colmax,
+                        const uint32_t* wmag, int64_t N, int64_t V, int64_t v0, float* ds, int64_t ld, uint32_t* rowmax, uint32_t* colmax,
                         float* db_part) {
   chain_begin();
   const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x, n0 = (int64_t)blockIdx.y * kGradRows;
@@ -892,7 +892,7 @@ lnll_grad_scores_kernel(const float* scores, int parts, const float* bias, const
   for (int k = 0; k < kGradRows; k++) {
     const int64_t n = n0 + k;
     if (n >= N) break;
-    const float d = v < V ? grad_score(t[k] + b, lse[n], lse[N + n], labels[n], v) : 0.0f;
+    const float d = v < V ? grad_score(t[k] + b, lse[n], lse[N + n], labels[n], v0 + v) : 0.0f;
     sum += d;
     if (v < V) ds[n * ld + v] = d;
     cm = fmaxf(cm, fabsf(d * magnitude(xmag[n])));

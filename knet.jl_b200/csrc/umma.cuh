@@ -3,7 +3,8 @@
 //
 // Rules the helpers rely on: one thread issues tcgen05.mma and its commits; TMEM is allocated and
 // freed by one whole warp; a warp reads the 32 TMEM lanes of its rank in its group of four; every
-// TMA load starts at a multiple of 16 bytes along the contiguous axis; no multicast form is used.
+// TMA load starts at a multiple of 16 bytes along the contiguous axis; no load is multicast.  (A pair's commit
+// signals the barriers of both its CTAs through tcgen05.commit's cluster form, which reads no memory.)
 #pragma once
 #include <cuda.h>
 

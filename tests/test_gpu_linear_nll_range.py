@@ -167,3 +167,81 @@ def test_terms_of_one_sign(K, trans, shape):
     p = c.p.abs() + hot
     within(c.matrix(dw), c.dw, t * (2 * top + 2) * (p.t() @ c.x.double()), "dw")
     within(dx.data.view(c.N, c.H), c.dx, t * (2 * top + 2) * (p @ c.w.double()), "dx")
+
+
+@pytest.mark.parametrize("trans", [False, True])
+@pytest.mark.parametrize("shape", [(1, 8192, 8192), (3001, 515, 700), (9000, 96, 3000), (2000, 4096, 500)], ids=str)
+def test_roundings_of_either_sign_mostly_cancel(K, trans, shape):
+    """The worst order of n roundings would hide the loss of a few of an operand's bits.  Of a product's terms t each
+    is off by less than 3 * 2^-23 |t| (the two splits and the product of the second terms), with either sign; an accumulator's 48
+    truncated additions, their mean made up for, by 2^-23 (48 / 12)^0.5 of a partial sum each in the mean square,
+    a partial sum being about |t|_2, the root of the sum of squares: about 2^-21.5 |t|_2 together.  Beyond 8 of those
+    standard deviations, 2^-18.5 |t|_2, is not rounding.  To the gradients adds what the probabilities' own error
+    does, a common factor per instance: as much as the scores' and lse's error together, with the sign of one."""
+    c = Case(*shape, torch.float32, trans, False, True, std=1.0)
+    kw, kx, _ = c.arrays(K)
+    res = K.ops.linear_nll_device(kw, kx, c.labels, trans=trans)
+    dw, dx, _ = K.ops.linear_nll_back(kw, kx, res, trans=trans)
+    c.solve()
+    t = 2.0 ** -18.5
+    w, x, p = c.w.double(), c.x.double(), c.p
+    score = t * ((x * x) @ (w * w).t()).sqrt() + 2.0 ** -24 * (x @ w.t()).abs()
+    if c.V == 1:                                                       # lse is the score
+        within(res.lse, c.lse, score[:, 0] + 2.0 ** -24, "lse")
+        return
+    ds = 2 * float(score.max()) + 2.0 ** -21                           # exponential, logarithm, lse's own rounding
+    within(res.lse, c.lse, torch.full_like(c.lse, ds), "lse")
+    hot = torch.zeros_like(p).scatter_(1, (c.labels.long() - 1).clamp_min(0).unsqueeze(1), 1.0 / c.count) * (c.labels != 0).unsqueeze(1)
+    soft = p + hot
+    within(dx.data.view(c.N, c.H), c.dx, t * ((p * p) @ (w * w)).sqrt() + ds * (soft @ w.abs()), "dx")
+    within(c.matrix(dw), c.dw, t * ((p * p).t() @ (x * x)).sqrt() + ds * (soft.t() @ x.abs()), "dw")
+
+
+@pytest.mark.parametrize("trans", [False, True])
+@pytest.mark.parametrize("shape", [(1001, 260, 301), (9000, 96, 3000)], ids=str)
+def test_gradients_one_at_a_time(K, trans, shape):
+    """dS is split for dx and for dW only where they are asked for; either alone has the bits that it has with the
+    others."""
+    c = Case(*shape, torch.float32, trans, True, True)
+    kw, kx, kb = c.arrays(K)
+    res = K.ops.linear_nll_device(kw, kx, c.labels, b=kb, trans=trans)
+    full = K.ops.linear_nll_back(kw, kx, res, b=kb, trans=trans)
+    for k in range(3):
+        part = K.ops.linear_nll_back(kw, kx, res, b=kb, trans=trans, need=tuple(i == k for i in range(3)))
+        assert [g is None for g in part] == [i != k for i in range(3)] and torch.equal(part[k].data, full[k].data)
+
+
+@pytest.mark.parametrize("shape", [(1000, 256, 300), (5001, 700, 400)], ids=str)
+def test_weights_in_columns_captured_and_on_two_streams(K, shape):
+    """The clusters that split W by columns, replayed on new inputs and side by side."""
+    cs = [Case(*shape, torch.float32, False, True, True, seed=s) for s in (1, 2)]
+    held = [c.arrays(K) for c in cs]
+
+    def step(c, arrays):
+        res = K.ops.linear_nll_device(*arrays[:2], c.labels, b=arrays[2])
+        return [res.total, res.lse] + [g.data for g in K.ops.linear_nll_back(*arrays[:2], res, b=arrays[2])]
+
+    want = [[t.clone() for t in step(c, a)] for c, a in zip(cs, held)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [None, None]
+    for _ in range(4):
+        for k in (0, 1):
+            with torch.cuda.stream(streams[k]):
+                got[k] = step(cs[k], held[k])
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(a, b) for a, b in zip(g, w))
+    box = Case(*shape, torch.float32, False, True, True, seed=1)
+    arrays = box.arrays(K)
+    graphs, outs = [], []
+    for _ in range(2):                                                 # two graphs of one set of inputs
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(step(box, arrays))
+    for k, g in ((1, 0), (0, 1), (1, 1), (0, 0)):
+        for to, of in zip(arrays, held[k]):
+            to.data.copy_(of.data)
+        box.labels.copy_(cs[k].labels)
+        graphs[g].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs[g], want[k]))

@@ -369,7 +369,10 @@ KNET_BOTH_TYPES(KNET_DECL_NLL, nll)
  * Up to 2^24 scores may pass through the workspace where that is faster.
  * workspace: at least knet_linear_nll_workspace_S(V, H, N, backward) bytes (0 for sizes that the
  * entry points refuse), 256-byte aligned; calls that share one must be ordered on one stream.
- * Nothing is allocated, nothing synchronises, calls can be captured.  V, H, N <= 2^22 - 64. */
+ * Nothing is allocated, nothing synchronises, calls can be captured.  V, H, N <= 2^22 - 64.
+ * _max: the same with class_max of V, or NULL: what the forward found out about W's classes and
+ * the backward of the same W, sizes and layout otherwise reads W once more for (the tensor-core
+ * form of transW 0; other forms leave it as it is and do not read it). */
 #define KNET_DECL_LINEAR_NLL(f, S, T)                                                          \
   KNET_API size_t knet_linear_nll_workspace_##S(int64_t V, int64_t H, int64_t N, int backward); \
   KNET_API int knet_linear_nll_fwd_##S(const T *w, int transW, const T *b, const T *x,         \
@@ -381,7 +384,18 @@ KNET_BOTH_TYPES(KNET_DECL_NLL, nll)
                                        const int32_t *labels, int64_t V, int64_t H, int64_t N, \
                                        const T *lse, int average, T dy, const int32_t *count,  \
                                        T *dw, T *db, T *dx, void *workspace,                   \
-                                       size_t workspace_bytes, cudaStream_t s);
+                                       size_t workspace_bytes, cudaStream_t s);                \
+  KNET_API int knet_linear_nll_fwd_max_##S(const T *w, int transW, const T *b, const T *x,     \
+                                           const int32_t *labels, int64_t V, int64_t H,        \
+                                           int64_t N, T *total, int32_t *count, T *lse,        \
+                                           T *per_instance, T *class_max, void *workspace,     \
+                                           size_t workspace_bytes, cudaStream_t s);            \
+  KNET_API int knet_linear_nll_bwd_max_##S(const T *w, int transW, const T *b, const T *x,     \
+                                           const int32_t *labels, int64_t V, int64_t H,        \
+                                           int64_t N, const T *lse, const T *class_max,        \
+                                           int average, T dy, const int32_t *count, T *dw,     \
+                                           T *db, T *dx, void *workspace,                      \
+                                           size_t workspace_bytes, cudaStream_t s);
 KNET_BOTH_TYPES(KNET_DECL_LINEAR_NLL, linear_nll)
 
 /* Whole-array reduction to a device scalar without a synchronisation or an allocation.

@@ -193,12 +193,12 @@ constexpr size_t kBiasRoom = 2 * kPlanSMs * 32;
 //   kSmall   up to 2^24 scores and either few instances or little work: the scores go to the workspace
 //   kMma     Float32 beyond that
 //   kPieces  the rest (Float64 with many scores)
-// Few instances: kSmall reads W once per 8 instances, kMma about four times whatever their number (the
-// scale, the split, the product) and needs five launches.  50257x1024, forward / with gradients, us, kSmall and kMma:
-// 8 instances 63 and 171 / 249 and 469, 16 instances 110 and 173 / 417 and 470, 24 instances 156 and 173 / 562 and
-// 478, 32 instances 208 and 175 / 729 and 471.
+// Few instances: kSmall reads W once per 8 instances, kMma reads it, writes it in two planes and reads those whatever
+// their number.  50257x1024, forward / with gradients, us, kSmall and kMma: 8 instances 59 and 133 / 248 and 462,
+// 16 instances 103 and 133 / 419 and 465, 17 instances 147 and 134 / 524 and 477, 24 instances 148 and 133 / 562 and
+// 470, 32 instances 195 and 132 / 730 and 472.
 // Work: FMA tiles and kMma with gradients: 300x256, 400 instances (2^25) 65 and 77 us, 500x512, 512 instances (2^27)
-// 94 and 85 us, 1000x512, 512 instances (2^28) 123 and 91 us.
+// 92 and 81 us, 1000x512, 512 instances (2^28) 120 and 85 us.
 enum Form { kSmall, kMma, kPieces };
 constexpr int64_t kFewInstances = 16;
 template <typename T> Form form(int64_t V, int64_t H, int64_t N) {
@@ -563,27 +563,40 @@ struct SplitState {
   Planes w, x;
   const uint32_t *wmag, *xmag;
 };
-template <int GROUP, int LANES>
-void split_cols_launch(const SplitJob& w, const SplitJob& x, int64_t blocks_x, uint32_t* zeros, int64_t nzeros, cudaStream_t st) {
-  uint32_t ctas = 1;
-  while (ctas < kSplitCtas && w.rows >= 64 * (int64_t)ctas) ctas *= 2;
-  const int64_t bw = ceil_div(w.cols, 8 * LANES) * ctas, bx = ceil_div(blocks_x, ctas) * ctas;
-  launch_chained_cluster(ctas, lnll_split_cols_kernel<GROUP, LANES>, (unsigned)(bw + bx), 256, 0, st, w, x, (uint32_t)bw, ctas, zeros, nzeros);
-}
+// W by columns in one kernel (see there) where a CTA's share of the rows is 128 at most: the shares of all CTAs that run
+// at once then fit L2 (50257x1024 102 us; 32000x4096 so 258 us, by the two 271 us, but 25357x5169, rows of any
+// alignment, 363-569 and 280 us).  A backward that is given the maxima reads W once (66 and 166 us).
+constexpr int64_t kSplitRows = 128 * kSplitCtas;
 template <int GROUP>
-void split_launch(bool rows, const SplitJob& w, const SplitJob& x, bool with_x, uint32_t* zeros, int64_t nzeros, cudaStream_t st) {
+void split_launch(bool rows, const SplitJob& w, const SplitJob& x, bool with_x, bool given, uint32_t* zeros, int64_t nzeros, cudaStream_t st) {
   const int64_t per = 256 / GROUP, bx = with_x ? ceil_div(x.rows, per) : 0;
   if (rows) {
     const int64_t bw = ceil_div(w.rows, per);
     launch_chained(lnll_split_rows_kernel<GROUP>, (unsigned)(bw + bx), 256, 0, st, w, x, (uint32_t)bw, zeros, nzeros);
-  } else if (ceil_div(w.cols, 256) * kSplitCtas >= 2 * kPlanSMs) {
-    split_cols_launch<GROUP, 32>(w, x, bx, zeros, nzeros, st);
-  } else {                   // 64 classes to a cluster where 256 would make less than two CTAs per SM
-    split_cols_launch<GROUP, 8>(w, x, bx, zeros, nzeros, st);
+    return;
   }
+  if (w.rows <= kSplitRows && !given) {
+    uint32_t ctas = 1;
+    while (ctas < kSplitCtas && w.rows >= 64 * (int64_t)ctas) ctas *= 2;
+    const int64_t bw = ceil_div(w.cols, kSplitCols) * ctas, padded = ceil_div(bx, ctas) * ctas;
+    launch_chained_cluster(ctas, lnll_split_cols_kernel<GROUP>, (unsigned)(bw + padded), 256, 0, st, w, x, (uint32_t)bw, ctas, zeros, nzeros);
+    return;
+  }
+  const uint32_t groups = (uint32_t)ceil_div(w.cols, kSplitCols);
+  int64_t share = ceil_div(w.rows, ceil_div(8 * kPlanSMs, groups));      // eight CTAs per SM, 32 rows or more each
+  share = share < 32 ? 32 : share;
+  const int64_t bw = groups * ceil_div(w.rows, share);
+  // ordinary launches: placed under the tail of another kernel, equal shares land unevenly on the SMs (loss and gradients
+  // of 25357x5169, 24 instances 1511 us chained, 1456 so, 1427 with the split of dS launched so too)
+  if (!given) {
+    lnll_zero((float*)w.mag, w.cols, st);
+    lnll_colmax_kernel<<<(unsigned)bw, 256, 0, st>>>(w, groups, share);
+  }
+  lnll_split_wide_kernel<GROUP><<<(unsigned)(bw + bx), 256, 0, st>>>(w, x, (uint32_t)bw, groups, share, zeros, nzeros);
 }
-inline SplitState split_operands(const Head<float>& h, const MmaPlan& p, char* ws, int64_t v0, int64_t vp, uint32_t* zeros, int64_t nzeros,
-                                 cudaStream_t st) {
+// class_max: of W's columns, taken where `given`, else left there if not null
+inline SplitState split_operands(const Head<float>& h, const MmaPlan& p, char* ws, int64_t v0, int64_t vp, uint32_t* class_max, bool given,
+                                 uint32_t* zeros, int64_t nzeros, cudaStream_t st) {
   SplitJob w, x;
   w.src = h.trans ? h.w + v0 * h.H : h.w + v0;
   w.rows = h.trans ? vp : h.H;
@@ -593,7 +606,8 @@ inline SplitState split_operands(const Head<float>& h, const MmaPlan& p, char* w
   w.ld = p.wld;
   w.plane = w.rows * p.wld;
   w.labels = nullptr;
-  w.mag = (uint32_t*)(ws + p.wmag);
+  w.mag = class_max && !h.trans ? class_max + v0 : (uint32_t*)(ws + p.wmag);
+  given = given && class_max && !h.trans;
   x.src = h.x;
   x.rows = h.N;
   x.cols = x.pitch = h.H;
@@ -603,9 +617,9 @@ inline SplitState split_operands(const Head<float>& h, const MmaPlan& p, char* w
   x.labels = h.labels;
   x.mag = (uint32_t*)(ws + p.xmag);
   // threads per row of up to 32 features each
-  if (h.H <= 256) split_launch<8>(h.trans, w, x, v0 == 0, zeros, nzeros, st);
-  else if (h.H <= 1024) split_launch<32>(h.trans, w, x, v0 == 0, zeros, nzeros, st);
-  else split_launch<256>(h.trans, w, x, v0 == 0, zeros, nzeros, st);
+  if (h.H <= 256) split_launch<8>(h.trans, w, x, v0 == 0, given, zeros, nzeros, st);
+  else if (h.H <= 1024) split_launch<32>(h.trans, w, x, v0 == 0, given, zeros, nzeros, st);
+  else split_launch<256>(h.trans, w, x, v0 == 0, given, zeros, nzeros, st);
   return SplitState{Planes{w.dst, w.rows, w.cols, w.ld, w.plane}, Planes{x.dst, x.rows, x.cols, x.ld, x.plane}, w.mag, x.mag};
 }
 
@@ -646,7 +660,7 @@ void statistics(const Head<T>& h, const T* scores, int parts, int64_t chunks, T*
   }
 }
 
-inline int linear_nll_fwd_mma(const Head<float>& h, float* total, int32_t* count, float* lse, float* per_instance, char* ws,
+inline int linear_nll_fwd_mma(const Head<float>& h, float* total, int32_t* count, float* lse, float* per_instance, float* class_max, char* ws,
                               cudaStream_t st) {
   const MmaPlan p = mma_plan(h.V, h.H, h.N, h.trans, 0);
   const int64_t all = ceil_div(h.V, kTN);
@@ -654,7 +668,7 @@ inline int linear_nll_fwd_mma(const Head<float>& h, float* total, int32_t* count
   float *label = (float*)(ws + p.label), *pm = (float*)(ws + p.part_m), *ps = (float*)(ws + p.part_s);
   for (int64_t v0 = 0; v0 < h.V; v0 += p.piece) {
     const int64_t vp = h.V - v0 < p.piece ? h.V - v0 : p.piece;
-    const SplitState s = split_operands(h, p, ws, v0, vp, nullptr, 0, st);
+    const SplitState s = split_operands(h, p, ws, v0, vp, (uint32_t*)class_max, false, nullptr, 0, st);
     if (p.s_parts > 1) {      // one piece
       float* scores = (float*)(ws + p.scores);
       if (int rc = mma_scores(h, p, s, vp, scores, done, st)) return rc;
@@ -678,14 +692,14 @@ void bias_gradient(const T* ds, int64_t ld, int64_t rows, int64_t J, T* db, T* p
   if (grid.y > 1) sum_parts_to<T>(parts, 1, J, J, (int)grid.y, db, 0, g, st);
 }
 
-inline int linear_nll_bwd_mma(const Head<float>& h, const float* lse, GradScale<float> g, float* dw, float* db, float* dx, char* ws,
+inline int linear_nll_bwd_mma(const Head<float>& h, const float* lse, const float* class_max, GradScale<float> g, float* dw, float* db, float* dx, char* ws,
                               cudaStream_t st) {
   const MmaPlan p = mma_plan(h.V, h.H, h.N, h.trans, 1);
   float *parts = (float*)(ws + p.parts), *ds = (float*)(ws + p.ds), *dbp = db ? (float*)(ws + p.db) : nullptr;
   uint32_t *rowmax = (uint32_t*)(ws + p.maxima), *colmax = rowmax + h.N;
   for (int64_t v0 = 0; v0 < h.V; v0 += p.piece) {
     const int64_t vp = h.V - v0 < p.piece ? h.V - v0 : p.piece;
-    const SplitState s = split_operands(h, p, ws, v0, vp, rowmax, h.N + vp, st);
+    const SplitState s = split_operands(h, p, ws, v0, vp, (uint32_t*)class_max, true, rowmax, h.N + vp, st);
     if (p.s_parts > 1) {
       float* scores = (float*)(ws + p.scores);
       if (int rc = mma_scores(h, p, s, vp, scores, nullptr, st)) return rc;
@@ -700,8 +714,9 @@ inline int linear_nll_bwd_mma(const Head<float>& h, const float* lse, GradScale<
     if (!dx && !dw) continue;
     const int64_t plane = h.N * p.dld;
     const Planes for_dx{(__half*)(ws + p.dx_ds), h.N, vp, p.dld, plane}, for_dw{(__half*)(ws + p.dw_ds), h.N, vp, p.dld, plane};
-    launch_chained(lnll_grad_planes_kernel, dim3((unsigned)ceil_div(h.N, kPlaneRows), (unsigned)ceil_div(vp, 256)), 256, 0, st, ds, p.dld, h.N, vp, s.xmag,
-                   s.wmag, rowmax, colmax, dx ? (__half*)for_dx.p : nullptr, dw ? (__half*)for_dw.p : nullptr, plane);
+    // an ordinary launch, as above (10007x515, 333 instances 151 us chained, 145 so)
+    lnll_grad_planes_kernel<<<dim3((unsigned)ceil_div(h.N, kPlaneRows), (unsigned)ceil_div(vp, 256)), 256, 0, st>>>(
+        ds, p.dld, h.N, vp, s.xmag, s.wmag, rowmax, colmax, dx ? (__half*)for_dx.p : nullptr, dw ? (__half*)for_dw.p : nullptr, plane);
     if (dx) {
       const int k = mma_parts(vp, p.x_parts);
       const MmaStore e2{rowmax, nullptr, k == 1 ? dx : parts, h.N, h.H, h.H, k == 1 ? 0 : h.N * h.H, k == 1 && v0 > 0, nullptr, g};
@@ -817,9 +832,9 @@ int linear_nll_bwd_pieces(const Head<T>& h, const T* lse, GradScale<T> g, T* dw,
 }
 
 template <typename T>
-int linear_nll_fwd(const Head<T>& h, T* total, int32_t* count, T* lse, T* per_instance, void* ws, size_t have, cudaStream_t st) {
+int linear_nll_fwd(const Head<T>& h, T* total, int32_t* count, T* lse, T* per_instance, T* class_max, void* ws, size_t have, cudaStream_t st) {
   if (!total || !count || (h.N > 0 && (!lse || !per_instance))) return KN_EINVAL;
-  if (odd(total) || odd(lse) || odd(per_instance) || (uintptr_t)count % 4) return KN_EALIGN;
+  if (odd(total) || odd(lse) || odd(per_instance) || odd(class_max) || (uintptr_t)count % 4) return KN_EALIGN;
   const size_t need = h.V > 0 && h.H > 0 && h.N > 0 && sizes_ok(h.V, h.H, h.N) ? workspace<T>(h.V, h.H, h.N, h.trans, 0) : 0;
   if (int rc = check(h, ws, have, need)) return rc;
   if (h.N == 0) {
@@ -828,7 +843,7 @@ int linear_nll_fwd(const Head<T>& h, T* total, int32_t* count, T* lse, T* per_in
   }
   const Form f = form<T>(h.V, h.H, h.N);
   if constexpr (sizeof(T) == 4) {
-    if (f == kMma) return linear_nll_fwd_mma(h, total, count, lse, per_instance, (char*)ws, st);
+    if (f == kMma) return linear_nll_fwd_mma(h, total, count, lse, per_instance, class_max, (char*)ws, st);
   } else if (f == kPieces) {
     return linear_nll_fwd_pieces<T>(h, total, count, lse, per_instance, (char*)ws, st);
   }
@@ -836,10 +851,10 @@ int linear_nll_fwd(const Head<T>& h, T* total, int32_t* count, T* lse, T* per_in
 }
 
 template <typename T>
-int linear_nll_bwd(const Head<T>& h, const T* lse, int average, T dy, const int32_t* count, T* dw, T* db, T* dx, void* ws,
+int linear_nll_bwd(const Head<T>& h, const T* lse, const T* class_max, int average, T dy, const int32_t* count, T* dw, T* db, T* dx, void* ws,
                    size_t have, cudaStream_t st) {
   if (h.N > 0 && (!lse || (average && !count))) return KN_EINVAL;
-  if (odd(lse) || odd(dw) || odd(db) || odd(dx) || (uintptr_t)count % 4) return KN_EALIGN;
+  if (odd(lse) || odd(class_max) || odd(dw) || odd(db) || odd(dx) || (uintptr_t)count % 4) return KN_EALIGN;
   const size_t need = h.V > 0 && h.H > 0 && h.N > 0 && sizes_ok(h.V, h.H, h.N) ? workspace<T>(h.V, h.H, h.N, h.trans, 1) : 0;
   if (int rc = check(h, ws, have, need)) return rc;
   if (h.N == 0) {
@@ -850,7 +865,7 @@ int linear_nll_bwd(const Head<T>& h, const T* lse, int average, T dy, const int3
   const GradScale<T> g{average ? count : nullptr, dy};
   const Form f = form<T>(h.V, h.H, h.N);
   if constexpr (sizeof(T) == 4) {
-    if (f == kMma) return linear_nll_bwd_mma(h, lse, g, dw, db, dx, (char*)ws, st);
+    if (f == kMma) return linear_nll_bwd_mma(h, lse, class_max, g, dw, db, dx, (char*)ws, st);
   } else if (f == kPieces) {
     return linear_nll_bwd_pieces<T>(h, lse, g, dw, db, dx, (char*)ws, st);
   }
@@ -864,19 +879,33 @@ using namespace kn;
 #define KN_DEF_LNLL(f_, S, T)                                                                                       \
   KN_EXPORT size_t knet_linear_nll_workspace_##S(int64_t V, int64_t H, int64_t N, int backward) {                   \
     if (V <= 0 || H <= 0 || N <= 0 || !sizes_ok(V, H, N)) return 0;                                                 \
-    return workspace_any<T>(V, H, N, backward != 0);                                                                         \
+    return workspace_any<T>(V, H, N, backward != 0);                                                                \
+  }                                                                                                                 \
+  KN_EXPORT int knet_linear_nll_fwd_max_##S(const T* w, int transW, const T* b, const T* x, const int32_t* labels,  \
+                                            int64_t V, int64_t H, int64_t N, T* total, int32_t* count, T* lse,      \
+                                            T* per_instance, T* class_max, void* workspace,                         \
+                                            size_t workspace_bytes, cudaStream_t s) {                               \
+    return linear_nll_fwd<T>(Head<T>{w, transW, b, x, labels, V, H, N}, total, count, lse, per_instance, class_max, \
+                             workspace, workspace_bytes, s);                                                        \
+  }                                                                                                                 \
+  KN_EXPORT int knet_linear_nll_bwd_max_##S(const T* w, int transW, const T* b, const T* x, const int32_t* labels,  \
+                                            int64_t V, int64_t H, int64_t N, const T* lse, const T* class_max,      \
+                                            int average, T dy, const int32_t* count, T* dw, T* db, T* dx,           \
+                                            void* workspace, size_t workspace_bytes, cudaStream_t s) {              \
+    return linear_nll_bwd<T>(Head<T>{w, transW, b, x, labels, V, H, N}, lse, class_max, average, dy, count, dw, db, \
+                             dx, workspace, workspace_bytes, s);                                                    \
   }                                                                                                                 \
   KN_EXPORT int knet_linear_nll_fwd_##S(const T* w, int transW, const T* b, const T* x, const int32_t* labels,      \
                                         int64_t V, int64_t H, int64_t N, T* total, int32_t* count, T* lse,          \
                                         T* per_instance, void* workspace, size_t workspace_bytes, cudaStream_t s) { \
-    return linear_nll_fwd<T>(Head<T>{w, transW, b, x, labels, V, H, N}, total, count, lse, per_instance, workspace, \
-                             workspace_bytes, s);                                                                   \
+    return knet_linear_nll_fwd_max_##S(w, transW, b, x, labels, V, H, N, total, count, lse, per_instance, nullptr,  \
+                                       workspace, workspace_bytes, s);                                              \
   }                                                                                                                 \
   KN_EXPORT int knet_linear_nll_bwd_##S(const T* w, int transW, const T* b, const T* x, const int32_t* labels,      \
                                         int64_t V, int64_t H, int64_t N, const T* lse, int average, T dy,           \
                                         const int32_t* count, T* dw, T* db, T* dx, void* workspace,                 \
                                         size_t workspace_bytes, cudaStream_t s) {                                   \
-    return linear_nll_bwd<T>(Head<T>{w, transW, b, x, labels, V, H, N}, lse, average, dy, count, dw, db, dx,        \
-                             workspace, workspace_bytes, s);                                                        \
+    return knet_linear_nll_bwd_max_##S(w, transW, b, x, labels, V, H, N, lse, nullptr, average, dy, count, dw, db,  \
+                                       dx, workspace, workspace_bytes, s);                                          \
   }
 KNET_BOTH_TYPES(KN_DEF_LNLL, lnll)

@@ -467,109 +467,146 @@ lnll_split_rows_kernel(SplitJob w, SplitJob x, uint32_t blocks_w, uint32_t* zero
   else split_rows<GROUP>(w, blockIdx.x, red);
 }
 
-// W whose classes are columns: a cluster of CTAs takes 8 * LANES of them, each CTA a share of the rows (the features)
-// and a thread eight classes.  The maxima of the shares meet through the cluster's shared memory; the second read
-// of a share, from its end, finds part of it in L1 and most in L2.
+// W whose classes are columns.  A thread takes eight of them and every eighth row (the features), so that its rows
+// have one offset in their 16-byte words; a CTA 256 classes.
+constexpr int kSplitCols = 256;
+template <int UN, int OFF>
+__device__ __forceinline__ void col_maxima(const SplitJob& w, int64_t c, int64_t r0, int64_t hi, uint32_t (&m)[8]) {
+  for (int64_t r = r0; r < hi; r += 8 * UN) {
+    float v[UN][8];
+#pragma unroll
+    for (int u = 0; u < UN; u++)
+      if (r + 8 * u < hi) load_at<OFF>(w.src + (r + 8 * u) * w.pitch + c, w.cols - c, v[u]);
+#pragma unroll
+    for (int u = 0; u < UN; u++)
+      if (r + 8 * u < hi) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) m[e] = max(m[e], finite_bits(v[u][e]));
+      }
+  }
+}
+// from the last row, which the maxima's pass has left in the caches
+template <int UN, int OFF>
+__device__ __forceinline__ void col_split(const SplitJob& w, int64_t c, int64_t r0, int64_t hi, const float (&f)[8]) {
+  for (int64_t r = r0 + (hi - 1 - r0) / 8 * 8; r >= r0; r -= 8 * UN) {
+    float v[UN][8];
+#pragma unroll
+    for (int u = 0; u < UN; u++)
+      if (r - 8 * u >= r0) load_at<OFF>(w.src + (r - 8 * u) * w.pitch + c, w.cols - c, v[u]);
+#pragma unroll
+    for (int u = 0; u < UN; u++)
+      if (r - 8 * u >= r0) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[u][e] *= f[e];
+        store_split(w, r - 8 * u, c, v[u]);
+      }
+  }
+}
+struct ColumnShare {
+  int64_t c, r0, hi;           // this thread's first class, first row and the end of the CTA's rows
+  bool in;
+  int how;                     // offset in a word, 4 at the ends of a row
+  __device__ __forceinline__ ColumnShare(const SplitJob& w, int64_t group, int64_t lo, int64_t hi_)
+      : c(group * kSplitCols + (threadIdx.x & 31) * 8), r0(lo + (threadIdx.x >> 5)), hi(min(w.rows, hi_)) {
+    in = c < w.cols && r0 < hi;
+    const int off = in ? offset_of(w.src + r0 * w.pitch + c) : 0;
+    how = words_inside(off, c, w.cols) ? off : 4;
+  }
+  template <int UN> __device__ __forceinline__ void maxima(const SplitJob& w, uint32_t (*part)[kSplitCols]) const {
+    uint32_t m[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (in) switch (how) {
+        case 0: col_maxima<UN, 0>(w, c, r0, hi, m); break;
+        case 1: col_maxima<UN, 1>(w, c, r0, hi, m); break;
+        case 2: col_maxima<UN, 2>(w, c, r0, hi, m); break;
+        case 3: col_maxima<UN, 3>(w, c, r0, hi, m); break;
+        default: col_maxima<UN, 4>(w, c, r0, hi, m);
+      }
+#pragma unroll
+    for (int e = 0; e < 8; e++) part[threadIdx.x >> 5][(threadIdx.x & 31) * 8 + e] = m[e];
+  }
+  template <int UN> __device__ __forceinline__ void split(const SplitJob& w, const float (&f)[8]) const {
+    switch (how) {
+      case 0: return col_split<UN, 0>(w, c, r0, hi, f);
+      case 1: return col_split<UN, 1>(w, c, r0, hi, f);
+      case 2: return col_split<UN, 2>(w, c, r0, hi, f);
+      case 3: return col_split<UN, 3>(w, c, r0, hi, f);
+      default: return col_split<UN, 4>(w, c, r0, hi, f);
+    }
+  }
+};
+__device__ __forceinline__ uint32_t joined(const uint32_t (*part)[kSplitCols]) {      // of column threadIdx.x
+  uint32_t a = 0;
+#pragma unroll
+  for (int k = 0; k < 8; k++) a = max(a, part[k][threadIdx.x]);
+  return a;
+}
+
+// Few features: a cluster of CTAs takes the 256 classes, each CTA a share of the rows.  The maxima of the shares meet
+// through the cluster's shared memory; the second read of a share finds it in L1 and L2.  The clusters of the first
+// blocks take W, the other blocks x.
 __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
   uint32_t v;
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
 constexpr int kSplitCtas = 8;
-template <int STEP, int OFF>
-__device__ __forceinline__ void col_maxima(const SplitJob& w, int64_t c, int64_t r0, int64_t hi, uint32_t (&m)[8]) {
-  constexpr int UN = 2;
-  for (int64_t r = r0; r < hi; r += STEP * UN) {
-    float v[UN][8];
-#pragma unroll
-    for (int u = 0; u < UN; u++)
-      if (r + STEP * u < hi) load_at<OFF>(w.src + (r + STEP * u) * w.pitch + c, w.cols - c, v[u]);
-#pragma unroll
-    for (int u = 0; u < UN; u++)
-      if (r + STEP * u < hi) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) m[e] = max(m[e], finite_bits(v[u][e]));
-      }
-  }
-}
-template <int STEP, int OFF>
-__device__ __forceinline__ void col_split(const SplitJob& w, int64_t c, int64_t r0, int64_t hi, const float (&f)[8]) {
-  constexpr int UN = 2;
-  for (int64_t r = r0 + (hi - 1 - r0) / STEP * STEP; r >= r0; r -= STEP * UN) {
-    float v[UN][8];
-#pragma unroll
-    for (int u = 0; u < UN; u++)
-      if (r - STEP * u >= r0) load_at<OFF>(w.src + (r - STEP * u) * w.pitch + c, w.cols - c, v[u]);
-#pragma unroll
-    for (int u = 0; u < UN; u++)
-      if (r - STEP * u >= r0) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) v[u][e] *= f[e];
-        store_split(w, r - STEP * u, c, v[u]);
-      }
-  }
-}
-// the clusters of the first blocks take W, the other blocks x
-template <int GROUP, int LANES>
+template <int GROUP>
 __global__ void __launch_bounds__(256, 4)
 lnll_split_cols_kernel(SplitJob w, SplitJob x, uint32_t blocks_w, uint32_t ctas, uint32_t* zeros, int64_t nzeros) {
   chain_begin();
   clear(zeros, nzeros);
-  constexpr int COLS = LANES * 8, STEP = 256 / LANES;    // a multiple of 4, so that a thread's rows have one offset
-  __shared__ uint32_t part[8][COLS], mine[COLS], all[COLS];
+  __shared__ uint32_t part[8][kSplitCols], mine[kSplitCols], all[kSplitCols];
   if (blockIdx.x >= blocks_w) return split_rows<GROUP>(x, blockIdx.x - blocks_w, mine);
   const uint32_t rank = ctas > 1 ? cluster_rank() : 0;
-  const int64_t g0 = (int64_t)(blockIdx.x / ctas) * COLS, share = (w.rows + ctas - 1) / ctas;
-  const int64_t lo = rank * share, hi = min(w.rows, lo + share);
-  const int lane = threadIdx.x % LANES;
-  const int64_t c = g0 + lane * 8, r0 = lo + threadIdx.x / LANES;
-  const bool in = c < w.cols && r0 < hi;
-  const int off = in ? offset_of(w.src + r0 * w.pitch + c) : 0, how = words_inside(off, c, w.cols) ? off : 4;
-  uint32_t m[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  if (in) switch (how) {
-      case 0: col_maxima<STEP, 0>(w, c, r0, hi, m); break;
-      case 1: col_maxima<STEP, 1>(w, c, r0, hi, m); break;
-      case 2: col_maxima<STEP, 2>(w, c, r0, hi, m); break;
-      case 3: col_maxima<STEP, 3>(w, c, r0, hi, m); break;
-      default: col_maxima<STEP, 4>(w, c, r0, hi, m);
-    }
-  __syncwarp();
-#pragma unroll
-  for (int e = 0; e < 8; e++) {
-#pragma unroll
-    for (int o = LANES; o < 32; o <<= 1) m[e] = max(m[e], __shfl_xor_sync(0xffffffffu, m[e], o));
-    if ((threadIdx.x & 31) < LANES) part[threadIdx.x >> 5][lane * 8 + e] = m[e];
-  }
+  const int64_t group = blockIdx.x / ctas, share = (w.rows + ctas - 1) / ctas, col = group * kSplitCols + threadIdx.x;
+  const ColumnShare s(w, group, rank * share, (rank + 1) * share);
+  s.maxima<2>(w, part);
   __syncthreads();
-  if (threadIdx.x < COLS) {
-    uint32_t a = 0;
-#pragma unroll
-    for (int k = 0; k < 8; k++) a = max(a, part[k][threadIdx.x]);
-    mine[threadIdx.x] = a;
-    all[threadIdx.x] = a;
-  }
+  uint32_t a = joined(part);
+  mine[threadIdx.x] = a;
   if (ctas > 1) {
     cluster_barrier();
-    if (threadIdx.x < COLS) {
-      uint32_t a = 0;
-      for (uint32_t k = 0; k < ctas; k++) a = max(a, ld_cluster_u32(mapa_u32(&mine[threadIdx.x], k)));
-      all[threadIdx.x] = a;
-    }
+    for (uint32_t k = 0; k < ctas; k++) a = max(a, ld_cluster_u32(mapa_u32(&mine[threadIdx.x], k)));
     cluster_barrier();                                   // no CTA leaves while another reads its share
   }
+  all[threadIdx.x] = a;
   __syncthreads();
-  if (rank == 0 && threadIdx.x < COLS && g0 + threadIdx.x < w.cols) w.mag[g0 + threadIdx.x] = all[threadIdx.x];
-  if (!in) return;
+  if (rank == 0 && col < w.cols) w.mag[col] = a;
+  if (!s.in) return;
   float f[8];
 #pragma unroll
-  for (int e = 0; e < 8; e++) f[e] = scale_of(magnitude(all[lane * 8 + e]));
-  switch (how) {
-    case 0: return col_split<STEP, 0>(w, c, r0, hi, f);
-    case 1: return col_split<STEP, 1>(w, c, r0, hi, f);
-    case 2: return col_split<STEP, 2>(w, c, r0, hi, f);
-    case 3: return col_split<STEP, 3>(w, c, r0, hi, f);
-    default: return col_split<STEP, 4>(w, c, r0, hi, f);
-  }
+  for (int e = 0; e < 8; e++) f[e] = scale_of(magnitude(all[(threadIdx.x & 31) * 8 + e]));
+  s.split<2>(w, f);
+}
+
+// Many features, or maxima that are known: the maxima (which begin at 0) by one kernel, the split by another, whose last
+// blocks take x.
+__global__ void __launch_bounds__(256, 4)
+lnll_colmax_kernel(SplitJob w, uint32_t groups, int64_t share) {
+  chain_begin();
+  __shared__ uint32_t part[8][kSplitCols];
+  const uint32_t group = blockIdx.x % groups, turn = blockIdx.x / groups;
+  const ColumnShare s(w, group, turn * share, (turn + 1) * share);
+  s.maxima<4>(w, part);
+  __syncthreads();
+  const uint32_t a = joined(part);
+  const int64_t col = (int64_t)group * kSplitCols + threadIdx.x;
+  if (col < w.cols && a) atomicMax(w.mag + col, a);
+}
+template <int GROUP>
+__global__ void __launch_bounds__(256, 4)
+lnll_split_wide_kernel(SplitJob w, SplitJob x, uint32_t blocks_w, uint32_t groups, int64_t share, uint32_t* zeros, int64_t nzeros) {
+  chain_begin();
+  clear(zeros, nzeros);
+  __shared__ uint32_t red[32];
+  if (blockIdx.x >= blocks_w) return split_rows<GROUP>(x, blockIdx.x - blocks_w, red);
+  const uint32_t group = blockIdx.x % groups, turn = blockIdx.x / groups;
+  const ColumnShare s(w, group, turn * share, (turn + 1) * share);
+  if (!s.in) return;
+  float f[8];
+#pragma unroll
+  for (int e = 0; e < 8; e++) f[e] = s.c + e < w.cols ? scale_of(magnitude(w.mag[s.c + e])) : 0.0f;
+  s.split<2>(w, f);
 }
 
 // ---- epilogues -------------------------------------------------------------------------------------------

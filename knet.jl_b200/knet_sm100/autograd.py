@@ -457,7 +457,9 @@ def nll(scores, labels, dims=1, average=True):
 def linear_nll(w, x, labels, b=None, trans=False, average=True):
     """nll(w*x .+ b, labels) (w' * x with `trans`) as one fused primitive that never holds the
     scores; w, x and b may be tracked.  A backward sweep that is itself recorded (a gradient of a
-    gradient) spells the gradients with the primitives of this module instead, scores included."""
+    gradient) spells the gradients with the primitives of this module instead, scores included.
+    The sweep reads dy on the host, as nll's does: it waits for the loss and cannot be captured into a
+    graph (ops.linear_nll_device and ops.linear_nll_back can)."""
     wv, xv, bv = _val(w), _val(x), _val(b)
     res = ops.linear_nll_device(wv, xv, labels, bv, trans)
     if not _tracked(w, x, b):

@@ -373,12 +373,13 @@ def nll_back(scores, labels, dims=1, average=True, dy=1.0, count=None):
 
 
 class LinearNllResult(NllResult):
-    """Device-side result of linear_nll_device: NllResult plus `saved`, what the backward pass reads: log
-    sum exp per instance as its rounded value (`lse`) and the remainder of that rounding."""
+    """Device-side result of linear_nll_device: NllResult plus what the backward pass reads: `saved`, log
+    sum exp per instance as its rounded value (`lse`) and the remainder of that rounding, and `class_max` (or
+    None), the largest magnitudes of the classes of w."""
 
-    def __init__(self, total, count, per_instance, labels, saved):
+    def __init__(self, total, count, per_instance, labels, saved, class_max=None):
         super().__init__(total, count, per_instance, labels)
-        self.saved = saved
+        self.saved, self.class_max = saved, class_max
 
     @property
     def lse(self):
@@ -423,11 +424,13 @@ def linear_nll_device(w, x, labels, b=None, trans=False):
         count = torch.empty(1, dtype=torch.int32, device=dev)
         per = torch.empty(max(N, 1), dtype=dt, device=dev)
         lse = torch.empty(2 * N, dtype=dt, device=dev)
+        top = None if trans or dt != torch.float32 else torch.empty(V, dtype=dt, device=dev)
         size = getattr(libknet, f"knet_linear_nll_workspace_{S}")(V, H, N, 0)
         ws = torch.empty(max(size, 1), dtype=torch.uint8, device=dev)
-        knet(f"knet_linear_nll_fwd_{S}", _address(w), 1 if trans else 0, _address(b), _address(x), lab.data_ptr(), V, H, N,
-             total.data_ptr(), count.data_ptr(), lse.data_ptr(), per.data_ptr(), ws.data_ptr(), size)
-    return LinearNllResult(total, count, per, lab, lse)
+        knet(f"knet_linear_nll_fwd_max_{S}", _address(w), 1 if trans else 0, _address(b), _address(x), lab.data_ptr(), V, H, N,
+             total.data_ptr(), count.data_ptr(), lse.data_ptr(), per.data_ptr(), None if top is None else top.data_ptr(), ws.data_ptr(),
+             size)
+    return LinearNllResult(total, count, per, lab, lse, top)
 
 
 def linear_nll(w, x, labels, b=None, trans=False, average=True):
@@ -440,7 +443,8 @@ def linear_nll_back(w, x, res, b=None, trans=False, average=True, dy=1.0, need=(
     None without b.  `need` leaves some of them out (None); `out` gives arrays to write them to."""
     V, H, N = _head_sizes(w, x, b, trans)
     dev, dt = w.data.device, w.data.dtype
-    if res.labels.numel() != N or res.saved.dtype != dt or res.labels.device != dev:
+    top = None if trans else res.class_max
+    if res.labels.numel() != N or res.saved.dtype != dt or res.labels.device != dev or (top is not None and top.numel() != V):
         raise ValueError("DimensionMismatch: the forward result belongs to other arrays")
     S = sfx(dt)
     with on_device(dev):
@@ -459,8 +463,8 @@ def linear_nll_back(w, x, res, b=None, trans=False, average=True, dy=1.0, need=(
             return None, None, None
         size = getattr(libknet, f"knet_linear_nll_workspace_{S}")(V, H, N, 1)
         ws = torch.empty(max(size, 1), dtype=torch.uint8, device=dev)
-        knet(f"knet_linear_nll_bwd_{S}", _address(w), 1 if trans else 0, _address(b), _address(x), res.labels.data_ptr(), V, H, N,
-             res.saved.data_ptr(), 1 if average else 0, dy, res.count.data_ptr(), _address(dw), _address(db), _address(dx),
+        knet(f"knet_linear_nll_bwd_max_{S}", _address(w), 1 if trans else 0, _address(b), _address(x), res.labels.data_ptr(), V, H, N,
+             res.saved.data_ptr(), None if top is None else top.data_ptr(), 1 if average else 0, dy, res.count.data_ptr(), _address(dw), _address(db), _address(dx),
              ws.data_ptr(), size)
     return dw, dx, db
 

@@ -245,3 +245,25 @@ def test_weights_in_columns_captured_and_on_two_streams(K, shape):
         graphs[g].replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs[g], want[k]))
+
+
+@pytest.mark.parametrize("off", [0, 1])
+@pytest.mark.parametrize("shape", [(1000, 256, 300), (1001, 260, 301), (3000, 2000, 300), (2501, 1100, 200), (9000, 96, 3000)], ids=str)
+def test_maxima_handed_to_the_backward_or_not(K, shape, off):
+    """With W's maxima from the forward the backward reads W once, without them it finds them again: the same bits, at
+    any alignment of W."""
+    c = Case(*shape, torch.float32, False, True, True)
+    kw, kx, kb = c.arrays(K)
+    big = torch.zeros(len(kw) + 4, device="cuda")
+    big[off:off + len(kw)] = kw.data
+    kw = K.KnetArray(big[off:off + len(kw)], kw.shape)
+    res = K.ops.linear_nll_device(kw, kx, c.labels, b=kb)
+    top = c.w.abs().max(1).values
+    assert torch.equal(res.class_max, top)
+    got = [g.data.clone() for g in K.ops.linear_nll_back(kw, kx, res, b=kb)]
+    assert torch.equal(res.class_max, top)                             # read, not written
+    res.class_max = None
+    assert all(torch.equal(g, h.data) for g, h in zip(got, K.ops.linear_nll_back(kw, kx, res, b=kb)))
+    c.solve()
+    within(c.matrix(K.KnetArray(got[0], kw.shape)), c.dw, c.ddw, "dw")
+    within(got[1].view(c.N, c.H), c.dx, c.ddx, "dx")

@@ -71,3 +71,14 @@ def test_workspace_holds_no_room_that_nothing_uses(lib):
     scores = 10 * 100_000
     assert lib.knet_linear_nll_workspace_64(10, 4096, 100_000, 1) < 2 * 8 * scores + (64 << 20) + (1 << 20)
     assert lib.knet_linear_nll_workspace_32(10, 64, 100_000, 1) < 4 * scores + (1 << 20)
+
+
+def test_the_forms_that_hand_maxima_over(lib):
+    """knet_linear_nll_*_max_S refuse what the forms without `class_max` refuse, and one of odd alignment."""
+    for S in ("32", "64"):
+        f = lambda class_max=P, V=V, ws=P, need=1 << 40: getattr(lib, f"knet_linear_nll_fwd_max_{S}")(
+            P, 0, None, P, P, V, H, N, P, P, P, P, class_max, ws, need, None)
+        b = lambda class_max=P, V=V, ws=P, need=1 << 40: getattr(lib, f"knet_linear_nll_bwd_max_{S}")(
+            P, 0, None, P, P, V, H, N, P, class_max, 1, 1.0, P, P, None, P, ws, need, None)
+        for g in (f, b):
+            assert g(V=0) == -1 and g(V=1 << 22) == -2 and g(ws=None) == -3 and g(need=0) == -3 and g(class_max=P + 2) == -4

@@ -360,8 +360,17 @@ __device__ __forceinline__ void split_pair(float v0, float v1, uint32_t& hi, uin
 // Eight consecutive floats at p, of which `left` are inside the row (0 past its end).  OFF 0..3: p lies OFF floats past a
 // multiple of 16 bytes and the aligned 16-byte words around the eight are inside the row; the shift is the same for
 // all rows that a thread walks, so it is a constant here.  OFF 4: single loads.
+// OFF 5: as 0..3 but by the address (rows of a warp that differ in it would else take turns).
+__device__ __forceinline__ int offset_of(const float* p) { return (int)(((uintptr_t)p >> 2) & 3); }
 template <int OFF> __device__ __forceinline__ void load_at(const float* p, int64_t left, float (&v)[8]) {
-  if constexpr (OFF < 4) {
+  if constexpr (OFF == 5) {
+    const int off = offset_of(p);
+    const float4* q = reinterpret_cast<const float4*>(p - off);
+    const float4 a = q[0], b = q[1], d = off ? q[2] : b;
+    const float t[12] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, d.x, d.y, d.z, d.w};
+#pragma unroll
+    for (int k = 0; k < 8; k++) v[k] = off == 0 ? t[k] : off == 1 ? t[k + 1] : off == 2 ? t[k + 2] : t[k + 3];
+  } else if constexpr (OFF < 4) {
     const float4* q = reinterpret_cast<const float4*>(p - OFF);
     const float4 a = q[0], b = q[1], d = OFF ? q[2] : b;
     const float t[12] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, d.x, d.y, d.z, d.w};
@@ -372,7 +381,6 @@ template <int OFF> __device__ __forceinline__ void load_at(const float* p, int64
     for (int k = 0; k < 8; k++) v[k] = k < left ? p[k] : 0.0f;
   }
 }
-__device__ __forceinline__ int offset_of(const float* p) { return (int)(((uintptr_t)p >> 2) & 3); }
 __device__ __forceinline__ bool words_inside(int off, int64_t c, int64_t cols) { return c - off >= 0 && c - off + (off ? 12 : 8) <= cols; }
 
 // 8 values times their scales in two planes; the pitch is a multiple of 8
@@ -386,9 +394,17 @@ __device__ __forceinline__ void store_split(const SplitJob& j, int64_t r, int64_
   *reinterpret_cast<uint4*>(j.dst + j.plane + r * j.ld + c) = lo;
 }
 
-// x, or W whose classes are rows: GROUP threads take a row, read it (up to 32 values per thread stay in registers,
-// what is longer comes from L1 the second time) and scale it by its own maximum.  In a skipped instance
-// (label 0) whatever has no fp16 value becomes 0: its dS is 0, which times infinity would be NaN in dW.
+// x, or W whose classes are rows, which lie one behind the other: GROUP threads take a row, read it (up to 32 values per
+// thread stay in registers, what is longer comes from L1 the second time) and scale it by its own maximum.  In a
+// skipped instance (label 0) whatever has no fp16 value becomes 0: its dS is 0, which times infinity would be NaN in dW.
+template <int OFF> __device__ __forceinline__ void load_of_row(const float* p, int64_t left, float (&v)[8]) {
+  load_at<OFF>(p, left, v);                              // the words around the eight may reach into the rows beside this one
+  if (OFF != 4 && left < 8) {
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+      if (k >= left) v[k] = 0.0f;
+  }
+}
 template <int GROUP, int OFF>
 __device__ __forceinline__ void split_row(const SplitJob& j, int64_t r, bool live, uint32_t* red) {
   constexpr int KEEP = 4;
@@ -396,16 +412,12 @@ __device__ __forceinline__ void split_row(const SplitJob& j, int64_t r, bool liv
   const float* row = j.src + r * j.pitch;
   const bool skipped = j.labels && j.labels[r] == 0;
   const bool kept = j.cols <= KEEP * GROUP * 8;
-  auto load = [&](int64_t c, float (&v)[8]) {
-    if (words_inside(OFF, c, j.cols)) load_at<OFF>(row + c, 8, v);
-    else load_at<4>(row + c, j.cols - c, v);
-  };
   float v[KEEP][8];
   uint32_t m = 0;
   for (int64_t c0 = t * 8; c0 < j.cols; c0 += KEEP * GROUP * 8) {
 #pragma unroll
     for (int k = 0; k < KEEP; k++)
-      if (c0 + k * GROUP * 8 < j.cols) load(c0 + k * GROUP * 8, v[k]);
+      if (c0 + k * GROUP * 8 < j.cols) load_of_row<OFF>(row + c0 + k * GROUP * 8, j.cols - c0 - k * GROUP * 8, v[k]);
 #pragma unroll
     for (int k = 0; k < KEEP; k++)
       if (c0 + k * GROUP * 8 < j.cols) {
@@ -428,7 +440,7 @@ __device__ __forceinline__ void split_row(const SplitJob& j, int64_t r, bool liv
     for (int k = 0; k < KEEP; k++) {
       const int64_t c = c0 + k * GROUP * 8;
       if (c >= j.cols) break;
-      if (!kept) load(c, v[k]);
+      if (!kept) load_of_row<OFF>(row + c, j.cols - c, v[k]);
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         v[k][e] *= f;
@@ -442,12 +454,16 @@ template <int GROUP> __device__ __forceinline__ void split_rows(const SplitJob& 
   const int64_t at = block * (256 / GROUP) + threadIdx.x / GROUP;
   const bool live = at < j.rows;
   const int64_t r = live ? at : j.rows - 1;
-  switch (offset_of(j.src + r * j.pitch)) {              // one row per CTA where it has barriers
-    case 0: return split_row<GROUP, 0>(j, r, live, red);
-    case 1: return split_row<GROUP, 1>(j, r, live, red);
-    case 2: return split_row<GROUP, 2>(j, r, live, red);
-    default: return split_row<GROUP, 3>(j, r, live, red);
-  }
+  // a row's words lie inside the array but at its two ends; one row per CTA where it has barriers
+  const bool inside = r * j.pitch >= 3 && (j.rows - 1 - r) * j.pitch >= 12;
+  if constexpr (GROUP < 32) return inside ? split_row<GROUP, 5>(j, r, live, red) : split_row<GROUP, 4>(j, r, live, red);
+  else switch (inside ? offset_of(j.src + r * j.pitch) : 4) {
+      case 0: return split_row<GROUP, 0>(j, r, live, red);
+      case 1: return split_row<GROUP, 1>(j, r, live, red);
+      case 2: return split_row<GROUP, 2>(j, r, live, red);
+      case 3: return split_row<GROUP, 3>(j, r, live, red);
+      default: return split_row<GROUP, 4>(j, r, live, red);
+    }
 }
 
 // maxima of dS's rows and columns, which a kernel that follows takes, begin at 0
@@ -915,6 +931,7 @@ lnll_grad_scores_kernel(const float* scores, int parts, const float* bias, const
                         const uint32_t* wmag, int64_t N, int64_t V, int64_t v0, float* ds, int64_t ld, uint32_t* rowmax, uint32_t* colmax,
                         float* db_part) {
   chain_begin();
+  __shared__ float row_top[8][kGradRows];                // one atomic per CTA and row: thousands to one address queue up
   const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x, n0 = (int64_t)blockIdx.y * kGradRows;
   const float b = bias && v < V ? bias[v] : 0.0f, mw = v < V ? magnitude(wmag[v]) : 0.0f;
   float t[kGradRows], sum = 0.0f, cm = 0.0f;
@@ -934,7 +951,14 @@ lnll_grad_scores_kernel(const float* scores, int parts, const float* bias, const
     if (v < V) ds[n * ld + v] = d;
     cm = fmaxf(cm, fabsf(d * magnitude(xmag[n])));
     const float rm = warp_reduce(fmaxf(0.0f, fabsf(d * mw)), [](float x, float y) { return fmaxf(x, y); });
-    if ((threadIdx.x & 31) == 0 && rm > 0.0f) atomicMax(rowmax + n, __float_as_uint(rm));
+    if ((threadIdx.x & 31) == 0) row_top[threadIdx.x >> 5][k] = rm;
+  }
+  __syncthreads();
+  if (threadIdx.x < kGradRows && n0 + threadIdx.x < N) {
+    float rm = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; k++) rm = fmaxf(rm, row_top[k][threadIdx.x]);
+    if (rm > 0.0f) atomicMax(rowmax + n0 + threadIdx.x, __float_as_uint(rm));
   }
   if (v < V && cm > 0.0f) atomicMax(colmax + v, __float_as_uint(cm));
   if (db_part && v < V) db_part[(int64_t)blockIdx.y * V + v] = sum;

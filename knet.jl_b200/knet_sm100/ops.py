@@ -424,7 +424,8 @@ def linear_nll_device(w, x, labels, b=None, trans=False):
         count = torch.empty(1, dtype=torch.int32, device=dev)
         per = torch.empty(max(N, 1), dtype=dt, device=dev)
         lse = torch.empty(2 * N, dtype=dt, device=dev)
-        top = None if trans or dt != torch.float32 else torch.empty(V, dtype=dt, device=dev)
+        tensor_core = dt == torch.float32 and (V * H * N >= 1 << 26 or V * N > 1 << 24)      # the form that fills it
+        top = torch.empty(V, dtype=dt, device=dev) if tensor_core and not trans else None
         size = getattr(libknet, f"knet_linear_nll_workspace_{S}")(V, H, N, 0)
         ws = torch.empty(max(size, 1), dtype=torch.uint8, device=dev)
         knet(f"knet_linear_nll_fwd_max_{S}", _address(w), 1 if trans else 0, _address(b), _address(x), lab.data_ptr(), V, H, N,

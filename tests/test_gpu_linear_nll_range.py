@@ -267,3 +267,28 @@ def test_maxima_handed_to_the_backward_or_not(K, shape, off):
     c.solve()
     within(c.matrix(K.KnetArray(got[0], kw.shape)), c.dw, c.ddw, "dw")
     within(got[1].view(c.N, c.H), c.dx, c.ddx, "dx")
+
+
+@pytest.mark.parametrize("trans", [False, True])
+@pytest.mark.parametrize("shape", [(70000, 1, 1000), (40000, 3, 700), (3000, 73, 400), (2000, 300, 200), (700, 700, 200), (1000, 1352, 100),
+                                   (301, 2049, 150), (300, 5169, 60), (33, 9001, 250)], ids=str)
+def test_rows_of_every_length_and_alignment(K, trans, shape):
+    """W and x that start 0 to 3 values past a 16-byte word, with NaN just before and behind them: each row has its own
+    offset in a word, and what lies beside an array is not read into it."""
+    c = Case(*shape, torch.float32, trans, True, True)
+    kw, kx, kb = c.arrays(K)
+    res = K.ops.linear_nll_device(kw, kx, c.labels, b=kb, trans=trans)
+    want = [res.total, res.lse] + [g.data for g in K.ops.linear_nll_back(kw, kx, res, b=kb, trans=trans)]
+    c.solve()
+    within(res.lse, c.lse, c.dlse, "lse")
+    within(c.matrix(K.KnetArray(want[2], kw.shape)), c.dw, c.ddw, "dw")
+    within(want[3].view(c.N, c.H), c.dx, c.ddx, "dx")
+    for off in (1, 2, 3):
+        views = []
+        for a in (kw, kx):
+            buf = torch.full((len(a) + 16,), float("nan"), device="cuda")
+            buf[4 + off:4 + off + len(a)] = a.data
+            views.append(K.KnetArray(buf[4 + off:4 + off + len(a)], a.shape))
+        res = K.ops.linear_nll_device(*views, c.labels, b=kb, trans=trans)
+        got = [res.total, res.lse] + [g.data for g in K.ops.linear_nll_back(*views, res, b=kb, trans=trans)]
+        assert all(torch.equal(g, w) for g, w in zip(got, want)), off

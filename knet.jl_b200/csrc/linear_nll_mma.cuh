@@ -359,8 +359,7 @@ __device__ __forceinline__ void split_pair(float v0, float v1, uint32_t& hi, uin
 
 // Eight consecutive floats at p, of which `left` are inside the row (0 past its end).  OFF 0..3: p lies OFF floats past a
 // multiple of 16 bytes and the aligned 16-byte words around the eight are inside the row; the shift is the same for
-// all rows that a thread walks, so it is a constant here.  OFF 4: single loads.
-// OFF 5: as 0..3 but by the address (rows of a warp that differ in it would else take turns).
+// all rows that a thread walks, so it is a constant here.  OFF 4: single loads.  OFF 5: as 0..3 but by the address (rows of a warp that differ in it would else take turns).
 __device__ __forceinline__ int offset_of(const float* p) { return (int)(((uintptr_t)p >> 2) & 3); }
 template <int OFF> __device__ __forceinline__ void load_at(const float* p, int64_t left, float (&v)[8]) {
   if constexpr (OFF == 5) {
@@ -394,9 +393,7 @@ __device__ __forceinline__ void store_split(const SplitJob& j, int64_t r, int64_
   *reinterpret_cast<uint4*>(j.dst + j.plane + r * j.ld + c) = lo;
 }
 
-// x, or W whose classes are rows, which lie one behind the other: GROUP threads take a row, read it (up to 32 values per
-// thread stay in registers, what is longer comes from L1 the second time) and scale it by its own maximum.  In a
-// skipped instance (label 0) whatever has no fp16 value becomes 0: its dS is 0, which times infinity would be NaN in dW.
+// of rows that lie one behind the other
 template <int OFF> __device__ __forceinline__ void load_of_row(const float* p, int64_t left, float (&v)[8]) {
   load_at<OFF>(p, left, v);                              // the words around the eight may reach into the rows beside this one
   if (OFF != 4 && left < 8) {
@@ -405,6 +402,9 @@ template <int OFF> __device__ __forceinline__ void load_of_row(const float* p, i
       if (k >= left) v[k] = 0.0f;
   }
 }
+// x, or W whose classes are rows, which lie one behind the other: GROUP threads take a row, read it (up to 32 values per
+// thread stay in registers, what is longer comes from L1 the second time) and scale it by its own maximum.  In a
+// skipped instance (label 0) whatever has no fp16 value becomes 0: its dS is 0, which times infinity would be NaN in dW.
 template <int GROUP, int OFF>
 __device__ __forceinline__ void split_row(const SplitJob& j, int64_t r, bool live, uint32_t* red) {
   constexpr int KEEP = 4;
